@@ -1,0 +1,120 @@
+"""The paged 4-bit KV cache of include/cactus_hip.h from Python: the cache
+descriptor as a ctypes structure, and an owner of its device buffers."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+
+from . import DeviceBuffer, call, hip
+
+NO_PAGES = 1       # CACTUS_HIP_KV4_NO_PAGES
+BAD_REQUEST = 2    # CACTUS_HIP_KV4_BAD_REQUEST
+
+
+class CacheDesc(ctypes.Structure):
+    """cactus_hip_kv4_cache: pass `desc.ref` as the entry points' cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("pages", "table", "lens", "refs", "state")] + \
+               [(n, ctypes.c_size_t) for n in ("layers", "kv_heads", "head_dim", "page_size", "num_pages", "max_seqs",
+                                               "max_pages")]
+
+    @property
+    def ref(self):
+        return ctypes.byref(self)
+
+
+class KV4Cache:
+    """Pages, tables and workspace of one cache, set up by cactus_hip_kv4_reset.
+
+    The methods take device pointers (DeviceBuffer.ptr, or any integer) where
+    the entry points do; slot and page lists may be sequences of ints, which
+    are uploaded first."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, page_size: int, num_pages: int, max_seqs: int,
+                 max_pages: int, stream=None):
+        self.desc = CacheDesc(layers=layers, kv_heads=kv_heads, head_dim=head_dim, page_size=page_size,
+                              num_pages=num_pages, max_seqs=max_seqs, max_pages=max_pages)
+        n = ctypes.c_size_t()
+        call("cactus_hip_kv4_bytes", self.desc.ref, ctypes.byref(n))
+        self._buf = {"pages": DeviceBuffer(n.value), "table": DeviceBuffer(4 * max_seqs * max_pages),
+                     "lens": DeviceBuffer(4 * max_seqs), "refs": DeviceBuffer(4 * num_pages), "state": DeviceBuffer(16)}
+        for name, b in self._buf.items():
+            setattr(self.desc, name, b.ptr)
+        self._work, self._lists = [], []
+        self.reset(stream)
+
+    def _lst(self, v, stream=None):
+        """A device pointer as it is; a sequence of ints uploaded (kept until the next such call ends)."""
+        if v is None or isinstance(v, int):
+            return v
+        b = DeviceBuffer.from_numpy(np.asarray(v, np.int32), stream)
+        self._lists.append(b)
+        return b.ptr
+
+    def _call(self, name, *args, stream=None):
+        call(name, self.desc.ref, *args, stream)
+        if self._lists:                       # uploaded lists go once the call has read them
+            call("cactus_hip_stream_sync", stream)
+            self._lists.clear()
+
+    def workspace(self, nbytes: int, stream=None):
+        """At least nbytes of scratch memory, the first 4096 bytes zero."""
+        if not self._work or self._work[-1].nbytes < nbytes:
+            # a smaller one stays: a captured graph may hold its address
+            self._work.append(DeviceBuffer(max(nbytes, 4096)))
+            call("cactus_hip_memset", self._work[-1].ptr, 0, 4096, stream)
+        return self._work[-1].ptr, self._work[-1].nbytes
+
+    def reset(self, stream=None):
+        self._call("cactus_hip_kv4_reset", stream=stream)
+
+    def status(self, stream=None) -> int:
+        s = ctypes.c_int()
+        call("cactus_hip_kv4_status", self.desc.ref, ctypes.byref(s), stream)
+        return s.value
+
+    def extend(self, batch: int, count: int = 0, seqs=None, counts=None, stream=None):
+        self._call("cactus_hip_kv4_extend", self._lst(seqs, stream), self._lst(counts, stream), batch, count,
+                   stream=stream)
+
+    def append(self, layer: int, k: int, v: int, batch: int, seq_len: int, kv_stride: int | None = None, seqs=None,
+               counts=None, stream=None):
+        stride = kv_stride or self.desc.kv_heads * self.desc.head_dim
+        self._call("cactus_hip_kv4_append_f16", layer, self._lst(seqs, stream), self._lst(counts, stream), k, v, batch,
+                   seq_len, stride, stream=stream)
+
+    def read(self, layer: int, k: int, v: int, batch: int, seq_len: int, seqs=None, starts=None, counts=None, stream=None):
+        self._call("cactus_hip_kv4_read_f16", layer, self._lst(seqs, stream), self._lst(starts, stream),
+                   self._lst(counts, stream), k, v, batch, seq_len, stream=stream)
+
+    def attention(self, layer: int, q: int, o: int, batch: int, seq_len: int, num_q_heads: int, scale: float = 0.0,
+                  window: int = 0, sink: int = 0, causal: bool = True, q_stride: int | None = None, seqs=None,
+                  counts=None, stream=None):
+        need = hip().cactus_hip_attention_kv4_workspace(self.desc.ref, batch, seq_len, num_q_heads)
+        work, size = self.workspace(need, stream)
+        stride = q_stride or num_q_heads * self.desc.head_dim
+        self._call("cactus_hip_attention_kv4_f16", layer, self._lst(seqs, stream), self._lst(counts, stream), q, stride,
+                   o, batch, seq_len, num_q_heads, scale, window, sink, int(causal), work, size, stream=stream)
+
+    def fork(self, src, dst, n: int | None = None, stream=None):
+        n = len(src) if n is None else n
+        work, size = self.workspace(hip().cactus_hip_kv4_pages_workspace(self.desc.ref, n), stream)
+        self._call("cactus_hip_kv4_fork", self._lst(src, stream), self._lst(dst, stream), n, work, size, stream=stream)
+
+    def free(self, seqs, n: int | None = None, stream=None):
+        n = len(seqs) if n is None else n
+        self._call("cactus_hip_kv4_free", self._lst(seqs, stream), n, stream=stream)
+
+    def compact(self, stream=None):
+        work, size = self.workspace(hip().cactus_hip_kv4_pages_workspace(self.desc.ref, 0), stream)
+        self._call("cactus_hip_kv4_compact", work, size, stream=stream)
+
+    def copy_pages(self, src, dst, n: int | None = None, stream=None):
+        n = len(src) if n is None else n
+        self._call("cactus_hip_kv4_copy_pages", self._lst(src, stream), self._lst(dst, stream), n, stream=stream)
+
+    def tables(self, stream=None) -> dict:
+        """Host copies of table, lens, refs and state."""
+        d = self.desc
+        shapes = {"table": (d.max_seqs, d.max_pages), "lens": (d.max_seqs,), "refs": (d.num_pages,), "state": (4,)}
+        return {n: self._buf[n].to_numpy(np.int32, s, stream) for n, s in shapes.items()}

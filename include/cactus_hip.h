@@ -434,6 +434,132 @@ int cactus_hip_kv_window_shift(const cactus_hip_kv_layer* layers, size_t nlayers
                                void* temp, size_t temp_bytes, uint32_t* state, uint32_t cache_len,
                                void* stream);
 
+/* ------------------------------------------------ paged 4-bit KV cache
+ * No reference counterpart (the reference's cache is one INT8 sequence).  Many
+ * sequences share one pool of pages; a page holds page_size tokens of one
+ * layer, all KV heads, keys and values, in 4-bit codes.  Per token, KV head
+ * and group of 32 dims, keys and values alike:
+ *   s = fp16(bf16(max|x| / 7)),  code = clamp(rne(x / s), -7, 7),  value = code * s
+ * (code 0 where s = 0).  The scale has 8 significant bits, so that code * s is
+ * an exact FP16 number: whoever reads a page computes with the same values.
+ * A group with a NaN or an infinity reads as NaN.  9/16 byte per value.
+ *
+ * The caller owns every buffer.  `table`, `lens`, `refs` and `state` live on
+ * the device, and the calls below change them there in stream order, so that a
+ * step that allocates pages can be captured into a graph and replayed.  Calls on
+ * one cache from several streams have to be ordered by the caller; attention
+ * and read calls on one cache may overlap.
+ *
+ * table[slot][j] is the page of the slot's tokens [j page_size, (j + 1)
+ * page_size), -1 behind its last page; lens[slot] its tokens; refs[page] how many slots
+ * hold the page (0: free); state[0] the number of free pages, state[1] a
+ * page below which none is free, state[2] status bits (sticky, see
+ * cactus_hip_kv4_status), state[3] 0.  Full pages may be shared by slots, a
+ * partly filled one never is.  cactus_hip_kv4_reset sets up all four.
+ *
+ * `seqs` (device, NULL: request i is slot i) names the slot of each request;
+ * `counts` (device, NULL: seq_len each) its rows, the first counts[i] of
+ * seq_len.  A slot number outside the cache makes no access: append, read and
+ * attention skip the request (attention leaves its output rows as they were).
+ * Page numbers in `table` are checked by every kernel: keys on a page that
+ * does not exist are as if they were not there. */
+#define CACTUS_HIP_KV4_GROUP        32
+#define CACTUS_HIP_KV4_NO_PAGES     1   /* status: an extend or fork found too few free pages */
+#define CACTUS_HIP_KV4_BAD_REQUEST  2   /* status: slot or page out of range or named twice, negative count, table full */
+typedef struct {
+    void*    pages;      /* cactus_hip_kv4_bytes bytes, 128-byte aligned */
+    int32_t* table;      /* [max_seqs][max_pages] */
+    int32_t* lens;       /* [max_seqs] */
+    int32_t* refs;       /* [num_pages] */
+    int32_t* state;      /* [4] */
+    size_t layers, kv_heads, head_dim;      /* head_dim 64, 128 or 256 */
+    size_t page_size;                       /* tokens: a power of two, 16 to 4096 */
+    size_t num_pages, max_seqs, max_pages;  /* max_seqs at most 65536; max_pages: per slot */
+} cactus_hip_kv4_cache;
+/* bytes of `pages`: layers * num_pages * kv_heads * page_size * head_dim * 9 / 8.
+ * Within: [layer][page][kv head][tile of 16 tokens], a tile of 18 head_dim bytes:
+ *   K codes  [h 4][token 16][head_dim / 64][t 8], byte: dims 64 p + 8 h + t (low
+ *            nibble) and 64 p + 32 + 8 h + t of p = head_dim / 64 index, code + 8
+ *   K scales [h 4][head_dim / 32][i 4] fp16, token 4 h + i
+ *   V codes  [h 4][x 16][head_dim / 32][i 4], byte: dims 32 g + x (low nibble) and
+ *            32 g + 16 + x of token 4 h + i, code + 8
+ *   V scales as the K scales */
+int cactus_hip_kv4_bytes(const cactus_hip_kv4_cache* cache, size_t* bytes);
+/* no tokens in any slot, every page free, status 0 (page contents stay) */
+int cactus_hip_kv4_reset(const cactus_hip_kv4_cache* cache, void* stream);
+/* Status bits since the last call or reset, which clears them; waits for the
+ * stream.  While a bit is set, appends write nothing. */
+int cactus_hip_kv4_status(const cactus_hip_kv4_cache* cache, int* status, void* stream);
+/* Slot seqs[i] grows by counts[i] tokens (counts NULL: by `count` each): the
+ * pages that it needs are the lowest free ones, in request order.  All or
+ * nothing: if pages are missing or a request is wrong, nothing changes and
+ * the status says so.  The new tokens' contents are what their pages hold
+ * until cactus_hip_kv4_append_f16 writes them, once per layer. */
+int cactus_hip_kv4_extend(const cactus_hip_kv4_cache* cache, const int32_t* seqs, const int32_t* counts,
+                          size_t batch, size_t count, void* stream);
+/* Quantizes k, v [batch][seq_len] rows of [kv_heads][head_dim] fp16, kv_stride
+ * values from row to row (a multiple of 8, at least kv_heads * head_dim; k and
+ * v 16-byte aligned), into layer `layer`: request i's rows become the last
+ * counts[i] tokens of its slot.  Slots have to differ from each other. */
+int cactus_hip_kv4_append_f16(const cactus_hip_kv4_cache* cache, size_t layer, const int32_t* seqs,
+                              const int32_t* counts, const uint16_t* k, const uint16_t* v, size_t batch,
+                              size_t seq_len, size_t kv_stride, void* stream);
+/* The values of layer `layer`'s tokens: request i's tokens [starts[i],
+ * starts[i] + counts[i]), or with starts NULL its last counts[i], into
+ * k, v [batch][seq_len][kv_heads][head_dim] fp16 (16-byte aligned; either may
+ * be NULL).  Rows behind counts[i] and tokens that the slot does not have are
+ * left as they were. */
+int cactus_hip_kv4_read_f16(const cactus_hip_kv4_cache* cache, size_t layer, const int32_t* seqs,
+                            const int32_t* starts, const int32_t* counts, uint16_t* k, uint16_t* v, size_t batch,
+                            size_t seq_len, void* stream);
+/* Attention of the newest rows over the pages: q [batch][seq_len] rows of
+ * [num_q_heads][head_dim] fp16, q_stride values from row to row (a multiple of
+ * 8), o [batch][seq_len][num_q_heads][head_dim], both 16-byte aligned.  Request i
+ * has n = lens tokens (its own new ones appended) and m = counts[i] rows; row
+ * r stands at position p = n - m + r and sees key j iff
+ *   (not is_causal or j <= p) and (window_size == 0 or p - j <= window_size or j < sink_size)
+ * o = sum_j softmax_j(scale q.k_j) v_j (scale 0: 1 / sqrt(head_dim)); a row
+ * that sees no key gets zeros, rows behind m are left as they were.
+ * window_size counts as cactus_hip_attention_f16's; sink_size without a
+ * window has no effect.  Scores, softmax and sums in FP32; the weights are
+ * rounded to FP16 for the matrix product with the values.
+ * workspace: device memory of at least cactus_hip_attention_kv4_workspace
+ * bytes, 256-byte aligned, its first 4096 bytes zero before the first call
+ * that uses it (every call leaves them zero); calls that may overlap need
+ * workspaces of their own, captured graphs among them. */
+size_t cactus_hip_attention_kv4_workspace(const cactus_hip_kv4_cache* cache, size_t batch, size_t seq_len,
+                                          size_t num_q_heads);
+int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer, const int32_t* seqs,
+                                 const int32_t* counts, const uint16_t* q, size_t q_stride, uint16_t* o,
+                                 size_t batch, size_t seq_len, size_t num_q_heads, float scale, size_t window_size,
+                                 size_t sink_size, int is_causal, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+/* Slot dst[i] takes over slot src[i]'s tokens (src, dst: device, n entries),
+ * all sources as they are before the call, so that beams may swap slots:
+ * dst's own pages are released, src's full pages shared, and a partly filled
+ * last page copied, in every layer, to the lowest page that is free before
+ * the call.  src[i] == dst[i] changes nothing.  A dst named twice, a slot out
+ * of range or too few free pages: nothing changes, and the status says so.
+ * workspace: cactus_hip_kv4_pages_workspace(cache, n) bytes (its first 4096
+ * bytes are left alone, so that it may be an attention workspace). */
+size_t cactus_hip_kv4_pages_workspace(const cactus_hip_kv4_cache* cache, size_t n);
+int cactus_hip_kv4_fork(const cactus_hip_kv4_cache* cache, const int32_t* src, const int32_t* dst, size_t n,
+                        void* workspace, size_t workspace_bytes, void* stream);
+/* Slots seqs[i] (NULL: 0 to n - 1) give up their pages; pages that no other
+ * slot shares are free.  An empty slot, or one named again, stays empty; one
+ * out of range sets the status. */
+int cactus_hip_kv4_free(const cactus_hip_kv4_cache* cache, const int32_t* seqs, size_t n, void* stream);
+/* Moves the pages in use to the front of the pool: with L pages in use, the
+ * used pages from L on go, ascending, to the free ones below L, ascending, in
+ * every layer; tables and reference counts follow.  workspace:
+ * cactus_hip_kv4_pages_workspace(cache, 0) bytes, as for the fork. */
+int cactus_hip_kv4_compact(const cactus_hip_kv4_cache* cache, void* workspace, size_t workspace_bytes, void* stream);
+/* Copies pages src[i] to dst[i] (device, n entries) in every layer; tables and
+ * counts stay.  No page may be a dst twice, or both src and dst.  Pairs with
+ * a page out of range are skipped and set the status. */
+int cactus_hip_kv4_copy_pages(const cactus_hip_kv4_cache* cache, const int32_t* src, const int32_t* dst, size_t n,
+                              void* stream);
+
 /* ------------------------------------------------ fused decode step
  * Each entry point computes a run of consecutive graph nodes of
  * QwenModel::forward (models/model_qwen.cpp:51-172) for ONE token with the

@@ -1,0 +1,411 @@
+"""The paged 4-bit KV cache on the GPU against its plain restatement."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from _kv4 import Model, attention, quantize, values
+
+pytestmark = pytest.mark.gpu
+
+
+class Cache:
+    """A KV4Cache and its model side by side; fresh pages hold 0xFF bytes (NaN scales)."""
+
+    def __init__(self, cm, layers=1, kv_heads=2, head_dim=64, page_size=16, num_pages=40, max_seqs=6, max_pages=12):
+        from cactus_amd.kv4 import KV4Cache
+        self.cm, self.shape = cm, (layers, kv_heads, head_dim, page_size, num_pages, max_seqs, max_pages)
+        self.gpu, self.cpu = KV4Cache(*self.shape), Model(*self.shape)
+        self.put_pages()
+
+    def put_pages(self):
+        self.gpu._buf["pages"].upload(self.cpu.pages)
+
+    def pages(self):
+        return self.gpu._buf["pages"].to_numpy(np.uint8, self.cpu.pages.shape)
+
+    def check(self):
+        t = self.gpu.tables()
+        for name in ("table", "lens", "refs"):
+            np.testing.assert_array_equal(t[name], getattr(self.cpu, name), err_msg=name)
+        assert t["state"][0] == (self.cpu.refs == 0).sum()
+        assert (self.cpu.refs[:t["state"][1]] > 0).all()
+        np.testing.assert_array_equal(self.pages(), self.cpu.pages)
+
+    def extend(self, seqs, counts):
+        want = self.cpu.extend(seqs, counts)
+        self.gpu.extend(len(seqs), seqs=seqs, counts=counts)
+        assert self.gpu.status() == want
+        return want
+
+    def append(self, layer, seqs, counts, k, v, stride=None, named=True):
+        """k, v [B][S][H][d]; the model and the GPU write the rows."""
+        B, S, H, d = k.shape
+        stride = stride or H * d
+        rows = np.full((2, B * S, stride), 0x7E00, np.uint16).view(np.float16)
+        rows[0, :, :H * d], rows[1, :, :H * d] = k.reshape(B * S, -1), v.reshape(B * S, -1)
+        dk, dv = (self.cm.DeviceBuffer.from_numpy(r) for r in rows)
+        self.gpu.append(layer, dk.ptr, dv.ptr, B, S, stride, seqs=list(seqs) if named else None, counts=list(counts))
+        for b, (s, m) in enumerate(zip(seqs, counts)):
+            for r in range(m):
+                self.cpu.write(layer, s, self.cpu.lens[s] - m + r, k[b, r], v[b, r])
+
+    def fill(self, rng, lens, seqs=None, layers=None, scale=1.0):
+        """Random tokens for slots `seqs`, all layers."""
+        seqs = list(range(len(lens))) if seqs is None else list(seqs)
+        assert self.extend(seqs, lens) == 0
+        S = max(max(lens), 1)
+        for layer in range(self.cpu.layers):
+            k = kv_rows(rng, len(lens), S, self.cpu.H, self.cpu.d, scale)
+            self.append(layer, seqs, lens, k, kv_rows(rng, len(lens), S, self.cpu.H, self.cpu.d, scale))
+
+    def attend(self, q, seqs, counts, layer=0, scale=0.0, window=0, sink=0, causal=True, stride=None, call=None):
+        """Runs the kernel on q [B][S][Hq][d] and holds every row to the plain attention."""
+        B, S, Hq, d = q.shape
+        stride = stride or Hq * d
+        rows = np.full((B * S, stride), np.float16(np.nan))
+        rows[:, :Hq * d] = q.reshape(B * S, -1)
+        mark = np.float16(-77.25)      # rows that are not there stay as they are
+        dq, do = self.cm.DeviceBuffer.from_numpy(rows), self.cm.DeviceBuffer.from_numpy(np.full(q.shape, mark))
+        self.gpu.attention(layer, dq.ptr, do.ptr, B, S, Hq, scale, window, sink, causal, stride, seqs=list(seqs),
+                           counts=list(counts))
+        o = do.to_numpy(np.float16, q.shape)
+        for b, (s, m) in enumerate(zip(seqs, counts)):
+            if not 0 <= s < self.cpu.max_seqs:
+                m = 0
+            assert (o[b, m:] == mark).all(), f"request {b}: rows behind the last one changed"
+            if m == 0:
+                continue
+            (kc, ks), (vc, vs) = self.cpu.read(layer, s)
+            want, tol = attention(q[b, :m], kc, ks, vc, vs, len(kc), scale or 1 / math.sqrt(d), window, sink, causal)
+            got = o[b, :m].astype(np.float64)
+            np.testing.assert_array_equal(np.isnan(got), np.isnan(want), err_msg=f"request {b}: NaN")
+            off = np.where(np.isnan(want), 0, np.abs(got - want) - tol)
+            assert (off <= 0).all(), f"request {b}: off by {np.nanmax(np.abs(got - want))}, {np.max(off)} over the bound"
+        return o
+
+
+def kv_rows(rng, B, S, H, d, scale=1.0):
+    x = rng.standard_normal((B, S, H, d)) * scale + rng.standard_normal((H, d)) * scale
+    return (x * np.exp(0.7 * rng.standard_normal((H, d)))).astype(np.float16)
+
+
+# ------------------------------------------------------------------ append and read
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("ps,S,lens", [(16, 1, [0, 15, 16, 17]), (16, 37, [0, 3, 29, 0]), (64, 70, [0, 63, 1, 40]),
+                                       (256, 5, [250, 0, 14, 12])])
+def test_append_writes_the_documented_bytes(hip_ready, d, ps, S, lens):
+    rng = np.random.default_rng(d + ps + S)
+    c = Cache(hip_ready, 2, 3, d, ps, 40, 6, 12)
+    c.fill(rng, lens, seqs=[4, 0, 2, 1])
+    counts = [S, max(1, S // 2), 0, max(1, S - 1)]
+    seqs = [2, 4, 0, 1]
+    assert c.extend(seqs, counts) == 0
+    c.append(1, seqs, counts, kv_rows(rng, 4, S, 3, d), kv_rows(rng, 4, S, 3, d), stride=3 * d + 8)
+    c.check()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_append_of_extreme_values(hip_ready, d):
+    rng = np.random.default_rng(5)
+    x = kv_rows(rng, 1, 40, 1, d)
+    x[0, 0] = 0
+    x[0, 1] = 65504
+    x[0, 2] = np.float16(2.0 ** -24) * rng.integers(-9, 10, (1, d))      # subnormals, scales that round to 0
+    x[0, 3] = np.where(np.arange(d) % 32 == 5, 65504, 1)
+    x[0, 4, 0, 7] = np.nan
+    x[0, 5, 0, d - 1] = np.inf
+    x[0, 6, 0, 40] = -np.inf
+    x[0, 7] = (np.arange(d) % 15 - 7) * np.float16(0.5)                   # codes exactly on the grid
+    x[0, 8] = (np.arange(d) % 14 - 6.5)                                   # ties
+    x[0, 8, 0, ::32] = 7
+    x[0, 9] = np.float16(2.0 ** -14) * rng.standard_normal((1, d)).astype(np.float16)
+    c = Cache(hip_ready, 1, 1, d)
+    assert c.extend([0], [40]) == 0
+    c.append(0, [0], [40], x, -x[:, ::-1])
+    c.check()
+    dk, dv = (c.cm.DeviceBuffer(x.nbytes) for _ in range(2))
+    c.gpu.read(0, dk.ptr, dv.ptr, 1, 40)
+    for buf, src in ((dk, x), (dv, -x[:, ::-1])):
+        got = buf.to_numpy(np.float16, x.shape)
+        want = values(*quantize(src)).reshape(x.shape)
+        np.testing.assert_array_equal(got.astype(np.float64), want)      # exact, NaN included
+
+
+@pytest.mark.parametrize("d", [64, 256])
+def test_read_ranges(hip_ready, d):
+    rng = np.random.default_rng(9)
+    c = Cache(hip_ready, 2, 2, d, 32, 20, 4, 6)
+    c.fill(rng, [70, 1, 0, 33])
+    S = 40
+    # a window in the middle, one that begins before the first token, one that ends behind the last, an empty slot
+    seqs, starts, counts = [0, 3, 0, 2, 9, 1], [21, -5, 60, 0, 0, 0], [40, 12, 40, 7, 3, 1]
+    mark = np.full((6, S, 2, d), 11.0, np.float16)
+    dk, dv = c.cm.DeviceBuffer.from_numpy(mark), c.cm.DeviceBuffer.from_numpy(mark)
+    c.gpu.read(1, dk.ptr, dv.ptr, 6, S, seqs=seqs, starts=starts, counts=counts)
+    for is_v, buf in ((0, dk), (1, dv)):
+        want = mark.astype(np.float64)
+        for b in range(6):
+            if seqs[b] >= 4:
+                continue
+            x = values(*c.cpu.read(1, seqs[b])[is_v]).reshape(-1, 2, d)
+            for r in range(counts[b]):
+                if 0 <= starts[b] + r < len(x):
+                    want[b, r] = x[starts[b] + r]
+        np.testing.assert_array_equal(buf.to_numpy(np.float16, mark.shape).astype(np.float64), want)
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("G", [1, 2, 3, 8, 17])
+def test_decode_lengths(hip_ready, d, G):
+    rng = np.random.default_rng(d * 100 + G)
+    lens = [1, 15, 16, 17, 31, 33, 64, 150]
+    c = Cache(hip_ready, 1, 2, d, 16, 40, 8, 12)
+    c.fill(rng, lens)
+    q = rng.standard_normal((8, 1, 2 * G, d)).astype(np.float16)
+    c.attend(q, range(8), [1] * 8)
+
+
+@pytest.mark.parametrize("d,ps", [(64, 16), (128, 64), (256, 32), (128, 256)])
+@pytest.mark.parametrize("S", [2, 5, 16, 33, 90])
+@pytest.mark.parametrize("window,sink,causal", [(0, 0, True), (0, 0, False), (20, 0, True), (31, 5, True), (1, 40, True),
+                                                (17, 3, False), (1 << 40, 2, True)])
+def test_rows_and_masks(hip_ready, d, ps, S, window, sink, causal):
+    rng = np.random.default_rng(S * 7 + d)
+    c = Cache(hip_ready, 1, 2, d, ps, 48, 5, 16)
+    lens = [S, S + 1, 150, S + 47, 97 if S <= 97 else S]
+    c.fill(rng, lens)
+    q = rng.standard_normal((5, S, 4, d)).astype(np.float16)
+    c.attend(q, [3, 1, 0, 2, 4], [S, S, 0, max(1, S - 1), max(1, S // 2)], window=window, sink=sink, causal=causal,
+             stride=4 * d + 16)
+
+
+def test_long_decode_and_sharp_softmax(hip_ready):
+    rng = np.random.default_rng(3)
+    c = Cache(hip_ready, 1, 1, 128, 64, 40, 3, 34)
+    c.fill(rng, [2100, 3, 300], scale=2.0)
+    q = (4 * rng.standard_normal((3, 1, 4, 128))).astype(np.float16)
+    c.attend(q, [0, 1, 2], [1, 1, 1])
+    c.attend(q, [0, 0, 2], [1, 1, 1], scale=0.004)          # the same slot twice
+    c.attend(np.zeros_like(q), [0, 1, 2], [1, 1, 1])        # a mean
+    c.attend(q, [2, -1, 5], [1, 1, 1])                      # slots that do not exist
+
+
+def test_rows_without_keys_are_zero(hip_ready):
+    rng = np.random.default_rng(4)
+    c = Cache(hip_ready, 1, 2, 64, 16, 20, 3, 8)
+    c.fill(rng, [40], seqs=[1])
+    q = rng.standard_normal((2, 3, 4, 64)).astype(np.float16)
+    do = c.cm.DeviceBuffer.from_numpy(np.full(q.shape, np.float16(5)))
+    dq = c.cm.DeviceBuffer.from_numpy(q)
+    c.gpu.attention(0, dq.ptr, do.ptr, 2, 3, 4, seqs=[0, 1])
+    o = do.to_numpy(np.float16, q.shape)
+    assert (o[0] == 0).all() and np.isfinite(o).all() and (o[1] != 5).all()
+
+
+@pytest.mark.parametrize("S", [1, 4, 70])
+def test_non_finite_keys_reach_only_the_rows_that_see_them(hip_ready, S):
+    rng = np.random.default_rng(6)
+    c = Cache(hip_ready, 1, 1, 64, 16, 20, 2, 8)
+    n = 100
+    assert c.extend([0], [n]) == 0
+    k, v = kv_rows(rng, 1, n, 1, 64), kv_rows(rng, 1, n, 1, 64)
+    k[0, 20, 0, 3] = np.inf        # seen by every row from 20 on
+    v[0, 60, 0, 40] = np.nan       # dims 32 to 63 only
+    v[0, 98, 0, 2] = np.inf
+    c.append(0, [0], [n], k, v)
+    q = rng.standard_normal((1, S, 2, 64)).astype(np.float16)
+    c.attend(q, [0], [S], window=25)
+    c.attend(q, [0], [S], window=5)
+    c.attend(q, [0], [S])
+
+
+def test_pages_that_do_not_exist_are_not_there(hip_ready):
+    rng = np.random.default_rng(8)
+    c = Cache(hip_ready, 1, 1, 64, 16, 20, 2, 8)
+    c.fill(rng, [60, 20])
+    whole = c.cpu.table.copy()
+    for bad in (-1, 20, 1 << 30, -(1 << 31)):
+        c.cpu.table = whole.copy()
+        c.cpu.table[:, 1] = bad
+        c.gpu._buf["table"].upload(c.cpu.table)
+        q = rng.standard_normal((1, 1, 2, 64)).astype(np.float16)
+        dq, do = c.cm.DeviceBuffer.from_numpy(q), c.cm.DeviceBuffer(q.nbytes)
+        c.gpu.attention(0, dq.ptr, do.ptr, 1, 1, 2, seqs=[0])
+        # the same keys without those of the missing page
+        c.cpu.table = whole.copy()
+        (kc, ks), (vc, vs) = c.cpu.read(0, 0)
+        at = np.r_[0:16, 32:60]
+        want, tol = attention(q[0], kc[at], ks[at], vc[at], vs[at], 44, 1 / 8, causal=False)
+        assert (np.abs(do.to_numpy(np.float16, q.shape)[0] - want) <= tol).all()
+        c.gpu.append(0, do.ptr, do.ptr, 1, 1, 64, seqs=[1])        # slot 1's last token stands on it: nothing is written
+        np.testing.assert_array_equal(c.pages(), c.cpu.pages)
+        dk = c.cm.DeviceBuffer.from_numpy(np.full((60, 64), np.float16(3)))
+        c.gpu.read(0, dk.ptr, None, 1, 60, seqs=[0])
+        got = dk.to_numpy(np.float16, (60, 64))
+        assert (got[16:32] == 3).all()
+
+
+# ------------------------------------------------------------------ pages
+def test_extend_fork_free_compact_follow_the_model(hip_ready):
+    rng = np.random.default_rng(10)
+    c = Cache(hip_ready, 2, 1, 64, 16, 50, 9, 8)
+    c.fill(rng, [40, 16, 1, 33, 64], seqs=[0, 2, 3, 5, 8])
+    c.check()
+    for step in range(40):
+        op = rng.integers(0, 5)
+        if op == 0:
+            n = int(rng.integers(1, 6))
+            c.extend([int(s) for s in rng.permutation(9)[:n]], [int(x) for x in rng.integers(0, 40, n)])
+        elif op == 1:
+            n = int(rng.integers(1, 10))
+            src, dst = [int(s) for s in rng.integers(0, 9, n)], [int(s) for s in rng.permutation(9)[:n]]
+            want = c.cpu.fork(src, dst)
+            c.gpu.fork(src, dst)
+            assert c.gpu.status() == want
+        elif op == 2:
+            seqs = [int(s) for s in rng.integers(0, 9, 2)]
+            c.cpu.free(seqs)
+            c.gpu.free(seqs)
+        elif op == 3:
+            c.cpu.compact()
+            c.gpu.compact()
+        else:
+            a = [int(x) for x in rng.permutation(50)[:6]]
+            c.cpu.pages[:, a[3:]] = c.cpu.pages[:, a[:3]]
+            c.gpu.copy_pages(a[:3], a[3:])
+        c.check()
+
+
+def test_large_pools(hip_ready):
+    """More pages than one round of the allocation takes, more than one workgroup counts, and many requests."""
+    rng = np.random.default_rng(11)
+    c = Cache(hip_ready, 1, 1, 64, 16, 21000, 1500, 900)
+    counts = [int(x) for x in rng.integers(0, 160, 1500)]
+    counts[7], counts[1400] = 16 * 900, 16 * 900
+    assert c.extend(list(range(1500)), counts) == 0
+    c.cpu.pages[0, :, 0, 0, :4] = np.arange(21000, dtype=np.int32).view(np.uint8).reshape(-1, 4)
+    c.put_pages()
+    c.check()
+    gone = [int(s) for s in rng.permutation(1500)[:700]] + [7]
+    c.cpu.free(gone)
+    c.gpu.free(gone)
+    c.check()
+    dst = list(dict.fromkeys(gone))[:600]
+    src = [int(s) for s in rng.integers(0, 1500, len(dst))]
+    assert c.cpu.fork(src, dst) == 0
+    c.gpu.fork(src, dst)
+    c.check()
+    c.cpu.compact()
+    c.gpu.compact()
+    c.check()
+    assert c.extend([3, 4], [16 * 300, 100]) == 0
+    c.check()
+
+
+def test_refused_requests_change_nothing(hip_ready):
+    rng = np.random.default_rng(12)
+    c = Cache(hip_ready, 1, 1, 64, 16, 10, 4, 8)
+    c.fill(rng, [40, 17])
+    assert c.extend([2, 3], [64, 32]) == 1          # six pages, five free
+    assert c.extend([2, 2], [1, 1]) == 2            # named twice
+    assert c.extend([2, 4], [1, 1]) == 2            # no such slot
+    assert c.extend([2, 3], [1, -1]) == 2
+    assert c.extend([2, 0], [1, 200]) == 2          # more than a table row holds
+    c.check()
+    for src, dst, want in (([0, 1], [2, 2], 2), ([0, -1], [2, 3], 2), ([0, 1], [2, 4], 2)):
+        assert c.cpu.fork(src, dst) == want
+        c.gpu.fork(src, dst)
+        assert c.gpu.status() == want
+    c.check()
+    assert c.extend([2, 3], [16, 64]) == 0          # the pool is full
+    assert c.cpu.fork([0], [3]) == 1
+    c.gpu.fork([0], [3])
+    # until the status is read, appends write nothing
+    k = kv_rows(rng, 1, 1, 1, 64)
+    d = c.cm.DeviceBuffer.from_numpy(k)
+    c.gpu.append(0, d.ptr, d.ptr, 1, 1, seqs=[0])
+    c.check()
+    assert c.gpu.status() == 1 and c.gpu.status() == 0
+    c.gpu.free([1, 77])
+    c.cpu.free([1, 77])
+    assert c.gpu.status() == 2
+    c.gpu.copy_pages([0, 1, -3], [1, 10, 2])
+    c.cpu.pages[:, 1] = c.cpu.pages[:, 0]
+    assert c.gpu.status() == 2
+    c.check()
+
+
+# ------------------------------------------------------------------ together
+def test_a_serving_run(hip_ready):
+    """Prompts, beams, drafted tokens, conversations that end and a packed pool, every step's attention checked."""
+    rng = np.random.default_rng(13)
+    H, G, d, layers = 2, 2, 64, 2
+    c = Cache(hip_ready, layers, H, d, 16, 60, 8, 20)
+
+    def step(seqs, counts):
+        assert c.extend(seqs, counts) == 0
+        S = max(counts)
+        for layer in range(layers):
+            c.append(layer, seqs, counts, kv_rows(rng, len(seqs), S, H, d), kv_rows(rng, len(seqs), S, H, d))
+            q = rng.standard_normal((len(seqs), S, H * G, d)).astype(np.float16)
+            c.attend(q, seqs, counts, layer, window=int(rng.integers(0, 2)) * 40, sink=4)
+
+    step([0, 1, 5], [75, 33, 120])
+    step([0, 1, 5], [1, 1, 1])
+    c.cpu.fork([0, 0, 5], [2, 3, 1])
+    c.gpu.fork([0, 0, 5], [2, 3, 1])
+    for _ in range(3):
+        step([0, 1, 2, 3, 5], [1, 4, 1, 1, 2])
+    c.cpu.fork([3, 0, 3], [0, 3, 6])
+    c.gpu.fork([3, 0, 3], [0, 3, 6])
+    step([0, 3, 6], [1, 1, 1])
+    c.cpu.free([1, 2])
+    c.gpu.free([1, 2])
+    c.cpu.compact()
+    c.gpu.compact()
+    c.check()
+    step([0, 3, 5, 6, 7], [1, 1, 1, 1, 50])
+    c.check()
+
+
+def test_a_captured_step(hip_ready):
+    """extend, append and attention captured once and replayed, eager work in between; the lengths grow on the device."""
+    cm = hip_ready
+    rng = np.random.default_rng(14)
+    H, G, d, B = 2, 2, 128, 3
+    c = Cache(cm, 1, H, d, 16, 60, 4, 16)
+    c.fill(rng, [30, 5, 64])
+    stream = cm.Stream()
+    st = stream.handle
+    kv = [cm.DeviceBuffer(B * H * d * 2) for _ in range(2)]
+    dq, do = cm.DeviceBuffer(B * H * G * d * 2), cm.DeviceBuffer(B * H * G * d * 2)
+    need = cm.hip().cactus_hip_attention_kv4_workspace(c.gpu.desc.ref, B, 1, H * G)
+    work = cm.DeviceBuffer(need)
+    cm.call("cactus_hip_memset", work.ptr, 0, 4096, st)
+    cm.call("cactus_hip_stream_sync", st)
+    graph = ctypes.c_void_p()
+    cm.call("cactus_hip_graph_capture_begin", st)
+    cm.call("cactus_hip_kv4_extend", c.gpu.desc.ref, None, None, B, 1, st)
+    cm.call("cactus_hip_kv4_append_f16", c.gpu.desc.ref, 0, None, None, kv[0].ptr, kv[1].ptr, B, 1, H * d, st)
+    cm.call("cactus_hip_attention_kv4_f16", c.gpu.desc.ref, 0, None, None, dq.ptr, H * G * d, do.ptr, B, 1, H * G, 0.0, 0, 0,
+            1, work.ptr, need, st)
+    cm.call("cactus_hip_graph_capture_end", st, ctypes.byref(graph))
+    for i in range(20):
+        k, v = kv_rows(rng, B, 1, H, d), kv_rows(rng, B, 1, H, d)
+        q = rng.standard_normal((B, 1, H * G, d)).astype(np.float16)
+        kv[0].upload(k, st), kv[1].upload(v, st), dq.upload(q, st)
+        cm.call("cactus_hip_graph_launch", graph, st)
+        o = do.to_numpy(np.float16, q.shape, st)
+        assert c.cpu.extend([0, 1, 2], [1, 1, 1]) == 0
+        for b in range(B):
+            c.cpu.write(0, b, c.cpu.lens[b] - 1, k[b, 0], v[b, 0])
+            (kc, ks), (vc, vs) = c.cpu.read(0, b)
+            want, tol = attention(q[b], kc, ks, vc, vs, len(kc), 1 / math.sqrt(d))
+            assert (np.abs(o[b] - want) <= tol).all(), (i, b)
+        eager = c.attend(q, [0, 1, 2], [1, 1, 1])          # on the default stream, with a workspace of its own
+        np.testing.assert_array_equal(o, eager)
+    cm.call("cactus_hip_graph_destroy", graph)
+    c.check()

@@ -1,0 +1,128 @@
+"""The paged 4-bit KV cache without a GPU: refusals before any launch, sizes,
+and the restatement's own quantization."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from _kv4 import code_at, quantize, scale_at, values
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import cactus_amd
+    return cactus_amd.hip()
+
+
+def desc(**kw):
+    from cactus_amd.kv4 import CacheDesc
+    shape = dict(layers=2, kv_heads=2, head_dim=128, page_size=64, num_pages=8, max_seqs=4, max_pages=4)
+    ptrs = dict(pages=1 << 20, table=1 << 21, lens=1 << 22, refs=1 << 23, state=1 << 24)   # never dereferenced
+    return CacheDesc(**{**shape, **ptrs, **kw})
+
+
+def refused(lib, rc, text):
+    assert rc == -1
+    assert text in lib.cactus_hip_last_error(), lib.cactus_hip_last_error()
+
+
+BAD = [(dict(head_dim=96), b"head_dim"), (dict(head_dim=0), b"head_dim"), (dict(page_size=48), b"page_size"),
+       (dict(page_size=8), b"page_size"), (dict(page_size=8192), b"page_size"), (dict(kv_heads=0), b"kv_heads"),
+       (dict(layers=0), b"layers"), (dict(num_pages=0), b"num_pages"), (dict(num_pages=1 << 40), b"num_pages"),
+       (dict(max_seqs=0), b"max_seqs"), (dict(max_seqs=70000), b"max_seqs"), (dict(max_pages=1 << 26), b"max_pages")]
+
+
+@pytest.mark.parametrize("change,text", BAD + [(dict(pages=None), b"null buffer"), (dict(table=None), b"null buffer"),
+                                               (dict(state=None), b"null buffer"), (dict(pages=(1 << 20) + 64), b"aligned")])
+def test_every_call_checks_the_cache(lib, change, text):
+    c = desc(**change).ref
+    p = 4096
+    refused(lib, lib.cactus_hip_kv4_reset(c, None), text)
+    refused(lib, lib.cactus_hip_kv4_extend(c, None, None, 1, 1, None), text)
+    refused(lib, lib.cactus_hip_kv4_append_f16(c, 0, None, None, p, p, 1, 1, 256, None), text)
+    refused(lib, lib.cactus_hip_kv4_read_f16(c, 0, None, None, None, p, p, 1, 1, None), text)
+    refused(lib, lib.cactus_hip_attention_kv4_f16(c, 0, None, None, p, 256, p, 1, 1, 2, 0.0, 0, 0, 1, p, 1 << 30, None), text)
+    refused(lib, lib.cactus_hip_kv4_fork(c, p, p, 1, p, 1 << 30, None), text)
+    refused(lib, lib.cactus_hip_kv4_free(c, None, 1, None), text)
+    refused(lib, lib.cactus_hip_kv4_compact(c, p, 1 << 30, None), text)
+    refused(lib, lib.cactus_hip_kv4_copy_pages(c, p, p, 1, None), text)
+    refused(lib, lib.cactus_hip_kv4_status(c, p, None), text)
+
+
+@pytest.mark.parametrize("change,text", BAD)
+def test_sizes_check_the_shape(lib, change, text):
+    c = desc(**change).ref
+    n = ctypes.c_size_t()
+    refused(lib, lib.cactus_hip_kv4_bytes(c, ctypes.byref(n)), text)
+    assert lib.cactus_hip_kv4_pages_workspace(c, 1) == 0
+    assert lib.cactus_hip_attention_kv4_workspace(c, 1, 1, 2) == 0
+
+
+def test_null_cache_and_sizes(lib):
+    n = ctypes.c_size_t()
+    refused(lib, lib.cactus_hip_kv4_bytes(None, ctypes.byref(n)), b"null")
+    refused(lib, lib.cactus_hip_kv4_bytes(desc().ref, None), b"null")
+    assert lib.cactus_hip_kv4_bytes(desc().ref, ctypes.byref(n)) == 0
+    assert n.value == 2 * 8 * 2 * 64 * 128 * 9 // 8
+    assert lib.cactus_hip_kv4_pages_workspace(desc().ref, 3) >= 4096
+    assert lib.cactus_hip_attention_kv4_workspace(desc().ref, 1, 1, 4) >= 4096
+
+
+def test_refused_arguments(lib):
+    c, p, big = desc().ref, 4096, 1 << 30
+    refused(lib, lib.cactus_hip_kv4_append_f16(c, 2, None, None, p, p, 1, 1, 256, None), b"layer")
+    refused(lib, lib.cactus_hip_kv4_append_f16(c, 0, None, None, None, p, 1, 1, 256, None), b"null")
+    refused(lib, lib.cactus_hip_kv4_append_f16(c, 0, None, None, p, p + 8, 1, 1, 256, None), b"aligned")
+    refused(lib, lib.cactus_hip_kv4_append_f16(c, 0, None, None, p, p, 1, 1, 260, None), b"aligned")
+    refused(lib, lib.cactus_hip_kv4_append_f16(c, 0, None, None, p, p, 1, 1, 248, None), b"kv_stride")
+    refused(lib, lib.cactus_hip_kv4_append_f16(c, 0, None, None, p, p, 5, 1, 256, None), b"slots")
+    refused(lib, lib.cactus_hip_kv4_read_f16(c, 0, None, None, None, p, p + 2, 1, 1, None), b"aligned")
+    refused(lib, lib.cactus_hip_kv4_extend(c, None, None, 5, 1, None), b"slots")
+    refused(lib, lib.cactus_hip_kv4_extend(c, None, None, 1, 1 << 31, None), b"count")
+    att = lib.cactus_hip_attention_kv4_f16
+    refused(lib, att(c, 0, None, None, None, 256, p, 1, 1, 2, 0.0, 0, 0, 1, p, big, None), b"null")
+    refused(lib, att(c, 0, None, None, p, 384, p, 1, 1, 3, 0.0, 0, 0, 1, p, big, None), b"num_q_heads")
+    refused(lib, att(c, 0, None, None, p, 128, p, 1, 1, 2, 0.0, 0, 0, 1, p, big, None), b"q_stride")
+    refused(lib, att(c, 0, None, None, p + 2, 256, p, 1, 1, 2, 0.0, 0, 0, 1, p, big, None), b"aligned")
+    refused(lib, att(c, 0, None, None, p, 256, p + 8, 1, 1, 2, 0.0, 0, 0, 1, p, big, None), b"aligned")
+    refused(lib, att(c, 0, None, None, p, 256, p, 1, 1, 2, 0.0, 0, 0, 1, None, big, None), b"workspace")
+    refused(lib, att(c, 0, None, None, p, 256, p, 1, 1, 2, 0.0, 0, 0, 1, p + 128, big, None), b"workspace")
+    refused(lib, att(c, 0, None, None, p, 256, p, 1, 1, 2, 0.0, 0, 0, 1, p, 64, None), b"workspace")
+    refused(lib, att(c, 0, None, None, p, 256, p, 1, 1 << 30, 2, 0.0, 0, 0, 1, p, big, None), b"seq_len")
+    refused(lib, att(c, 2, None, None, p, 256, p, 1, 1, 2, 0.0, 0, 0, 1, p, big, None), b"layer")
+    refused(lib, lib.cactus_hip_kv4_fork(c, None, p, 1, p, big, None), b"null")
+    refused(lib, lib.cactus_hip_kv4_fork(c, p, p, 5, p, big, None), b"slots")
+    refused(lib, lib.cactus_hip_kv4_fork(c, p, p, 1, p, 4096, None), b"workspace")
+    refused(lib, lib.cactus_hip_kv4_compact(c, p, 4096, None), b"workspace")
+    refused(lib, lib.cactus_hip_kv4_copy_pages(c, p, None, 1, None), b"null")
+    refused(lib, lib.cactus_hip_kv4_copy_pages(c, p, p, 9, None), b"pages")
+    refused(lib, lib.cactus_hip_kv4_status(c, None, None), b"null")
+    # nothing to do is no error and no launch
+    assert lib.cactus_hip_kv4_append_f16(c, 0, None, None, None, None, 0, 1, 256, None) == 0
+    assert att(c, 0, None, None, None, 0, None, 1, 0, 2, 0.0, 0, 0, 1, None, 0, None) == 0
+    assert lib.cactus_hip_kv4_extend(c, None, None, 0, 1, None) == 0
+    assert lib.cactus_hip_kv4_fork(c, None, None, 0, None, 0, None) == 0
+    assert lib.cactus_hip_kv4_free(c, None, 0, None) == 0
+    assert lib.cactus_hip_kv4_copy_pages(c, None, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_the_layout_gives_every_code_and_scale_a_place_of_its_own(d):
+    nibbles = {code_at(d, k, i, v) for k in range(16) for i in range(d) for v in (False, True)}
+    scales = {scale_at(d, k, g, v) + b for k in range(16) for g in range(d // 32) for v in (False, True) for b in (0, 1)}
+    assert len(nibbles) == 2 * 16 * d and len(scales) == 2 * 16 * (d // 32) * 2
+    assert {b for b, _ in nibbles} | scales == set(range(18 * d)) and not {b for b, _ in nibbles} & scales
+
+
+def test_the_quantized_values_are_exact_fp16_numbers_near_the_input():
+    rng = np.random.default_rng(1)
+    x = (rng.standard_normal((400, 64)) * np.exp(3 * rng.standard_normal((400, 1)))).astype(np.float16)
+    x[0], x[1], x[2] = 0, 65504, np.float16(2.0 ** -24)
+    c, s = quantize(x)
+    y = values(c, s).reshape(x.shape)
+    assert np.abs(c).max() == 7
+    np.testing.assert_array_equal(y, y.astype(np.float16).astype(np.float64))
+    # half a step, and what the rounded scale leaves of the largest value (2^-9 of it, or half of 2^-24 per code)
+    g = np.abs(x.astype(np.float64)).reshape(400, -1, 32).max(-1).repeat(32, -1)
+    bound = np.repeat(s.astype(np.float64), 32, -1).reshape(x.shape) / 2 + g * 2.0 ** -9 + 7 * 2.0 ** -25
+    assert (np.abs(y - x) <= bound).all()
