@@ -49,6 +49,8 @@ HIP_FILE_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     # the prefill attention scales its output accumulators every key tile
     "attention_fast.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    # likewise the attention over the 4-bit cache, where a maximum grows
+    "attention_kv4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     # the decode value chains: the next block's scalar weight loads must stay
     # ahead of this block's FMAs (machine sinking moves them behind)
     "chain_stream.hip": ["-mllvm", "-disable-machine-sink"],

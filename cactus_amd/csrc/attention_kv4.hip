@@ -37,7 +37,7 @@ struct Kv4AttnArgs {
     int window, sink, causal; // window 0: none
     float scale;              // times log2(e): the softmax runs in powers of two
     uint32_t* counters;       // [workgroups] zero between calls
-    float* part;              // [workgroups][2][16 (D + 2)]: output, maxima, sums
+    float* part;              // [workgroups][2][vectors][D + 4]: output, maximum, sum
 };
 
 // rows and keys of one request
@@ -47,11 +47,11 @@ struct Kv4Seq {
 };
 constexpr int KV4_STEP = 32;
 
-__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b) {
+__device__ __forceinline__ Kv4Seq kv4_span(const Kv4AttnArgs& a, int slot, int len, int rows) {
     Kv4Seq s;
-    s.slot = kv4_slot(a.c, a.seqs, b);
-    s.rows = s.slot < 0 ? 0 : kv4_count(a.counts, b, a.S);
-    s.len = s.slot < 0 ? 0 : kv4_len(a.c, s.slot);
+    s.slot = slot;
+    s.len = len;
+    s.rows = rows;
     const int p0 = s.len - s.rows;                       // first row's position: its window reaches furthest back
     int lo = a.window > 0 && p0 > a.window ? p0 - a.window : 0;
     s.main0 = lo / KV4_STEP;
@@ -59,10 +59,14 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b) {
     s.steps = s.sinks + (s.len + KV4_STEP - 1) / KV4_STEP - s.main0;
     return s;
 }
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b) {
+    const int slot = kv4_slot(a.c, a.seqs, b);
+    return kv4_span(a, slot, slot < 0 ? 0 : kv4_len(a.c, slot), slot < 0 ? 0 : kv4_count(a.counts, b, a.S));
+}
 
 // whether the row at position p sees key j of n
 __device__ __forceinline__ bool kv4_sees(const Kv4AttnArgs& a, int p, int j, int n) {
-    return j < n && (!a.causal || j <= p) && (a.window == 0 || p - j <= a.window || j < a.sink);
+    return (j < n) & (!a.causal | (j <= p)) & ((a.window == 0) | (p - j <= a.window) | (j < a.sink));
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -99,11 +103,14 @@ __device__ __forceinline__ uint32_t pack_h(float a, float b) {
 }
 
 constexpr float LOG2E_F = 1.4426950408889634f;
-__device__ __forceinline__ float agent_load(const float* p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// pairs of values that workgroups hand to each other
+__device__ __forceinline__ float2 agent_load2(const float* p) {
+    const uint64_t u = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(bits_f((uint32_t)u), bits_f((uint32_t)(u >> 32)));
 }
-__device__ __forceinline__ void agent_store(float* p, float v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ void agent_store2(float* p, float x, float y) {
+    const uint64_t u = __builtin_bit_cast(uint32_t, x) | (uint64_t)__builtin_bit_cast(uint32_t, y) << 32;
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 // inclusive sum over the wave's lanes: row_shr 1, 2, 4, 8 within each 16-lane
 // row, then row_bcast:15 and row_bcast:31 across rows
@@ -132,7 +139,6 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
         }
     }
 }
-__device__ __forceinline__ float half_of(uint32_t w, int i) { return h2f((uint16_t)(i ? w >> 16 : w)); }
 
 // ------------------------------------------------------------ few rows
 // The work is a line of block steps (KV4_BLOCK keys of one unit: a request's
@@ -144,124 +150,136 @@ __device__ __forceinline__ float half_of(uint32_t w, int i) { return h2f((uint16
 // in their order.
 constexpr int KV4_WAVES = 4;
 constexpr int KV4_BLOCK = KV4_STEP * KV4_WAVES;   // a wave takes a step of 32 keys
-constexpr int KV4_GRID = 512;                     // two workgroups per CU
 constexpr int KV4_PARTS = 128;                    // a unit's stretches at most
 constexpr size_t KV4_COUNTERS = 4096;             // bytes: one counter per workgroup
 
-// block steps of a unit and units of a request (0: no rows)
+// block steps of a unit (one at least: a request without tokens gets its zeros)
 __device__ __forceinline__ uint32_t unit_blocks(const Kv4Seq& s) {
     return (uint32_t)max(1, (s.steps + KV4_WAVES - 1) / KV4_WAVES);
 }
-__device__ __forceinline__ uint32_t seq_units(const Kv4AttnArgs& a, const Kv4Seq& s) {
-    return (uint32_t)((s.rows * a.G + 15) / 16) * (uint32_t)a.c.Hkv;
+
+// Query vectors of a unit.  PACK: a vector takes NG = d / 32 of the product's
+// 16 columns, one per scale group, so that a lane multiplies by one group's
+// scale and the softmax runs once per lane, not per group; the products' other
+// groups' columns are computed and not used.  Otherwise a column is a vector
+// and each lane scales all its groups.
+template <int D, bool PACK>
+constexpr int kv4_vectors() { return PACK ? 16 / (D / 32) : 16; }
+// Steps of a wave's ring in LDS, workgroups per CU
+template <int D, bool PACK>
+constexpr int kv4_ring() { return D == 64 ? 4 : PACK ? 2 : 3; }
+template <int D, bool PACK>
+constexpr int kv4_per_cu() { return D == 256 ? (PACK ? 2 : 1) : PACK ? 4 : 2; }
+
+// a times half I of w plus c, one instruction (v_fma_mix_f32; as a builtin, so that
+// the compiler knows what waits for the matrix and transcendental units' results)
+template <int I>
+__device__ __forceinline__ float fma_half(float a, uint32_t w, float c) {
+    return __builtin_fmaf(a, h2f((uint16_t)(I ? w >> 16 : w)), c);
 }
+template <int I>
+__device__ __forceinline__ float mul_half(float a, uint32_t w) { return fma_half<I>(a, w, 0.0f); }
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+// sum over the N lanes of a group (consecutive lanes, N = 2, 4 or 8), in each of them
+template <int N>
+__device__ __forceinline__ float sum_lanes(float v) {
+    v = add_dpp<0xB1>(v);                        // quad_perm [1,0,3,2]
+    if constexpr (N > 2) v = add_dpp<0x4E>(v);   // quad_perm [2,3,0,1]
+    if constexpr (N > 4) v = add_dpp<0x141>(v);  // row_half_mirror
+    return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_fmaxf(__builtin_fmaxf(a, b), c); }
 
-// Steps of a wave's ring in LDS: as many as leave room for two workgroups per CU
-template <int D>
-constexpr int kv4_ring() { return 4 - D / 256; }
-
-template <int D>
-__global__ void __launch_bounds__(64 * KV4_WAVES, D == 256 ? 1 : 2) attn_kv4_kernel(Kv4AttnArgs a) {
-    constexpr int NG = D / 32, NB = D / 16, OS = D + 4;
+template <int D, bool PACK>
+__global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_kv4_kernel(Kv4AttnArgs a) {
+    constexpr int NG = D / 32, NB = D / 16, OS = D + 4, QV = kv4_vectors<D, PACK>();
+    constexpr int SG = PACK ? 1 : NG;                          // scale groups of a lane
     constexpr int TB = 18 * D, SLOT = 2 * TB;                  // bytes of a tile and of a step
     constexpr int NI = 2 * ((TB + 1023) / 1024);               // LDS loads of a step
-    constexpr int R = kv4_ring<D>();
-    static_assert(R * SLOT >= 16 * OS * 4 && R * SLOT >= KV4_PARTS * 64 + 64, "the ring holds the wave's sums, then the parts' weights");
+    constexpr int R = kv4_ring<D, PACK>();
+    static_assert(R * SLOT >= QV * OS * 4 && KV4_WAVES * R * SLOT >= 64 * KV4_WAVES * 24,
+                  "the ring holds a wave's sums, then the joined parts'");
     __shared__ __align__(16) uint8_t ring[KV4_WAVES][R][SLOT];
-    __shared__ float m_sh[KV4_WAVES][16], l_sh[KV4_WAVES][16];
+    __shared__ float m_sh[KV4_WAVES][QV], l_sh[KV4_WAVES][QV];
     __shared__ int last_sh;
-    float (*o_sh)[R * SLOT / 4] = reinterpret_cast<float (*)[R * SLOT / 4]>(&ring[0][0][0]);   // [wave][16][OS]
-    float (*w_sh)[16] = reinterpret_cast<float (*)[16]>(&ring[0][0][0]);   // a part's weight in each column, then the sum
+    float (*o_sh)[R * SLOT / 4] = reinterpret_cast<float (*)[R * SLOT / 4]>(&ring[0][0][0]);   // [wave][QV][OS]
+    float* j_sh = reinterpret_cast<float*>(&ring[0][0][0]);    // [threads][6]: sums of parts
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, h = lane >> 4;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int qi = PACK ? col / NG : col, gi = PACK ? col % NG : 0;    // the lane's query vector and group
     const Kv4View& c = a.c;
-    const float kscale = a.scale * 16777216.0f;
+    // PACK: odd groups' codes are 16 times theirs
+    const float kscale = a.scale * 16777216.0f * (PACK && (gi & 1) ? 0.0625f : 1.0f);
 
-    // ---- this workgroup's stretch [at, end) of the line
-    uint32_t total = 0, longest = 1;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-        uint32_t cost = 0, blocks = 0;
+    // ---- 64 requests at a time, one per lane: slot, tokens, rows, block steps
+    // of a unit, and how far the line reaches with this request
+    int r_slot = -1, r_len = 0, r_rows = 0;
+    uint32_t r_blocks = 0, r_cost = 0, r_upto = 0;
+    auto look = [&](int b0) {
+        r_rows = 0;
+        r_blocks = r_cost = 0;
         if (b0 + lane < a.B) {
             const Kv4Seq s = kv4_seq(a, b0 + lane);
-            blocks = s.rows > 0 ? unit_blocks(s) : 0;
-            cost = blocks * seq_units(a, s);
+            r_slot = s.slot;
+            r_len = s.len;
+            r_rows = s.rows;
+            r_blocks = s.rows > 0 ? unit_blocks(s) : 0;
+            r_cost = r_blocks * (uint32_t)((s.rows * a.G + QV - 1) / QV) * (uint32_t)c.Hkv;
         }
-        total += lane_u(wave_scan_add(cost), 63);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) blocks = max(blocks, (uint32_t)__shfl_xor((int)blocks, o, 64));
-        longest = max(longest, (uint32_t)__builtin_amdgcn_readfirstlane((int)blocks));
+        r_upto = wave_scan_add(r_cost);
+    };
+    // ---- this workgroup's stretch [at, end) of the line
+    uint32_t total = 0;
+    int longest = 1;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        look(b0);
+        total += lane_u(r_upto, 63);
+        longest = max(longest, __builtin_amdgcn_readlane(wave_scan_max((int)r_blocks), 63));
     }
-    const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, (longest + KV4_PARTS - 2) / (KV4_PARTS - 1));
+    const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1));
     uint32_t at = blockIdx.x * per;
     const uint32_t end = min(total, at + per);
 
     while (at < end) {
-        // ---- the unit at `at`: request, KV head, columns, its block steps
-        uint32_t base = 0, blocks = 0;
-        int b = 0;
+        // ---- the unit at `at`: request, KV head, vectors, its block steps
+        uint32_t base = 0;
+        int b = 0, j = 0;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
-            uint32_t cost = 0, mine = 0;
-            if (b0 + lane < a.B) {
-                const Kv4Seq s = kv4_seq(a, b0 + lane);
-                mine = unit_blocks(s);
-                cost = s.rows > 0 ? mine * seq_units(a, s) : 0;
-            }
-            const uint32_t incl = wave_scan_add(cost);
-            const unsigned long long over = __ballot(base + incl > at);
+            if (a.B > 64) look(b0);
+            const unsigned long long over = __ballot(base + r_upto > at);
             if (over) {
-                const int j = __builtin_ctzll(over);
+                j = __builtin_ctzll(over);
                 b = b0 + j;
-                base += lane_u(incl - cost, j);
-                blocks = lane_u(mine, j);
+                base += lane_u(r_upto - r_cost, j);
                 break;
             }
-            base += lane_u(incl, 63);
+            base += lane_u(r_upto, 63);
         }
-        const Kv4Seq sq = kv4_seq(a, b);
+        const uint32_t blocks = lane_u(r_blocks, j);
+        const Kv4Seq sq = kv4_span(a, __builtin_amdgcn_readlane(r_slot, j), __builtin_amdgcn_readlane(r_len, j),
+                                   __builtin_amdgcn_readlane(r_rows, j));
         const uint32_t rel = at - base, unit = rel / blocks, s0 = rel % blocks;
         const uint32_t nblk = min(blocks - s0, end - at);
-        const int ncg = (sq.rows * a.G + 15) / 16;
-        const int head = (int)unit / ncg, cg = (int)unit % ncg;
-        const int ncol = min(16, sq.rows * a.G - 16 * cg);
-
-        // ---- this lane's column: row, query head and position
-        const int vec = 16 * cg + col, row = vec / a.G;
-        const bool live = col < ncol;
-        const int pos = sq.len - sq.rows + row;
-        h16x8 qf[NG];
-        f32x4 start[NG];
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (live)
-                u = *reinterpret_cast<const uint4*>(a.q + ((size_t)b * a.S + row) * a.q_stride +
-                                                    (size_t)(head * a.G + vec % a.G) * D + 32 * g + 8 * h);
-            qf[g] = code_order(u);
-            start[g] = mfma16(minus8(g & 1), qf[g], (f32x4){0, 0, 0, 0});
-        }
-        // keys that every column of the unit sees: below `all`, and within the last column's window
-        const int first_pos = sq.len - sq.rows + 16 * cg / a.G;
-        const int last_pos = sq.len - sq.rows + (16 * cg + ncol - 1) / a.G;
-        const int all = a.causal ? min(first_pos + 1, sq.len) : sq.len;
-
-        float m = -__builtin_inff(), mbase = 0.0f, l = 0.0f;
-        f32x4 acc[NB], off[NG];       // O^T 2^-24 (odd blocks 2^-20) before the 8 comes off, -8 2^-24 sum p s_g
-#pragma unroll
-        for (int i = 0; i < NB; i++) acc[i] = (f32x4){0, 0, 0, 0};
-#pragma unroll
-        for (int g = 0; g < NG; g++) off[g] = (f32x4){0, 0, 0, 0};
+        const int ncg = (sq.rows * a.G + QV - 1) / QV;
+        const int head = (int)unit / ncg, v0 = (int)unit % ncg * QV;
+        const int nvec = min(QV, sq.rows * a.G - v0);
 
         // ---- pages of the run, 64 table entries in the lanes at a time
         int page_first = 0, pages = -1;
         bool have_pages = false;
         auto page_of = [&](int key) -> int {
-            const int j = key >> c.ps_log2;
-            if (!have_pages || j < page_first || j >= page_first + 64) {
-                page_first = j;
+            const int e = key >> c.ps_log2;
+            if (!have_pages || e < page_first || e >= page_first + 64) {
+                page_first = e;
                 have_pages = true;
-                pages = j + lane < c.max_pages ? c.table[(size_t)sq.slot * c.max_pages + j + lane] : -1;
+                pages = c.table[(size_t)sq.slot * c.max_pages + min(e + lane, c.max_pages - 1)];
+                // waited for here: at its use a wait would hold up the tiles under way each time
+                __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0)
             }
-            return __builtin_amdgcn_readlane(pages, j - page_first);
+            return __builtin_amdgcn_readlane(pages, e - page_first);
         };
         auto key_of = [&](int i) { return KV4_STEP * (i < sq.sinks ? i : sq.main0 + i - sq.sinks); };
         const uint32_t ring_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&ring[wid][0][0];
@@ -284,50 +302,105 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, D == 256 ? 1 : 2) attn_kv4_ker
             }
             return there;
         };
-        auto compute = [&](int key0, int s, uint32_t there) {
+        // ---- this wave's steps, the first R - 1 on their way
+        const int last = min(sq.steps, (int)(s0 + nblk) * KV4_WAVES), i0 = (int)s0 * KV4_WAVES + wid;
+        const int n = i0 < last ? (last - i0 + KV4_WAVES - 1) / KV4_WAVES : 0;
+        uint32_t there = 0;          // two bits per slot of the ring
+        auto put = [&](int k) {
+            const int s = k % R;
+            there = (there & ~(3u << 2 * s)) | fetch(i0 + KV4_WAVES * k, s) << 2 * s;
+        };
+#pragma unroll
+        for (int k = 0; k < R - 1; k++)
+            if (k < n) put(k);
+
+        // ---- this lane's vector: row, query head and position
+        const int vec = v0 + qi, row = vec / a.G;
+        const bool live = qi < nvec;
+        const int pos = sq.len - sq.rows + row;
+        h16x8 qf[NG];
+        f32x4 start[SG];
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (live && (!PACK || g == gi))
+                u = *reinterpret_cast<const uint4*>(a.q + ((size_t)b * a.S + row) * a.q_stride +
+                                                    (size_t)(head * a.G + vec % a.G) * D + 32 * g + 8 * h);
+            qf[g] = code_order(u);
+        }
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+            start[PACK ? 0 : g] = mfma16(minus8(g & 1), qf[g], PACK && g > 0 ? start[0] : (f32x4){0, 0, 0, 0});
+        // keys that every vector of the unit sees: below `all`, and within the last one's window
+        const int first_pos = sq.len - sq.rows + v0 / a.G;
+        const int last_pos = sq.len - sq.rows + (v0 + nvec - 1) / a.G;
+        const int all = a.causal ? min(first_pos + 1, sq.len) : sq.len;
+
+        float m = -__builtin_inff(), mbase = 0.0f, l = 0.0f;
+        f32x4 acc[NB], off[SG];       // O^T 2^-24 (odd blocks 2^-20) before the 8 comes off, -8 2^-24 sum p s_g
+#pragma unroll
+        for (int i = 0; i < NB; i++) acc[i] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int g = 0; g < SG; g++) off[g] = (f32x4){0, 0, 0, 0};
+
+        auto compute = [&](bool whole, int key0, int s, uint32_t there) {
             const uint8_t* slot = &ring[wid][s][0];
             float x[2][4];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                uint32_t k[D / 32], ks[D / 16];
+                uint32_t k[D / 32], ks[2 * SG];
                 load_words(k, slot + t * TB + lane * (D / 8));
-                load_words(ks, slot + t * TB + 8 * D + h * (D / 4));
-                float even[4] = {0, 0, 0, 0}, odd[4] = {0, 0, 0, 0};
+                load_words(ks, slot + t * TB + 8 * D + h * (D / 4) + gi * 8);
+                if constexpr (PACK) {
+                    f32x4 st = start[0];
 #pragma unroll
-                for (int p = 0; p < NG / 2; p++) {
-                    const uint32_t w0 = k[2 * p], w1 = k[2 * p + 1];
-                    const f32x4 lo = mfma16(low_codes(w0, w1), qf[2 * p], start[2 * p]);
-                    const f32x4 hi = mfma16(high_codes(w0, w1), qf[2 * p + 1], start[2 * p + 1]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        even[i] = __builtin_fmaf(lo[i], half_of(ks[4 * p + i / 2], i & 1), even[i]);
-                        odd[i] = __builtin_fmaf(hi[i], half_of(ks[4 * p + 2 + i / 2], i & 1), odd[i]);
+                    for (int p = 0; p < NG / 2; p++) {
+                        st = mfma16(low_codes(k[2 * p], k[2 * p + 1]), qf[2 * p], st);
+                        st = mfma16(high_codes(k[2 * p], k[2 * p + 1]), qf[2 * p + 1], st);
                     }
-                }
+                    x[t][0] = sum_lanes<NG>(mul_half<0>(st[0] * kscale, ks[0]));
+                    x[t][1] = sum_lanes<NG>(mul_half<1>(st[1] * kscale, ks[0]));
+                    x[t][2] = sum_lanes<NG>(mul_half<0>(st[2] * kscale, ks[1]));
+                    x[t][3] = sum_lanes<NG>(mul_half<1>(st[3] * kscale, ks[1]));
+                } else {
+                    float even[4] = {0, 0, 0, 0}, odd[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[t][i] = __builtin_fmaf(odd[i], kscale * 0.0625f, even[i] * kscale);
+                    for (int p = 0; p < NG / 2; p++) {
+                        const f32x4 lo = mfma16(low_codes(k[2 * p], k[2 * p + 1]), qf[2 * p], start[2 * p]);
+                        const f32x4 hi = mfma16(high_codes(k[2 * p], k[2 * p + 1]), qf[2 * p + 1], start[2 * p + 1]);
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            even[2 * i] = fma_half<0>(lo[2 * i], ks[4 * p + i], even[2 * i]);
+                            even[2 * i + 1] = fma_half<1>(lo[2 * i + 1], ks[4 * p + i], even[2 * i + 1]);
+                            odd[2 * i] = fma_half<0>(hi[2 * i], ks[4 * p + 2 + i], odd[2 * i]);
+                            odd[2 * i + 1] = fma_half<1>(hi[2 * i + 1], ks[4 * p + 2 + i], odd[2 * i + 1]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[t][i] = __builtin_fmaf(odd[i], kscale * 0.0625f, even[i] * kscale);
+                }
             }
-            uint32_t v[2][D / 32], vs[2][D / 16];
+            uint32_t v[2][D / 32], vs[2][2 * SG];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 load_words(v[t], slot + t * TB + 9 * D + lane * (D / 8));
-                load_words(vs[t], slot + t * TB + 17 * D + h * (D / 4));
+                load_words(vs[t], slot + t * TB + 17 * D + h * (D / 4) + gi * 8);
             }
-            const bool whole = there == 3 && key0 + KV4_STEP <= all &&
-                               (a.window == 0 || last_pos - key0 <= a.window || key0 + KV4_STEP <= a.sink);
-            if (!whole) {
+            if (!whole) {     // a key that is not seen adds nothing, whatever its scales are
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (!((there >> t & 1) && kv4_sees(a, pos, key0 + 16 * t + 4 * h + i, sq.len)))
-                            x[t][i] = -__builtin_inff();
+                    for (int i = 0; i < 4; i++) {
+                        const bool sees = (there >> t & 1) & kv4_sees(a, pos, key0 + 16 * t + 4 * h + i, sq.len);
+                        x[t][i] = sees ? x[t][i] : -__builtin_inff();
+#pragma unroll
+                        for (int g = 0; g < SG; g++)
+                            vs[t][2 * g + i / 2] = sees ? vs[t][2 * g + i / 2] : vs[t][2 * g + i / 2] & (i & 1 ? 0xFFFFu : 0xFFFF0000u);
+                    }
             }
             // the running maximum, where one of the step's scores is above it (a
             // NaN score reaches the sum by itself)
-            float top = x[0][0];
-#pragma unroll
-            for (int i = 1; i < 8; i++) top = __builtin_fmaxf(top, x[i >> 2][i & 3]);
+            float top = max3(max3(x[0][0], x[0][1], x[0][2]), max3(x[0][3], x[1][0], x[1][1]), __builtin_fmaxf(x[1][2], x[1][3]));
             if (__ballot(top > m)) {
                 top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
                 top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
@@ -339,7 +412,7 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, D == 256 ? 1 : 2) attn_kv4_ker
 #pragma unroll
                 for (int i = 0; i < NB; i++) acc[i] *= f;
 #pragma unroll
-                for (int g = 0; g < NG; g++) off[g] *= f;
+                for (int g = 0; g < SG; g++) off[g] *= f;
             }
             float p[2][4];
 #pragma unroll
@@ -349,66 +422,68 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, D == 256 ? 1 : 2) attn_kv4_ker
                     p[t][i] = exp2_fast(x[t][i] - mbase);
                     l += p[t][i];
                 }
+            h16x8 pf[SG];
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
+            for (int g = 0; g < SG; g++) {
                 float w[2][4];
 #pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) w[t][i] = p[t][i] * half_of(vs[t][2 * g + i / 2], i & 1);
-                if (!whole) {      // a key that is not seen adds nothing, whatever its scale is
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (x[t][i] == -__builtin_inff()) w[t][i] = 0.0f;
+                for (int t = 0; t < 2; t++) {
+                    w[t][0] = mul_half<0>(p[t][0], vs[t][2 * g]);
+                    w[t][1] = mul_half<1>(p[t][1], vs[t][2 * g]);
+                    w[t][2] = mul_half<0>(p[t][2], vs[t][2 * g + 1]);
+                    w[t][3] = mul_half<1>(p[t][3], vs[t][2 * g + 1]);
                 }
-                const h16x8 pf = frag(pack_h(w[0][0], w[0][2]), pack_h(w[0][1], w[0][3]), pack_h(w[1][0], w[1][2]),
-                                      pack_h(w[1][1], w[1][3]));
-                acc[2 * g] = mfma16(low_codes(v[0][g], v[1][g]), pf, acc[2 * g]);
-                acc[2 * g + 1] = mfma16(high_codes(v[0][g], v[1][g]), pf, acc[2 * g + 1]);
-                off[g] = mfma16(minus8(false), pf, off[g]);
+                pf[g] = frag(pack_h(w[0][0], w[0][2]), pack_h(w[0][1], w[0][3]), pack_h(w[1][0], w[1][2]),
+                             pack_h(w[1][1], w[1][3]));
+                off[g] = mfma16(minus8(false), pf[g], off[g]);
+            }
+            // the codes of the groups that follow are not taken apart ahead of their
+            // products (the registers that this holds spilled)
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                __builtin_amdgcn_sched_barrier(0);
+                acc[2 * g] = mfma16(low_codes(v[0][g], v[1][g]), pf[PACK ? 0 : g], acc[2 * g]);
+                acc[2 * g + 1] = mfma16(high_codes(v[0][g], v[1][g]), pf[PACK ? 0 : g], acc[2 * g + 1]);
             }
         };
-
-        // ---- this wave's steps, the next R - 1 on their way
-        const int last = min(sq.steps, (int)(s0 + nblk) * KV4_WAVES), i0 = (int)s0 * KV4_WAVES + wid;
-        const int n = i0 < last ? (last - i0 + KV4_WAVES - 1) / KV4_WAVES : 0;
-        uint32_t there = 0;          // two bits per slot of the ring
-        auto put = [&](int j) {
-            const int s = j % R;
-            there = (there & ~(3u << 2 * s)) | fetch(i0 + KV4_WAVES * j, s) << 2 * s;
-        };
-#pragma unroll
-        for (int j = 0; j < R - 1; j++)
-            if (j < n) put(j);
-        for (int j = 0; j < n; j++) {
-            if (j + R - 1 < n) {
-                put(j + R - 1);
+        for (int k = 0; k < n; k++) {
+            if (k + R - 1 < n) {
+                put(k + R - 1);
                 wait_dma<NI * (R - 1)>();
-            } else if (R > 2 && j + R - 2 < n) {
+            } else if (R > 2 && k + R - 2 < n) {
                 wait_dma<NI * (R - 2)>();
-            } else if (R > 3 && j + R - 3 < n) {
+            } else if (R > 3 && k + R - 3 < n) {
                 wait_dma<NI * (R - 3)>();
             } else {
                 wait_dma<0>();
             }
-            compute(key_of(i0 + KV4_WAVES * j), j % R, there >> 2 * (j % R) & 3u);
+            const int key0 = key_of(i0 + KV4_WAVES * k), s = k % R;
+            const uint32_t ok = there >> 2 * s & 3u;
+            const bool whole = ok == 3 && key0 + KV4_STEP <= all &&
+                               (a.window == 0 || last_pos - key0 <= a.window || key0 + KV4_STEP <= a.sink);
+            compute(whole, key0, s, ok);
         }
 
         // ---- the waves' shares of the keys meet
+        // (the thread's number hidden from the compiler, which would hold what follows
+        // from it in registers over the steps: 40 of them, a workgroup per CU less)
+        int et = tid;
+        asm volatile("" : "+v"(et));
+        const int eh = (et & 63) >> 4;
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (live) {
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                *reinterpret_cast<f32x4*>(&o_sh[wid][col * OS + 32 * g + 4 * h]) = (acc[2 * g] + off[g]) * 16777216.0f;
-                *reinterpret_cast<f32x4*>(&o_sh[wid][col * OS + 32 * g + 16 + 4 * h]) =
-                    (acc[2 * g + 1] * 0.0625f + off[g]) * 16777216.0f;
+                if (PACK && g != gi) continue;
+                const f32x4 o8 = off[PACK ? 0 : g];
+                *reinterpret_cast<f32x4*>(&o_sh[wid][qi * OS + 32 * g + 4 * eh]) = (acc[2 * g] + o8) * 16777216.0f;
+                *reinterpret_cast<f32x4*>(&o_sh[wid][qi * OS + 32 * g + 16 + 4 * eh]) =
+                    (acc[2 * g + 1] * 0.0625f + o8) * 16777216.0f;
             }
-            if (h == 0) {
-                m_sh[wid][col] = m;
-                l_sh[wid][col] = l;
+            if (eh == 0 && gi == 0) {
+                m_sh[wid][qi] = m;
+                l_sh[wid][qi] = l;
             }
         }
         __syncthreads();
@@ -417,30 +492,42 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, D == 256 ? 1 : 2) attn_kv4_ker
         // (slot 1), the others at the start of theirs (slot 0)
         const uint32_t unit0 = base + unit * blocks;
         const uint32_t wg0 = unit0 / per, nparts = (unit0 + blocks - 1) / per - wg0 + 1;
-        float* part = a.part + (size_t)(2 * blockIdx.x + (blockIdx.x == wg0)) * 16 * (D + 2);
-        for (int e = tid; e < ncol * D; e += 64 * KV4_WAVES) {
-            const int cc = e / D, d = e % D;
-            float mw = -__builtin_inff();
+        // rows of D sums, maximum, sum of weights
+        auto part_row = [&](uint32_t wg, int cc) {
+            return a.part + ((size_t)(2 * wg + (wg == wg0)) * QV + cc) * (D + 4);
+        };
+        auto write_row = [&](int cc, int d, f32x4 num, float den) {
+            const int vv = v0 + cc;
+            uint16_t r[4];
 #pragma unroll
-            for (int w = 0; w < KV4_WAVES; w++) mw = __builtin_fmaxf(mw, m_sh[w][cc]);
-            float num = 0.0f, den = 0.0f;
+            for (int i = 0; i < 4; i++) r[i] = f2h(den != 0.0f ? num[i] / den : 0.0f);
+            *reinterpret_cast<uint2*>(a.o + (((size_t)b * a.S + vv / a.G) * a.Hq + (size_t)head * a.G + vv % a.G) * D + d) =
+                make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
+        };
+        const int nquad = nvec * (D / 4);
+        for (int e = et; e < nquad; e += 64 * KV4_WAVES) {
+            const int cc = e / (D / 4), d = e % (D / 4) * 4;
+            float mw = m_sh[0][cc];
+#pragma unroll
+            for (int w = 1; w < KV4_WAVES; w++) mw = __builtin_fmaxf(mw, m_sh[w][cc]);
+            f32x4 num = {0, 0, 0, 0};
+            float den = 0.0f;
 #pragma unroll
             for (int w = 0; w < KV4_WAVES; w++) {
                 // without a maximum the wave's sums are zero, or NaN from a NaN score
                 const float f = m_sh[w][cc] > -__builtin_inff() ? exp2_fast(m_sh[w][cc] - mw) : 1.0f;
-                num = __builtin_fmaf(f, o_sh[w][cc * OS + d], num);
+                const f32x4 y = *reinterpret_cast<const f32x4*>(&o_sh[w][cc * OS + d]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) num[i] = __builtin_fmaf(f, y[i], num[i]);
                 den = __builtin_fmaf(f, l_sh[w][cc], den);
             }
             if (alone) {
-                const int vv = 16 * cg + cc;
-                a.o[(((size_t)b * a.S + vv / a.G) * a.Hq + (size_t)head * a.G + vv % a.G) * D + d] =
-                    f2h(den != 0.0f ? num / den : 0.0f);
+                write_row(cc, d, num, den);
             } else {
-                agent_store(part + e, num);
-                if (d == 0) {
-                    agent_store(part + 16 * D + cc, mw);
-                    agent_store(part + 16 * D + 16 + cc, den);
-                }
+                float* row_at = part_row(blockIdx.x, cc);
+                agent_store2(row_at + d, num[0], num[1]);
+                agent_store2(row_at + d + 2, num[2], num[3]);
+                if (d == 0) agent_store2(row_at + D, mw, den);
             }
         }
         if (!alone) {
@@ -448,48 +535,72 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, D == 256 ? 1 : 2) attn_kv4_ker
             // partials are agent-scope stores) before the count goes up
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
-            if (tid == 0)
+            if (et == 0)
                 last_sh = __hip_atomic_fetch_add(a.counters + wg0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nparts - 1;
             __syncthreads();
             if (last_sh) {
-                auto part_of = [&](uint32_t p) {
-                    return a.part + (size_t)(2 * (wg0 + p) + (p == 0)) * 16 * (D + 2);
-                };
-                // 16 threads per column: the parts' maxima and sums
-                if (tid < 16 * ncol) {
-                    const int cc = tid >> 4;
-                    float mx = -__builtin_inff();
-                    for (uint32_t p = tid & 15; p < nparts; p += 16) {
-                        const float v = agent_load(part_of(p) + 16 * D + cc);
-                        w_sh[p][cc] = v;
-                        mx = __builtin_fmaxf(mx, v);
-                    }
+                // a thread takes a quad of dims and every (threads / quads)-th part,
+                // eight parts' loads at a time: 4096 keys in 32 parts take one round of
+                // loads (a part after the other: 4 us more)
+                const int share = max(1, 64 * KV4_WAVES / nquad);
+                for (int e0 = 0; e0 < nquad; e0 += 64 * KV4_WAVES) {
+                    const int e = e0 + (share > 1 ? et % nquad : et), pl = share > 1 ? et / nquad : 0;
+                    const bool in = e < nquad && pl < share;
+                    const int cc = in ? e / (D / 4) : 0, d = in ? e % (D / 4) * 4 : 0;
+                    f32x4 num = {0, 0, 0, 0};
+                    float mx = -__builtin_inff(), den = 0.0f;
+                    for (int p0 = pl; in && p0 < (int)nparts; p0 += 8 * share) {
+                        f32x4 y[8];
+                        float2 ml[8];
 #pragma unroll
-                    for (int o = 1; o < 16; o <<= 1) mx = __builtin_fmaxf(mx, __shfl_xor(mx, o, 64));
-                    float sum = 0.0f;
-                    for (uint32_t p = tid & 15; p < nparts; p += 16) {
-                        const float v = w_sh[p][cc];
-                        const float f = v > -__builtin_inff() ? exp2_fast(v - mx) : 1.0f;
-                        w_sh[p][cc] = f;
-                        sum = __builtin_fmaf(f, agent_load(part_of(p) + 16 * D + 16 + cc), sum);
-                    }
+                        for (int u = 0; u < 8; u++) {
+                            y[u] = (f32x4){0, 0, 0, 0};
+                            ml[u] = make_float2(-__builtin_inff(), 0.0f);
+                            if (p0 + u * share < (int)nparts) {
+                                const float* row_at = part_row(wg0 + p0 + u * share, cc);
+                                const float2 lo = agent_load2(row_at + d), hi = agent_load2(row_at + d + 2);
+                                y[u] = (f32x4){lo.x, lo.y, hi.x, hi.y};
+                                ml[u] = agent_load2(row_at + D);
+                            }
+                        }
+                        float mn = mx;
 #pragma unroll
-                    for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor(sum, o, 64);
-                    if ((tid & 15) == 0) w_sh[KV4_PARTS][cc] = sum;
+                        for (int u = 0; u < 8; u++) mn = __builtin_fmaxf(mn, ml[u].x);
+                        const float f0 = mx > -__builtin_inff() ? exp2_fast(mx - mn) : 1.0f;
+                        mx = mn;
+                        num *= f0;
+                        den *= f0;
+#pragma unroll
+                        for (int u = 0; u < 8; u++) {
+                            const float f = ml[u].x > -__builtin_inff() ? exp2_fast(ml[u].x - mx) : 1.0f;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) num[i] = __builtin_fmaf(f, y[u][i], num[i]);
+                            den = __builtin_fmaf(f, ml[u].y, den);
+                        }
+                    }
+                    if (share > 1) {
+                        if (in) {
+                            float* s = &j_sh[(pl * nquad + e) * 6];
+                            s[0] = num[0], s[1] = num[1], s[2] = num[2], s[3] = num[3], s[4] = mx, s[5] = den;
+                        }
+                        __syncthreads();
+                        if (et < nquad) {
+                            mx = j_sh[e * 6 + 4];
+                            for (int u = 1; u < share; u++) mx = __builtin_fmaxf(mx, j_sh[(u * nquad + e) * 6 + 4]);
+                            num = (f32x4){0, 0, 0, 0};
+                            den = 0.0f;
+                            for (int u = 0; u < share; u++) {
+                                const float* s = &j_sh[(u * nquad + e) * 6];
+                                const float f = s[4] > -__builtin_inff() ? exp2_fast(s[4] - mx) : 1.0f;
+#pragma unroll
+                                for (int i = 0; i < 4; i++) num[i] = __builtin_fmaf(f, s[i], num[i]);
+                                den = __builtin_fmaf(f, s[5], den);
+                            }
+                        }
+                    }
+                    if (share > 1 ? et < nquad : in) write_row(cc, d, num, den);
                 }
-                __syncthreads();
-                for (int e = tid; e < ncol * D; e += 64 * KV4_WAVES) {
-                    const int cc = e / D, d = e % D;
-                    float num = 0.0f;
-#pragma unroll 8
-                    for (uint32_t p = 0; p < nparts; p++)
-                        num = __builtin_fmaf(w_sh[p][cc], agent_load(part_of(p) + e), num);
-                    const float den = w_sh[KV4_PARTS][cc];
-                    const int vv = 16 * cg + cc;
-                    a.o[(((size_t)b * a.S + vv / a.G) * a.Hq + (size_t)head * a.G + vv % a.G) * D + d] =
-                        f2h(den != 0.0f ? num / den : 0.0f);
-                }
-                if (tid == 0) __hip_atomic_store(a.counters + wg0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (et == 0) __hip_atomic_store(a.counters + wg0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
         __syncthreads();
@@ -507,7 +618,7 @@ size_t cactus_hip_attention_kv4_workspace(const cactus_hip_kv4_cache* cache, siz
                                           size_t num_q_heads) {
     (void)batch; (void)seq_len; (void)num_q_heads;
     if (kv4_view(cache, 0, "attention_kv4_workspace", nullptr)) return 0;
-    return KV4_COUNTERS + (size_t)KV4_GRID * 2 * 16 * (cache->head_dim + 2) * 4;
+    return KV4_COUNTERS + (size_t)512 * 2 * 16 * (cache->head_dim + 4) * 4;   // (packed: 1024 of 4 vectors)
 }
 
 int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer, const int32_t* seqs,
@@ -546,18 +657,24 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     a.scale = (scale == 0.0f ? 1.0f / sqrtf((float)cache->head_dim) : scale) * LOG2E_F;
     a.counters = static_cast<uint32_t*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + KV4_COUNTERS);
+    const hipStream_t st = as_stream(stream);
     // block steps at most, by what the tables can hold
     const size_t blocks = (cache->max_pages * cache->page_size + KV4_BLOCK - 1) / KV4_BLOCK;
-    const size_t units = batch * cache->kv_heads * ceil_div(seq_len * G, 16);
-    if (units >= (1u << 31) / blocks)
-        return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows times table length is too large");
-    const dim3 grid((unsigned)std::min<size_t>(KV4_GRID, units * blocks)), block(64 * KV4_WAVES);
-    const hipStream_t st = as_stream(stream);
-    switch (a.c.d) {
-        case 64: hipLaunchKernelGGL(attn_kv4_kernel<64>, grid, block, 0, st, a); break;
-        case 128: hipLaunchKernelGGL(attn_kv4_kernel<128>, grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL(attn_kv4_kernel<256>, grid, block, 0, st, a);
-    }
+    auto launch = [&](auto kernel, int vectors, int per_cu) {
+        const size_t units = batch * cache->kv_heads * ceil_div(seq_len * G, vectors);
+        if (units >= (1u << 31) / blocks)
+            return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows times table length is too large");
+        const dim3 grid((unsigned)std::min<size_t>(256 * per_cu, units * blocks));
+        hipLaunchKernelGGL(kernel, grid, dim3(64 * KV4_WAVES), 0, st, a);
+        return (int)CACTUS_HIP_OK;
+    };
+#define KV4_LAUNCH(D)                                                                                              \
+    (seq_len * G <= (size_t)kv4_vectors<D, true>()                                                                 \
+         ? launch(attn_kv4_kernel<D, true>, kv4_vectors<D, true>(), kv4_per_cu<D, true>())                         \
+         : launch(attn_kv4_kernel<D, false>, kv4_vectors<D, false>(), kv4_per_cu<D, false>()))
+    rc = a.c.d == 64 ? KV4_LAUNCH(64) : a.c.d == 128 ? KV4_LAUNCH(128) : KV4_LAUNCH(256);
+#undef KV4_LAUNCH
+    if (rc) return rc;
     return check_launch("attention_kv4");
 }
 
