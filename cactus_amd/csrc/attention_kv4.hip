@@ -193,6 +193,17 @@ __device__ __forceinline__ float sum_lanes(float v) {
 }
 __device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_fmaxf(__builtin_fmaxf(a, b), c); }
 
+// 16 bytes per active lane to LDS; ONCE: not to be kept in the caches
+template <bool ONCE>
+__device__ __forceinline__ void tile_dma(const void* src, uint32_t lds_addr) {
+    if constexpr (ONCE) {
+        const uint32_t lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr);
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "s"(lds) : "memory");
+    } else {
+        lds_dma<16>(src, lds_addr);
+    }
+}
+
 template <int D, bool PACK>
 __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_kv4_kernel(Kv4AttnArgs a) {
     constexpr int NG = D / 32, NB = D / 16, OS = D + 4, QV = kv4_vectors<D, PACK>();
@@ -297,8 +308,8 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_
                 const uint8_t* tile = kv4_tile(c, ok ? page : 0, head, (k0 & ((1 << c.ps_log2) - 1)) >> 4) + 16 * lane;
                 const uint32_t to = ring_lds + s * SLOT + t * TB;
 #pragma unroll
-                for (int o = 0; o + 1024 <= TB; o += 1024) lds_dma<16>(tile + o, to + o);
-                if (16 * lane < TB % 1024) lds_dma<16>(tile + TB / 1024 * 1024, to + TB / 1024 * 1024);
+                for (int o = 0; o + 1024 <= TB; o += 1024) tile_dma<PACK>(tile + o, to + o);
+                if (16 * lane < TB % 1024) tile_dma<PACK>(tile + TB / 1024 * 1024, to + TB / 1024 * 1024);
             }
             return there;
         };
@@ -608,6 +619,542 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_
     }
 }
 
+// ------------------------------------------------------------ many rows
+// A workgroup takes 32 W query vectors of one KV head, 32 per wave in two
+// column blocks of 16, and walks the keys PF_KEYS at a time.  Each stage's codes
+// become FP16 values once for all the waves: (u - 8) s is exact in FP16 (the
+// scale has 8 significant bits), so nothing is rounded that the few-row kernel
+// does not round, and the scores and outputs are plain products without a scale
+// per group.  The waves write the values to LDS in the order of the matrix
+// operands, two stages in turn: stage t + 1 is written while stage t is used, and
+// stage t + 2's codes are on their way to registers.
+//
+// A column's maximum is raised only when a score exceeds it by 2^PF_SLACK: the
+// weights stay below 2^8 (FP16 holds 2^16), and the outputs are rescaled a few
+// times per row instead of at every new maximum.  The sum of the weights is a
+// product with ones, of the rounded weights that the outputs use.
+constexpr int PF_SLACK = 8;
+constexpr size_t PF_FROM = 32;   // more query vectors per KV head than this
+constexpr int PF_MIN = 4;        // stages of a stretch at least
+
+
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ h16x2 as_h2(uint32_t u) { return __builtin_bit_cast(h16x2, u); }
+// pairs of codes (bits 0 and 16, or 4 and 20, of w on) times the scales s: as
+// 1024 + u, exactly u - 8, times s
+__device__ __forceinline__ uint32_t low_values(uint32_t w, h16x2 s) {
+    const h16x2 x = as_h2((w & 0x000F000Fu) | 0x64006400u) - (h16x2){(_Float16)1032.0f, (_Float16)1032.0f};
+    return __builtin_bit_cast(uint32_t, x * s);
+}
+__device__ __forceinline__ uint32_t high_values(uint32_t w, h16x2 s) {
+    const h16x2 x = __builtin_elementwise_fma(as_h2((w & 0x00F000F0u) | 0x64006400u),
+                                              (h16x2){(_Float16)0.0625f, (_Float16)0.0625f},
+                                              (h16x2){(_Float16)-72.0f, (_Float16)-72.0f});
+    return __builtin_bit_cast(uint32_t, x * s);
+}
+
+// The line of stages: units (request, block of NV vectors, KV head) in that
+// order; 64 (request, block) pairs at a time, one per lane.
+template <int NV, int KT>
+struct PrefillLine {
+    const Kv4AttnArgs& a;
+    int lane, nvb, npairs;
+    int slot = -1, len = 0, rows = 0;                // of the lane's pair
+    uint32_t blocks = 0, cost = 0, upto = 0;         // stages of a unit, of the pair, of the pairs up to it
+    uint32_t total = 0, base = 0;                    // base: stages before the pair that find() found
+    int pair = 0;
+
+    struct Span { int slot, len, rows, main0, sinks, steps; };
+    __device__ Span span(int slot, int len, int rows, int vb) const {
+        Span s{slot, len, rows, 0, 0, 0};
+        const int nv = rows * a.G, v0 = vb * NV;
+        if (v0 >= nv) return s;
+        const int p0 = len - rows + v0 / a.G, p1 = len - rows + (min(v0 + NV, nv) - 1) / a.G;
+        const int hi = max(0, a.causal ? min(len, p1 + 1) : len);
+        const int lo = a.window > 0 && p0 > a.window ? min(p0 - a.window, hi) : 0;
+        s.main0 = lo / KT;
+        s.sinks = a.window > 0 ? min((min(a.sink, hi) + KT - 1) / KT, s.main0) : 0;
+        s.steps = s.sinks + (hi + KT - 1) / KT - s.main0;
+        return s;
+    }
+    __device__ PrefillLine(const Kv4AttnArgs& args, int l)
+        : a(args), lane(l), nvb((args.S * args.G + NV - 1) / NV), npairs(args.B * nvb) {}
+    __device__ void look(int i0) {
+        rows = 0;
+        blocks = cost = 0;
+        const int i = i0 + lane;
+        if (i < npairs) {
+            const int b = i / nvb, vb = i % nvb;
+            slot = kv4_slot(a.c, a.seqs, b);
+            rows = slot < 0 ? 0 : kv4_count(a.counts, b, a.S);
+            len = slot < 0 ? 0 : kv4_len(a.c, slot);
+            blocks = vb * NV < rows * a.G ? (uint32_t)max(1, span(slot, len, rows, vb).steps) : 0;
+            cost = blocks * (uint32_t)a.c.Hkv;
+        }
+        upto = wave_scan_add(cost);
+    }
+    // stages of a workgroup's stretch
+    __device__ uint32_t stretch(uint32_t workgroups) {
+        int longest = 1;
+        for (int i0 = 0; i0 < npairs; i0 += 64) {
+            look(i0);
+            total += lane_u(upto, 63);
+            longest = max(longest, __builtin_amdgcn_readlane(wave_scan_max((int)blocks), 63));
+        }
+        return max(max((total + workgroups - 1) / workgroups, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1)),
+                   (uint32_t)PF_MIN);
+    }
+    // the lane of the pair that stage `at` of the line belongs to
+    __device__ int find(uint32_t at) {
+        base = 0;
+        for (int i0 = 0; i0 < npairs; i0 += 64) {
+            if (npairs > 64) look(i0);
+            const unsigned long long over = __ballot(base + upto > at);
+            if (over) {
+                const int j = __builtin_ctzll(over);
+                pair = i0 + j;
+                base += lane_u(upto - cost, j);
+                return j;
+            }
+            base += lane_u(upto, 63);
+        }
+        return 0;   // (not reached: at < total)
+    }
+};
+
+template <int D, int W>
+__global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kernel(Kv4AttnArgs a) {
+    constexpr int NG = D / 32, NB = D / 16, NT = W, KT = 16 * NT, NV = 32 * W;
+    constexpr int NQ = NT / 2;                       // 32-key parts of a stage
+    __shared__ __align__(16) uint4 kf[2][NT][NG][64];          // K operands: [tile][group][lane]
+    __shared__ __align__(16) uint4 vf[2][NT / 2][NB][64];      // V operands: [32 keys][16 dims][lane]
+    __shared__ uint32_t nan_sh[2][KT];               // stage << 8 | value groups of a key that read as NaN
+    __shared__ int any_sh[2];                        // the last stage (plus 1) that has such a key
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, h = lane >> 4;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Kv4View& c = a.c;
+    const float kscale = __builtin_fabsf(a.scale);   // (a negative one turns the sign of q)
+    const uint32_t qsign = a.scale < 0.0f ? 0x80008000u : 0u;
+
+    PrefillLine<NV, KT> line(a, lane);
+    const uint32_t per = line.stretch(gridDim.x), total = line.total;
+    uint32_t at = blockIdx.x * per;
+    const uint32_t end = min(total, at + per);
+
+    while (at < end) {
+        const int j = line.find(at);
+        const uint32_t base = line.base, blocks = lane_u(line.blocks, j);
+        const int b = line.pair / line.nvb, vb = line.pair % line.nvb;
+        const auto sq = line.span(__builtin_amdgcn_readlane(line.slot, j), __builtin_amdgcn_readlane(line.len, j),
+                                  __builtin_amdgcn_readlane(line.rows, j), vb);
+        const uint32_t rel = at - base;
+        const int head = (int)(rel / blocks);
+        const uint32_t s0 = rel % blocks, nblk = min(blocks - s0, end - at);
+        const int nvec = min(NV, sq.rows * a.G - vb * NV);          // of the workgroup
+        const int w0 = 32 * wid, wvec = max(0, min(32, nvec - w0)); // of this wave
+        const int row0 = sq.len - sq.rows;
+
+        // ---- pages, 64 table entries in the lanes at a time
+        int page_first = 0, pages = -1;
+        bool have_pages = false;
+        auto key_of = [&](int i) { return KT * (i < sq.sinks ? i : sq.main0 + i - sq.sinks); };
+        // ---- the wave's tile of a stage (tile `wid`), in registers
+        uint32_t kraw[D / 32], kscl[NG], vraw[D / 32], vscl[D / 16];
+        uint32_t there = 0;          // tiles of that stage that have a page, a bit each
+        auto fetch = [&](int i) {
+            const int key0 = key_of(i), e0 = key0 >> c.ps_log2, e1 = (key0 + KT - 1) >> c.ps_log2;
+            if (!have_pages || e0 < page_first || e1 >= page_first + 64) {
+                page_first = e0;
+                have_pages = true;
+                pages = c.table[(size_t)sq.slot * c.max_pages + min(e0 + lane, c.max_pages - 1)];
+                __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0), see the few-row kernel
+            }
+            const int k0 = key0 + 16 * wid;
+            int page = __builtin_amdgcn_readlane(pages, (k0 >> c.ps_log2) - page_first);
+            bool ok = kv4_page_ok(c, page);
+            if (e0 == e1) {
+                there = ok ? (1u << NT) - 1 : 0;
+            } else {
+                there = 0;
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+                    there |= (uint32_t)kv4_page_ok(c, __builtin_amdgcn_readlane(pages, ((key0 + 16 * t) >> c.ps_log2) - page_first)) << t;
+            }
+            const uint8_t* p = kv4_tile(c, ok ? page : 0, head, (k0 & ((1 << c.ps_log2) - 1)) >> 4);
+            load_words(kraw, p + lane * (D / 8));
+#pragma unroll
+            for (int g = 0; g < NG; g++)                         // of key `col`
+                kscl[g] = *reinterpret_cast<const uint16_t*>(p + 8 * D + (((col >> 2) * NG + g) * 4 + (col & 3)) * 2);
+            load_words(vraw, p + 9 * D + lane * (D / 8));
+            load_words(vscl, p + 17 * D + h * (D / 4));          // of keys 4 h + i
+        };
+        // A NaN or infinite scale of a value group: the key is marked and the group
+        // reads as 0 (0 times NaN would reach the rows that do not see the key)
+        auto mark = [&](int i) {
+            uint32_t bad = 0;        // an exponent of all ones carries into bits 15 and 31
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) bad |= (vscl[k] & 0x7C007C00u) + 0x04000400u;
+            if (__builtin_expect(__ballot((bad & 0x80008000u) != 0) != 0, 0)) {
+                uint32_t groups[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < D / 16; k++)
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        if ((vscl[k] >> 16 * half & 0x7C00u) != 0x7C00u) continue;
+                        vscl[k] &= half ? 0xFFFFu : 0xFFFF0000u;
+                        groups[2 * (k & 1) + half] |= 1u << (k >> 1);
+                    }
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int key = 16 * wid + 4 * h + r;
+                    if (groups[r] && key_of(i) + key < sq.len && (there >> wid & 1)) {
+                        nan_sh[i & 1][key] = (uint32_t)i << 8 | groups[r];
+                        any_sh[i & 1] = i + 1;
+                    }
+                }
+            }
+        };
+        // a quarter of the tile's codes to the operands of buffer `buf`: groups
+        // [g0, g1) of the keys, then of the values
+        auto put_keys = [&](int buf, int p0, int p1) {
+#pragma unroll
+            for (int p = p0; p < p1; p++) {
+                const uint32_t x0 = kraw[2 * p], x1 = kraw[2 * p + 1];
+                const h16x2 sl = as_h2(kscl[2 * p] | kscl[2 * p] << 16);
+                const h16x2 sh = as_h2(kscl[2 * p + 1] | kscl[2 * p + 1] << 16);
+                kf[buf][wid][2 * p][lane] = make_uint4(low_values(x0, sl), low_values(x0 >> 8, sl), low_values(x1, sl),
+                                                       low_values(x1 >> 8, sl));
+                kf[buf][wid][2 * p + 1][lane] = make_uint4(high_values(x0, sh), high_values(x0 >> 8, sh),
+                                                           high_values(x1, sh), high_values(x1 >> 8, sh));
+            }
+        };
+        auto put_vals = [&](int buf, int g0, int g1) {
+#pragma unroll
+            for (int g = g0; g < g1; g++) {
+                const uint32_t s01 = vscl[2 * g], s23 = vscl[2 * g + 1], w = vraw[g];
+                const h16x2 se = as_h2(__builtin_amdgcn_perm(s23, s01, 0x05040100u));    // keys 4 h, 4 h + 2
+                const h16x2 so = as_h2(__builtin_amdgcn_perm(s23, s01, 0x07060302u));    // keys 4 h + 1, 4 h + 3
+                reinterpret_cast<uint2*>(&vf[buf][wid >> 1][2 * g][lane])[wid & 1] =
+                    make_uint2(low_values(w, se), low_values(w >> 8, so));
+                reinterpret_cast<uint2*>(&vf[buf][wid >> 1][2 * g + 1][lane])[wid & 1] =
+                    make_uint2(high_values(w, se), high_values(w >> 8, so));
+            }
+        };
+        // part n of m of all that
+        auto put = [&](int buf, int n, int m) {
+            if (m == 1 || n < m / 2) put_keys(buf, m == 1 ? 0 : NG / 2 * n / (m / 2), m == 1 ? NG / 2 : NG / 2 * (n + 1) / (m / 2));
+            if (m == 1 || n >= m / 2) put_vals(buf, m == 1 ? 0 : NG * (n - m / 2) / (m / 2), m == 1 ? NG : NG * (n + 1 - m / 2) / (m / 2));
+        };
+
+        // ---- this wave's vectors: lane's column in two blocks of 16
+        h16x8 qf[2][NG];
+        int pos[2];
+#pragma unroll
+        for (int cb = 0; cb < 2; cb++) {
+            const int vec = vb * NV + w0 + 16 * cb + col, row = vec / a.G;
+            pos[cb] = row0 + row;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (16 * cb + col < wvec)
+                    u = *reinterpret_cast<const uint4*>(a.q + ((size_t)b * a.S + row) * a.q_stride +
+                                                        (size_t)(head * a.G + vec % a.G) * D + 32 * g + 8 * h);
+                u.x ^= qsign, u.y ^= qsign, u.z ^= qsign, u.w ^= qsign;
+                qf[cb][g] = code_order(u);
+            }
+        }
+        const int first_pos = row0 + (vb * NV + w0) / a.G;
+        const int last_pos = row0 + (vb * NV + w0 + max(wvec, 1) - 1) / a.G;
+        const int all = a.causal ? min(first_pos + 1, sq.len) : sq.len;      // keys that each of them sees (but for a window)
+
+        float m[2], mbase[2];
+        f32x4 acc[2][NB], lsum[2];
+#pragma unroll
+        for (int cb = 0; cb < 2; cb++) {
+            m[cb] = -__builtin_inff();
+            mbase[cb] = 0.0f;
+            lsum[cb] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < NB; i++) acc[cb][i] = (f32x4){0, 0, 0, 0};
+        }
+        u32x4 one4 = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+        asm volatile("" : "+v"(one4));               // in registers: not made anew at each stage
+        const h16x8 ones = __builtin_bit_cast(h16x8, one4);
+
+        // ---- a stage: its 32-key parts in turn, the next part's scores beside this
+        // one's powers of two, then this part's outputs beside a share of the next
+        // stage's values.  Operands are read from LDS a group of products ahead; the
+        // barriers and groups keep the compiler from moving them together.
+        constexpr int VG = 4, NVG = NB / VG;
+        auto stage = [&](int i, int buf, uint32_t there, bool more) {
+            const int key0 = key_of(i);
+            const bool active = wvec > 0 && (!a.causal || key0 <= last_pos);
+            if (!active) {
+                if (more) put(buf ^ 1, 0, 1);
+                return;
+            }
+            f32x4 st[2][2][2];                        // [part parity][column block][tile]
+            h16x8 pf[2], ka[NG], kb[NG], va[VG], vb2[VG];
+            auto read_k = [&](int t, h16x8 (&to)[NG]) {
+#pragma unroll
+                for (int g = 0; g < NG; g++) to[g] = __builtin_bit_cast(h16x8, kf[buf][t][g][lane]);
+            };
+            auto read_v = [&](int q, int n, h16x8 (&to)[VG]) {
+#pragma unroll
+                for (int u = 0; u < VG; u++) to[u] = __builtin_bit_cast(h16x8, vf[buf][q][n * VG + u][lane]);
+            };
+            auto scores = [&](int q, int t, const h16x8 (&k)[NG]) {
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+#pragma unroll
+                    for (int cb = 0; cb < 2; cb++)
+                        st[q & 1][cb][t] = mfma16(k[g], qf[cb][g], g ? st[q & 1][cb][t] : (f32x4){0, 0, 0, 0});
+            };
+            // part q's scores: masked where not every vector sees every key, and the maxima
+            auto check = [&](int q) {
+                const int k0 = key0 + 32 * q;
+                f32x4 (&s)[2][2] = st[q & 1];
+                const bool whole = (there >> 2 * q & 3u) == 3u && k0 + 32 <= all &&
+                                   (a.window == 0 || last_pos - k0 <= a.window || k0 + 32 <= a.sink);
+                if (!whole) {
+#pragma unroll
+                    for (int cb = 0; cb < 2; cb++)
+#pragma unroll
+                        for (int t = 0; t < 2; t++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const bool sees = (there >> (2 * q + t) & 1) & kv4_sees(a, pos[cb], k0 + 16 * t + 4 * h + r, sq.len);
+                                s[cb][t][r] = sees ? s[cb][t][r] : -__builtin_inff();
+                            }
+                }
+                float top[2];
+#pragma unroll
+                for (int cb = 0; cb < 2; cb++)
+                    top[cb] = kscale * max3(max3(s[cb][0][0], s[cb][0][1], s[cb][0][2]), max3(s[cb][0][3], s[cb][1][0], s[cb][1][1]),
+                                            __builtin_fmaxf(s[cb][1][2], s[cb][1][3]));
+                if (__ballot((top[0] > m[0] + PF_SLACK) | (top[1] > m[1] + PF_SLACK))) {
+#pragma unroll
+                    for (int cb = 0; cb < 2; cb++) {
+                        float y = top[cb];
+                        y = __builtin_fmaxf(y, __shfl_xor(y, 16, 64));
+                        y = __builtin_fmaxf(y, __shfl_xor(y, 32, 64));
+                        const float mn = __builtin_fmaxf(m[cb], y);
+                        mbase[cb] = mn > -__builtin_inff() ? mn : 0.0f;
+                        const float f = exp2_fast(m[cb] - mbase[cb]);
+                        m[cb] = mn;
+                        lsum[cb] *= f;
+#pragma unroll
+                        for (int n = 0; n < NB; n++) acc[cb][n] *= f;
+                    }
+                }
+            };
+            auto weights = [&](int q) {
+#pragma unroll
+                for (int cb = 0; cb < 2; cb++) {
+                    float p[2][4];
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) p[t][r] = exp2_fast(__builtin_fmaf(st[q & 1][cb][t][r], kscale, -mbase[cb]));
+                    pf[cb] = frag(pack_h(p[0][0], p[0][2]), pack_h(p[0][1], p[0][3]), pack_h(p[1][0], p[1][2]),
+                                  pack_h(p[1][1], p[1][3]));
+                }
+            };
+            auto values = [&](int n, const h16x8 (&v)[VG]) {
+#pragma unroll
+                for (int u = 0; u < VG; u++)
+#pragma unroll
+                    for (int cb = 0; cb < 2; cb++) acc[cb][n * VG + u] = mfma16(v[u], pf[cb], acc[cb][n * VG + u]);
+            };
+            read_k(0, ka);
+            read_k(1, kb);
+            __builtin_amdgcn_sched_barrier(0);
+            scores(0, 0, ka);
+            scores(0, 1, kb);
+            if (NQ > 1) read_k(2, ka);
+            __builtin_amdgcn_sched_barrier(0);
+            check(0);
+#pragma unroll
+            for (int q = 0; q < NQ; q++) {
+                // A: scores of part q + 1, weights of part q
+                if (q + 1 < NQ) read_k(2 * q + 3, kb);
+                __builtin_amdgcn_sched_barrier(0);
+                if (q + 1 < NQ) scores(q + 1, 0, ka);
+                weights(q);
+                if (q + 1 < NQ) scores(q + 1, 1, kb);
+                read_v(q, 0, va);
+                if (q + 1 < NQ) {
+#pragma unroll
+                    for (int n = 0; n < 4 * NG; n++) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x402, (40 + 4 * NG - 1) / (4 * NG), 0);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x100, VG, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                // B: outputs of part q, the next stage's values
+#pragma unroll
+                for (int n = 0; n < NVG; n++) {
+                    h16x8 (&cur)[VG] = n & 1 ? vb2 : va;
+                    h16x8 (&nxt)[VG] = n & 1 ? va : vb2;
+                    if (n + 1 < NVG) read_v(q, n + 1, nxt);
+                    else if (q + 2 < NQ) read_k(2 * q + 4, ka);
+                    __builtin_amdgcn_sched_barrier(0x606);      // vector and scalar instructions and LDS writes may pass
+                    values(n, cur);
+                    if (n == 0) put(buf ^ 1, q, NQ);
+                    if (n + 1 == NVG) {
+#pragma unroll
+                        for (int cb = 0; cb < 2; cb++) lsum[cb] = mfma16(ones, pf[cb], lsum[cb]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2 * VG; u++) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0x606);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (q + 1 < NQ) check(q + 1);
+            }
+            if (__builtin_expect(any_sh[buf] == i + 1, 0)) {
+                for (int key = 0; key < KT; key++) {
+                    const uint32_t w = nan_sh[buf][key];
+                    if (w >> 8 != ((uint32_t)i & 0xFFFFFFu) || !(w & 0xFFu)) continue;
+#pragma unroll
+                    for (int cb = 0; cb < 2; cb++) {
+                        const bool sees = kv4_sees(a, pos[cb], key0 + key, sq.len);
+#pragma unroll
+                        for (int n = 0; n < NB; n++)
+                            if (sees && (w >> (n >> 1) & 1))
+                                acc[cb][n] = (f32x4){__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+                    }
+                }
+            }
+        };
+
+        // ---- the stages
+        const int i0 = (int)s0, i1 = min(sq.steps, (int)(s0 + nblk));
+        for (int e = tid; e < 2 * KT; e += 64 * W) (&nan_sh[0][0])[e] = 0;
+        if (tid < 2) any_sh[tid] = 0;
+        __syncthreads();
+        if (i0 < i1) {
+            fetch(i0);
+            mark(i0);
+            put(i0 & 1, 0, 1);
+            uint32_t now = there;
+            fetch(min(i0 + 1, i1 - 1));
+            __syncthreads();
+            for (int i = i0; i < i1; i++) {
+                const uint32_t next = there;
+                if (i + 1 < i1) mark(i + 1);
+                stage(i, i & 1, now, i + 1 < i1);
+                fetch(min(i + 2, i1 - 1));
+                now = next;
+                __syncthreads();
+            }
+        }
+
+        // ---- outputs, or this workgroup's part of them
+        const bool alone = nblk == blocks;
+        const uint32_t unit0 = base + (uint32_t)head * blocks;
+        const uint32_t wg0 = unit0 / per;    // the unit's first workgroup has it in slot 1 (see the few-row kernel)
+        auto out_row = [&](int v) {
+            const int vv = vb * NV + v;
+            return a.o + (((size_t)b * a.S + vv / a.G) * a.Hq + (size_t)head * a.G + vv % a.G) * D;
+        };
+        auto write4 = [&](uint16_t* p, f32x4 num, float den) {
+            uint16_t r[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) r[k] = f2h(den != 0.0f ? num[k] / den : 0.0f);
+            *reinterpret_cast<uint2*>(p) = make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
+        };
+#pragma unroll
+        for (int cb = 0; cb < 2; cb++) {
+            const int v = w0 + 16 * cb + col;
+            if (v >= nvec) continue;
+            if (alone) {
+                uint16_t* o = out_row(v);
+#pragma unroll
+                for (int n = 0; n < NB; n++) write4(o + 16 * n + 4 * h, acc[cb][n], lsum[cb][0]);
+            } else {
+                float* row_at = a.part + ((size_t)(2 * blockIdx.x + (blockIdx.x == wg0)) * NV + v) * (D + 4);
+#pragma unroll
+                for (int n = 0; n < NB; n++) *reinterpret_cast<f32x4*>(row_at + 16 * n + 4 * h) = acc[cb][n];
+                if (h == 0) *reinterpret_cast<float2*>(row_at + D) = make_float2(m[cb], lsum[cb][0]);
+            }
+        }
+        __syncthreads();
+        at += nblk;
+    }
+}
+
+// The joining of units that several workgroups shared, PJ_VEC vectors per
+// workgroup.  A launch of its own: the last workgroup of a unit, joining 256
+// vectors' parts alone, took longer than the products of a few hundred rows.
+constexpr int PJ_VEC = 16;
+template <int D, int W>
+__global__ void __launch_bounds__(256) attn_kv4_join_kernel(Kv4AttnArgs a, uint32_t workgroups) {
+    constexpr int NV = 32 * W, KT = 16 * W, NVJ = NV / PJ_VEC;
+    const int tid = threadIdx.x, lane = tid & 63;
+    PrefillLine<NV, KT> line(a, lane);
+    const uint32_t per = line.stretch(workgroups);
+    // this workgroup's unit: the pair's place in the line, then the head
+    const int v0 = (int)(blockIdx.x % NVJ) * PJ_VEC, head = (int)(blockIdx.x / NVJ % a.c.Hkv);
+    const int pair = (int)(blockIdx.x / NVJ / a.c.Hkv), j = pair & 63;
+    uint32_t base = 0;
+    for (int i0 = 0; i0 <= pair; i0 += 64) {
+        if (line.npairs > 64) line.look(i0);
+        base += lane_u(i0 + 64 <= pair ? line.upto : line.upto - line.cost, i0 + 64 <= pair ? 63 : j);
+    }
+    const uint32_t blocks = lane_u(line.blocks, j);
+    if (blocks == 0) return;
+    const int b = pair / line.nvb, vb = pair % line.nvb;
+    const int nvec = min(NV, __builtin_amdgcn_readlane(line.rows, j) * a.G - vb * NV);
+    const uint32_t unit0 = base + (uint32_t)head * blocks;
+    const uint32_t wg0 = unit0 / per, nparts = (unit0 + blocks - 1) / per - wg0 + 1;
+    if (nparts == 1) return;
+    for (int e = tid; e < PJ_VEC * (D / 4); e += 256) {
+        const int v = v0 + e / (D / 4), d = e % (D / 4) * 4;
+        if (v >= nvec) break;
+        f32x4 num = {0, 0, 0, 0};
+        float mx = -__builtin_inff(), den = 0.0f;
+        for (int p0 = 0; p0 < (int)nparts; p0 += 4) {
+            f32x4 y[4];
+            float2 ml[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                y[u] = (f32x4){0, 0, 0, 0};
+                ml[u] = make_float2(-__builtin_inff(), 0.0f);
+                if (p0 + u < (int)nparts) {
+                    const float* row_at = a.part + ((size_t)(2 * (wg0 + p0 + u) + (p0 + u == 0)) * NV + v) * (D + 4);
+                    y[u] = *reinterpret_cast<const f32x4*>(row_at + d);
+                    ml[u] = *reinterpret_cast<const float2*>(row_at + D);
+                }
+            }
+            float mn = mx;
+#pragma unroll
+            for (int u = 0; u < 4; u++) mn = __builtin_fmaxf(mn, ml[u].x);
+            const float f0 = mx > -__builtin_inff() ? exp2_fast(mx - mn) : 1.0f;
+            mx = mn;
+            num *= f0;
+            den *= f0;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float f = ml[u].x > -__builtin_inff() ? exp2_fast(ml[u].x - mx) : 1.0f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) num[k] = __builtin_fmaf(f, y[u][k], num[k]);
+                den = __builtin_fmaf(f, ml[u].y, den);
+            }
+        }
+        const int vv = vb * NV + v;
+        uint16_t r[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) r[k] = f2h(den != 0.0f ? num[k] / den : 0.0f);
+        *reinterpret_cast<uint2*>(a.o + (((size_t)b * a.S + vv / a.G) * a.Hq + (size_t)head * a.G + vv % a.G) * D + d) =
+            make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
+    }
+}
+
 }  // namespace cactus_hip
 
 using namespace cactus_hip;
@@ -616,9 +1163,12 @@ extern "C" {
 
 size_t cactus_hip_attention_kv4_workspace(const cactus_hip_kv4_cache* cache, size_t batch, size_t seq_len,
                                           size_t num_q_heads) {
-    (void)batch; (void)seq_len; (void)num_q_heads;
     if (kv4_view(cache, 0, "attention_kv4_workspace", nullptr)) return 0;
-    return KV4_COUNTERS + (size_t)512 * 2 * 16 * (cache->head_dim + 4) * 4;   // (packed: 1024 of 4 vectors)
+    const size_t vectors = seq_len * (num_q_heads / cache->kv_heads);
+    const size_t few = (size_t)512 * 2 * 16;                  // (packed: 1024 workgroups of 4 vectors)
+    const size_t many = (size_t)256 * 2 * (cache->head_dim == 256 ? 128 : 256);
+    (void)batch;
+    return KV4_COUNTERS + (vectors > PF_FROM ? many : few) * (cache->head_dim + 4) * 4;
 }
 
 int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer, const int32_t* seqs,
@@ -660,20 +1210,32 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     const hipStream_t st = as_stream(stream);
     // block steps at most, by what the tables can hold
     const size_t blocks = (cache->max_pages * cache->page_size + KV4_BLOCK - 1) / KV4_BLOCK;
-    auto launch = [&](auto kernel, int vectors, int per_cu) {
-        const size_t units = batch * cache->kv_heads * ceil_div(seq_len * G, vectors);
-        if (units >= (1u << 31) / blocks)
+    const size_t vectors = seq_len * G;
+    auto launch = [&](auto kernel, int per_unit, int per_cu, int waves, unsigned* workgroups) {
+        const size_t units = batch * cache->kv_heads * ceil_div(vectors, per_unit);
+        if (units >= (1u << 31) / blocks / PJ_VEC)
             return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows times table length is too large");
-        const dim3 grid((unsigned)std::min<size_t>(256 * per_cu, units * blocks));
-        hipLaunchKernelGGL(kernel, grid, dim3(64 * KV4_WAVES), 0, st, a);
+        *workgroups = (unsigned)std::min<size_t>(256 * per_cu, units * blocks);
+        hipLaunchKernelGGL(kernel, dim3(*workgroups), dim3(64 * waves), 0, st, a);
         return (int)CACTUS_HIP_OK;
     };
-#define KV4_LAUNCH(D)                                                                                              \
-    (seq_len * G <= (size_t)kv4_vectors<D, true>()                                                                 \
-         ? launch(attn_kv4_kernel<D, true>, kv4_vectors<D, true>(), kv4_per_cu<D, true>())                         \
-         : launch(attn_kv4_kernel<D, false>, kv4_vectors<D, false>(), kv4_per_cu<D, false>()))
-    rc = a.c.d == 64 ? KV4_LAUNCH(64) : a.c.d == 128 ? KV4_LAUNCH(128) : KV4_LAUNCH(256);
+    auto many = [&](auto kernel, auto join, int waves) {
+        unsigned workgroups = 0;
+        const int r = launch(kernel, 32 * waves, 1, waves, &workgroups);
+        if (r) return r;
+        const unsigned units = (unsigned)(batch * cache->kv_heads * ceil_div(vectors, 32 * waves));
+        hipLaunchKernelGGL(join, dim3(units * (32 * waves / PJ_VEC)), dim3(256), 0, st, a, workgroups);
+        return (int)CACTUS_HIP_OK;
+    };
+    unsigned n = 0;
+#define KV4_FEW(D, PACK) launch(attn_kv4_kernel<D, PACK>, kv4_vectors<D, PACK>(), kv4_per_cu<D, PACK>(), KV4_WAVES, &n)
+#define KV4_LAUNCH(D, W)                                                              \
+    (vectors <= (size_t)kv4_vectors<D, true>() ? KV4_FEW(D, true)                     \
+     : vectors <= PF_FROM                      ? KV4_FEW(D, false)                    \
+                                               : many(attn_kv4_prefill_kernel<D, W>, attn_kv4_join_kernel<D, W>, W))
+    rc = a.c.d == 64 ? KV4_LAUNCH(64, 8) : a.c.d == 128 ? KV4_LAUNCH(128, 8) : KV4_LAUNCH(256, 4);
 #undef KV4_LAUNCH
+#undef KV4_FEW
     if (rc) return rc;
     return check_launch("attention_kv4");
 }

@@ -182,6 +182,18 @@ def test_rows_and_masks(hip_ready, d, ps, S, window, sink, causal):
              stride=4 * d + 16)
 
 
+@pytest.mark.parametrize("d,G,lens,counts", [(64, 4, [700, 0, 333], [300, 5, 257]), (128, 1, [900, 130], [513, 1]),
+                                             (256, 3, [260, 41], [130, 41]), (128, 8, [1500], [40])])
+@pytest.mark.parametrize("window,sink,causal,scale", [(0, 0, True, 0.0), (100, 70, True, 0.3), (0, 0, False, -0.2)])
+def test_many_rows(hip_ready, d, G, lens, counts, window, sink, causal, scale):
+    """Several blocks of query vectors, key ranges that workgroups share, scores far apart, a negative scale."""
+    rng = np.random.default_rng(d + G + window)
+    c = Cache(hip_ready, 1, 2, d, 32, 80, len(lens), 50)
+    c.fill(rng, lens, scale=1.5)
+    q = (2 * rng.standard_normal((len(lens), max(counts), 2 * G, d))).astype(np.float16)
+    c.attend(q, range(len(lens)), counts, window=window, sink=sink, causal=causal, scale=scale)
+
+
 def test_long_decode_and_sharp_softmax(hip_ready):
     rng = np.random.default_rng(3)
     c = Cache(hip_ready, 1, 1, 128, 64, 40, 3, 34)
