@@ -635,7 +635,6 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_
 // product with ones, of the rounded weights that the outputs use.
 constexpr int PF_SLACK = 8;
 constexpr size_t PF_FROM = 32;   // more query vectors per KV head than this
-constexpr int PF_MIN = 4;        // stages of a stretch at least
 
 
 typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
@@ -701,8 +700,7 @@ struct PrefillLine {
             total += lane_u(upto, 63);
             longest = max(longest, __builtin_amdgcn_readlane(wave_scan_max((int)blocks), 63));
         }
-        return max(max((total + workgroups - 1) / workgroups, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1)),
-                   (uint32_t)PF_MIN);
+        return max((total + workgroups - 1) / workgroups, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1));
     }
     // the lane of the pair that stage `at` of the line belongs to
     __device__ int find(uint32_t at) {
@@ -728,6 +726,8 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
     constexpr int NQ = NT / 2;                       // 32-key parts of a stage
     __shared__ __align__(16) uint4 kf[2][NT][NG][64];          // K operands: [tile][group][lane]
     __shared__ __align__(16) uint4 vf[2][NT / 2][NB][64];      // V operands: [32 keys][16 dims][lane]
+    constexpr int TB = 18 * D;
+    __shared__ __align__(16) uint8_t raw_sh[W][TB];            // a wave's tile of the stage after the next, as it is stored
     __shared__ uint32_t nan_sh[2][KT];               // stage << 8 | value groups of a key that read as NaN
     __shared__ int any_sh[2];                        // the last stage (plus 1) that has such a key
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, h = lane >> 4;
@@ -758,8 +758,8 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         int page_first = 0, pages = -1;
         bool have_pages = false;
         auto key_of = [&](int i) { return KT * (i < sq.sinks ? i : sq.main0 + i - sq.sinks); };
-        // ---- the wave's tile of a stage (tile `wid`), in registers
-        uint32_t kraw[D / 32], kscl[NG], vraw[D / 32], vscl[D / 16];
+        // ---- the wave's tile of a stage (tile `wid`), to LDS
+        const uint32_t raw_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)&raw_sh[wid][0];
         uint32_t there = 0;          // tiles of that stage that have a page, a bit each
         auto fetch = [&](int i) {
             const int key0 = key_of(i), e0 = key0 >> c.ps_log2, e1 = (key0 + KT - 1) >> c.ps_log2;
@@ -781,16 +781,14 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                     there |= (uint32_t)kv4_page_ok(c, __builtin_amdgcn_readlane(pages, ((key0 + 16 * t) >> c.ps_log2) - page_first)) << t;
             }
             const uint8_t* p = kv4_tile(c, ok ? page : 0, head, (k0 & ((1 << c.ps_log2) - 1)) >> 4);
-            load_words(kraw, p + lane * (D / 8));
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // the last tile has been read
 #pragma unroll
-            for (int g = 0; g < NG; g++)                         // of key `col`
-                kscl[g] = *reinterpret_cast<const uint16_t*>(p + 8 * D + (((col >> 2) * NG + g) * 4 + (col & 3)) * 2);
-            load_words(vraw, p + 9 * D + lane * (D / 8));
-            load_words(vscl, p + 17 * D + h * (D / 4));          // of keys 4 h + i
+            for (int o = 0; o + 1024 <= TB; o += 1024) lds_dma<16>(p + 16 * lane + o, raw_lds + o);
+            if (16 * lane < TB % 1024) lds_dma<16>(p + 16 * lane + TB / 1024 * 1024, raw_lds + TB / 1024 * 1024);
         };
         // A NaN or infinite scale of a value group: the key is marked and the group
         // reads as 0 (0 times NaN would reach the rows that do not see the key)
-        auto mark = [&](int i) {
+        auto mark = [&](int i, uint32_t (&vscl)[D / 16]) {
             uint32_t bad = 0;        // an exponent of all ones carries into bits 15 and 31
 #pragma unroll
             for (int k = 0; k < D / 16; k++) bad |= (vscl[k] & 0x7C007C00u) + 0x04000400u;
@@ -814,24 +812,32 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                 }
             }
         };
-        // a quarter of the tile's codes to the operands of buffer `buf`: groups
-        // [g0, g1) of the keys, then of the values
-        auto put_keys = [&](int buf, int p0, int p1) {
+        // stage i's tile, once it has arrived, to the operands of buffer `buf`
+        auto put = [&](int i, int buf) {
+            wait_dma<0>();
+            const uint8_t* raw = &raw_sh[wid][0];
+            {
+                uint32_t x[D / 32];
+                load_words(x, raw + lane * (D / 8));
 #pragma unroll
-            for (int p = p0; p < p1; p++) {
-                const uint32_t x0 = kraw[2 * p], x1 = kraw[2 * p + 1];
-                const h16x2 sl = as_h2(kscl[2 * p] | kscl[2 * p] << 16);
-                const h16x2 sh = as_h2(kscl[2 * p + 1] | kscl[2 * p + 1] << 16);
-                kf[buf][wid][2 * p][lane] = make_uint4(low_values(x0, sl), low_values(x0 >> 8, sl), low_values(x1, sl),
-                                                       low_values(x1 >> 8, sl));
-                kf[buf][wid][2 * p + 1][lane] = make_uint4(high_values(x0, sh), high_values(x0 >> 8, sh),
-                                                           high_values(x1, sh), high_values(x1 >> 8, sh));
+                for (int p = 0; p < NG / 2; p++) {
+                    // scales of key `col`
+                    const uint16_t* s = reinterpret_cast<const uint16_t*>(raw + 8 * D) + ((col >> 2) * NG + 2 * p) * 4 + (col & 3);
+                    const h16x2 sl = as_h2(s[0] | (uint32_t)s[0] << 16), sh = as_h2(s[4] | (uint32_t)s[4] << 16);
+                    const uint32_t x0 = x[2 * p], x1 = x[2 * p + 1];
+                    kf[buf][wid][2 * p][lane] = make_uint4(low_values(x0, sl), low_values(x0 >> 8, sl), low_values(x1, sl),
+                                                           low_values(x1 >> 8, sl));
+                    kf[buf][wid][2 * p + 1][lane] = make_uint4(high_values(x0, sh), high_values(x0 >> 8, sh),
+                                                               high_values(x1, sh), high_values(x1 >> 8, sh));
+                }
             }
-        };
-        auto put_vals = [&](int buf, int g0, int g1) {
+            uint32_t x[D / 32], vscl[D / 16];        // scales of keys 4 h + i
+            load_words(x, raw + 9 * D + lane * (D / 8));
+            load_words(vscl, raw + 17 * D + h * (D / 4));
+            mark(i, vscl);
 #pragma unroll
-            for (int g = g0; g < g1; g++) {
-                const uint32_t s01 = vscl[2 * g], s23 = vscl[2 * g + 1], w = vraw[g];
+            for (int g = 0; g < NG; g++) {
+                const uint32_t s01 = vscl[2 * g], s23 = vscl[2 * g + 1], w = x[g];
                 const h16x2 se = as_h2(__builtin_amdgcn_perm(s23, s01, 0x05040100u));    // keys 4 h, 4 h + 2
                 const h16x2 so = as_h2(__builtin_amdgcn_perm(s23, s01, 0x07060302u));    // keys 4 h + 1, 4 h + 3
                 reinterpret_cast<uint2*>(&vf[buf][wid >> 1][2 * g][lane])[wid & 1] =
@@ -839,11 +845,6 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                 reinterpret_cast<uint2*>(&vf[buf][wid >> 1][2 * g + 1][lane])[wid & 1] =
                     make_uint2(high_values(w, se), high_values(w >> 8, so));
             }
-        };
-        // part n of m of all that
-        auto put = [&](int buf, int n, int m) {
-            if (m == 1 || n < m / 2) put_keys(buf, m == 1 ? 0 : NG / 2 * n / (m / 2), m == 1 ? NG / 2 : NG / 2 * (n + 1) / (m / 2));
-            if (m == 1 || n >= m / 2) put_vals(buf, m == 1 ? 0 : NG * (n - m / 2) / (m / 2), m == 1 ? NG : NG * (n + 1 - m / 2) / (m / 2));
         };
 
         // ---- this wave's vectors: lane's column in two blocks of 16
@@ -886,13 +887,10 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         // stage's values.  Operands are read from LDS a group of products ahead; the
         // barriers and groups keep the compiler from moving them together.
         constexpr int VG = 4, NVG = NB / VG;
-        auto stage = [&](int i, int buf, uint32_t there, bool more) {
+        auto stage = [&](int i, int buf, uint32_t there) {
             const int key0 = key_of(i);
             const bool active = wvec > 0 && (!a.causal || key0 <= last_pos);
-            if (!active) {
-                if (more) put(buf ^ 1, 0, 1);
-                return;
-            }
+            if (!active) return;
             f32x4 st[2][2][2];                        // [part parity][column block][tile]
             h16x8 pf[2], ka[NG], kb[NG], va[VG], vb2[VG];
             auto read_k = [&](int t, h16x8 (&to)[NG]) {
@@ -917,15 +915,23 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                 const bool whole = (there >> 2 * q & 3u) == 3u && k0 + 32 <= all &&
                                    (a.window == 0 || last_pos - k0 <= a.window || k0 + 32 <= a.sink);
                 if (!whole) {
+                    // a column sees keys below its upper limit and, under a window, from its
+                    // lower one on or below the sink (computed here: held over the
+                    // stages, the limits' registers spilled the accumulators)
+                    int k4 = k0 + 4 * h;
+                    asm volatile("" : "+v"(k4));
 #pragma unroll
-                    for (int cb = 0; cb < 2; cb++)
+                    for (int cb = 0; cb < 2; cb++) {
+                        const int hi = (a.causal ? min(pos[cb] + 1, sq.len) : sq.len) - k4;
+                        const int lo = a.window > 0 ? pos[cb] - a.window - k4 : -64, sink = a.sink - k4;
 #pragma unroll
                         for (int t = 0; t < 2; t++)
 #pragma unroll
                             for (int r = 0; r < 4; r++) {
-                                const bool sees = (there >> (2 * q + t) & 1) & kv4_sees(a, pos[cb], k0 + 16 * t + 4 * h + r, sq.len);
-                                s[cb][t][r] = sees ? s[cb][t][r] : -__builtin_inff();
+                                const int k = 16 * t + r;
+                                s[cb][t][r] = (there >> (2 * q + t) & 1) & (k < hi) & ((k >= lo) | (k < sink)) ? s[cb][t][r] : -__builtin_inff();
                             }
+                    }
                 }
                 float top[2];
 #pragma unroll
@@ -992,26 +998,20 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                     __builtin_amdgcn_sched_group_barrier(0x100, VG, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                // B: outputs of part q, the next stage's values
+                // B: outputs of part q
 #pragma unroll
                 for (int n = 0; n < NVG; n++) {
                     h16x8 (&cur)[VG] = n & 1 ? vb2 : va;
                     h16x8 (&nxt)[VG] = n & 1 ? va : vb2;
                     if (n + 1 < NVG) read_v(q, n + 1, nxt);
                     else if (q + 2 < NQ) read_k(2 * q + 4, ka);
-                    __builtin_amdgcn_sched_barrier(0x606);      // vector and scalar instructions and LDS writes may pass
+                    __builtin_amdgcn_sched_barrier(0);
                     values(n, cur);
-                    if (n == 0) put(buf ^ 1, q, NQ);
                     if (n + 1 == NVG) {
 #pragma unroll
                         for (int cb = 0; cb < 2; cb++) lsum[cb] = mfma16(ones, pf[cb], lsum[cb]);
                     }
-#pragma unroll
-                    for (int u = 0; u < 2 * VG; u++) {
-                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
-                    }
-                    __builtin_amdgcn_sched_barrier(0x606);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 if (q + 1 < NQ) check(q + 1);
@@ -1037,21 +1037,26 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         for (int e = tid; e < 2 * KT; e += 64 * W) (&nan_sh[0][0])[e] = 0;
         if (tid < 2) any_sh[tid] = 0;
         __syncthreads();
-        if (i0 < i1) {
-            fetch(i0);
-            mark(i0);
-            put(i0 & 1, 0, 1);
-            uint32_t now = there;
-            fetch(min(i0 + 1, i1 - 1));
+        // Iteration i writes stage i + 1's operands and uses stage i's (from i0 - 1 on:
+        // one copy of the code).  Two waves share a SIMD's units: the first four prepare
+        // the next stage before their products, the others after theirs, so that one
+        // wave's vector instructions run beside the other's matrix ones.
+        uint32_t now = 0;
+        if (i0 < i1) fetch(i0);
+#pragma unroll 1
+        for (int i = i0 - 1; i < i1; i++) {
+            const uint32_t next = there;
+            auto prepare = [&]() {
+                if (i + 1 < i1) {
+                    put(i + 1, (i + 1) & 1);
+                    if (i + 2 < i1) fetch(i + 2);
+                }
+            };
+            if (wid < 4) prepare();
+            if (i >= i0) stage(i, i & 1, now);
+            if (wid >= 4) prepare();
+            now = next;
             __syncthreads();
-            for (int i = i0; i < i1; i++) {
-                const uint32_t next = there;
-                if (i + 1 < i1) mark(i + 1);
-                stage(i, i & 1, now, i + 1 < i1);
-                fetch(min(i + 2, i1 - 1));
-                now = next;
-                __syncthreads();
-            }
         }
 
         // ---- outputs, or this workgroup's part of them
