@@ -141,21 +141,20 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
 }
 
 // ------------------------------------------------------------ few rows
-// The work is a line of block steps (KV4_BLOCK keys of one unit: a request's
+// The work is a line of block steps (32 keys per wave of one unit: a request's
 // KV head and up to 16 query vectors), unit after unit, request after
 // request; each workgroup takes an equal stretch of it, whatever the lengths
 // of the sequences are.  A unit that lies in one stretch is written at once;
 // one that several workgroups share is written as partial (maximum, sum,
 // output) to the workspace, and the last of them to finish joins the parts
 // in their order.
-constexpr int KV4_WAVES = 4;
-constexpr int KV4_BLOCK = KV4_STEP * KV4_WAVES;   // a wave takes a step of 32 keys
 constexpr int KV4_PARTS = 128;                    // a unit's stretches at most
 constexpr size_t KV4_COUNTERS = 4096;             // bytes: one counter per workgroup
 
 // block steps of a unit (one at least: a request without tokens gets its zeros)
+template <int W>
 __device__ __forceinline__ uint32_t unit_blocks(const Kv4Seq& s) {
-    return (uint32_t)max(1, (s.steps + KV4_WAVES - 1) / KV4_WAVES);
+    return (uint32_t)max(1, (s.steps + W - 1) / W);
 }
 
 // Query vectors of a unit.  PACK: a vector takes NG = d / 32 of the product's
@@ -167,9 +166,14 @@ template <int D, bool PACK>
 constexpr int kv4_vectors() { return PACK ? 16 / (D / 32) : 16; }
 // Steps of a wave's ring in LDS, workgroups per CU
 template <int D, bool PACK>
-constexpr int kv4_ring() { return D == 64 ? 4 : PACK ? 2 : 3; }
+constexpr int kv4_ring() { return D == 64 ? 4 : PACK || D == 256 ? 2 : 3; }
+// Waves of a workgroup: with 16 vectors, twice the keys per part, whose joining
+// costs as much as the keys (16 rows at 4096 keys, 16 / 8 heads of 128: 24 us with
+// four waves, 14 with eight; one row 9.2 against 10.4)
 template <int D, bool PACK>
-constexpr int kv4_per_cu() { return D == 256 ? (PACK ? 2 : 1) : PACK ? 4 : 2; }
+constexpr int kv4_waves() { return PACK ? 4 : 8; }
+template <int D, bool PACK>
+constexpr int kv4_per_cu() { return PACK ? (D == 256 ? 2 : 4) : D == 64 ? 2 : 1; }
 
 // a times half I of w plus c, one instruction (v_fma_mix_f32; as a builtin, so that
 // the compiler knows what waits for the matrix and transcendental units' results)
@@ -205,16 +209,17 @@ __device__ __forceinline__ void tile_dma(const void* src, uint32_t lds_addr) {
 }
 
 template <int D, bool PACK>
-__global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_kv4_kernel(Kv4AttnArgs a) {
+__global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PACK>() * kv4_waves<D, PACK>() / 4)) attn_kv4_kernel(Kv4AttnArgs a) {
+    constexpr int W = kv4_waves<D, PACK>();
     constexpr int NG = D / 32, NB = D / 16, OS = D + 4, QV = kv4_vectors<D, PACK>();
     constexpr int SG = PACK ? 1 : NG;                          // scale groups of a lane
     constexpr int TB = 18 * D, SLOT = 2 * TB;                  // bytes of a tile and of a step
     constexpr int NI = 2 * ((TB + 1023) / 1024);               // LDS loads of a step
     constexpr int R = kv4_ring<D, PACK>();
-    static_assert(R * SLOT >= QV * OS * 4 && KV4_WAVES * R * SLOT >= 64 * KV4_WAVES * 24,
+    static_assert(R * SLOT >= QV * OS * 4 && W * R * SLOT >= 64 * W * 24,
                   "the ring holds a wave's sums, then the joined parts'");
-    __shared__ __align__(16) uint8_t ring[KV4_WAVES][R][SLOT];
-    __shared__ float m_sh[KV4_WAVES][QV], l_sh[KV4_WAVES][QV];
+    __shared__ __align__(16) uint8_t ring[W][R][SLOT];
+    __shared__ float m_sh[W][QV], l_sh[W][QV];
     __shared__ int last_sh;
     float (*o_sh)[R * SLOT / 4] = reinterpret_cast<float (*)[R * SLOT / 4]>(&ring[0][0][0]);   // [wave][QV][OS]
     float* j_sh = reinterpret_cast<float*>(&ring[0][0][0]);    // [threads][6]: sums of parts
@@ -237,7 +242,7 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_
             r_slot = s.slot;
             r_len = s.len;
             r_rows = s.rows;
-            r_blocks = s.rows > 0 ? unit_blocks(s) : 0;
+            r_blocks = s.rows > 0 ? unit_blocks<W>(s) : 0;
             r_cost = r_blocks * (uint32_t)((s.rows * a.G + QV - 1) / QV) * (uint32_t)c.Hkv;
         }
         r_upto = wave_scan_add(r_cost);
@@ -314,16 +319,15 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_
             return there;
         };
         // ---- this wave's steps, the first R - 1 on their way
-        const int last = min(sq.steps, (int)(s0 + nblk) * KV4_WAVES), i0 = (int)s0 * KV4_WAVES + wid;
-        const int n = i0 < last ? (last - i0 + KV4_WAVES - 1) / KV4_WAVES : 0;
+        const int last = min(sq.steps, (int)(s0 + nblk) * W), i0 = (int)s0 * W + wid;
+        const int n = i0 < last ? (last - i0 + W - 1) / W : 0;
         uint32_t there = 0;          // two bits per slot of the ring
         auto put = [&](int k) {
             const int s = k % R;
-            there = (there & ~(3u << 2 * s)) | fetch(i0 + KV4_WAVES * k, s) << 2 * s;
+            there = (there & ~(3u << 2 * s)) | fetch(i0 + W * k, s) << 2 * s;
         };
-#pragma unroll
-        for (int k = 0; k < R - 1; k++)
-            if (k < n) put(k);
+#pragma unroll 1
+        for (int k = 0; k < min(R - 1, n); k++) put(k);
 
         // ---- this lane's vector: row, query head and position
         const int vec = v0 + qi, row = vec / a.G;
@@ -457,6 +461,7 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_
                 acc[2 * g + 1] = mfma16(high_codes(v[0][g], v[1][g]), pf[PACK ? 0 : g], acc[2 * g + 1]);
             }
         };
+#pragma unroll 1
         for (int k = 0; k < n; k++) {
             if (k + R - 1 < n) {
                 put(k + R - 1);
@@ -468,7 +473,7 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_
             } else {
                 wait_dma<0>();
             }
-            const int key0 = key_of(i0 + KV4_WAVES * k), s = k % R;
+            const int key0 = key_of(i0 + W * k), s = k % R;
             const uint32_t ok = there >> 2 * s & 3u;
             const bool whole = ok == 3 && key0 + KV4_STEP <= all &&
                                (a.window == 0 || last_pos - key0 <= a.window || key0 + KV4_STEP <= a.sink);
@@ -516,15 +521,15 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_
                 make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
         };
         const int nquad = nvec * (D / 4);
-        for (int e = et; e < nquad; e += 64 * KV4_WAVES) {
+        for (int e = et; e < nquad; e += 64 * W) {
             const int cc = e / (D / 4), d = e % (D / 4) * 4;
             float mw = m_sh[0][cc];
 #pragma unroll
-            for (int w = 1; w < KV4_WAVES; w++) mw = __builtin_fmaxf(mw, m_sh[w][cc]);
+            for (int w = 1; w < W; w++) mw = __builtin_fmaxf(mw, m_sh[w][cc]);
             f32x4 num = {0, 0, 0, 0};
             float den = 0.0f;
 #pragma unroll
-            for (int w = 0; w < KV4_WAVES; w++) {
+            for (int w = 0; w < W; w++) {
                 // without a maximum the wave's sums are zero, or NaN from a NaN score
                 const float f = m_sh[w][cc] > -__builtin_inff() ? exp2_fast(m_sh[w][cc] - mw) : 1.0f;
                 const f32x4 y = *reinterpret_cast<const f32x4*>(&o_sh[w][cc * OS + d]);
@@ -553,8 +558,8 @@ __global__ void __launch_bounds__(64 * KV4_WAVES, (kv4_per_cu<D, PACK>())) attn_
                 // a thread takes a quad of dims and every (threads / quads)-th part,
                 // eight parts' loads at a time: 4096 keys in 32 parts take one round of
                 // loads (a part after the other: 4 us more)
-                const int share = max(1, 64 * KV4_WAVES / nquad);
-                for (int e0 = 0; e0 < nquad; e0 += 64 * KV4_WAVES) {
+                const int share = max(1, 64 * W / nquad);
+                for (int e0 = 0; e0 < nquad; e0 += 64 * W) {
                     const int e = e0 + (share > 1 ? et % nquad : et), pl = share > 1 ? et / nquad : 0;
                     const bool in = e < nquad && pl < share;
                     const int cc = in ? e / (D / 4) : 0, d = in ? e % (D / 4) * 4 : 0;
@@ -1170,7 +1175,7 @@ size_t cactus_hip_attention_kv4_workspace(const cactus_hip_kv4_cache* cache, siz
                                           size_t num_q_heads) {
     if (kv4_view(cache, 0, "attention_kv4_workspace", nullptr)) return 0;
     const size_t vectors = seq_len * (num_q_heads / cache->kv_heads);
-    const size_t few = (size_t)512 * 2 * 16;                  // (packed: 1024 workgroups of 4 vectors)
+    const size_t few = (size_t)512 * 2 * 16;                  // (packed: 1024 workgroups of 8 vectors at most)
     const size_t many = (size_t)256 * 2 * (cache->head_dim == 256 ? 128 : 256);
     (void)batch;
     return KV4_COUNTERS + (vectors > PF_FROM ? many : few) * (cache->head_dim + 4) * 4;
@@ -1214,7 +1219,7 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + KV4_COUNTERS);
     const hipStream_t st = as_stream(stream);
     // block steps at most, by what the tables can hold
-    const size_t blocks = (cache->max_pages * cache->page_size + KV4_BLOCK - 1) / KV4_BLOCK;
+    const size_t blocks = (cache->max_pages * cache->page_size + 127) / 128;    // (of 128 keys or more)
     const size_t vectors = seq_len * G;
     auto launch = [&](auto kernel, int per_unit, int per_cu, int waves, unsigned* workgroups) {
         const size_t units = batch * cache->kv_heads * ceil_div(vectors, per_unit);
@@ -1233,7 +1238,7 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
         return (int)CACTUS_HIP_OK;
     };
     unsigned n = 0;
-#define KV4_FEW(D, PACK) launch(attn_kv4_kernel<D, PACK>, kv4_vectors<D, PACK>(), kv4_per_cu<D, PACK>(), KV4_WAVES, &n)
+#define KV4_FEW(D, PACK) launch(attn_kv4_kernel<D, PACK>, kv4_vectors<D, PACK>(), kv4_per_cu<D, PACK>(), kv4_waves<D, PACK>(), &n)
 #define KV4_LAUNCH(D, W)                                                              \
     (vectors <= (size_t)kv4_vectors<D, true>() ? KV4_FEW(D, true)                     \
      : vectors <= PF_FROM                      ? KV4_FEW(D, false)                    \

@@ -7,145 +7,232 @@
 
 namespace cactus_hip {
 
-typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+// ------------------------------------------------------------ append and read
+// A wave takes the keys or the values of one 16-token tile of a KV head, lane 16 h +
+// token with dims 8 h to 8 h + 7 of each 32-dim group.  For the keys that is the lane
+// order of the page.  For the values the page holds, per dim, the four tokens of a
+// quad of lanes: the quads transpose 4 x 4 bytes in registers, so that pages are
+// read and written 4 bytes per group and lane, contiguous over the groups.
+//
+// Per value: x / s to the nearest integer, ties to even.  x has 11 significant
+// bits and (k + 1/2) s at most 12, so x / s is either exactly k + 1/2 or at least
+// 2^-13 away from it; x times the FP32 reciprocal of s is within 2^-20 of x / s, and
+// rounded to a multiple of 2^-14 it falls on the same side, ties included (an
+// exact division took twice the instructions).
+//
+// Bound by memory for prompts, by the chain of loads (slot, length, page, row) for
+// single tokens.
 
-// ------------------------------------------------------------ append
-// Scale of a 32-dim group from the largest magnitude: a / 7 rounded to 8
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+
+// Scale of a group from the bits of its largest magnitude: a / 7 rounded to 8
 // significant bits (bf16) and then to fp16, which only rounds again where the
-// scale is an fp16 subnormal.  NaN for a group with a NaN or an infinity.
-__device__ __forceinline__ uint16_t kv4_scale(float amax, bool bad) {
-    const float q = amax / 7.0f;
+// scale is an fp16 subnormal.  NaN for a NaN or an infinity.
+__device__ __forceinline__ uint16_t kv4_scale(uint32_t abits) {
+    const float q = h2f((uint16_t)abits) / 7.0f;
     uint32_t b = __builtin_bit_cast(uint32_t, q);
     b = (b + 0x7FFFu + ((b >> 16) & 1u)) & 0xFFFF0000u;   // finite: to nearest, ties to even
-    return bad ? (uint16_t)0x7E00u : f2h(bits_f(b));
+    return abits >= 0x7C00u ? (uint16_t)0x7E00u : f2h(bits_f(b));
 }
-// code + 8 of x under scale s
-__device__ __forceinline__ uint32_t kv4_code(float x, float s) {
-    const float c = __builtin_rintf(x / s);
-    const float t = __builtin_fminf(__builtin_fmaxf(c, -7.0f), 7.0f);
-    return (s > 0.0f) ? (uint32_t)((int)t + 8) : 8u;   // s NaN or 0: code 0
+// code + 8 in the low byte of the result; inv: 1 / s, 0 where every code is 0
+__device__ __forceinline__ uint32_t kv4_code(uint16_t x, float inv) {
+    const float v = (h2f(x) * inv + 768.0f) - 768.0f;    // a multiple of 2^-14 (|v| < 16)
+    const float w = __builtin_amdgcn_fmed3f(v, -7.0f, 7.0f);
+    return __builtin_bit_cast(uint32_t, w + 12582920.0f);  // 3 2^22 + 8: the integer in the low bits
 }
-
-// One wave per (request, KV head, 16-key tile): lane 16 h + key takes dims 8 h
-// to 8 h + 7 of each 32-dim group of its key, which are the K codes of the
-// lane of that number in the page; a group's maximum meets over the four
-// lanes of the key.
-template <int D>
-__global__ void __launch_bounds__(64) kv4_append_kernel(Kv4View c, const int32_t* seqs, const int32_t* counts,
-                                                        const uint16_t* k, const uint16_t* v, int seq_len, size_t stride) {
-    constexpr int NG = D / 32;
-    const int lane = threadIdx.x, key = lane & 15, h = lane >> 4;
-    const int head = blockIdx.y, req = blockIdx.z;
-    if (c.state[KV4_STATUS] != 0) return;
-    const int slot = kv4_slot(c, seqs, req);
-    if (slot < 0) return;
-    const int len = kv4_len(c, slot), first = len - kv4_count(counts, req, seq_len);   // (negative: rows without a token)
-    const int lo = max(first, 0);
-    const int pos0 = (lo & ~15) + 16 * (int)blockIdx.x;      // first position of this wave's tile
-    if (pos0 >= len) return;
-    const int page = c.table[(size_t)slot * c.max_pages + (pos0 >> c.ps_log2)];
-    if (!kv4_page_ok(c, page)) return;
-    uint8_t* tile = kv4_tile(c, page, head, (pos0 & ((1 << c.ps_log2) - 1)) >> 4);
-    const int pos = pos0 + key;
-    const bool mine = pos >= lo && pos < len;
-    const size_t row = ((size_t)req * seq_len + (mine ? pos - first : 0)) * stride + (size_t)head * D;
-    uint8_t codes[NG][8];
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(b, a, 0x0C0C0400u) | __builtin_amdgcn_perm(d, c, 0x04000C0Cu);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+// byte j of lane i's result: byte i of lane j's v, within each quad of lanes
+__device__ __forceinline__ uint32_t quad_transpose(uint32_t v, int i) {
+    // bytes (0, 1) and (2, 3) change places between lanes 1 apart, then pairs between lanes 2 apart
+    uint32_t o = quad<0xB1>(v);
+    v = i & 1 ? __builtin_amdgcn_perm(v, o, 0x07030501u) : __builtin_amdgcn_perm(o, v, 0x06020400u);
+    o = quad<0x4E>(v);
+    return i & 2 ? __builtin_amdgcn_perm(v, o, 0x07060302u) : __builtin_amdgcn_perm(o, v, 0x05040100u);
+}
+// N dwords at p, 4 N bytes aligned up to 16
+template <int N>
+__device__ __forceinline__ void load_dwords(uint32_t (&w)[N], const uint8_t* p) {
+    if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x, w[1] = u.y;
+    } else {
 #pragma unroll
-    for (int kv = 0; kv < 2; kv++) {
-        const uint16_t* src = (kv ? v : k) + row;
-        uint8_t* out = tile + kv * 9 * D;
-        uint16_t* scales = reinterpret_cast<uint16_t*>(out + 8 * D);
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            const h16x8 x = *reinterpret_cast<const h16x8*>(src + 32 * g + 8 * h);
-            float amax = 0.0f;
-            int bad = 0;
-#pragma unroll
-            for (int t = 0; t < 8; t++) {
-                const float a = __builtin_fabsf((float)x[t]);
-                bad |= !(a <= 65504.0f);
-                amax = __builtin_fmaxf(amax, a);
-            }
-            amax = __builtin_fmaxf(amax, __shfl_xor(amax, 16, 64));
-            amax = __builtin_fmaxf(amax, __shfl_xor(amax, 32, 64));
-            bad |= __shfl_xor(bad, 16, 64);
-            bad |= __shfl_xor(bad, 32, 64);
-            const uint16_t sb = kv4_scale(amax, bad != 0);
-            const float s = h2f(sb);
-#pragma unroll
-            for (int t = 0; t < 8; t++) codes[g][t] = (uint8_t)kv4_code((float)x[t], s);
-            if (mine && h == (g & 3)) scales[((key >> 2) * NG + g) * 4 + (key & 3)] = sb;
-        }
-        if (kv == 0) {
-            // byte 8 p + t: groups 2 p and 2 p + 1
-#pragma unroll
-            for (int p = 0; p < NG / 2; p++) {
-                uint64_t w = 0;
-#pragma unroll
-                for (int t = 0; t < 8; t++)
-                    w |= (uint64_t)(codes[2 * p][t] | codes[2 * p + 1][t] << 4) << (8 * t);
-                if (mine) *reinterpret_cast<uint64_t*>(out + lane * (D / 8) + 8 * p) = w;
-            }
-        } else {
-            // lane h < 2 holds dims x = 8 h + t of each group, its partner h + 2 dims x + 16
-#pragma unroll
-            for (int g = 0; g < NG; g++)
-#pragma unroll
-                for (int t = 0; t < 8; t++) {
-                    const int hi = __shfl_xor((int)codes[g][t], 32, 64);
-                    if (mine && h < 2)
-                        out[(key >> 2) * 2 * D + (8 * h + t) * (D / 8) + 4 * g + (key & 3)] =
-                            (uint8_t)(codes[g][t] | hi << 4);
-                }
+        for (int k = 0; k < N / 4; k++) {
+            const uint4 u = reinterpret_cast<const uint4*>(p)[k];
+            w[4 * k] = u.x, w[4 * k + 1] = u.y, w[4 * k + 2] = u.z, w[4 * k + 3] = u.w;
         }
     }
 }
+template <int N>
+__device__ __forceinline__ void store_dwords(uint8_t* p, const uint32_t (&w)[N]) {
+    if constexpr (N == 2) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N / 4; k++)
+            reinterpret_cast<uint4*>(p)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    }
+}
 
-// ------------------------------------------------------------ read
-// One wave per (request, KV head, 16-key tile), lane = 16 h + key as above.
-// code * scale is an exact fp16 value.
+// grid (tile, KV head, request), two waves: keys and values
 template <int D>
-__global__ void __launch_bounds__(64) kv4_read_kernel(Kv4View c, const int32_t* seqs, const int32_t* starts,
-                                                      const int32_t* counts, uint16_t* k, uint16_t* v, int seq_len) {
+__global__ void __launch_bounds__(128) kv4_append_kernel(Kv4View c, const int32_t* seqs, const int32_t* counts,
+                                                         const uint16_t* k, const uint16_t* v, int seq_len, size_t stride) {
     constexpr int NG = D / 32;
-    const int lane = threadIdx.x, key = lane & 15, h = lane >> 4;
+    const int lane = threadIdx.x & 63, key = lane & 15, h = lane >> 4, i = lane & 3;
+    const bool vals = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) != 0;
     const int head = blockIdx.y, req = blockIdx.z;
+    const int status = c.state[KV4_STATUS];
     const int slot = kv4_slot(c, seqs, req);
-    if (slot < 0) return;
+    if (slot < 0 || status != 0) return;
+    const int len = kv4_len(c, slot), first = len - kv4_count(counts, req, seq_len);   // (negative: rows without a token)
+    const int lo = max(first, 0);
+    const int pos0 = (lo & ~15) + 16 * (int)blockIdx.x;      // first position of this tile
+    if (pos0 >= len) return;
+    const int pos = pos0 + key;
+    const bool mine = pos >= lo && pos < len;
+    const uint16_t* src = (vals ? v : k) + ((size_t)req * seq_len + (mine ? pos - first : lo - first)) * stride +
+                          (size_t)head * D + 8 * h;
+    uint4 x[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) x[g] = *reinterpret_cast<const uint4*>(src + 32 * g);
+    const int page = c.table[(size_t)slot * c.max_pages + (pos0 >> c.ps_log2)];
+    if (!kv4_page_ok(c, page)) return;
+    uint8_t* out = kv4_tile(c, page, head, (pos0 & ((1 << c.ps_log2) - 1)) >> 4) + (vals ? 9 * D : 0);
+
+    // the groups' largest magnitudes, as fp16 bits (a NaN's or an infinity's are above every number's)
+    uint32_t amax[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const uint32_t m = 0x7FFF7FFFu;
+        u16x2 y = __builtin_bit_cast(u16x2, x[g].x & m);
+        y = __builtin_elementwise_max(y, __builtin_bit_cast(u16x2, x[g].y & m));
+        y = __builtin_elementwise_max(y, __builtin_bit_cast(u16x2, x[g].z & m));
+        y = __builtin_elementwise_max(y, __builtin_bit_cast(u16x2, x[g].w & m));
+        amax[g] = max((uint32_t)y[0], (uint32_t)y[1]);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; g++) amax[g] = max(amax[g], (uint32_t)__shfl_xor((int)amax[g], 16, 64));
+#pragma unroll
+    for (int g = 0; g < NG; g++) amax[g] = max(amax[g], (uint32_t)__shfl_xor((int)amax[g], 32, 64));
+    uint32_t c0[NG], c1[NG];                                 // codes of dims 0-3 and 4-7, a byte each
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const uint16_t sb = kv4_scale(amax[g]);
+        const float s = h2f(sb), inv = s > 0.0f ? 1.0f / s : 0.0f;      // (NaN: codes 0)
+        // (a NaN or infinite value times 0 is NaN: its code is 0 too)
+        const bool zero = !(s > 0.0f);
+        const uint32_t w[4] = {x[g].x, x[g].y, x[g].z, x[g].w};
+        uint32_t u[8];
+#pragma unroll
+        for (int t = 0; t < 8; t++) u[t] = kv4_code((uint16_t)(t & 1 ? w[t / 2] >> 16 : w[t / 2]), inv);
+        c0[g] = zero ? 0x08080808u : low_bytes(u[0], u[1], u[2], u[3]);
+        c1[g] = zero ? 0x08080808u : low_bytes(u[4], u[5], u[6], u[7]);
+        if (mine && h == (g & 3))
+            reinterpret_cast<uint16_t*>(out + 8 * D)[((key >> 2) * NG + g) * 4 + (key & 3)] = sb;
+    }
+    if (!vals) {
+        uint32_t b[NG];
+#pragma unroll
+        for (int p = 0; p < NG / 2; p++) {
+            b[2 * p] = c0[2 * p] | c0[2 * p + 1] << 4;
+            b[2 * p + 1] = c1[2 * p] | c1[2 * p + 1] << 4;
+        }
+        if (mine) store_dwords(out + lane * (D / 8), b);
+        return;
+    }
+    // lanes h and h + 2 hold dims x and x + 16, which share a byte: lane h < 2 takes
+    // x = 8 h to 8 h + 3, lane h + 2 the four dims behind them
+    uint32_t b[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const uint32_t got = (uint32_t)__shfl_xor((int)(h < 2 ? c1[g] : c0[g]), 32, 64);
+        b[g] = h < 2 ? c0[g] | got << 4 : got | c1[g] << 4;
+    }
+    const int x0 = 8 * (h & 1) + (h < 2 ? 0 : 4);
+    const bool whole = pos0 >= lo && pos0 + 16 <= len;       // (the same for the wave)
+    if (whole) {
+#pragma unroll
+        for (int g = 0; g < NG; g++) b[g] = quad_transpose(b[g], i);
+        store_dwords(out + (key >> 2) * 2 * D + (x0 + i) * (D / 8), b);
+    } else if (mine) {
+        // other tokens of the tile stay: a byte at a time
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                out[(key >> 2) * 2 * D + (x0 + t) * (D / 8) + 4 * g + i] = (uint8_t)(b[g] >> (8 * t));
+    }
+}
+
+// four codes (a byte each, low nibble: code + 8) times s, an exact fp16 value
+__device__ __forceinline__ uint2 kv4_values(uint32_t b, h16x2 s) {
+    const h16x2 bias = {(_Float16)1032.0f, (_Float16)1032.0f};
+    const h16x2 y0 = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - bias;
+    const h16x2 y1 = __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - bias;
+    return make_uint2(__builtin_bit_cast(uint32_t, y0 * s), __builtin_bit_cast(uint32_t, y1 * s));
+}
+
+template <int D>
+__global__ void __launch_bounds__(128) kv4_read_kernel(Kv4View c, const int32_t* seqs, const int32_t* starts,
+                                                       const int32_t* counts, uint16_t* k, uint16_t* v, int seq_len) {
+    constexpr int NG = D / 32;
+    const int lane = threadIdx.x & 63, key = lane & 15, h = lane >> 4, i = lane & 3;
+    const bool vals = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) != 0;
+    const int head = blockIdx.y, req = blockIdx.z;
+    uint16_t* dst = vals ? v : k;
+    const int slot = kv4_slot(c, seqs, req);
+    if (slot < 0 || !dst) return;
     const int len = kv4_len(c, slot), m = kv4_count(counts, req, seq_len);
     const int first = starts ? starts[req] : len - m;   // may lie outside the slot's tokens
     const int64_t end64 = (int64_t)first + m;
     const int end = end64 < len ? (int)end64 : len;
     const int lo = max(first, 0);
-    const int pos0 = (lo & ~15) + 16 * (int)blockIdx.x;
-    if (pos0 >= end) return;
+    const int64_t pos64 = (int64_t)(lo & ~15) + 16 * (int64_t)blockIdx.x;
+    if (pos64 >= end) return;
+    const int pos0 = (int)pos64;
     const int page = c.table[(size_t)slot * c.max_pages + (pos0 >> c.ps_log2)];
     if (!kv4_page_ok(c, page)) return;
-    const uint8_t* tile = kv4_tile(c, page, head, (pos0 & ((1 << c.ps_log2) - 1)) >> 4);
-    const int pos = pos0 + key;
-    if (pos < lo || pos >= end) return;
-    const size_t row = (((size_t)req * seq_len + (size_t)(pos - first)) * c.Hkv + head) * D;
+    const uint8_t* in = kv4_tile(c, page, head, (pos0 & ((1 << c.ps_log2) - 1)) >> 4) + (vals ? 9 * D : 0);
+    uint16_t s[NG];
 #pragma unroll
-    for (int kv = 0; kv < 2; kv++) {
-        uint16_t* dst = kv ? v : k;
-        if (!dst) continue;
-        const uint8_t* in = tile + kv * 9 * D;
-        const uint16_t* scales = reinterpret_cast<const uint16_t*>(in + 8 * D);
+    for (int g = 0; g < NG; g++) s[g] = reinterpret_cast<const uint16_t*>(in + 8 * D)[((key >> 2) * NG + g) * 4 + (key & 3)];
+    uint32_t c0[NG], c1[NG];                                 // codes of dims 0-3 and 4-7, low nibbles
+    if (!vals) {
+        uint32_t b[NG];
+        load_dwords(b, in + lane * (D / 8));
+#pragma unroll
+        for (int p = 0; p < NG / 2; p++) {
+            c0[2 * p] = b[2 * p] & 0x0F0F0F0Fu;
+            c1[2 * p] = b[2 * p + 1] & 0x0F0F0F0Fu;
+            c0[2 * p + 1] = (b[2 * p] >> 4) & 0x0F0F0F0Fu;
+            c1[2 * p + 1] = (b[2 * p + 1] >> 4) & 0x0F0F0F0Fu;
+        }
+    } else {
+        const uint8_t* at = in + (key >> 2) * 2 * D + (8 * (h & 1) + i) * (D / 8);
+        load_dwords(c0, at);
+        load_dwords(c1, at + 4 * (D / 8));
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            const float s = h2f(scales[((key >> 2) * NG + g) * 4 + (key & 3)]);
-            h16x8 y;
-#pragma unroll
-            for (int t = 0; t < 8; t++) {
-                // dim 32 g + 8 h + t
-                const int x = 8 * (h & 1) + t;
-                const int byte = kv == 0 ? in[lane * (D / 8) + 8 * (g >> 1) + t]
-                                         : in[(key >> 2) * 2 * D + x * (D / 8) + 4 * g + (key & 3)];
-                const int up = kv == 0 ? (g & 1) : (h >> 1);
-                y[t] = (_Float16)((float)(((byte >> (4 * up)) & 15) - 8) * s);
-            }
-            *reinterpret_cast<h16x8*>(dst + row + 32 * g + 8 * h) = y;
+            c0[g] = (quad_transpose(c0[g], i) >> (h & 2 ? 4 : 0)) & 0x0F0F0F0Fu;
+            c1[g] = (quad_transpose(c1[g], i) >> (h & 2 ? 4 : 0)) & 0x0F0F0F0Fu;
         }
+    }
+    const int pos = pos0 + key;
+    if (pos < lo || pos >= end) return;
+    uint16_t* row = dst + (((size_t)req * seq_len + (size_t)(pos - first)) * c.Hkv + head) * D + 8 * h;
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const h16x2 ss = {hbits(s[g]), hbits(s[g])};
+        const uint2 y0 = kv4_values(c0[g], ss), y1 = kv4_values(c1[g], ss);
+        *reinterpret_cast<uint4*>(row + 32 * g) = make_uint4(y0.x, y0.y, y1.x, y1.y);
     }
 }
 
@@ -566,20 +653,20 @@ __global__ void kv4_copy_kernel(Kv4View c, const int32_t* src, const int32_t* ds
 
 // ------------------------------------------------------------ host side
 int kv4_view(const cactus_hip_kv4_cache* c, size_t layer, const char* what, Kv4View* out) {
-    const std::string w(what);
-    CH_REQUIRE(c, w + ": null cache");
-    CH_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, w + ": head_dim is 64, 128 or 256");
+    using std::string;
+    CH_REQUIRE(c, string(what) + ": null cache");
+    CH_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, string(what) + ": head_dim is 64, 128 or 256");
     CH_REQUIRE(c->page_size >= 16 && c->page_size <= 4096 && (c->page_size & (c->page_size - 1)) == 0,
-               w + ": page_size is a power of two from 16 to 4096");
-    CH_REQUIRE(c->layers >= 1 && c->layers < 65535 && c->kv_heads >= 1 && c->kv_heads <= 4096, w + ": layers or kv_heads out of range");
+               string(what) + ": page_size is a power of two from 16 to 4096");
+    CH_REQUIRE(c->layers >= 1 && c->layers < 65535 && c->kv_heads >= 1 && c->kv_heads <= 4096, string(what) + ": layers or kv_heads out of range");
     CH_REQUIRE(c->num_pages >= 1 && c->num_pages < (1u << 30) && c->max_seqs >= 1 && c->max_seqs <= KV4_MAX_SEQS &&
                    c->max_pages >= 1 && c->max_pages < (1u << 30) / c->page_size &&
                    c->max_seqs * c->max_pages < (1u << 31),
-               w + ": num_pages, max_seqs or max_pages out of range");
+               string(what) + ": num_pages, max_seqs or max_pages out of range");
     if (!out) return CACTUS_HIP_OK;
-    CH_REQUIRE(c->pages && c->table && c->lens && c->refs && c->state, w + ": null buffer");
-    CH_REQUIRE(((uintptr_t)c->pages & 127) == 0, w + ": pages is not 128-byte aligned");
-    CH_REQUIRE(layer < c->layers, w + ": no such layer");
+    CH_REQUIRE(c->pages && c->table && c->lens && c->refs && c->state, string(what) + ": null buffer");
+    CH_REQUIRE(((uintptr_t)c->pages & 127) == 0, string(what) + ": pages is not 128-byte aligned");
+    CH_REQUIRE(layer < c->layers, string(what) + ": no such layer");
     Kv4View v;
     v.table = c->table;
     v.lens = c->lens;
@@ -671,9 +758,9 @@ int cactus_hip_kv4_append_f16(const cactus_hip_kv4_cache* cache, size_t layer, c
     CH_REQUIRE(seq_len < (1u << 30), "kv4_append: seq_len out of range");
     const dim3 grid(ceil_div(seq_len + 15, 16), c.Hkv, (unsigned)batch);
     switch (c.d) {
-        case 64: hipLaunchKernelGGL(kv4_append_kernel<64>, grid, dim3(64), 0, as_stream(stream), c, seqs, counts, k, v, (int)seq_len, kv_stride); break;
-        case 128: hipLaunchKernelGGL(kv4_append_kernel<128>, grid, dim3(64), 0, as_stream(stream), c, seqs, counts, k, v, (int)seq_len, kv_stride); break;
-        default: hipLaunchKernelGGL(kv4_append_kernel<256>, grid, dim3(64), 0, as_stream(stream), c, seqs, counts, k, v, (int)seq_len, kv_stride);
+        case 64: hipLaunchKernelGGL(kv4_append_kernel<64>, grid, dim3(128), 0, as_stream(stream), c, seqs, counts, k, v, (int)seq_len, kv_stride); break;
+        case 128: hipLaunchKernelGGL(kv4_append_kernel<128>, grid, dim3(128), 0, as_stream(stream), c, seqs, counts, k, v, (int)seq_len, kv_stride); break;
+        default: hipLaunchKernelGGL(kv4_append_kernel<256>, grid, dim3(128), 0, as_stream(stream), c, seqs, counts, k, v, (int)seq_len, kv_stride);
     }
     return check_launch("kv4_append");
 }
@@ -690,9 +777,9 @@ int cactus_hip_kv4_read_f16(const cactus_hip_kv4_cache* cache, size_t layer, con
     CH_REQUIRE(seq_len < (1u << 30), "kv4_read: seq_len out of range");
     const dim3 grid(ceil_div(seq_len + 15, 16), c.Hkv, (unsigned)batch);
     switch (c.d) {
-        case 64: hipLaunchKernelGGL(kv4_read_kernel<64>, grid, dim3(64), 0, as_stream(stream), c, seqs, starts, counts, k, v, (int)seq_len); break;
-        case 128: hipLaunchKernelGGL(kv4_read_kernel<128>, grid, dim3(64), 0, as_stream(stream), c, seqs, starts, counts, k, v, (int)seq_len); break;
-        default: hipLaunchKernelGGL(kv4_read_kernel<256>, grid, dim3(64), 0, as_stream(stream), c, seqs, starts, counts, k, v, (int)seq_len);
+        case 64: hipLaunchKernelGGL(kv4_read_kernel<64>, grid, dim3(128), 0, as_stream(stream), c, seqs, starts, counts, k, v, (int)seq_len); break;
+        case 128: hipLaunchKernelGGL(kv4_read_kernel<128>, grid, dim3(128), 0, as_stream(stream), c, seqs, starts, counts, k, v, (int)seq_len); break;
+        default: hipLaunchKernelGGL(kv4_read_kernel<256>, grid, dim3(128), 0, as_stream(stream), c, seqs, starts, counts, k, v, (int)seq_len);
     }
     return check_launch("kv4_read");
 }
