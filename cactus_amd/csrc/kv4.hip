@@ -283,8 +283,12 @@ __device__ int collect_free(const Kv4View& c, int* at, int want, int* ids, int* 
     while (have < want && pos < c.num_pages) {
         const int i = pos + (int)threadIdx.x * 4;
         int z = 0;
-#pragma unroll
-        for (int u = 0; u < 4; u++) z |= (i + u < c.num_pages && c.refs[i + u] == 0) << u;
+        if (i + 4 <= c.num_pages) {
+            const int r0 = c.refs[i], r1 = c.refs[i + 1], r2 = c.refs[i + 2], r3 = c.refs[i + 3];
+            z = (r0 == 0) | (r1 == 0) << 1 | (r2 == 0) << 2 | (r3 == 0) << 3;
+        } else {
+            for (int u = 0; i + u < c.num_pages; u++) z |= (c.refs[i + u] == 0) << u;
+        }
         int got;
         int rank = have + block_scan(__popc(z), wave_sums, &got);
 #pragma unroll
@@ -317,6 +321,7 @@ __global__ void __launch_bounds__(BK_THREADS) kv4_extend_kernel(Kv4View c, const
     __shared__ int ids[BK_IDS], off[BK_THREADS], wave_sums[16];
     __shared__ int bad, total_s;
     const int tid = threadIdx.x, cap = c.max_pages << c.ps_log2;
+    const int free_pages = c.state[KV4_FREE], hint = c.state[KV4_HINT];   // (before anything is waited for)
     for (int i = tid; i < (c.max_seqs + 31) / 32; i += BK_THREADS) bits[i] = 0;
     if (tid == 0) {
         bad = 0;
@@ -341,14 +346,13 @@ __global__ void __launch_bounds__(BK_THREADS) kv4_extend_kernel(Kv4View c, const
     }
     __syncthreads();
     const int total = total_s;
-    if (bad || total > c.state[KV4_FREE]) {
+    if (bad || total > free_pages) {
         if (tid == 0) atomicOr((uint32_t*)c.state + KV4_STATUS, bad ? CACTUS_HIP_KV4_BAD_REQUEST : CACTUS_HIP_KV4_NO_PAGES);
         return;
     }
     // free pages in rounds of BK_IDS, each handed to the requests whose share
     // of the sequence of new pages falls into the round
-    int at = c.state[KV4_HINT], done = 0;
-    at = at < 0 ? 0 : at;
+    int at = max(hint, 0), done = 0;
     while (done < total) {
         const int got = collect_free(c, &at, total - done, ids, wave_sums);
         if (got == 0) {                    // the free count was wrong: no page is handed out twice
@@ -393,55 +397,76 @@ __global__ void __launch_bounds__(BK_THREADS) kv4_extend_kernel(Kv4View c, const
 
 // Lists of a fork in the workspace, behind the attention's counters.
 struct ForkPlan {
-    int32_t* ok;         // [1]
+    int32_t* ok;         // [2] whether the call is carried out, pages it takes
     int32_t* tail;       // [n] new page of the partly filled last one, -1
     int32_t* len;        // [n] the source's tokens before the call
     int32_t* rows;       // [n][max_pages] the source's pages before the call
 };
 constexpr size_t KV4_WORK_SKIP = 4096;
 
-// Requests checked and the copies' pages allocated, before anything changes
-// that a wrong call would have to undo.
+// The whole workgroup: whether the pairs are right, and how many pages they need.
+__device__ bool fork_checked(const Kv4View& c, const int32_t* src, const int32_t* dst, int n, uint32_t* bits, int* counts,
+                             int* total) {
+    const int tid = threadIdx.x, ps1 = (1 << c.ps_log2) - 1;
+    for (int i = tid; i < (c.max_seqs + 31) / 32; i += blockDim.x) bits[i] = 0;
+    if (tid < 2) counts[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += blockDim.x) {
+        const int s = kv4_slot(c, src, i), d = kv4_slot(c, dst, i);
+        if (s < 0 || d < 0 || mark_twice(bits, d)) {
+            counts[0] = 1;
+            continue;
+        }
+        if (s != d && (kv4_len(c, s) & ps1)) atomicAdd(&counts[1], 1);
+    }
+    __syncthreads();
+    *total = counts[1];
+    return counts[0] == 0;
+}
+
+// Workgroup 0 allocates the copies' pages; workgroup 1 + i sets pair i's source
+// aside (row and length) and raises its full pages' counts.  Each checks the call
+// by itself, so that one launch does both: the counts of pages in use are raised
+// while workgroup 0 looks for pages whose count is 0, and the number of free
+// pages, which all of them read, changes in the second launch.
 __global__ void __launch_bounds__(BK_THREADS) kv4_fork_plan_kernel(Kv4View c, ForkPlan p, const int32_t* src,
                                                                    const int32_t* dst, int n) {
     __shared__ uint32_t bits[KV4_MAX_SEQS / 32];
-    __shared__ int ids[BK_IDS], wave_sums[16];
-    __shared__ int bad, total_s;
+    __shared__ int ids[BK_IDS], wave_sums[16], counts[2];
     const int tid = threadIdx.x, ps1 = (1 << c.ps_log2) - 1;
-    for (int i = tid; i < (c.max_seqs + 31) / 32; i += BK_THREADS) bits[i] = 0;
-    if (tid == 0) {
-        bad = 0;
-        total_s = 0;
-    }
-    __syncthreads();
-    for (int i = tid; i < n; i += BK_THREADS) {
-        const int s = kv4_slot(c, src, i), d = kv4_slot(c, dst, i);
-        if (s < 0 || d < 0 || mark_twice(bits, d)) {
-            bad = 1;
-            continue;
-        }
-        if (s != d && (kv4_len(c, s) & ps1)) atomicAdd(&total_s, 1);
-    }
-    __syncthreads();
-    const int total = total_s;
-    if (bad || total > c.state[KV4_FREE]) {
-        if (tid == 0) {
-            atomicOr((uint32_t*)c.state + KV4_STATUS, bad ? CACTUS_HIP_KV4_BAD_REQUEST : CACTUS_HIP_KV4_NO_PAGES);
-            *p.ok = 0;
+    const int free_pages = c.state[KV4_FREE], hint = c.state[KV4_HINT];   // (before anything is waited for)
+    int total;
+    const bool right = fork_checked(c, src, dst, n, bits, counts, &total);
+    const bool ok = right && total <= free_pages;
+    if (blockIdx.x > 0) {
+        const int i = blockIdx.x - 1;
+        if (!ok) return;
+        const int s = kv4_slot(c, src, i);
+        if (s == kv4_slot(c, dst, i)) return;
+        const int len = kv4_len(c, s), full = len >> c.ps_log2, np = kv4_pages_of(c, len);
+        if (tid == 0) p.len[i] = len;
+        for (int j = tid; j < np; j += BK_THREADS) {
+            const int id = c.table[(size_t)s * c.max_pages + j];
+            p.rows[(size_t)i * c.max_pages + j] = id;
+            if (j < full && kv4_page_ok(c, id)) atomicAdd(&c.refs[id], 1);
         }
         return;
     }
+    if (tid == 0) {
+        p.ok[0] = ok;
+        p.ok[1] = total;
+        if (!ok) atomicOr((uint32_t*)c.state + KV4_STATUS, right ? CACTUS_HIP_KV4_NO_PAGES : CACTUS_HIP_KV4_BAD_REQUEST);
+    }
+    if (!ok) return;
     // at most max_seqs pages: dst slots differ
-    int at = c.state[KV4_HINT], done = 0;
-    at = at < 0 ? 0 : at;
+    int at = max(hint, 0), done = 0;
     do {
         const int got = done < total ? collect_free(c, &at, total - done, ids, wave_sums) : 0;
         if (got == 0 && done < total) {
-            if (tid == 0) {
-                atomicOr((uint32_t*)c.state + KV4_STATUS, CACTUS_HIP_KV4_NO_PAGES);
-                *p.ok = 0;
-            }
-            return;
+            // the free count was wrong: the pairs behind are left without a last page
+            if (tid == 0) atomicOr((uint32_t*)c.state + KV4_STATUS, CACTUS_HIP_KV4_NO_PAGES);
+            for (int i = tid; i < n; i += BK_THREADS) p.tail[i] = done ? p.tail[i] : -1;
+            break;
         }
         int base = 0;
         for (int i0 = 0; i0 < n; i0 += BK_THREADS) {
@@ -454,65 +479,76 @@ __global__ void __launch_bounds__(BK_THREADS) kv4_fork_plan_kernel(Kv4View c, Fo
             int chunk;
             const int o = base + block_scan(part, wave_sums, &chunk) - done;
             if (i < n) {
-                if (!part) p.tail[i] = -1;
-                else if (o >= 0 && o < got) p.tail[i] = ids[o];
+                if (!part || o >= got) {
+                    if (done == 0) p.tail[i] = -1;
+                } else if (o >= 0) {
+                    p.tail[i] = ids[o];
+                    c.refs[ids[o]] = 1;
+                }
             }
             base += chunk;
         }
         done += got;
         __syncthreads();
     } while (done < total);
-    if (tid == 0) {
-        *p.ok = 1;
-        if (total > 0) {
-            c.state[KV4_FREE] -= total;
-            c.state[KV4_HINT] = at;
-        }
-    }
+    if (tid == 0 && total > 0) c.state[KV4_HINT] = at;
 }
-// the sources' rows and lengths set aside, their full pages' counts raised
-__global__ void kv4_fork_share_kernel(Kv4View c, ForkPlan p, const int32_t* src, const int32_t* dst) {
-    if (!*p.ok) return;
-    const int i = blockIdx.x, s = kv4_slot(c, src, i);
-    if (s == kv4_slot(c, dst, i)) return;
-    const int len = kv4_len(c, s), full = len >> c.ps_log2, np = kv4_pages_of(c, len);
-    if (threadIdx.x == 0) {
-        p.len[i] = len;
-        if (p.tail[i] >= 0) c.refs[p.tail[i]] = 1;
-    }
-    for (int j = threadIdx.x; j < np; j += blockDim.x) {
-        const int id = c.table[(size_t)s * c.max_pages + j];
-        p.rows[(size_t)i * c.max_pages + j] = id;
-        if (j < full && kv4_page_ok(c, id)) atomicAdd(&c.refs[id], 1);
-    }
-}
-// a slot's pages given up (its row as it stands)
+// a slot's pages given up (its row as it stands); whole waves
 __device__ __forceinline__ void release_row(const Kv4View& c, int slot, int len) {
-    const int np = kv4_pages_of(c, len);
+    const int np = kv4_pages_of(c, len), lane = threadIdx.x & 63;
+    int freed = 0, lowest = 0x7FFFFFFF;
     for (int j = threadIdx.x; j < np; j += blockDim.x) {
         const int id = c.table[(size_t)slot * c.max_pages + j];
         if (kv4_page_ok(c, id) && atomicSub(&c.refs[id], 1) == 1) {
-            atomicAdd(&c.state[KV4_FREE], 1);
-            atomicMin(&c.state[KV4_HINT], id);
+            freed++;
+            lowest = min(lowest, id);
         }
     }
+    // one update of the shared words per wave
+    freed = wave_sum_i32(freed);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) lowest = min(lowest, __shfl_xor(lowest, o, 64));
+    if (lane == 0 && freed) {
+        atomicAdd(&c.state[KV4_FREE], freed);
+        atomicMin(&c.state[KV4_HINT], lowest);
+    }
 }
-__device__ __forceinline__ void copy_bytes16(uint8_t* dst, const uint8_t* src, size_t bytes, size_t first, size_t step) {
-    for (size_t o = first * 16; o < bytes; o += step * 16)
-        *reinterpret_cast<uint4*>(dst + o) = *reinterpret_cast<const uint4*>(src + o);
+// Pages are copied in pieces of COPY_PIECE bytes, a workgroup of 256 each, every
+// load of a piece before its stores (a whole page per workgroup, load by load:
+// 15 pages of 28 layers 17 us, 62 MB).
+constexpr int COPY_PIECE = 16384;
+__device__ __forceinline__ void copy_piece(uint8_t* dst, const uint8_t* src, size_t bytes, int piece) {
+    const uint32_t at = (uint32_t)piece * COPY_PIECE + 16 * threadIdx.x;
+    const uint32_t end = min((uint32_t)bytes, (uint32_t)(piece + 1) * COPY_PIECE);
+    if (end - (uint32_t)piece * COPY_PIECE == COPY_PIECE) {
+        // (an array of four was moved to LDS, for which the kernel read its launch
+        // packet in host memory: 13 us)
+        const uint4* s = reinterpret_cast<const uint4*>(src + at);
+        uint4* d = reinterpret_cast<uint4*>(dst + at);
+        const uint4 w0 = s[0], w1 = s[256], w2 = s[512], w3 = s[768];
+        d[0] = w0;
+        d[256] = w1;
+        d[512] = w2;
+        d[768] = w3;
+    } else {
+        for (uint32_t o = at; o < end; o += 4096) *reinterpret_cast<uint4*>(dst + o) = *reinterpret_cast<const uint4*>(src + o);
+    }
 }
-// block y 0: the destination's table row; blocks from 1 on: the last page, a layer each
-__global__ void kv4_fork_apply_kernel(Kv4View c, ForkPlan p, const int32_t* src, const int32_t* dst) {
-    if (!*p.ok) return;
+
+// block y 0: the destination's table row; from 1 on: a piece of the last page, a layer
+__global__ void __launch_bounds__(256) kv4_fork_apply_kernel(Kv4View c, ForkPlan p, const int32_t* src, const int32_t* dst,
+                                                             int pieces) {
+    if (!p.ok[0]) return;
     const int i = blockIdx.x, d = kv4_slot(c, dst, i);
+    if (blockIdx.y == 0 && i == 0 && threadIdx.x == 0) atomicSub(&c.state[KV4_FREE], p.ok[1]);
     if (kv4_slot(c, src, i) == d) return;
     const int32_t* row = p.rows + (size_t)i * c.max_pages;
     const int len = p.len[i], full = len >> c.ps_log2, tail = p.tail[i];
     if (blockIdx.y > 0) {
         if (tail < 0 || !kv4_page_ok(c, row[full])) return;
-        const size_t layer = (size_t)(blockIdx.y - 1) * c.layer_bytes;
-        copy_bytes16(c.pages + layer + (size_t)tail * c.page_bytes, c.pages + layer + (size_t)row[full] * c.page_bytes,
-                     c.page_bytes, threadIdx.x, blockDim.x);
+        const size_t layer = (size_t)((blockIdx.y - 1) / pieces) * c.layer_bytes;
+        copy_piece(c.pages + layer + (size_t)tail * c.page_bytes, c.pages + layer + (size_t)row[full] * c.page_bytes,
+                   c.page_bytes, (blockIdx.y - 1) % pieces);
         return;
     }
     release_row(c, d, kv4_len(c, d));
@@ -540,7 +576,7 @@ __global__ void kv4_free_kernel(Kv4View c, const int32_t* seqs) {
 }
 
 // ------------------------------------------------------------ compact
-constexpr int CP_THREADS = 256, CP_PER = 16, CP_BLOCK = CP_THREADS * CP_PER;   // pages per workgroup
+constexpr int CP_THREADS = 1024, CP_PER = 4, CP_BLOCK = CP_THREADS * CP_PER;   // pages per workgroup
 struct CompactPlan {
     int32_t* moves;      // [1]
     int32_t* live;       // [1] pages in use
@@ -549,48 +585,54 @@ struct CompactPlan {
     int32_t* from;       // [num_pages] pages that move, ascending
     int32_t* to;         // [num_pages] free pages below `live`, ascending
 };
+// bit u: page i0 + u is in use
+__device__ __forceinline__ uint32_t pages_in_use(const Kv4View& c, int i0) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int u = 0; u < CP_PER; u++) bits |= (uint32_t)(i0 + u < c.num_pages && c.refs[i0 + u] > 0) << u;
+    return bits;
+}
+__device__ __forceinline__ uint32_t bits_below(int i0, int top) {   // of pages i0 on, those below `top`
+    return top <= i0 ? 0 : top - i0 >= CP_PER ? (1u << CP_PER) - 1 : (1u << (top - i0)) - 1;
+}
+// (pools of more than CP_BLOCK pages)
 __global__ void __launch_bounds__(CP_THREADS) kv4_compact_count_kernel(Kv4View c, CompactPlan p) {
-    __shared__ int sums[4];
-    int n = 0;
-    for (int u = 0; u < CP_PER; u++) {
-        const int i = blockIdx.x * CP_BLOCK + u * CP_THREADS + threadIdx.x;
-        n += i < c.num_pages && c.refs[i] > 0;
-    }
+    __shared__ int sums[16];
     int total;
-    block_scan(n, sums, &total);
+    block_scan(__popc(pages_in_use(c, (blockIdx.x * CP_THREADS + threadIdx.x) * CP_PER)), sums, &total);
     if (threadIdx.x == 0) p.used[blockIdx.x] = total;
 }
 __global__ void __launch_bounds__(CP_THREADS) kv4_compact_list_kernel(Kv4View c, CompactPlan p) {
-    __shared__ int sums[4];
+    __shared__ int sums[16];
     const int tid = threadIdx.x, blocks = gridDim.x, me = blockIdx.x;
-    int before_me = 0, all = 0, t;
-    for (int b0 = 0; b0 < blocks; b0 += CP_THREADS) {
-        const int b = b0 + tid, v = b < blocks ? p.used[b] : 0;
-        block_scan(b < me ? v : 0, sums, &t);
-        before_me += t;
-        block_scan(v, sums, &t);
-        all += t;
-    }
-    const int live = all;
-    // pages in use below `live`
-    const int edge = live / CP_BLOCK;
-    int below = 0;
-    for (int b0 = 0; b0 < edge; b0 += CP_THREADS) {
-        block_scan(b0 + tid < edge ? p.used[b0 + tid] : 0, sums, &t);
+    const int i0 = (me * CP_THREADS + tid) * CP_PER;
+    const uint32_t in_use = pages_in_use(c, i0);
+    int mine, t, before_me = 0, live, below = 0;
+    const int inside = block_scan(__popc(in_use), sums, &mine);
+    if (blocks == 1) {
+        live = mine;
+        block_scan(__popc(in_use & bits_below(i0, live)), sums, &below);
+    } else {
+        live = 0;
+        for (int b0 = 0; b0 < blocks; b0 += CP_THREADS) {
+            const int b = b0 + tid, v = b < blocks ? p.used[b] : 0;
+            block_scan(b < me ? v : 0, sums, &t);
+            before_me += t;
+            block_scan(v, sums, &t);
+            live += t;
+        }
+        // pages in use below `live`: whole workgroups' shares and a part of one
+        const int edge = live / CP_BLOCK;
+        for (int b0 = 0; b0 < edge; b0 += CP_THREADS) {
+            block_scan(b0 + tid < edge ? p.used[b0 + tid] : 0, sums, &t);
+            below += t;
+        }
+        const int e0 = (edge * CP_THREADS + tid) * CP_PER;
+        block_scan(__popc(pages_in_use(c, e0) & bits_below(e0, live)), sums, &t);
         below += t;
     }
-    int n = 0;
-    for (int u = 0; u < CP_PER; u++) {
-        const int i = edge * CP_BLOCK + u * CP_THREADS + tid;
-        n += i < live && c.refs[i] > 0;
-    }
-    block_scan(n, sums, &t);
-    below += t;
-    // this workgroup's pages, CP_PER consecutive ones per thread
-    const int i0 = me * CP_BLOCK + tid * CP_PER;
-    uint32_t in_use = 0;
-    for (int u = 0; u < CP_PER; u++) in_use |= (uint32_t)(i0 + u < c.num_pages && c.refs[i0 + u] > 0) << u;
-    int r = before_me + block_scan(__popc(in_use), sums, &t);   // pages in use before page i0
+    int r = before_me + inside;                   // pages in use before page i0
+#pragma unroll
     for (int u = 0; u < CP_PER; u++) {
         const int i = i0 + u;
         if (i >= c.num_pages) break;
@@ -608,31 +650,30 @@ __global__ void __launch_bounds__(CP_THREADS) kv4_compact_list_kernel(Kv4View c,
         *p.live = live;
     }
 }
-// grid x: page copies first (one workgroup per move and layer in turn), the
-// last CP_TABLE workgroups tables and counts
+// the first CP_TABLE workgroups tables and counts, the others pieces of pages in turn
 constexpr int CP_TABLE = 64;
-__global__ void __launch_bounds__(CP_THREADS) kv4_compact_apply_kernel(Kv4View c, CompactPlan p) {
+__global__ void __launch_bounds__(256) kv4_compact_apply_kernel(Kv4View c, CompactPlan p, int pieces) {
     const int moves = *p.moves, live = *p.live;
-    const int ncopy = gridDim.x - CP_TABLE;
-    if ((int)blockIdx.x < ncopy) {
-        for (int64_t w = blockIdx.x; w < (int64_t)moves * c.layers; w += ncopy) {
-            const int m = (int)(w % moves);
-            const size_t layer = (size_t)(w / moves) * c.layer_bytes;
-            copy_bytes16(c.pages + layer + (size_t)p.to[m] * c.page_bytes, c.pages + layer + (size_t)p.from[m] * c.page_bytes,
-                         c.page_bytes, threadIdx.x, blockDim.x);
+    if (blockIdx.x >= CP_TABLE) {
+        const uint64_t per_page = (uint64_t)pieces * c.layers;
+        for (uint64_t w = blockIdx.x - CP_TABLE; w < moves * per_page; w += gridDim.x - CP_TABLE) {
+            const int m = (int)(w / per_page), r = (int)(w % per_page);
+            const size_t layer = (size_t)(r / pieces) * c.layer_bytes;
+            copy_piece(c.pages + layer + (size_t)p.to[m] * c.page_bytes, c.pages + layer + (size_t)p.from[m] * c.page_bytes,
+                       c.page_bytes, r % pieces);
         }
         return;
     }
-    const int me = (blockIdx.x - ncopy) * CP_THREADS + threadIdx.x, step = CP_TABLE * CP_THREADS;
+    const int me = blockIdx.x * 256 + threadIdx.x, step = CP_TABLE * 256;
     for (int m = me; m < moves; m += step) {
         c.refs[p.to[m]] = c.refs[p.from[m]];
         c.refs[p.from[m]] = 0;
     }
-    for (int64_t e = me; e < (int64_t)c.max_seqs * c.max_pages; e += step) {
-        const int s = (int)(e / c.max_pages), j = (int)(e % c.max_pages);
-        if (j >= kv4_pages_of(c, kv4_len(c, s))) continue;
+    for (uint32_t e = me; e < (uint32_t)c.max_seqs * (uint32_t)c.max_pages; e += step) {
         const int id = c.table[e];
-        if (kv4_page_ok(c, id) && id >= live) c.table[e] = p.to[p.rank[id]];
+        if (!kv4_page_ok(c, id) || id < live) continue;
+        const int s = (int)(e / (uint32_t)c.max_pages), j = (int)(e % (uint32_t)c.max_pages);
+        if (j < kv4_pages_of(c, kv4_len(c, s)) && p.rank[id] < moves) c.table[e] = p.to[p.rank[id]];
     }
     if (me == 0) {
         c.state[KV4_FREE] = c.num_pages - live;
@@ -640,15 +681,15 @@ __global__ void __launch_bounds__(CP_THREADS) kv4_compact_apply_kernel(Kv4View c
     }
 }
 
-__global__ void kv4_copy_kernel(Kv4View c, const int32_t* src, const int32_t* dst) {
+__global__ void __launch_bounds__(256) kv4_copy_kernel(Kv4View c, const int32_t* src, const int32_t* dst, int pieces) {
     const int s = src[blockIdx.x], d = dst[blockIdx.x];
     if (!kv4_page_ok(c, s) || !kv4_page_ok(c, d)) {
         if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr((uint32_t*)c.state + KV4_STATUS, CACTUS_HIP_KV4_BAD_REQUEST);
         return;
     }
-    const size_t layer = (size_t)blockIdx.y * c.layer_bytes;
-    copy_bytes16(c.pages + layer + (size_t)d * c.page_bytes, c.pages + layer + (size_t)s * c.page_bytes, c.page_bytes,
-                 threadIdx.x, blockDim.x);
+    const size_t layer = (size_t)(blockIdx.y / pieces) * c.layer_bytes;
+    copy_piece(c.pages + layer + (size_t)d * c.page_bytes, c.pages + layer + (size_t)s * c.page_bytes, c.page_bytes,
+               blockIdx.y % pieces);
 }
 
 // ------------------------------------------------------------ host side
@@ -658,7 +699,11 @@ int kv4_view(const cactus_hip_kv4_cache* c, size_t layer, const char* what, Kv4V
     CH_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, string(what) + ": head_dim is 64, 128 or 256");
     CH_REQUIRE(c->page_size >= 16 && c->page_size <= 4096 && (c->page_size & (c->page_size - 1)) == 0,
                string(what) + ": page_size is a power of two from 16 to 4096");
-    CH_REQUIRE(c->layers >= 1 && c->layers < 65535 && c->kv_heads >= 1 && c->kv_heads <= 4096, string(what) + ": layers or kv_heads out of range");
+    CH_REQUIRE(c->layers >= 1 && c->layers <= 4096 && c->kv_heads >= 1 && c->kv_heads <= 4096,
+               string(what) + ": layers or kv_heads out of range");
+    // a page in pieces, all layers, is a launch dimension
+    CH_REQUIRE(c->layers * ceil_div(c->kv_heads * (c->page_size / 16) * (18 * c->head_dim), 16384) < 65535,
+               string(what) + ": layers times page bytes out of range");
     CH_REQUIRE(c->num_pages >= 1 && c->num_pages < (1u << 30) && c->max_seqs >= 1 && c->max_seqs <= KV4_MAX_SEQS &&
                    c->max_pages >= 1 && c->max_pages < (1u << 30) / c->page_size &&
                    c->max_seqs * c->max_pages < (1u << 31),
@@ -803,9 +848,9 @@ int cactus_hip_kv4_fork(const cactus_hip_kv4_cache* cache, const int32_t* src, c
     int32_t* w = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + KV4_WORK_SKIP);
     ForkPlan p{w, w + 64, w + 64 + n, w + 64 + 2 * n};
     const hipStream_t st = as_stream(stream);
-    hipLaunchKernelGGL(kv4_fork_plan_kernel, dim3(1), dim3(BK_THREADS), 0, st, c, p, src, dst, (int)n);
-    hipLaunchKernelGGL(kv4_fork_share_kernel, dim3((unsigned)n), dim3(256), 0, st, c, p, src, dst);
-    hipLaunchKernelGGL(kv4_fork_apply_kernel, dim3((unsigned)n, c.layers + 1), dim3(256), 0, st, c, p, src, dst);
+    const int pieces = (int)ceil_div(c.page_bytes, COPY_PIECE);
+    hipLaunchKernelGGL(kv4_fork_plan_kernel, dim3((unsigned)n + 1), dim3(BK_THREADS), 0, st, c, p, src, dst, (int)n);
+    hipLaunchKernelGGL(kv4_fork_apply_kernel, dim3((unsigned)n, c.layers * pieces + 1), dim3(256), 0, st, c, p, src, dst, pieces);
     return check_launch("kv4_fork");
 }
 
@@ -830,9 +875,10 @@ int cactus_hip_kv4_compact(const cactus_hip_kv4_cache* cache, void* workspace, s
     const size_t np = cache->num_pages;
     CompactPlan p{w, w + 1, w + 64, w + 64 + blocks, w + 64 + blocks + np, w + 64 + blocks + 2 * np};
     const hipStream_t st = as_stream(stream);
-    hipLaunchKernelGGL(kv4_compact_count_kernel, dim3(blocks), dim3(CP_THREADS), 0, st, c, p);
+    const int pieces = (int)ceil_div(c.page_bytes, COPY_PIECE);
+    if (blocks > 1) hipLaunchKernelGGL(kv4_compact_count_kernel, dim3(blocks), dim3(CP_THREADS), 0, st, c, p);
     hipLaunchKernelGGL(kv4_compact_list_kernel, dim3(blocks), dim3(CP_THREADS), 0, st, c, p);
-    hipLaunchKernelGGL(kv4_compact_apply_kernel, dim3(2048 + CP_TABLE), dim3(CP_THREADS), 0, st, c, p);
+    hipLaunchKernelGGL(kv4_compact_apply_kernel, dim3(2048 + CP_TABLE), dim3(256), 0, st, c, p, pieces);
     return check_launch("kv4_compact");
 }
 
@@ -844,7 +890,8 @@ int cactus_hip_kv4_copy_pages(const cactus_hip_kv4_cache* cache, const int32_t* 
     if (n == 0) return CACTUS_HIP_OK;
     CH_REQUIRE(src && dst, "kv4_copy_pages: null pointer");
     CH_REQUIRE(n <= cache->num_pages, "kv4_copy_pages: more pairs than pages");
-    hipLaunchKernelGGL(kv4_copy_kernel, dim3((unsigned)n, c.layers), dim3(256), 0, as_stream(stream), c, src, dst);
+    const int pieces = (int)ceil_div(c.page_bytes, COPY_PIECE);
+    hipLaunchKernelGGL(kv4_copy_kernel, dim3((unsigned)n, c.layers * pieces), dim3(256), 0, as_stream(stream), c, src, dst, pieces);
     return check_launch("kv4_copy_pages");
 }
 
