@@ -26,6 +26,18 @@ namespace cactus_hip {
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// n / d for 0 <= n < 2^31: n m / 2^(31 + s) with 2^s the power of two at or above d
+// and m = 2^(31 + s) / d + 1, whose error n / 2^(31 + s) stays below 1 / d
+struct FastDiv {
+    uint32_t m = 0;
+    int s = 0;
+    void set(uint32_t d) {
+        for (s = 0; (1ull << s) < d; s++) {}
+        m = (uint32_t)((1ull << (31 + s)) / d + 1);
+    }
+    __device__ __forceinline__ int operator()(int n) const { return s == 0 ? n : (int)(__umulhi((uint32_t)n, m) >> (s - 1)); }
+};
+
 struct Kv4AttnArgs {
     Kv4View c;
     const int32_t* seqs;
@@ -34,6 +46,7 @@ struct Kv4AttnArgs {
     uint16_t* o;
     size_t q_stride;
     int B, S, Hq, G;          // G query heads per KV head
+    FastDiv by_g, by_nvb;     // division by G, and by the blocks of query vectors of a request
     int window, sink, causal; // window 0: none
     float scale;              // times log2(e): the softmax runs in powers of two
     uint32_t* counters;       // [workgroups] zero between calls
@@ -69,6 +82,11 @@ __device__ __forceinline__ bool kv4_sees(const Kv4AttnArgs& a, int p, int j, int
     return (j < n) & (!a.causal | (j <= p)) & ((a.window == 0) | (p - j <= a.window) | (j < a.sink));
 }
 
+// row of o, in heads, that query vector vv of a KV head has within its request
+__device__ __forceinline__ size_t out_offset(const Kv4AttnArgs& a, int head, int vv) {
+    const int row = a.by_g(vv);
+    return (size_t)row * a.Hq + (size_t)(head * a.G + vv - row * a.G);
+}
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ h16x8 frag(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_bit_cast(h16x8, (u32x4){a, b, c, d});
@@ -255,9 +273,29 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
         total += lane_u(r_upto, 63);
         longest = max(longest, __builtin_amdgcn_readlane(wave_scan_max((int)r_blocks), 63));
     }
-    const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1));
-    uint32_t at = blockIdx.x * per;
-    const uint32_t end = min(total, at + per);
+    uint32_t per = max((total + gridDim.x - 1) / gridDim.x, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1));
+    // Stretches that end inside a unit cost their workgroup another unit's start (7
+    // us, where a block step takes 0.5 to 3).  If units cut into whole parts of at
+    // most `per` steps, or one or two more, make no more parts than there are
+    // workgroups, each takes a part (up to five rows of 8 sequences 18.7 -> 16.7 us);
+    // the line then counts parts.  (Of long stretches the ends matter less than
+    // equal lengths.)
+    bool parts = false;
+    if (a.B <= 64 && per > 1 && per <= 12) {
+        const uint32_t units = r_blocks ? r_cost / r_blocks : 0;
+        for (uint32_t q = per; q <= per + 2 && !parts; q++) {
+            const uint32_t cost = units * ((r_blocks + q - 1) / q), upto = wave_scan_add(cost);
+            if (lane_u(upto, 63) <= gridDim.x) {
+                parts = true;
+                per = q;
+                total = lane_u(upto, 63);
+                r_cost = cost;
+                r_upto = upto;
+            }
+        }
+    }
+    uint32_t at = parts ? blockIdx.x : blockIdx.x * per;
+    const uint32_t end = min(total, parts ? at + 1 : at + per);
 
     while (at < end) {
         // ---- the unit at `at`: request, KV head, vectors, its block steps
@@ -277,10 +315,12 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
         const uint32_t blocks = lane_u(r_blocks, j);
         const Kv4Seq sq = kv4_span(a, __builtin_amdgcn_readlane(r_slot, j), __builtin_amdgcn_readlane(r_len, j),
                                    __builtin_amdgcn_readlane(r_rows, j));
-        const uint32_t rel = at - base, unit = rel / blocks, s0 = rel % blocks;
-        const uint32_t nblk = min(blocks - s0, end - at);
+        const uint32_t nparts = (blocks + per - 1) / per;            // (of a unit in parts)
+        const uint32_t rel = at - base, unit = rel / (parts ? nparts : blocks), first = rel - unit * (parts ? nparts : blocks);
+        const uint32_t s0 = parts ? first * per : first;
+        const uint32_t nblk = min(blocks - s0, parts ? per : end - at);
         const int ncg = (sq.rows * a.G + QV - 1) / QV;
-        const int head = (int)unit / ncg, v0 = (int)unit % ncg * QV;
+        const int head = ncg == 1 ? (int)unit : (int)unit / ncg, v0 = ncg == 1 ? 0 : (int)unit % ncg * QV;
         const int nvec = min(QV, sq.rows * a.G - v0);
 
         // ---- pages of the run, 64 table entries in the lanes at a time
@@ -330,7 +370,7 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
         for (int k = 0; k < min(R - 1, n); k++) put(k);
 
         // ---- this lane's vector: row, query head and position
-        const int vec = v0 + qi, row = vec / a.G;
+        const int vec = v0 + qi, row = a.by_g(vec);
         const bool live = qi < nvec;
         const int pos = sq.len - sq.rows + row;
         h16x8 qf[NG];
@@ -340,15 +380,15 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
             uint4 u = make_uint4(0, 0, 0, 0);
             if (live && (!PACK || g == gi))
                 u = *reinterpret_cast<const uint4*>(a.q + ((size_t)b * a.S + row) * a.q_stride +
-                                                    (size_t)(head * a.G + vec % a.G) * D + 32 * g + 8 * h);
+                                                    (size_t)(head * a.G + vec - row * a.G) * D + 32 * g + 8 * h);
             qf[g] = code_order(u);
         }
 #pragma unroll
         for (int g = 0; g < NG; g++)
             start[PACK ? 0 : g] = mfma16(minus8(g & 1), qf[g], PACK && g > 0 ? start[0] : (f32x4){0, 0, 0, 0});
         // keys that every vector of the unit sees: below `all`, and within the last one's window
-        const int first_pos = sq.len - sq.rows + v0 / a.G;
-        const int last_pos = sq.len - sq.rows + (v0 + nvec - 1) / a.G;
+        const int first_pos = sq.len - sq.rows + a.by_g(v0);
+        const int last_pos = sq.len - sq.rows + a.by_g(v0 + nvec - 1);
         const int all = a.causal ? min(first_pos + 1, sq.len) : sq.len;
 
         float m = -__builtin_inff(), mbase = 0.0f, l = 0.0f;
@@ -507,17 +547,19 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
         // parts of the unit: the first workgroup has it at the end of its stretch
         // (slot 1), the others at the start of theirs (slot 0)
         const uint32_t unit0 = base + unit * blocks;
-        const uint32_t wg0 = unit0 / per, nparts = (unit0 + blocks - 1) / per - wg0 + 1;
+        const uint32_t wg0 = alone ? 0 : parts ? blockIdx.x - first : unit0 / per;
+        const uint32_t joined = parts ? nparts : (unit0 + blocks - 1) / per - wg0 + 1;
         // rows of D sums, maximum, sum of weights
         auto part_row = [&](uint32_t wg, int cc) {
             return a.part + ((size_t)(2 * wg + (wg == wg0)) * QV + cc) * (D + 4);
         };
         auto write_row = [&](int cc, int d, f32x4 num, float den) {
             const int vv = v0 + cc;
+            const float inv = den != 0.0f ? 1.0f / den : 0.0f;
             uint16_t r[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) r[i] = f2h(den != 0.0f ? num[i] / den : 0.0f);
-            *reinterpret_cast<uint2*>(a.o + (((size_t)b * a.S + vv / a.G) * a.Hq + (size_t)head * a.G + vv % a.G) * D + d) =
+            for (int i = 0; i < 4; i++) r[i] = f2h(num[i] * inv);
+            *reinterpret_cast<uint2*>(a.o + ((size_t)b * a.S * a.Hq + out_offset(a, head, vv)) * D + d) =
                 make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
         };
         const int nquad = nvec * (D / 4);
@@ -552,7 +594,7 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
             if (et == 0)
-                last_sh = __hip_atomic_fetch_add(a.counters + wg0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == nparts - 1;
+                last_sh = __hip_atomic_fetch_add(a.counters + wg0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == joined - 1;
             __syncthreads();
             if (last_sh) {
                 // a thread takes a quad of dims and every (threads / quads)-th part,
@@ -565,14 +607,14 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
                     const int cc = in ? e / (D / 4) : 0, d = in ? e % (D / 4) * 4 : 0;
                     f32x4 num = {0, 0, 0, 0};
                     float mx = -__builtin_inff(), den = 0.0f;
-                    for (int p0 = pl; in && p0 < (int)nparts; p0 += 8 * share) {
+                    for (int p0 = pl; in && p0 < (int)joined; p0 += 8 * share) {
                         f32x4 y[8];
                         float2 ml[8];
 #pragma unroll
                         for (int u = 0; u < 8; u++) {
                             y[u] = (f32x4){0, 0, 0, 0};
                             ml[u] = make_float2(-__builtin_inff(), 0.0f);
-                            if (p0 + u * share < (int)nparts) {
+                            if (p0 + u * share < (int)joined) {
                                 const float* row_at = part_row(wg0 + p0 + u * share, cc);
                                 const float2 lo = agent_load2(row_at + d), hi = agent_load2(row_at + d + 2);
                                 y[u] = (f32x4){lo.x, lo.y, hi.x, hi.y};
@@ -620,7 +662,7 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
             }
         }
         __syncthreads();
-        at += nblk;
+        at += parts ? 1 : nblk;
     }
 }
 
@@ -666,6 +708,7 @@ struct PrefillLine {
     int slot = -1, len = 0, rows = 0;                // of the lane's pair
     uint32_t blocks = 0, cost = 0, upto = 0;         // stages of a unit, of the pair, of the pairs up to it
     uint32_t total = 0, base = 0;                    // base: stages before the pair that find() found
+    bool whole = false;                              // the line counts units: each workgroup takes one
     int pair = 0;
 
     struct Span { int slot, len, rows, main0, sinks, steps; };
@@ -673,7 +716,7 @@ struct PrefillLine {
         Span s{slot, len, rows, 0, 0, 0};
         const int nv = rows * a.G, v0 = vb * NV;
         if (v0 >= nv) return s;
-        const int p0 = len - rows + v0 / a.G, p1 = len - rows + (min(v0 + NV, nv) - 1) / a.G;
+        const int p0 = len - rows + a.by_g(v0), p1 = len - rows + a.by_g(min(v0 + NV, nv) - 1);
         const int hi = max(0, a.causal ? min(len, p1 + 1) : len);
         const int lo = a.window > 0 && p0 > a.window ? min(p0 - a.window, hi) : 0;
         s.main0 = lo / KT;
@@ -688,7 +731,7 @@ struct PrefillLine {
         blocks = cost = 0;
         const int i = i0 + lane;
         if (i < npairs) {
-            const int b = i / nvb, vb = i % nvb;
+            const int b = a.by_nvb(i), vb = i - b * nvb;
             slot = kv4_slot(a.c, a.seqs, b);
             rows = slot < 0 ? 0 : kv4_count(a.counts, b, a.S);
             len = slot < 0 ? 0 : kv4_len(a.c, slot);
@@ -705,7 +748,21 @@ struct PrefillLine {
             total += lane_u(upto, 63);
             longest = max(longest, __builtin_amdgcn_readlane(wave_scan_max((int)blocks), 63));
         }
-        return max((total + workgroups - 1) / workgroups, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1));
+        const uint32_t per = max((total + workgroups - 1) / workgroups, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1));
+        // Where there is a workgroup for each unit and the longest is hardly longer
+        // than an equal share, a unit each saves the parts' way through memory (2048
+        // rows at 16384 keys, 32 / 8 heads of 128: 611 -> 591 us)
+        if (npairs <= 64 && (uint32_t)longest <= per + per / 8) {
+            const uint32_t units = blocks ? (uint32_t)a.c.Hkv : 0, sum = wave_scan_add(units);
+            if (lane_u(sum, 63) <= workgroups) {
+                whole = true;
+                total = lane_u(sum, 63);
+                cost = units;
+                upto = sum;
+                return (uint32_t)longest;
+            }
+        }
+        return per;
     }
     // the lane of the pair that stage `at` of the line belongs to
     __device__ int find(uint32_t at) {
@@ -742,19 +799,19 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
     const uint32_t qsign = a.scale < 0.0f ? 0x80008000u : 0u;
 
     PrefillLine<NV, KT> line(a, lane);
-    const uint32_t per = line.stretch(gridDim.x), total = line.total;
-    uint32_t at = blockIdx.x * per;
-    const uint32_t end = min(total, at + per);
+    const uint32_t per = line.stretch(gridDim.x);
+    uint32_t at = line.whole ? blockIdx.x : blockIdx.x * per;
+    const uint32_t end = min(line.total, line.whole ? at + 1 : at + per);
 
     while (at < end) {
         const int j = line.find(at);
         const uint32_t base = line.base, blocks = lane_u(line.blocks, j);
-        const int b = line.pair / line.nvb, vb = line.pair % line.nvb;
+        const int b = a.by_nvb(line.pair), vb = line.pair - b * line.nvb;
         const auto sq = line.span(__builtin_amdgcn_readlane(line.slot, j), __builtin_amdgcn_readlane(line.len, j),
                                   __builtin_amdgcn_readlane(line.rows, j), vb);
         const uint32_t rel = at - base;
-        const int head = (int)(rel / blocks);
-        const uint32_t s0 = rel % blocks, nblk = min(blocks - s0, end - at);
+        const int head = (int)(line.whole ? rel : rel / blocks);
+        const uint32_t s0 = line.whole ? 0 : rel % blocks, nblk = line.whole ? blocks : min(blocks - s0, end - at);
         const int nvec = min(NV, sq.rows * a.G - vb * NV);          // of the workgroup
         const int w0 = 32 * wid, wvec = max(0, min(32, nvec - w0)); // of this wave
         const int row0 = sq.len - sq.rows;
@@ -857,20 +914,20 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         int pos[2];
 #pragma unroll
         for (int cb = 0; cb < 2; cb++) {
-            const int vec = vb * NV + w0 + 16 * cb + col, row = vec / a.G;
+            const int vec = vb * NV + w0 + 16 * cb + col, row = a.by_g(vec);
             pos[cb] = row0 + row;
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 uint4 u = make_uint4(0, 0, 0, 0);
                 if (16 * cb + col < wvec)
                     u = *reinterpret_cast<const uint4*>(a.q + ((size_t)b * a.S + row) * a.q_stride +
-                                                        (size_t)(head * a.G + vec % a.G) * D + 32 * g + 8 * h);
+                                                        (size_t)(head * a.G + vec - row * a.G) * D + 32 * g + 8 * h);
                 u.x ^= qsign, u.y ^= qsign, u.z ^= qsign, u.w ^= qsign;
                 qf[cb][g] = code_order(u);
             }
         }
-        const int first_pos = row0 + (vb * NV + w0) / a.G;
-        const int last_pos = row0 + (vb * NV + w0 + max(wvec, 1) - 1) / a.G;
+        const int first_pos = row0 + a.by_g(vb * NV + w0);
+        const int last_pos = row0 + a.by_g(vb * NV + w0 + max(wvec, 1) - 1);
         const int all = a.causal ? min(first_pos + 1, sq.len) : sq.len;      // keys that each of them sees (but for a window)
 
         float m[2], mbase[2];
@@ -1070,12 +1127,12 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         const uint32_t wg0 = unit0 / per;    // the unit's first workgroup has it in slot 1 (see the few-row kernel)
         auto out_row = [&](int v) {
             const int vv = vb * NV + v;
-            return a.o + (((size_t)b * a.S + vv / a.G) * a.Hq + (size_t)head * a.G + vv % a.G) * D;
+            return a.o + ((size_t)b * a.S * a.Hq + out_offset(a, head, vv)) * D;
         };
-        auto write4 = [&](uint16_t* p, f32x4 num, float den) {
+        auto write4 = [&](uint16_t* p, f32x4 num, float inv) {
             uint16_t r[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) r[k] = f2h(den != 0.0f ? num[k] / den : 0.0f);
+            for (int k = 0; k < 4; k++) r[k] = f2h(num[k] * inv);
             *reinterpret_cast<uint2*>(p) = make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
         };
 #pragma unroll
@@ -1084,8 +1141,9 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
             if (v >= nvec) continue;
             if (alone) {
                 uint16_t* o = out_row(v);
+                const float inv = lsum[cb][0] != 0.0f ? 1.0f / lsum[cb][0] : 0.0f;
 #pragma unroll
-                for (int n = 0; n < NB; n++) write4(o + 16 * n + 4 * h, acc[cb][n], lsum[cb][0]);
+                for (int n = 0; n < NB; n++) write4(o + 16 * n + 4 * h, acc[cb][n], inv);
             } else {
                 float* row_at = a.part + ((size_t)(2 * blockIdx.x + (blockIdx.x == wg0)) * NV + v) * (D + 4);
 #pragma unroll
@@ -1094,7 +1152,7 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
             }
         }
         __syncthreads();
-        at += nblk;
+        at += line.whole ? 1 : nblk;
     }
 }
 
@@ -1108,6 +1166,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(Kv4AttnArgs a, uint3
     const int tid = threadIdx.x, lane = tid & 63;
     PrefillLine<NV, KT> line(a, lane);
     const uint32_t per = line.stretch(workgroups);
+    if (line.whole) return;
     // this workgroup's unit: the pair's place in the line, then the head
     const int v0 = (int)(blockIdx.x % NVJ) * PJ_VEC, head = (int)(blockIdx.x / NVJ % a.c.Hkv);
     const int pair = (int)(blockIdx.x / NVJ / a.c.Hkv), j = pair & 63;
@@ -1118,7 +1177,7 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(Kv4AttnArgs a, uint3
     }
     const uint32_t blocks = lane_u(line.blocks, j);
     if (blocks == 0) return;
-    const int b = pair / line.nvb, vb = pair % line.nvb;
+    const int b = a.by_nvb(pair), vb = pair - b * line.nvb;
     const int nvec = min(NV, __builtin_amdgcn_readlane(line.rows, j) * a.G - vb * NV);
     const uint32_t unit0 = base + (uint32_t)head * blocks;
     const uint32_t wg0 = unit0 / per, nparts = (unit0 + blocks - 1) / per - wg0 + 1;
@@ -1157,10 +1216,11 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(Kv4AttnArgs a, uint3
             }
         }
         const int vv = vb * NV + v;
+        const float inv = den != 0.0f ? 1.0f / den : 0.0f;
         uint16_t r[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) r[k] = f2h(den != 0.0f ? num[k] / den : 0.0f);
-        *reinterpret_cast<uint2*>(a.o + (((size_t)b * a.S + vv / a.G) * a.Hq + (size_t)head * a.G + vv % a.G) * D + d) =
+        for (int k = 0; k < 4; k++) r[k] = f2h(num[k] * inv);
+        *reinterpret_cast<uint2*>(a.o + ((size_t)b * a.S * a.Hq + out_offset(a, head, vv)) * D + d) =
             make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
     }
 }
@@ -1211,6 +1271,7 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     a.S = (int)seq_len;
     a.Hq = (int)num_q_heads;
     a.G = (int)G;
+    a.by_g.set((uint32_t)G);
     a.window = (int)std::min(window_size, top);
     a.sink = (int)std::min(sink_size, top);
     a.causal = is_causal != 0;
@@ -1223,7 +1284,8 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     const size_t vectors = seq_len * G;
     auto launch = [&](auto kernel, int per_unit, int per_cu, int waves, unsigned* workgroups) {
         const size_t units = batch * cache->kv_heads * ceil_div(vectors, per_unit);
-        if (units >= (1u << 31) / blocks / PJ_VEC)
+        // (the line counts in 32 bits, and the joining launch has 16 workgroups of 256 for a unit)
+        if (units >= (1u << 31) / blocks || (waves == per_unit / 32 && units >= (1u << 20)))
             return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows times table length is too large");
         *workgroups = (unsigned)std::min<size_t>(256 * per_cu, units * blocks);
         hipLaunchKernelGGL(kernel, dim3(*workgroups), dim3(64 * waves), 0, st, a);
@@ -1231,6 +1293,7 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     };
     auto many = [&](auto kernel, auto join, int waves) {
         unsigned workgroups = 0;
+        a.by_nvb.set((uint32_t)ceil_div(vectors, 32 * waves));
         const int r = launch(kernel, 32 * waves, 1, waves, &workgroups);
         if (r) return r;
         const unsigned units = (unsigned)(batch * cache->kv_heads * ceil_div(vectors, 32 * waves));

@@ -684,7 +684,8 @@ __global__ void __launch_bounds__(256) kv4_compact_apply_kernel(Kv4View c, Compa
         const int id = c.table[e];
         if (!kv4_page_ok(c, id) || id < live) continue;
         const int s = (int)(e / (uint32_t)c.max_pages), j = (int)(e % (uint32_t)c.max_pages);
-        if (j < kv4_pages_of(c, kv4_len(c, s)) && p.rank[id] < moves) c.table[e] = p.to[p.rank[id]];
+        const uint32_t r = (uint32_t)p.rank[id];
+        if (j < kv4_pages_of(c, kv4_len(c, s)) && r < (uint32_t)moves) c.table[e] = p.to[r];
     }
     if (me == 0) {
         c.state[KV4_FREE] = c.num_pages - live;
@@ -810,8 +811,8 @@ int cactus_hip_kv4_append_f16(const cactus_hip_kv4_cache* cache, size_t layer, c
     CH_REQUIRE(((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0 && kv_stride % 8 == 0,
                "kv4_append: rows are not 16-byte aligned");
     CH_REQUIRE(kv_stride >= cache->kv_heads * cache->head_dim, "kv4_append: kv_stride is shorter than a row");
-    CH_REQUIRE(batch <= cache->max_seqs, "kv4_append: more requests than slots");
-    CH_REQUIRE(seq_len < (1u << 30), "kv4_append: seq_len out of range");
+    CH_REQUIRE(batch <= cache->max_seqs && batch <= 65535, "kv4_append: more requests than slots, or than 65535");
+    CH_REQUIRE(seq_len <= (1u << 28), "kv4_append: seq_len out of range");
     const dim3 grid(ceil_div(seq_len + 15, 16), c.Hkv, (unsigned)batch);
     switch (c.d) {
         case 64: hipLaunchKernelGGL(kv4_append_kernel<64>, grid, dim3(128), 0, as_stream(stream), c, seqs, counts, k, v, (int)seq_len, kv_stride); break;
@@ -830,7 +831,7 @@ int cactus_hip_kv4_read_f16(const cactus_hip_kv4_cache* cache, size_t layer, con
     if (batch == 0 || seq_len == 0 || (!k && !v)) return CACTUS_HIP_OK;
     CH_REQUIRE(((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0, "kv4_read: rows are not 16-byte aligned");
     CH_REQUIRE(batch <= 65535, "kv4_read: more than 65535 requests");
-    CH_REQUIRE(seq_len < (1u << 30), "kv4_read: seq_len out of range");
+    CH_REQUIRE(seq_len <= (1u << 28), "kv4_read: seq_len out of range");
     const dim3 grid(ceil_div(seq_len + 15, 16), c.Hkv, (unsigned)batch);
     switch (c.d) {
         case 64: hipLaunchKernelGGL(kv4_read_kernel<64>, grid, dim3(128), 0, as_stream(stream), c, seqs, starts, counts, k, v, (int)seq_len); break;
@@ -870,7 +871,7 @@ int cactus_hip_kv4_free(const cactus_hip_kv4_cache* cache, const int32_t* seqs, 
     int rc = kv4_view(cache, 0, "kv4_free", &c);
     if (rc) return rc;
     if (n == 0) return CACTUS_HIP_OK;
-    CH_REQUIRE(n < (1u << 31), "kv4_free: too many requests");
+    CH_REQUIRE(n < (1u << 24), "kv4_free: too many requests");
     hipLaunchKernelGGL(kv4_free_kernel, dim3((unsigned)n), dim3(256), 0, as_stream(stream), c, seqs);
     return check_launch("kv4_free");
 }
@@ -900,7 +901,7 @@ int cactus_hip_kv4_copy_pages(const cactus_hip_kv4_cache* cache, const int32_t* 
     if (rc) return rc;
     if (n == 0) return CACTUS_HIP_OK;
     CH_REQUIRE(src && dst, "kv4_copy_pages: null pointer");
-    CH_REQUIRE(n <= cache->num_pages, "kv4_copy_pages: more pairs than pages");
+    CH_REQUIRE(n <= cache->num_pages && n < (1u << 24), "kv4_copy_pages: more pairs than pages, or than 2^24");
     const int pieces = (int)ceil_div(c.page_bytes, COPY_PIECE);
     hipLaunchKernelGGL(kv4_copy_kernel, dim3((unsigned)n, c.layers * pieces), dim3(256), 0, as_stream(stream), c, src, dst, pieces);
     return check_launch("kv4_copy_pages");

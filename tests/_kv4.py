@@ -1,6 +1,7 @@
 """Plain restatement of the paged 4-bit KV cache in numpy, 64 bits: the
 quantization, the page layout byte by byte, the page bookkeeping and the
 attention, with the error that the kernels' roundings may make."""
+import functools
 import math
 
 import numpy as np
@@ -44,6 +45,13 @@ def code_at(d, key, dim, value):
 
 def scale_at(d, key, g, value):
     return (17 if value else 8) * d + 2 * ((key // 4 * (d // 32) + g) * 4 + key % 4)
+
+
+@functools.lru_cache(None)
+def places(d, key, value):
+    """Bytes and shifts of a token's codes, and bytes of its scales."""
+    at = np.array([code_at(d, key, i, value) for i in range(d)])
+    return at[:, 0], at[:, 1], np.array([scale_at(d, key, g, value) for g in range(d // GROUP)])
 
 
 class Model:
@@ -128,16 +136,16 @@ class Model:
     def write(self, layer, slot, pos, k, v):
         """k, v [H][d] fp16 as the token at `pos`."""
         page = self.pages[layer, self.table[slot, pos // self.ps]]
-        t, key = pos % self.ps // TILE, pos % TILE
+        tile, key = page[:, pos % self.ps // TILE], pos % TILE
         for x, is_v in ((k, False), (v, True)):
             c, s = quantize(x)
-            for dim in range(self.d):
-                at, up = code_at(self.d, key, dim, is_v)
-                keep = page[:, t, at] & (0xF0 if up == 0 else 0x0F)
-                page[:, t, at] = keep | ((c[:, dim] + 8) << up).astype(np.uint8)
-            for g in range(self.d // GROUP):
-                at = scale_at(self.d, key, g, is_v)
-                page[:, t, at:at + 2] = np.ascontiguousarray(s[:, g]).view(np.uint8).reshape(-1, 2)
+            at, up, sat = places(self.d, key, is_v)
+            for shift in (0, 4):                  # the two nibbles of the token's bytes
+                mine = up == shift
+                keep = tile[:, at[mine]] & (0xF0 if shift == 0 else 0x0F)
+                tile[:, at[mine]] = keep | ((c[:, mine] + 8) << shift).astype(np.uint8)
+            b = np.ascontiguousarray(s).view(np.uint8).reshape(self.H, -1, 2)
+            tile[:, sat], tile[:, sat + 1] = b[..., 0], b[..., 1]
 
     def read(self, layer, slot, n=None):
         """Codes [n][H][d] and scales [n][H][d / 32] of a slot's keys and values, from the page bytes."""
@@ -147,12 +155,10 @@ class Model:
             return (z, s), (z, s)
         ids = self.table[slot, :self.npages(n)]
         tiles = self.pages[layer, ids].transpose(0, 2, 1, 3).reshape(-1, self.H, 18 * self.d)
-        key, dim, g = np.arange(TILE), np.arange(self.d), np.arange(self.d // GROUP)
         out = []
         for is_v in (False, True):
-            at = np.array([[code_at(self.d, k, i, is_v) for i in dim] for k in key])
-            sa = np.array([[scale_at(self.d, k, i, is_v) for i in g] for k in key])
-            c = (tiles[:, :, at[..., 0]].astype(np.int64) >> at[..., 1]) % 16 - 8          # [tile][H][key][d]
+            at, up, sa = (np.stack(x) for x in zip(*(places(self.d, k, is_v) for k in range(TILE))))
+            c = (tiles[:, :, at].astype(np.int64) >> up) % 16 - 8          # [tile][H][key][d]
             raw = np.stack([tiles[:, :, sa], tiles[:, :, sa + 1]], -1)
             s = np.ascontiguousarray(raw).view(np.float16)[..., 0]
             c = c.transpose(0, 2, 1, 3).reshape(-1, self.H, self.d)[:n]
@@ -193,27 +199,32 @@ def attention(q, kc, ks, vc, vs, n, scale, window=0, sink=0, causal=True):
     seen = seen & (pos >= -(1 << 40))
     e = 2.0 ** -24
     for h in range(Hq):
-        kh, vh = k[:, h // G], v[:, h // G]
+        kh, vh, vch = k[:, h // G], v[:, h // G], np.abs(vc[:, h // G])
         qh = q[:, h].astype(np.float64)
-        x = qh @ kh.T * scale
-        err = (d + 16) * e * abs(scale) * (np.abs(qh) @ k16[:, h // G].T)
-        for r in range(m):
-            s = seen[r]
-            if not s.any():
-                continue
-            xr = x[r, s]
-            if np.isnan(xr).any():     # a key that reads as NaN; a value does so in its own dims only
-                o[r, h] = np.nan
-                continue
-            mx = xr.max()
-            p = np.exp(xr - mx)
-            L = p.sum()
-            o[r, h] = p @ vh[s] / L
-            ao, av = np.abs(o[r, h]), np.abs(vh[s])
-            w = err[r, s] + err[r, s].max() + 4 * e * (np.abs(xr) + abs(mx)) + 4 * e
-            ps = p[:, None] * v16[s, h // G] / 16
-            tol[r, h] += 2.0 ** -11 * ao + 2.0 ** -11 * (p @ av) / L
-            tol[r, h] += 2.0 ** -25 * ((ps < 2.0 ** -14) * np.abs(vc[s, h // G])).sum(0) / L
-            tol[r, h] += ((p * w) @ av + (p * w).sum() * ao) / L
-            tol[r, h] += 3 * (s.sum() + 64) * e * (ao + p @ v16[s, h // G] / L)
+        x = np.where(seen, qh @ kh.T * scale, -np.inf)
+        err = np.where(seen, (d + 16) * e * abs(scale) * (np.abs(qh) @ k16[:, h // G].T), 0)
+        bad = np.isnan(x).any(1)                       # rows that see a key that reads as NaN
+        mx = np.where(np.isfinite(x), x, -np.inf).max(1, initial=-np.inf)
+        some = (mx > -np.inf) & ~bad
+        base = np.where(some, mx, 0)[:, None]
+        p = np.where(seen & some[:, None], np.exp(np.where(seen, x, -np.inf) - base), 0)
+        L = np.where(some, p.sum(1), 1)[:, None]
+        # a value that reads as NaN does so in its own dims, for the rows that see its key
+        nan = np.isnan(vh)
+        hit = seen.astype(np.float64) @ nan > 0
+        vz, v16z = np.where(nan, 0, vh), np.where(np.isnan(v16[:, h // G]), 0, v16[:, h // G])
+        av = np.abs(vz)
+        oh = p @ vz / L
+        ao = np.abs(oh)
+        w = err + err.max(1, initial=0)[:, None] + 4 * e * (np.abs(np.where(seen, x, 0)) + np.abs(base)) + 4 * e
+        t = 2.0 ** -25 + 2.0 ** -11 * ao + 2.0 ** -11 * (p @ av) / L
+        for g in range(d // GROUP):
+            s = slice(g * GROUP, (g + 1) * GROUP)
+            small = seen & (p * v16z[:, g * GROUP] / 16 < 2.0 ** -14)
+            t[:, s] += 2.0 ** -25 * (small @ vch[:, s]) / L
+        pw = p * np.where(np.isnan(w), 0, w)
+        t += (pw @ av + pw.sum(1)[:, None] * ao) / L
+        t += 3 * (seen.sum(1)[:, None] + 64) * e * (ao + p @ v16z / L)
+        o[:, h] = np.where(bad[:, None] | (hit & (seen.any(1)[:, None])), np.nan, np.where(some[:, None], oh, 0))
+        tol[:, h] = t
     return o, tol

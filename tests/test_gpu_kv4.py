@@ -194,6 +194,86 @@ def test_many_rows(hip_ready, d, G, lens, counts, window, sink, causal, scale):
     c.attend(q, range(len(lens)), counts, window=window, sink=sink, causal=causal, scale=scale)
 
 
+@pytest.mark.parametrize("S", [3, 40])
+def test_more_rows_than_tokens(hip_ready, S):
+    """Rows before the first token: positions below 0, which causal rows see nothing from."""
+    rng = np.random.default_rng(S)
+    c = Cache(hip_ready, 1, 2, 64, 16, 20, 3, 8)
+    c.fill(rng, [2, 30])
+    q = rng.standard_normal((3, S, 4, 64)).astype(np.float16)
+    c.attend(q, [0, 1, 2], [S, S, S])
+    c.attend(q, [0, 1, 2], [S, S, S], causal=False)
+
+
+def test_offsets_past_32_bits(hip_ready):
+    """A pool of 4.9 GB of which only the last pages are used."""
+    from cactus_amd.kv4 import CacheDesc
+    cm, rng = hip_ready, np.random.default_rng(21)
+    H, d, ps, N, n = 8, 256, 256, 8300, 600
+    one = Cache(cm, 1, H, d, ps, 4, 1, 4)                     # the same tokens in a small pool
+    assert one.extend([0], [n]) == 0
+    k, v = kv_rows(rng, 1, n, H, d), kv_rows(rng, 1, n, H, d)
+    page = H * ps * d * 9 // 8
+    pool = cm.DeviceBuffer(N * page)
+    table = np.full((1, 4), -1, np.int32)
+    table[0, :3] = [N - 1, 8000, N - 7]
+    bufs = [cm.DeviceBuffer.from_numpy(x) for x in (table, np.array([n], np.int32), np.zeros(N, np.int32), np.zeros(4, np.int32))]
+    desc = CacheDesc(pages=pool.ptr, table=bufs[0].ptr, lens=bufs[1].ptr, refs=bufs[2].ptr, state=bufs[3].ptr, layers=1,
+                     kv_heads=H, head_dim=d, page_size=ps, num_pages=N, max_seqs=1, max_pages=4)
+    dk, dv = cm.DeviceBuffer.from_numpy(k), cm.DeviceBuffer.from_numpy(v)
+    for c in (desc, one.gpu.desc):
+        cm.call("cactus_hip_kv4_append_f16", c.ref, 0, None, None, dk.ptr, dv.ptr, 1, n, H * d, None)
+    for S, Hq in ((1, 16), (5, 32), (60, 8)):
+        q = rng.standard_normal((1, S, Hq, d)).astype(np.float16)
+        dq, outs = cm.DeviceBuffer.from_numpy(q), []
+        for c in (desc, one.gpu.desc):
+            need = cm.hip().cactus_hip_attention_kv4_workspace(c.ref, 1, S, Hq)
+            work, do = cm.DeviceBuffer(need), cm.DeviceBuffer(q.nbytes)
+            cm.call("cactus_hip_memset", work.ptr, 0, 4096, None)
+            cm.call("cactus_hip_attention_kv4_f16", c.ref, 0, None, None, dq.ptr, Hq * d, do.ptr, 1, S, Hq, 0.0, 0, 0, 1,
+                    work.ptr, need, None)
+            outs.append(do.to_numpy(np.uint16, q.shape))
+        np.testing.assert_array_equal(*outs)                  # the same bits wherever the pages lie
+    # pages far up copied far up
+    lists = [cm.DeviceBuffer.from_numpy(np.array(x, np.int32)) for x in ([N - 1, 8000], [N - 3, 7999])]
+    cm.call("cactus_hip_kv4_copy_pages", desc.ref, lists[0].ptr, lists[1].ptr, 2, None)
+    table[0, :2] = [N - 3, 7999]
+    bufs[0].upload(table)
+    back = [[cm.DeviceBuffer(k.nbytes) for _ in range(2)] for _ in range(2)]
+    for c, (bk, bv) in zip((desc, one.gpu.desc), back):
+        cm.call("cactus_hip_kv4_read_f16", c.ref, 0, None, None, None, bk.ptr, bv.ptr, 1, n, None)
+    for i in range(2):
+        np.testing.assert_array_equal(*(b[i].to_numpy(np.uint16, k.shape) for b in back))
+
+
+def test_two_streams_at_once(hip_ready):
+    """Calls that overlap, with a workspace each, give what they give alone."""
+    cm, rng = hip_ready, np.random.default_rng(22)
+    c = Cache(cm, 1, 4, 128, 16, 700, 3, 300)
+    c.fill(rng, [4000, 333, 2500])
+    cases = []
+    for S in (1, 7, 50):
+        q = rng.standard_normal((3, S, 8, 128)).astype(np.float16)
+        need = cm.hip().cactus_hip_attention_kv4_workspace(c.gpu.desc.ref, 3, S, 8)
+        alone = c.attend(q, [0, 1, 2], [S] * 3)
+        work = [cm.DeviceBuffer(need) for _ in range(2)]
+        for w in work:
+            cm.call("cactus_hip_memset", w.ptr, 0, 4096, None)
+        cases.append((S, cm.DeviceBuffer.from_numpy(q), alone, need, work, [cm.DeviceBuffer(q.nbytes) for _ in range(2)]))
+    cm.call("cactus_hip_stream_sync", None)
+    streams = [cm.Stream(), cm.Stream()]
+    for _ in range(5):
+        for S, dq, _, need, work, do in cases:
+            for i in range(2):
+                cm.call("cactus_hip_attention_kv4_f16", c.gpu.desc.ref, 0, None, None, dq.ptr, 8 * 128, do[i].ptr, 3, S, 8, 0.0,
+                        0, 0, 1, work[i].ptr, need, streams[i].handle)
+    for s in streams:
+        s.sync()
+    for S, _, alone, _, _, do in cases:
+        for b in do:
+            np.testing.assert_array_equal(b.to_numpy(np.float16, alone.shape), alone)
+
+
 def test_long_decode_and_sharp_softmax(hip_ready):
     rng = np.random.default_rng(3)
     c = Cache(hip_ready, 1, 1, 128, 64, 40, 3, 34)
