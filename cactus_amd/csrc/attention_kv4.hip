@@ -674,15 +674,21 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
 // does not round, and the scores and outputs are plain products without a scale
 // per group.  The waves write the values to LDS in the order of the matrix
 // operands, two stages in turn: stage t + 1 is written while stage t is used, and
-// stage t + 2's codes are on their way to registers.
+// stage t + 2's tiles are on their way to LDS as they are stored.
 //
 // A column's maximum is raised only when a score exceeds it by 2^PF_SLACK: the
 // weights stay below 2^8 (FP16 holds 2^16), and the outputs are rescaled a few
 // times per row instead of at every new maximum.  The sum of the weights is a
 // product with ones, of the rounded weights that the outputs use.
 constexpr int PF_SLACK = 8;
-constexpr size_t PF_FROM = 32;   // more query vectors per KV head than this
-
+//
+// More query vectors of a request per KV head than PF_FROM come here.  Its 256
+// columns (D = 256: 128) are dear for few vectors and its joining is a second
+// launch: 40 vectors at 4096 keys, 8 heads of 128: 14.2 us there, 20.6 here; 8
+// requests of 40 at 9000: 62 and 73; 16 of 64 at 2000: 41 and 46.  With more the
+// codes are unpacked too often there: 4 requests of 68 at 4096: 33.5 there, 27.5
+// here; one of 128 at 32000: 71 and 46 (at 8000 25 and 26, at 2000 13 and 20).
+constexpr size_t PF_FROM = 64;
 
 typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ h16x2 as_h2(uint32_t u) { return __builtin_bit_cast(h16x2, u); }
@@ -708,7 +714,8 @@ struct PrefillLine {
     int slot = -1, len = 0, rows = 0;                // of the lane's pair
     uint32_t blocks = 0, cost = 0, upto = 0;         // stages of a unit, of the pair, of the pairs up to it
     uint32_t total = 0, base = 0;                    // base: stages before the pair that find() found
-    bool whole = false;                              // the line counts units: each workgroup takes one
+    bool single = false;                             // and each unit is one part
+    bool parts = false;                              // the line counts parts of units: each workgroup takes one
     int pair = 0;
 
     struct Span { int slot, len, rows, main0, sinks, steps; };
@@ -749,18 +756,29 @@ struct PrefillLine {
             longest = max(longest, __builtin_amdgcn_readlane(wave_scan_max((int)blocks), 63));
         }
         const uint32_t per = max((total + workgroups - 1) / workgroups, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1));
-        // Where there is a workgroup for each unit and the longest is hardly longer
-        // than an equal share, a unit each saves the parts' way through memory (2048
-        // rows at 16384 keys, 32 / 8 heads of 128: 611 -> 591 us)
-        if (npairs <= 64 && (uint32_t)longest <= per + per / 8) {
-            const uint32_t units = blocks ? (uint32_t)a.c.Hkv : 0, sum = wave_scan_add(units);
-            if (lane_u(sum, 63) <= workgroups) {
-                whole = true;
-                total = lane_u(sum, 63);
-                cost = units;
-                upto = sum;
-                return (uint32_t)longest;
-            }
+        // Units cut into whole parts, as in the few-row kernel, where they make no more
+        // parts than there are workgroups (333 rows at 3333 keys, 16 / 8 heads of 128:
+        // 31 -> 27 us); one part where the longest unit is hardly longer than an equal
+        // share, which saves the parts' way through memory (2048 rows at 16384 keys,
+        // 32 / 8 heads: 611 -> 591 us with the joining).
+        if (npairs <= 64) {
+            const uint32_t units = blocks ? (uint32_t)a.c.Hkv : 0;
+            const uint32_t pair_cost = cost, pair_upto = upto;
+            auto fits = [&](uint32_t q) {
+                cost = units * ((blocks + q - 1) / q);
+                upto = wave_scan_add(cost);
+                if (lane_u(upto, 63) > workgroups) return false;
+                parts = true;
+                single = q >= (uint32_t)longest;
+                total = lane_u(upto, 63);
+                return true;
+            };
+            const uint32_t most = per <= 12 ? per + 2 : per;
+            for (uint32_t q = per; q <= most; q++)
+                if (fits(q)) return q;
+            if ((uint32_t)longest <= per + per / 8 && fits((uint32_t)longest)) return (uint32_t)longest;
+            cost = pair_cost;
+            upto = pair_upto;
         }
         return per;
     }
@@ -798,10 +816,17 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
     const float kscale = __builtin_fabsf(a.scale);   // (a negative one turns the sign of q)
     const uint32_t qsign = a.scale < 0.0f ? 0x80008000u : 0u;
 
+    // no marks: here, and behind each unit
+    auto clear_marks = [&]() {
+        for (int e = tid; e < 2 * KT; e += 64 * W) (&nan_sh[0][0])[e] = 0;
+        if (tid < 2) any_sh[tid] = 0;
+    };
+    clear_marks();
     PrefillLine<NV, KT> line(a, lane);
     const uint32_t per = line.stretch(gridDim.x);
-    uint32_t at = line.whole ? blockIdx.x : blockIdx.x * per;
-    const uint32_t end = min(line.total, line.whole ? at + 1 : at + per);
+    __syncthreads();
+    uint32_t at = line.parts ? blockIdx.x : blockIdx.x * per;
+    const uint32_t end = min(line.total, line.parts ? at + 1 : at + per);
 
     while (at < end) {
         const int j = line.find(at);
@@ -810,8 +835,10 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         const auto sq = line.span(__builtin_amdgcn_readlane(line.slot, j), __builtin_amdgcn_readlane(line.len, j),
                                   __builtin_amdgcn_readlane(line.rows, j), vb);
         const uint32_t rel = at - base;
-        const int head = (int)(line.whole ? rel : rel / blocks);
-        const uint32_t s0 = line.whole ? 0 : rel % blocks, nblk = line.whole ? blocks : min(blocks - s0, end - at);
+        const uint32_t nparts = (blocks + per - 1) / per, span = line.parts ? nparts : blocks;
+        const int head = (int)(rel / span);
+        const uint32_t first = rel - (uint32_t)head * span, s0 = line.parts ? first * per : first;
+        const uint32_t nblk = min(blocks - s0, line.parts ? per : end - at);
         const int nvec = min(NV, sq.rows * a.G - vb * NV);          // of the workgroup
         const int w0 = 32 * wid, wvec = max(0, min(32, nvec - w0)); // of this wave
         const int row0 = sq.len - sq.rows;
@@ -910,7 +937,8 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         };
 
         // ---- this wave's vectors: lane's column in two blocks of 16
-        h16x8 qf[2][NG];
+        // (their loads go ahead of the first tile's, which wait for its page number)
+        uint4 qraw[2][NG];
         int pos[2];
 #pragma unroll
         for (int cb = 0; cb < 2; cb++) {
@@ -922,10 +950,19 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                 if (16 * cb + col < wvec)
                     u = *reinterpret_cast<const uint4*>(a.q + ((size_t)b * a.S + row) * a.q_stride +
                                                         (size_t)(head * a.G + vec - row * a.G) * D + 32 * g + 8 * h);
-                u.x ^= qsign, u.y ^= qsign, u.z ^= qsign, u.w ^= qsign;
-                qf[cb][g] = code_order(u);
+                qraw[cb][g] = u;
             }
         }
+        const int i0 = (int)s0, i1 = min(sq.steps, (int)(s0 + nblk));
+        if (i0 < i1) fetch(i0);
+        h16x8 qf[2][NG];
+#pragma unroll
+        for (int cb = 0; cb < 2; cb++)
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint4 u = qraw[cb][g];
+                qf[cb][g] = code_order(make_uint4(u.x ^ qsign, u.y ^ qsign, u.z ^ qsign, u.w ^ qsign));
+            }
         const int first_pos = row0 + a.by_g(vb * NV + w0);
         const int last_pos = row0 + a.by_g(vb * NV + w0 + max(wvec, 1) - 1);
         const int all = a.causal ? min(first_pos + 1, sq.len) : sq.len;      // keys that each of them sees (but for a window)
@@ -945,9 +982,9 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         const h16x8 ones = __builtin_bit_cast(h16x8, one4);
 
         // ---- a stage: its 32-key parts in turn, the next part's scores beside this
-        // one's powers of two, then this part's outputs beside a share of the next
-        // stage's values.  Operands are read from LDS a group of products ahead; the
-        // barriers and groups keep the compiler from moving them together.
+        // one's powers of two, then this part's outputs.  Operands are read from LDS a
+        // group of products ahead; the barriers and groups keep the compiler from
+        // moving them together.
         constexpr int VG = 4, NVG = NB / VG;
         auto stage = [&](int i, int buf, uint32_t there) {
             const int key0 = key_of(i);
@@ -1095,16 +1132,11 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         };
 
         // ---- the stages
-        const int i0 = (int)s0, i1 = min(sq.steps, (int)(s0 + nblk));
-        for (int e = tid; e < 2 * KT; e += 64 * W) (&nan_sh[0][0])[e] = 0;
-        if (tid < 2) any_sh[tid] = 0;
-        __syncthreads();
         // Iteration i writes stage i + 1's operands and uses stage i's (from i0 - 1 on:
         // one copy of the code).  Two waves share a SIMD's units: the first four prepare
         // the next stage before their products, the others after theirs, so that one
         // wave's vector instructions run beside the other's matrix ones.
         uint32_t now = 0;
-        if (i0 < i1) fetch(i0);
 #pragma unroll 1
         for (int i = i0 - 1; i < i1; i++) {
             const uint32_t next = there;
@@ -1121,10 +1153,12 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
             __syncthreads();
         }
 
+        clear_marks();
+
         // ---- outputs, or this workgroup's part of them
         const bool alone = nblk == blocks;
         const uint32_t unit0 = base + (uint32_t)head * blocks;
-        const uint32_t wg0 = unit0 / per;    // the unit's first workgroup has it in slot 1 (see the few-row kernel)
+        const uint32_t wg0 = line.parts ? blockIdx.x - first : unit0 / per;    // the unit's first workgroup has it in slot 1
         auto out_row = [&](int v) {
             const int vv = vb * NV + v;
             return a.o + ((size_t)b * a.S * a.Hq + out_offset(a, head, vv)) * D;
@@ -1152,23 +1186,27 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
             }
         }
         __syncthreads();
-        at += line.whole ? 1 : nblk;
+        at += line.parts ? 1 : nblk;
     }
 }
 
-// The joining of units that several workgroups shared, PJ_VEC vectors per
-// workgroup.  A launch of its own: the last workgroup of a unit, joining 256
-// vectors' parts alone, took longer than the products of a few hundred rows.
-constexpr int PJ_VEC = 16;
+// The joining of units that several workgroups shared, a quad of dims per thread,
+// eight parts' loads at a time: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.  A
+// launch of its own: the last workgroup of a unit, joining 256 vectors' parts
+// alone, took longer than the products of a few hundred rows.  Bound by the
+// latency of the lengths, then of the parts (333 rows, 16 / 8 heads of 128: 7.9
+// us; 40 vectors in 32 parts 7.0, with a part after the other 12.9).
+template <int D>
+constexpr int pj_vec() { return 1024 / D; }       // vectors of a workgroup
 template <int D, int W>
 __global__ void __launch_bounds__(256) attn_kv4_join_kernel(Kv4AttnArgs a, uint32_t workgroups) {
-    constexpr int NV = 32 * W, KT = 16 * W, NVJ = NV / PJ_VEC;
+    constexpr int NV = 32 * W, KT = 16 * W, VEC = pj_vec<D>(), NVJ = NV / VEC;
     const int tid = threadIdx.x, lane = tid & 63;
     PrefillLine<NV, KT> line(a, lane);
     const uint32_t per = line.stretch(workgroups);
-    if (line.whole) return;
+    if (line.single) return;
     // this workgroup's unit: the pair's place in the line, then the head
-    const int v0 = (int)(blockIdx.x % NVJ) * PJ_VEC, head = (int)(blockIdx.x / NVJ % a.c.Hkv);
+    const int v0 = (int)(blockIdx.x % NVJ) * VEC, head = (int)(blockIdx.x / NVJ % a.c.Hkv);
     const int pair = (int)(blockIdx.x / NVJ / a.c.Hkv), j = pair & 63;
     uint32_t base = 0;
     for (int i0 = 0; i0 <= pair; i0 += 64) {
@@ -1179,19 +1217,20 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(Kv4AttnArgs a, uint3
     if (blocks == 0) return;
     const int b = a.by_nvb(pair), vb = pair - b * line.nvb;
     const int nvec = min(NV, __builtin_amdgcn_readlane(line.rows, j) * a.G - vb * NV);
-    const uint32_t unit0 = base + (uint32_t)head * blocks;
-    const uint32_t wg0 = unit0 / per, nparts = (unit0 + blocks - 1) / per - wg0 + 1;
+    const uint32_t own = (blocks + per - 1) / per;                  // parts of the unit, where the line counts parts
+    const uint32_t unit0 = base + (uint32_t)head * (line.parts ? own : blocks);
+    const uint32_t wg0 = line.parts ? unit0 : unit0 / per;
+    const uint32_t nparts = line.parts ? own : (unit0 + blocks - 1) / per - wg0 + 1;
     if (nparts == 1) return;
-    for (int e = tid; e < PJ_VEC * (D / 4); e += 256) {
-        const int v = v0 + e / (D / 4), d = e % (D / 4) * 4;
-        if (v >= nvec) break;
+    const int v = v0 + tid / (D / 4), d = tid % (D / 4) * 4;
+    if (v < nvec) {
         f32x4 num = {0, 0, 0, 0};
         float mx = -__builtin_inff(), den = 0.0f;
-        for (int p0 = 0; p0 < (int)nparts; p0 += 4) {
-            f32x4 y[4];
-            float2 ml[4];
+        for (int p0 = 0; p0 < (int)nparts; p0 += 8) {
+            f32x4 y[8];
+            float2 ml[8];
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
+            for (int u = 0; u < 8; u++) {
                 y[u] = (f32x4){0, 0, 0, 0};
                 ml[u] = make_float2(-__builtin_inff(), 0.0f);
                 if (p0 + u < (int)nparts) {
@@ -1202,13 +1241,13 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(Kv4AttnArgs a, uint3
             }
             float mn = mx;
 #pragma unroll
-            for (int u = 0; u < 4; u++) mn = __builtin_fmaxf(mn, ml[u].x);
+            for (int u = 0; u < 8; u++) mn = __builtin_fmaxf(mn, ml[u].x);
             const float f0 = mx > -__builtin_inff() ? exp2_fast(mx - mn) : 1.0f;
             mx = mn;
             num *= f0;
             den *= f0;
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
+            for (int u = 0; u < 8; u++) {
                 const float f = ml[u].x > -__builtin_inff() ? exp2_fast(ml[u].x - mx) : 1.0f;
 #pragma unroll
                 for (int k = 0; k < 4; k++) num[k] = __builtin_fmaf(f, y[u][k], num[k]);
@@ -1284,8 +1323,7 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     const size_t vectors = seq_len * G;
     auto launch = [&](auto kernel, int per_unit, int per_cu, int waves, unsigned* workgroups) {
         const size_t units = batch * cache->kv_heads * ceil_div(vectors, per_unit);
-        // (the line counts in 32 bits, and the joining launch has 16 workgroups of 256 for a unit)
-        if (units >= (1u << 31) / blocks || (waves == per_unit / 32 && units >= (1u << 20)))
+        if (units >= (1u << 31) / blocks)        // (the line counts in 32 bits)
             return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows times table length is too large");
         *workgroups = (unsigned)std::min<size_t>(256 * per_cu, units * blocks);
         hipLaunchKernelGGL(kernel, dim3(*workgroups), dim3(64 * waves), 0, st, a);
@@ -1294,10 +1332,12 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     auto many = [&](auto kernel, auto join, int waves) {
         unsigned workgroups = 0;
         a.by_nvb.set((uint32_t)ceil_div(vectors, 32 * waves));
+        const size_t units = batch * cache->kv_heads * ceil_div(vectors, 32 * waves);
+        if (units >= (1u << 19))                 // (the joining has 16 or 32 workgroups of 256 for each)
+            return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows is too large");
         const int r = launch(kernel, 32 * waves, 1, waves, &workgroups);
         if (r) return r;
-        const unsigned units = (unsigned)(batch * cache->kv_heads * ceil_div(vectors, 32 * waves));
-        hipLaunchKernelGGL(join, dim3(units * (32 * waves / PJ_VEC)), dim3(256), 0, st, a, workgroups);
+        hipLaunchKernelGGL(join, dim3((unsigned)(units * (32 * waves * cache->head_dim / 1024))), dim3(256), 0, st, a, workgroups);
         return (int)CACTUS_HIP_OK;
     };
     unsigned n = 0;

@@ -285,6 +285,22 @@ def test_long_decode_and_sharp_softmax(hip_ready):
     c.attend(q, [2, -1, 5], [1, 1, 1])                      # slots that do not exist
 
 
+@pytest.mark.parametrize("d,B,S", [(64, 64, 1), (64, 150, 1), (64, 64, 40), (128, 40, 40), (64, 130, 37), (256, 33, 70)])
+def test_many_short_requests(hip_ready, d, B, S):
+    """More units than workgroups, more requests than a wave has lanes, some without rows."""
+    rng = np.random.default_rng(B + S)
+    c = Cache(hip_ready, 1, 8, d, 16, 8 * B, B, 8)
+    lens = [int(x) for x in rng.integers(0, 100, B)]
+    lens[0], lens[-1] = 0, 100
+    c.fill(rng, lens)
+    q = rng.standard_normal((B, S, 16, d)).astype(np.float16)
+    counts = [int(x) for x in rng.integers(0, S + 1, B)]
+    counts[-1] = S
+    order = [int(x) for x in rng.permutation(B)]
+    c.attend(q, order, counts)
+    c.attend(q, order, counts, window=9, sink=3)
+
+
 def test_rows_without_keys_are_zero(hip_ready):
     rng = np.random.default_rng(4)
     c = Cache(hip_ready, 1, 2, 64, 16, 20, 3, 8)
