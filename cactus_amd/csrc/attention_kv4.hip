@@ -1318,11 +1318,11 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     a.counters = static_cast<uint32_t*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + KV4_COUNTERS);
     const hipStream_t st = as_stream(stream);
-    // block steps at most, by what the tables can hold
-    const size_t blocks = (cache->max_pages * cache->page_size + 127) / 128;    // (of 128 keys or more)
     const size_t vectors = seq_len * G;
-    auto launch = [&](auto kernel, int per_unit, int per_cu, int waves, unsigned* workgroups) {
+    auto launch = [&](auto kernel, int per_unit, int keys, int per_cu, int waves, unsigned* workgroups) {
         const size_t units = batch * cache->kv_heads * ceil_div(vectors, per_unit);
+        // block steps of a unit at most, by what the tables can hold
+        const size_t blocks = ceil_div(cache->max_pages * cache->page_size, keys);
         if (units >= (1u << 31) / blocks)        // (the line counts in 32 bits)
             return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows times table length is too large");
         *workgroups = (unsigned)std::min<size_t>(256 * per_cu, units * blocks);
@@ -1335,13 +1335,15 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
         const size_t units = batch * cache->kv_heads * ceil_div(vectors, 32 * waves);
         if (units >= (1u << 19))                 // (the joining has 16 or 32 workgroups of 256 for each)
             return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows is too large");
-        const int r = launch(kernel, 32 * waves, 1, waves, &workgroups);
+        const int r = launch(kernel, 32 * waves, 16 * waves, 1, waves, &workgroups);
         if (r) return r;
         hipLaunchKernelGGL(join, dim3((unsigned)(units * (32 * waves * cache->head_dim / 1024))), dim3(256), 0, st, a, workgroups);
         return (int)CACTUS_HIP_OK;
     };
     unsigned n = 0;
-#define KV4_FEW(D, PACK) launch(attn_kv4_kernel<D, PACK>, kv4_vectors<D, PACK>(), kv4_per_cu<D, PACK>(), kv4_waves<D, PACK>(), &n)
+#define KV4_FEW(D, PACK)                                                                                  \
+    launch(attn_kv4_kernel<D, PACK>, kv4_vectors<D, PACK>(), KV4_STEP * kv4_waves<D, PACK>(), kv4_per_cu<D, PACK>(), \
+           kv4_waves<D, PACK>(), &n)
 #define KV4_LAUNCH(D, W)                                                              \
     (vectors <= (size_t)kv4_vectors<D, true>() ? KV4_FEW(D, true)                     \
      : vectors <= PF_FROM                      ? KV4_FEW(D, false)                    \

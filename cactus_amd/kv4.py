@@ -3,6 +3,7 @@ descriptor as a ctypes structure, and an owner of its device buffers."""
 from __future__ import annotations
 
 import ctypes
+import numbers
 
 import numpy as np
 
@@ -28,7 +29,11 @@ class KV4Cache:
 
     The methods take device pointers (DeviceBuffer.ptr, or any integer) where
     the entry points do; slot and page lists may be sequences of ints, which
-    are uploaded first."""
+    are uploaded first (the call then waits for the stream).  `stream` is a
+    Stream's handle.  Scratch memory is kept per stream: calls on two streams may
+    overlap as the entry points say.  In a capture give pointers, and make the same
+    call once before it, so that the scratch memory is there; a graph that may
+    overlap eager calls needs the entry points and a workspace of its own."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, page_size: int, num_pages: int, max_seqs: int,
                  max_pages: int, stream=None):
@@ -40,14 +45,23 @@ class KV4Cache:
                      "lens": DeviceBuffer(4 * max_seqs), "refs": DeviceBuffer(4 * num_pages), "state": DeviceBuffer(16)}
         for name, b in self._buf.items():
             setattr(self.desc, name, b.ptr)
-        self._work, self._lists = [], []
+        self._work, self._lists = {}, []
         self.reset(stream)
 
-    def _lst(self, v, stream=None):
-        """A device pointer as it is; a sequence of ints uploaded (kept until the next such call ends)."""
-        if v is None or isinstance(v, int):
-            return v
-        b = DeviceBuffer.from_numpy(np.asarray(v, np.int32), stream)
+    def _lst(self, v, n: int, stream=None):
+        """A device pointer as it is; a sequence of n ints or more uploaded (kept until the next such call ends)."""
+        if v is None or isinstance(v, numbers.Integral):
+            return None if v is None else int(v)
+        a = np.asarray(v)
+        if a.ndim != 1 or len(a) < n:
+            raise ValueError(f"a list of {n} integers is needed")
+        if n == 0:
+            return None
+        if a.dtype.kind not in "iu":
+            raise TypeError("a list of integers is needed")
+        if a.min() < -(1 << 31) or a.max() >= 1 << 31:
+            raise OverflowError("a list of 32-bit integers is needed")
+        b = DeviceBuffer.from_numpy(a.astype(np.int32), stream)
         self._lists.append(b)
         return b.ptr
 
@@ -58,12 +72,14 @@ class KV4Cache:
             self._lists.clear()
 
     def workspace(self, nbytes: int, stream=None):
-        """At least nbytes of scratch memory, the first 4096 bytes zero."""
-        if not self._work or self._work[-1].nbytes < nbytes:
+        """At least nbytes of scratch memory for calls on `stream`, the first 4096 bytes zero."""
+        work = self._work.setdefault(stream or 0, [])
+        if not work or work[-1].nbytes < nbytes:
             # a smaller one stays: a captured graph may hold its address
-            self._work.append(DeviceBuffer(max(nbytes, 4096)))
-            call("cactus_hip_memset", self._work[-1].ptr, 0, 4096, stream)
-        return self._work[-1].ptr, self._work[-1].nbytes
+            new = DeviceBuffer(max(nbytes, 4096))
+            call("cactus_hip_memset", new.ptr, 0, 4096, stream)
+            work.append(new)
+        return work[-1].ptr, work[-1].nbytes
 
     def reset(self, stream=None):
         self._call("cactus_hip_kv4_reset", stream=stream)
@@ -74,18 +90,18 @@ class KV4Cache:
         return s.value
 
     def extend(self, batch: int, count: int = 0, seqs=None, counts=None, stream=None):
-        self._call("cactus_hip_kv4_extend", self._lst(seqs, stream), self._lst(counts, stream), batch, count,
+        self._call("cactus_hip_kv4_extend", self._lst(seqs, batch, stream), self._lst(counts, batch, stream), batch, count,
                    stream=stream)
 
     def append(self, layer: int, k: int, v: int, batch: int, seq_len: int, kv_stride: int | None = None, seqs=None,
                counts=None, stream=None):
         stride = kv_stride or self.desc.kv_heads * self.desc.head_dim
-        self._call("cactus_hip_kv4_append_f16", layer, self._lst(seqs, stream), self._lst(counts, stream), k, v, batch,
-                   seq_len, stride, stream=stream)
+        self._call("cactus_hip_kv4_append_f16", layer, self._lst(seqs, batch, stream), self._lst(counts, batch, stream), k, v,
+                   batch, seq_len, stride, stream=stream)
 
     def read(self, layer: int, k: int, v: int, batch: int, seq_len: int, seqs=None, starts=None, counts=None, stream=None):
-        self._call("cactus_hip_kv4_read_f16", layer, self._lst(seqs, stream), self._lst(starts, stream),
-                   self._lst(counts, stream), k, v, batch, seq_len, stream=stream)
+        self._call("cactus_hip_kv4_read_f16", layer, self._lst(seqs, batch, stream), self._lst(starts, batch, stream),
+                   self._lst(counts, batch, stream), k, v, batch, seq_len, stream=stream)
 
     def attention(self, layer: int, q: int, o: int, batch: int, seq_len: int, num_q_heads: int, scale: float = 0.0,
                   window: int = 0, sink: int = 0, causal: bool = True, q_stride: int | None = None, seqs=None,
@@ -93,17 +109,17 @@ class KV4Cache:
         need = hip().cactus_hip_attention_kv4_workspace(self.desc.ref, batch, seq_len, num_q_heads)
         work, size = self.workspace(need, stream)
         stride = q_stride or num_q_heads * self.desc.head_dim
-        self._call("cactus_hip_attention_kv4_f16", layer, self._lst(seqs, stream), self._lst(counts, stream), q, stride,
-                   o, batch, seq_len, num_q_heads, scale, window, sink, int(causal), work, size, stream=stream)
+        self._call("cactus_hip_attention_kv4_f16", layer, self._lst(seqs, batch, stream), self._lst(counts, batch, stream), q,
+                   stride, o, batch, seq_len, num_q_heads, scale, window, sink, int(causal), work, size, stream=stream)
 
     def fork(self, src, dst, n: int | None = None, stream=None):
         n = len(src) if n is None else n
         work, size = self.workspace(hip().cactus_hip_kv4_pages_workspace(self.desc.ref, n), stream)
-        self._call("cactus_hip_kv4_fork", self._lst(src, stream), self._lst(dst, stream), n, work, size, stream=stream)
+        self._call("cactus_hip_kv4_fork", self._lst(src, n, stream), self._lst(dst, n, stream), n, work, size, stream=stream)
 
     def free(self, seqs, n: int | None = None, stream=None):
         n = len(seqs) if n is None else n
-        self._call("cactus_hip_kv4_free", self._lst(seqs, stream), n, stream=stream)
+        self._call("cactus_hip_kv4_free", self._lst(seqs, n, stream), n, stream=stream)
 
     def compact(self, stream=None):
         work, size = self.workspace(hip().cactus_hip_kv4_pages_workspace(self.desc.ref, 0), stream)
@@ -111,7 +127,7 @@ class KV4Cache:
 
     def copy_pages(self, src, dst, n: int | None = None, stream=None):
         n = len(src) if n is None else n
-        self._call("cactus_hip_kv4_copy_pages", self._lst(src, stream), self._lst(dst, stream), n, stream=stream)
+        self._call("cactus_hip_kv4_copy_pages", self._lst(src, n, stream), self._lst(dst, n, stream), n, stream=stream)
 
     def tables(self, stream=None) -> dict:
         """Host copies of table, lens, refs and state."""

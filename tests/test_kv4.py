@@ -97,6 +97,12 @@ def test_refused_arguments(lib):
     refused(lib, lib.cactus_hip_kv4_copy_pages(c, p, None, 1, None), b"null")
     refused(lib, lib.cactus_hip_kv4_copy_pages(c, p, p, 9, None), b"pages")
     refused(lib, lib.cactus_hip_kv4_status(c, None, None), b"null")
+    # more stages of keys than the kernels count: 128 and, with dims of 256 and many rows, 64 keys each
+    for change, rows in ((dict(head_dim=256), 65), (dict(head_dim=64), 65), (dict(head_dim=256), 1)):
+        wide = desc(page_size=16, max_pages=1 << 20, kv_heads=1, **change).ref
+        batch = (8192 if change["head_dim"] == 256 else 16384) if rows > 1 else 16384
+        assert att(wide, 0, None, None, p, 256, p, batch, rows, 1, 0.0, 0, 0, 1, p, big, None) == -2
+        assert b"too large" in lib.cactus_hip_last_error()
     # nothing to do is no error and no launch
     assert lib.cactus_hip_kv4_append_f16(c, 0, None, None, None, None, 0, 1, 256, None) == 0
     assert att(c, 0, None, None, None, 0, None, 1, 0, 2, 0.0, 0, 0, 1, None, 0, None) == 0
@@ -104,6 +110,16 @@ def test_refused_arguments(lib):
     assert lib.cactus_hip_kv4_fork(c, None, None, 0, None, 0, None) == 0
     assert lib.cactus_hip_kv4_free(c, None, 0, None) == 0
     assert lib.cactus_hip_kv4_copy_pages(c, None, None, 0, None) == 0
+
+
+def test_lists_of_the_python_owner():
+    from cactus_amd.kv4 import KV4Cache
+    c = KV4Cache.__new__(KV4Cache)
+    assert c._lst(None, 3) is None and c._lst([], 0) is None
+    assert c._lst(np.int64(1 << 40), 3) == 1 << 40         # a pointer, whatever the integer's type
+    for bad in ([0], [[0, 1], [2, 3]], [0.5, 1, 2], [1, 2, 1 << 31]):      # too short, not a list, not numbers of slots
+        with pytest.raises((ValueError, TypeError, OverflowError)):
+            c._lst(bad, 2)
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
