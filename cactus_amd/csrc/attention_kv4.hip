@@ -1194,10 +1194,13 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
 // eight parts' loads at a time: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.  A
 // launch of its own: the last workgroup of a unit, joining 256 vectors' parts
 // alone, took longer than the products of a few hundred rows.  Bound by the
-// latency of the lengths, then of the parts (333 rows, 16 / 8 heads of 128: 7.9
-// us; 40 vectors in 32 parts 7.0, with a part after the other 12.9).
+// latency of the lengths, then of the parts (333 rows, 16 / 8 heads of 128: 7.7
+// us; 40 vectors in 32 parts 7.0, with a part after the other 12.9).  1024
+// workgroups: with one for each share, 2048 rows whose units are one part each take 10.5
+// us to find that there is nothing to join, 4.8 so.
 template <int D>
-constexpr int pj_vec() { return 1024 / D; }       // vectors of a workgroup
+constexpr int pj_vec() { return 1024 / D; }       // vectors of a workgroup's share
+constexpr size_t PJ_WORKGROUPS = 1024;
 template <int D, int W>
 __global__ void __launch_bounds__(256) attn_kv4_join_kernel(Kv4AttnArgs a, uint32_t workgroups) {
     constexpr int NV = 32 * W, KT = 16 * W, VEC = pj_vec<D>(), NVJ = NV / VEC;
@@ -1205,62 +1208,77 @@ __global__ void __launch_bounds__(256) attn_kv4_join_kernel(Kv4AttnArgs a, uint3
     PrefillLine<NV, KT> line(a, lane);
     const uint32_t per = line.stretch(workgroups);
     if (line.single) return;
-    // this workgroup's unit: the pair's place in the line, then the head
-    const int v0 = (int)(blockIdx.x % NVJ) * VEC, head = (int)(blockIdx.x / NVJ % a.c.Hkv);
-    const int pair = (int)(blockIdx.x / NVJ / a.c.Hkv), j = pair & 63;
-    uint32_t base = 0;
-    for (int i0 = 0; i0 <= pair; i0 += 64) {
-        if (line.npairs > 64) line.look(i0);
-        base += lane_u(i0 + 64 <= pair ? line.upto : line.upto - line.cost, i0 + 64 <= pair ? 63 : j);
-    }
-    const uint32_t blocks = lane_u(line.blocks, j);
-    if (blocks == 0) return;
-    const int b = a.by_nvb(pair), vb = pair - b * line.nvb;
-    const int nvec = min(NV, __builtin_amdgcn_readlane(line.rows, j) * a.G - vb * NV);
-    const uint32_t own = (blocks + per - 1) / per;                  // parts of the unit, where the line counts parts
-    const uint32_t unit0 = base + (uint32_t)head * (line.parts ? own : blocks);
-    const uint32_t wg0 = line.parts ? unit0 : unit0 / per;
-    const uint32_t nparts = line.parts ? own : (unit0 + blocks - 1) / per - wg0 + 1;
-    if (nparts == 1) return;
-    const int v = v0 + tid / (D / 4), d = tid % (D / 4) * 4;
-    if (v < nvec) {
-        f32x4 num = {0, 0, 0, 0};
-        float mx = -__builtin_inff(), den = 0.0f;
-        for (int p0 = 0; p0 < (int)nparts; p0 += 8) {
-            f32x4 y[8];
-            float2 ml[8];
+    // A workgroup takes shares in turn, a unit's vectors VEC at a time.  With many
+    // requests, whose lengths do not stay in the lanes, it looks for units from the main launch's
+    // workgroups instead (a unit that is shared is the last of its first
+    // workgroup's stretch), and takes eight times the vectors (64 requests of 600
+    // vectors 112 -> 20 us; with few units these would meet in few workgroups: 100
+    // rows at 4096 keys 8 -> 37).
+    const bool from_units = line.npairs <= 64;
+    const int steps = from_units ? 1 : 8;
+    const uint32_t per_unit = NVJ / steps, shares = (from_units ? (uint32_t)(line.npairs * a.c.Hkv) : workgroups) * per_unit;
+    for (uint32_t w = blockIdx.x; w < shares; w += gridDim.x) {
+        const uint32_t of = w / per_unit;                        // which unit, or workgroup
+        const int v0 = (int)(w - of * per_unit) * steps * VEC;
+        int j, head;
+        if (from_units) {
+            j = (int)of / a.c.Hkv;
+            head = (int)of - j * a.c.Hkv;
+            line.pair = j;
+            line.base = lane_u(line.upto - line.cost, j);
+        } else {
+            if (of * per >= line.total) return;
+            const uint32_t end = min(line.total, (of + 1) * per);
+            j = line.find(end - 1);
+            head = (int)((end - 1 - line.base) / lane_u(line.blocks, j));
+        }
+        const uint32_t blocks = lane_u(line.blocks, j), span = line.parts ? (blocks + per - 1) / per : blocks;
+        if (blocks == 0) continue;
+        const uint32_t unit0 = line.base + (uint32_t)head * span, wg0 = line.parts ? unit0 : unit0 / per;
+        const uint32_t nparts = line.parts ? span : (unit0 + span - 1) / per - wg0 + 1;
+        if (nparts == 1 || (!from_units && wg0 != of)) continue;
+        const int b = a.by_nvb(line.pair), vb = line.pair - b * line.nvb;
+        const int nvec = min(NV, __builtin_amdgcn_readlane(line.rows, j) * a.G - vb * NV);
+        for (int v = v0 + tid / (D / 4); v < min(v0 + steps * VEC, nvec); v += VEC) {
+            const int d = tid % (D / 4) * 4;
+            f32x4 num = {0, 0, 0, 0};
+            float mx = -__builtin_inff(), den = 0.0f;
+            for (int p0 = 0; p0 < (int)nparts; p0 += 8) {
+                f32x4 y[8];
+                float2 ml[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                y[u] = (f32x4){0, 0, 0, 0};
-                ml[u] = make_float2(-__builtin_inff(), 0.0f);
-                if (p0 + u < (int)nparts) {
-                    const float* row_at = a.part + ((size_t)(2 * (wg0 + p0 + u) + (p0 + u == 0)) * NV + v) * (D + 4);
-                    y[u] = *reinterpret_cast<const f32x4*>(row_at + d);
-                    ml[u] = *reinterpret_cast<const float2*>(row_at + D);
+                for (int u = 0; u < 8; u++) {
+                    y[u] = (f32x4){0, 0, 0, 0};
+                    ml[u] = make_float2(-__builtin_inff(), 0.0f);
+                    if (p0 + u < (int)nparts) {
+                        const float* row_at = a.part + ((size_t)(2 * (wg0 + p0 + u) + (p0 + u == 0)) * NV + v) * (D + 4);
+                        y[u] = *reinterpret_cast<const f32x4*>(row_at + d);
+                        ml[u] = *reinterpret_cast<const float2*>(row_at + D);
+                    }
+                }
+                float mn = mx;
+#pragma unroll
+                for (int u = 0; u < 8; u++) mn = __builtin_fmaxf(mn, ml[u].x);
+                const float f0 = mx > -__builtin_inff() ? exp2_fast(mx - mn) : 1.0f;
+                mx = mn;
+                num *= f0;
+                den *= f0;
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const float f = ml[u].x > -__builtin_inff() ? exp2_fast(ml[u].x - mx) : 1.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) num[k] = __builtin_fmaf(f, y[u][k], num[k]);
+                    den = __builtin_fmaf(f, ml[u].y, den);
                 }
             }
-            float mn = mx;
+            const int vv = vb * NV + v;
+            const float inv = den != 0.0f ? 1.0f / den : 0.0f;
+            uint16_t r[4];
 #pragma unroll
-            for (int u = 0; u < 8; u++) mn = __builtin_fmaxf(mn, ml[u].x);
-            const float f0 = mx > -__builtin_inff() ? exp2_fast(mx - mn) : 1.0f;
-            mx = mn;
-            num *= f0;
-            den *= f0;
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const float f = ml[u].x > -__builtin_inff() ? exp2_fast(ml[u].x - mx) : 1.0f;
-#pragma unroll
-                for (int k = 0; k < 4; k++) num[k] = __builtin_fmaf(f, y[u][k], num[k]);
-                den = __builtin_fmaf(f, ml[u].y, den);
-            }
+            for (int k = 0; k < 4; k++) r[k] = f2h(num[k] * inv);
+            *reinterpret_cast<uint2*>(a.o + ((size_t)b * a.S * a.Hq + out_offset(a, head, vv)) * D + d) =
+                make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
         }
-        const int vv = vb * NV + v;
-        const float inv = den != 0.0f ? 1.0f / den : 0.0f;
-        uint16_t r[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) r[k] = f2h(num[k] * inv);
-        *reinterpret_cast<uint2*>(a.o + ((size_t)b * a.S * a.Hq + out_offset(a, head, vv)) * D + d) =
-            make_uint2(r[0] | (uint32_t)r[1] << 16, r[2] | (uint32_t)r[3] << 16);
     }
 }
 
@@ -1323,7 +1341,8 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
         const size_t units = batch * cache->kv_heads * ceil_div(vectors, per_unit);
         // block steps of a unit at most, by what the tables can hold
         const size_t blocks = ceil_div(cache->max_pages * cache->page_size, keys);
-        if (units >= (1u << 31) / blocks)        // (the line counts in 32 bits)
+        // the line counts steps, and requests times blocks of vectors, in 32 bits
+        if (units >= (1u << 30) / blocks)
             return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows times table length is too large");
         *workgroups = (unsigned)std::min<size_t>(256 * per_cu, units * blocks);
         hipLaunchKernelGGL(kernel, dim3(*workgroups), dim3(64 * waves), 0, st, a);
@@ -1332,12 +1351,10 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
     auto many = [&](auto kernel, auto join, int waves) {
         unsigned workgroups = 0;
         a.by_nvb.set((uint32_t)ceil_div(vectors, 32 * waves));
-        const size_t units = batch * cache->kv_heads * ceil_div(vectors, 32 * waves);
-        if (units >= (1u << 19))                 // (the joining has 16 or 32 workgroups of 256 for each)
-            return fail(CACTUS_HIP_EUNSUPPORTED, "attention_kv4: batch times rows is too large");
         const int r = launch(kernel, 32 * waves, 16 * waves, 1, waves, &workgroups);
         if (r) return r;
-        hipLaunchKernelGGL(join, dim3((unsigned)(units * (32 * waves * cache->head_dim / 1024))), dim3(256), 0, st, a, workgroups);
+        const size_t shares = batch * cache->kv_heads * ceil_div(vectors, 32 * waves) * (32 * waves * cache->head_dim / 1024);
+        hipLaunchKernelGGL(join, dim3((unsigned)std::min(shares, PJ_WORKGROUPS)), dim3(256), 0, st, a, workgroups);
         return (int)CACTUS_HIP_OK;
     };
     unsigned n = 0;

@@ -301,6 +301,22 @@ def test_many_short_requests(hip_ready, d, B, S):
     c.attend(q, order, counts, window=9, sink=3)
 
 
+@pytest.mark.parametrize("d,B,S,H,longest", [(64, 70, 70, 2, 600), (128, 66, 40, 3, 500), (256, 33, 70, 1, 400),
+                                             (64, 150, 2, 2, 900)])
+def test_many_requests_whose_units_are_shared(hip_ready, d, B, S, H, longest):
+    """More requests, or blocks of query vectors, than a wave has lanes, and units that several workgroups take."""
+    rng = np.random.default_rng(B + d)
+    c = Cache(hip_ready, 1, H, d, 32, B * (longest // 32 + 1), B, longest // 32 + 1)
+    lens = [int(x) for x in rng.integers(0, longest + 1, B)]
+    lens[0], lens[1], lens[-1] = 0, 1, longest
+    c.fill(rng, lens)
+    q = rng.standard_normal((B, S, 2 * H, d)).astype(np.float16)
+    counts = [S if b % 3 else int(rng.integers(0, S + 1)) for b in range(B)]
+    c.attend(q, [int(x) for x in rng.permutation(B)], counts)
+    c.attend(q, range(B), counts, window=200, sink=70)
+    c.attend(q, range(B), counts, causal=False)
+
+
 def test_rows_without_keys_are_zero(hip_ready):
     rng = np.random.default_rng(4)
     c = Cache(hip_ready, 1, 2, 64, 16, 20, 3, 8)
