@@ -48,6 +48,7 @@ struct Kv4AttnArgs {
     int B, S, Hq, G;          // G query heads per KV head
     FastDiv by_g, by_nvb;     // division by G, and by the blocks of query vectors of a request
     int window, sink, causal; // window 0: none
+    int join_log2;            // parts that the few-row kernel joins at a time
     float scale;              // times log2(e): the softmax runs in powers of two
     uint32_t* counters;       // [workgroups] zero between calls
     float* part;              // [workgroups][2][vectors][D + 4]: output, maximum, sum
@@ -193,6 +194,12 @@ constexpr int kv4_waves() { return PACK ? 4 : 8; }
 template <int D, bool PACK>
 constexpr int kv4_per_cu() { return PACK ? (D == 256 ? 2 : 4) : D == 64 ? 2 : 1; }
 
+// threads that share a quad of dims, of `quads`, when parts are joined
+template <int D, bool PACK>
+__host__ __device__ constexpr int kv4_shares(int quads) {
+    return 64 * kv4_waves<D, PACK>() > quads ? 64 * kv4_waves<D, PACK>() / quads : 1;
+}
+
 // a times half I of w plus c, one instruction (v_fma_mix_f32; as a builtin, so that
 // the compiler knows what waits for the matrix and transcendental units' results)
 template <int I>
@@ -274,6 +281,17 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
         longest = max(longest, __builtin_amdgcn_readlane(wave_scan_max((int)r_blocks), 63));
     }
     uint32_t per = max((total + gridDim.x - 1) / gridDim.x, ((uint32_t)longest + KV4_PARTS - 2) / (KV4_PARTS - 1));
+    // The joining takes 2^join_log2 parts at a time, which costs as much as two steps:
+    // longer stretches, for one or two such rounds, where that saves more (one row at
+    // 9000 keys, 16 / 8 heads of 128, in stretches of 1, 2, 3 and 4 steps: 14.2, 12.8,
+    // 11.3 and 12.7 us; at 4096, one round in any case: 9.1, 10.3, 11.1 and 12.0; at
+    // 32000: 24.8 -> 16.8).  With 16 vectors a step costs more than a round.
+    if constexpr (PACK) {
+        const uint32_t one = ((uint32_t)longest + (1u << a.join_log2) - 1) >> a.join_log2;   // steps of a part for one round
+        const uint32_t rounds = (uint32_t)((float)(one + per - 1) * __builtin_amdgcn_rcpf((float)per));
+        const uint32_t q = one <= 3 ? one : (one + 1) / 2;
+        if (q > per && q + (one <= 3 ? 2 : 4) < per + 2 * rounds) per = q;
+    }
     // Stretches that end inside a unit cost their workgroup another unit's start (7
     // us, where a block step takes 0.5 to 3).  If units cut into whole parts of at
     // most `per` steps, or one or two more, make no more parts than there are
@@ -600,7 +618,7 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
                 // a thread takes a quad of dims and every (threads / quads)-th part,
                 // eight parts' loads at a time: 4096 keys in 32 parts take one round of
                 // loads (a part after the other: 4 us more)
-                const int share = max(1, 64 * W / nquad);
+                const int share = kv4_shares<D, PACK>(nquad);
                 for (int e0 = 0; e0 < nquad; e0 += 64 * W) {
                     const int e = e0 + (share > 1 ? et % nquad : et), pl = share > 1 ? et / nquad : 0;
                     const bool in = e < nquad && pl < share;
@@ -1358,6 +1376,9 @@ int cactus_hip_attention_kv4_f16(const cactus_hip_kv4_cache* cache, size_t layer
         return (int)CACTUS_HIP_OK;
     };
     unsigned n = 0;
+    const int quads = (int)std::min<size_t>(vectors, 16) * a.c.d / 4;     // (of up to 8 vectors: the packed kernel's)
+    const int shares = a.c.d == 64 ? kv4_shares<64, true>(quads) : a.c.d == 128 ? kv4_shares<128, true>(quads) : kv4_shares<256, true>(quads);
+    a.join_log2 = 31 - __builtin_clz(8 * shares);
 #define KV4_FEW(D, PACK)                                                                                  \
     launch(attn_kv4_kernel<D, PACK>, kv4_vectors<D, PACK>(), KV4_STEP * kv4_waves<D, PACK>(), kv4_per_cu<D, PACK>(), \
            kv4_waves<D, PACK>(), &n)

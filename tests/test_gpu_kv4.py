@@ -317,6 +317,17 @@ def test_many_requests_whose_units_are_shared(hip_ready, d, B, S, H, longest):
     c.attend(q, range(B), counts, causal=False)
 
 
+@pytest.mark.parametrize("d,G,lens", [(128, 2, [9000]), (64, 1, [9000, 130]), (64, 6, [5000]), (256, 1, [9000, 4000, 1])])
+def test_parts_joined_in_rounds(hip_ready, d, G, lens):
+    """Keys in more parts than the joining takes at a time, in stretches of one or more steps."""
+    rng = np.random.default_rng(d + G)
+    c = Cache(hip_ready, 1, 2, d, 64, 330, len(lens), 150)
+    c.fill(rng, lens)
+    q = rng.standard_normal((len(lens), 1, 2 * G, d)).astype(np.float16)
+    c.attend(q, range(len(lens)), [1] * len(lens))
+    c.attend(q, range(len(lens)), [1] * len(lens), window=5000, sink=200)
+
+
 def test_rows_without_keys_are_zero(hip_ready):
     rng = np.random.default_rng(4)
     c = Cache(hip_ready, 1, 2, 64, 16, 20, 3, 8)
