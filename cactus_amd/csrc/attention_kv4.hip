@@ -14,8 +14,9 @@
 //           already the operand's lane order; the 8 of u - 8 comes off once at
 //           the end through sum_j P'_g (a product with a constant)
 // The running maximum and the sum are FP32, kept per column.  The weights are
-// rounded to FP16 after the scale (2^-12 relative each): the matrix
-// instruction takes them so, and the sum of thousands averages it out.
+// rounded to FP16 after the scale (2^-11 relative each, lifted by a power of two
+// so that small ones keep their bits): the matrix instruction takes them so,
+// and the sum of thousands averages it out.
 #include "kv4_device.h"
 
 #include <algorithm>
@@ -25,6 +26,7 @@ namespace cactus_hip {
 
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 // n / d for 0 <= n < 2^31: n m / 2^(31 + s) with 2^s the power of two at or above d
 // and m = 2^(31 + s) / d + 1, whose error n / 2^(31 + s) stays below 1 / d
@@ -409,6 +411,15 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
         const int last_pos = sq.len - sq.rows + a.by_g(v0 + nvec - 1);
         const int all = a.causal ? min(first_pos + 1, sq.len) : sq.len;
 
+        // The products p s are lifted by 2^(26 - top_exp), top_exp the exponent field of
+        // the largest value scale seen: s 2^lift is below 2^12 then, and below 2^15, which FP16 holds,
+        // until one eight times as large is met.  (Without it the weights of small
+        // values, or of many keys beside one that takes most of the weight, fell
+        // to FP16 subnormals or to zero; it costs 2% of a decode step of 32 requests,
+        // 8% of five drafted rows of heads of 64.)
+        int top_exp = 0;
+        uint32_t scale_end = 0;      // a scale from here on raises top_exp
+        float lift = 0x1p26f;
         float m = -__builtin_inff(), mbase = 0.0f, l = 0.0f;
         f32x4 acc[NB], off[SG];       // O^T 2^-24 (odd blocks 2^-20) before the 8 comes off, -8 2^-24 sum p s_g
 #pragma unroll
@@ -474,18 +485,38 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
             // the running maximum, where one of the step's scores is above it (a
             // NaN score reaches the sum by itself)
             float top = max3(max3(x[0][0], x[0][1], x[0][2]), max3(x[0][3], x[1][0], x[1][1]), __builtin_fmaxf(x[1][2], x[1][3]));
-            if (__ballot(top > m)) {
+            u16x2 sc = __builtin_bit_cast(u16x2, vs[0][0]);
+#pragma unroll
+            for (int k = 1; k < 4 * SG; k++)
+                sc = __builtin_elementwise_max(sc, __builtin_bit_cast(u16x2, vs[k / (2 * SG)][k % (2 * SG)]));
+            const uint32_t top_scale = max((uint32_t)sc[0], (uint32_t)sc[1]);
+            if (__ballot((top > m) | (top_scale >= scale_end))) {
                 top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
                 top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
+                int se = (int)(top_scale >> 10);
+                if (__builtin_expect(__ballot(se > 30) != 0, 0)) {       // NaNs: not counted
+                    se = 0;
+#pragma unroll
+                    for (int k = 0; k < 4 * SG; k++) {
+                        const int lo = vs[k / (2 * SG)][k % (2 * SG)] >> 10 & 31, hi = vs[k / (2 * SG)][k % (2 * SG)] >> 26 & 31;
+                        se = max(se, max(lo > 30 ? 0 : lo, hi > 30 ? 0 : hi));
+                    }
+                }
+                se = max(se, __shfl_xor(se, 16, 64));
+                se = max(max(se, __shfl_xor(se, 32, 64)), top_exp);
                 const float mn = __builtin_fmaxf(m, top);
                 mbase = mn > -__builtin_inff() ? mn : 0.0f;
                 const float f = exp2_fast(m - mbase);      // 0 where nothing was there
                 m = mn;
                 l *= f;
+                const float fs = __builtin_ldexpf(f, top_exp - se);
+                top_exp = se;
+                scale_end = (uint32_t)(se + 4) << 10;
+                lift = __builtin_ldexpf(1.0f, 26 - se);
 #pragma unroll
-                for (int i = 0; i < NB; i++) acc[i] *= f;
+                for (int i = 0; i < NB; i++) acc[i] *= fs;
 #pragma unroll
-                for (int g = 0; g < SG; g++) off[g] *= f;
+                for (int g = 0; g < SG; g++) off[g] *= fs;
             }
             float p[2][4];
 #pragma unroll
@@ -494,6 +525,7 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
                 for (int i = 0; i < 4; i++) {
                     p[t][i] = exp2_fast(x[t][i] - mbase);
                     l += p[t][i];
+                    p[t][i] *= lift;
                 }
             h16x8 pf[SG];
 #pragma unroll
@@ -546,14 +578,15 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
         const int eh = (et & 63) >> 4;
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
+        const float drop = __builtin_ldexpf(1.0f, top_exp - 26 + 24);      // the lift, and the codes' 2^-24
         if (live) {
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 if (PACK && g != gi) continue;
                 const f32x4 o8 = off[PACK ? 0 : g];
-                *reinterpret_cast<f32x4*>(&o_sh[wid][qi * OS + 32 * g + 4 * eh]) = (acc[2 * g] + o8) * 16777216.0f;
+                *reinterpret_cast<f32x4*>(&o_sh[wid][qi * OS + 32 * g + 4 * eh]) = (acc[2 * g] + o8) * drop;
                 *reinterpret_cast<f32x4*>(&o_sh[wid][qi * OS + 32 * g + 16 + 4 * eh]) =
-                    (acc[2 * g + 1] * 0.0625f + o8) * 16777216.0f;
+                    (acc[2 * g + 1] * 0.0625f + o8) * drop;
             }
             if (eh == 0 && gi == 0) {
                 m_sh[wid][qi] = m;
@@ -694,11 +727,12 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
 // operands, two stages in turn: stage t + 1 is written while stage t is used, and
 // stage t + 2's tiles are on their way to LDS as they are stored.
 //
-// A column's maximum is raised only when a score exceeds it by 2^PF_SLACK: the
-// weights stay below 2^8 (FP16 holds 2^16), and the outputs are rescaled a few
-// times per row instead of at every new maximum.  The sum of the weights is a
+// A column's maximum is raised only when a score exceeds it by 2^PF_SLACK, and
+// the outputs are rescaled a few times per row instead of at every new maximum.  The
+// weights are 2^PF_LIFT times those of the maximum, below 2^15 (FP16 holds 2^16):
+// where one key takes most of the weight, the many small ones keep their bits.  The sum of the weights is a
 // product with ones, of the rounded weights that the outputs use.
-constexpr int PF_SLACK = 8;
+constexpr int PF_SLACK = 8, PF_LIFT = 7;
 //
 // More query vectors of a request per KV head than PF_FROM come here.  Its 256
 // columns (D = 256: 128) are dear for few vectors and its joining is a second
@@ -1061,9 +1095,9 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                         float y = top[cb];
                         y = __builtin_fmaxf(y, __shfl_xor(y, 16, 64));
                         y = __builtin_fmaxf(y, __shfl_xor(y, 32, 64));
-                        const float mn = __builtin_fmaxf(m[cb], y);
-                        mbase[cb] = mn > -__builtin_inff() ? mn : 0.0f;
-                        const float f = exp2_fast(m[cb] - mbase[cb]);
+                        const float mn = __builtin_fmaxf(m[cb], y), base = mn > -__builtin_inff() ? mn - PF_LIFT : 0.0f;
+                        const float f = m[cb] > -__builtin_inff() ? exp2_fast(mbase[cb] - base) : 0.0f;
+                        mbase[cb] = base;
                         m[cb] = mn;
                         lsum[cb] *= f;
 #pragma unroll
@@ -1200,7 +1234,8 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                 float* row_at = a.part + ((size_t)(2 * blockIdx.x + (blockIdx.x == wg0)) * NV + v) * (D + 4);
 #pragma unroll
                 for (int n = 0; n < NB; n++) *reinterpret_cast<f32x4*>(row_at + 16 * n + 4 * h) = acc[cb][n];
-                if (h == 0) *reinterpret_cast<float2*>(row_at + D) = make_float2(m[cb], lsum[cb][0]);
+                if (h == 0)
+                    *reinterpret_cast<float2*>(row_at + D) = make_float2(m[cb] > -__builtin_inff() ? mbase[cb] : m[cb], lsum[cb][0]);
             }
         }
         __syncthreads();

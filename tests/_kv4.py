@@ -167,7 +167,7 @@ class Model:
         return out
 
 
-def attention(q, kc, ks, vc, vs, n, scale, window=0, sink=0, causal=True):
+def attention(q, kc, ks, vc, vs, n, scale, window=0, sink=0, causal=True, small=True):
     """q [m][Hq][d] of the rows at positions n - m to n - 1 over n tokens' codes and scales.
     -> (o [m][Hq][d] in 64 bits, the largest error that the kernel may make in each output).
 
@@ -175,7 +175,8 @@ def attention(q, kc, ks, vc, vs, n, scale, window=0, sink=0, causal=True):
     to the value; 2^-25 absolute below FP16's normal range):
       * the output is rounded to FP16: 2^-11 |o| + 2^-25;
       * the weight p s of a key and group is rounded to FP16: 2^-11 sum p |v| / L,
-        and 2^-25 |code| / L where p s < 2^-14 (p <= 1 is relative to the maximum);
+        and 2^-25 |code| / L where p s < 2^-14 (p <= 1 is relative to the maximum;
+        not with small = False, for weights that the kernels lift above that);
       * a score is a sum of d products of |q| and at most 16 s (code + 8, and the
         8 that comes off): (d + 16) e scale sum |q| 16 s, its product with the
         scale and the difference from the maximum 4 e (|x| + |max|), the power of two 4 e
@@ -218,10 +219,10 @@ def attention(q, kc, ks, vc, vs, n, scale, window=0, sink=0, causal=True):
         ao = np.abs(oh)
         w = err + err.max(1, initial=0)[:, None] + 4 * e * (np.abs(np.where(seen, x, 0)) + np.abs(base)) + 4 * e
         t = 2.0 ** -25 + 2.0 ** -11 * ao + 2.0 ** -11 * (p @ av) / L
-        for g in range(d // GROUP):
+        for g in range(d // GROUP if small else 0):
             s = slice(g * GROUP, (g + 1) * GROUP)
-            small = seen & (p * v16z[:, g * GROUP] / 16 < 2.0 ** -14)
-            t[:, s] += 2.0 ** -25 * (small @ vch[:, s]) / L
+            tiny = seen & (p * v16z[:, g * GROUP] / 16 < 2.0 ** -14)
+            t[:, s] += 2.0 ** -25 * (tiny @ vch[:, s]) / L
         pw = p * np.where(np.isnan(w), 0, w)
         t += (pw @ av + pw.sum(1)[:, None] * ao) / L
         t += 3 * (seen.sum(1)[:, None] + 64) * e * (ao + p @ v16z / L)

@@ -60,7 +60,7 @@ class Cache:
             k = kv_rows(rng, len(lens), S, self.cpu.H, self.cpu.d, scale)
             self.append(layer, seqs, lens, k, kv_rows(rng, len(lens), S, self.cpu.H, self.cpu.d, scale))
 
-    def attend(self, q, seqs, counts, layer=0, scale=0.0, window=0, sink=0, causal=True, stride=None, call=None):
+    def attend(self, q, seqs, counts, layer=0, scale=0.0, window=0, sink=0, causal=True, stride=None, small=True):
         """Runs the kernel on q [B][S][Hq][d] and holds every row to the plain attention."""
         B, S, Hq, d = q.shape
         stride = stride or Hq * d
@@ -78,7 +78,8 @@ class Cache:
             if m == 0:
                 continue
             (kc, ks), (vc, vs) = self.cpu.read(layer, s)
-            want, tol = attention(q[b, :m], kc, ks, vc, vs, len(kc), scale or 1 / math.sqrt(d), window, sink, causal)
+            want, tol = attention(q[b, :m], kc, ks, vc, vs, len(kc), scale or 1 / math.sqrt(d), window, sink, causal,
+                                  small)
             got = o[b, :m].astype(np.float64)
             np.testing.assert_array_equal(np.isnan(got), np.isnan(want), err_msg=f"request {b}: NaN")
             off = np.where(np.isnan(want), 0, np.abs(got - want) - tol)
@@ -326,6 +327,54 @@ def test_parts_joined_in_rounds(hip_ready, d, G, lens):
     q = rng.standard_normal((len(lens), 1, 2 * G, d)).astype(np.float16)
     c.attend(q, range(len(lens)), [1] * len(lens))
     c.attend(q, range(len(lens)), [1] * len(lens), window=5000, sink=200)
+
+
+@pytest.mark.parametrize("d,S,G", [(64, 1, 1), (128, 1, 2), (256, 1, 2), (64, 5, 3), (128, 9, 2), (256, 4, 4), (64, 80, 1),
+                                   (128, 40, 2), (256, 70, 1)])
+@pytest.mark.parametrize("size", [0.02, 1e-3])
+def test_many_small_weights_beside_a_large_one(hip_ready, d, S, G, size):
+    """A first key that takes nearly all the weight and has no value, as attention sinks are: the others' weights,
+    2^-17 of its, and their small values keep their bits (2^-17 of the products with the kernels' factors stay above
+    2^-14, so that no rounding is absolute but that of the output)."""
+    rng = np.random.default_rng(d + S)
+    n = 3000
+    c = Cache(hip_ready, 1, 1, d, 64, 50, 1, 50)
+    assert c.extend([0], [n]) == 0
+    k = (0.1 * rng.standard_normal((1, n, 1, d))).astype(np.float16)
+    v = (size * (1 + 0.3 * rng.standard_normal((1, n, 1, d)))).astype(np.float16)
+    k[..., 0], k[0, 0, 0, 0], v[0, 0] = 0, 12, 0
+    c.append(0, [0], [n], k, v)
+    q = rng.standard_normal((1, S, G, d)).astype(np.float16)
+    q[..., 0] = 8
+    c.attend(q, [0], [S], scale=1 / 8, small=False)
+
+
+def test_a_query_that_is_not_finite_leaves_the_others(hip_ready):
+    rng = np.random.default_rng(23)
+    c = Cache(hip_ready, 1, 2, 128, 16, 40, 2, 20)
+    c.fill(rng, [300, 40])
+    for S in (1, 5, 40):
+        q = rng.standard_normal((2, S, 8, 128)).astype(np.float16)
+        clean = c.attend(q, [0, 1], [S, S])
+        q[0, S // 2, 1, 7], q[1, 0, 6, 100] = np.nan, np.inf
+        dq, do = c.cm.DeviceBuffer.from_numpy(q), c.cm.DeviceBuffer(q.nbytes)
+        c.gpu.attention(0, dq.ptr, do.ptr, 2, S, 8)
+        o = do.to_numpy(np.float16, q.shape)
+        o[0, S // 2, 1], o[1, 0, 6] = clean[0, S // 2, 1], clean[1, 0, 6]
+        np.testing.assert_array_equal(o, clean)
+
+
+@pytest.mark.parametrize("ps", [512, 4096])
+def test_large_pages(hip_ready, ps):
+    rng = np.random.default_rng(ps)
+    c = Cache(hip_ready, 2, 2, 64, ps, 6, 3, 2)
+    c.fill(rng, [ps + 70, 33])
+    c.cpu.fork([0], [2])
+    c.gpu.fork([0], [2])
+    c.check()
+    for S in (1, 4, 70):
+        q = rng.standard_normal((3, S, 4, 64)).astype(np.float16)
+        c.attend(q, [0, 1, 2], [S, min(S, 33), S], layer=1, window=ps - 40, sink=3)
 
 
 def test_rows_without_keys_are_zero(hip_ready):
