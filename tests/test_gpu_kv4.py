@@ -593,3 +593,60 @@ def test_a_captured_step(hip_ready):
         np.testing.assert_array_equal(o, eager)
     cm.call("cactus_hip_graph_destroy", graph)
     c.check()
+
+
+def test_captured_prompts_and_pages(hip_ready):
+    """Prompts of 40 rows (the many-row kernel), a fork, an end and a compaction in one graph, replayed with eager calls
+    between; graph and eager calls have a workspace each."""
+    cm = hip_ready
+    rng = np.random.default_rng(15)
+    H, G, d, B, S = 2, 2, 64, 2, 40
+    c = Cache(cm, 2, H, d, 16, 90, 5, 20)
+    c.fill(rng, [30, 130, 20])
+    stream = cm.Stream()
+    st = stream.handle
+    ref = c.gpu.desc.ref
+    kv = [cm.DeviceBuffer(B * S * H * d * 2) for _ in range(2)]
+    dq, do = cm.DeviceBuffer(B * S * H * G * d * 2), cm.DeviceBuffer(B * S * H * G * d * 2)
+    lists = {n: cm.DeviceBuffer.from_numpy(np.array(v, np.int32)) for n, v in
+             (("seqs", [1, 3]), ("counts", [40, 33]), ("src", [1, 3]), ("dst", [4, 1]), ("gone", [3, 4]))}
+    p = {n: b.ptr for n, b in lists.items()}
+    hip = cm.hip()
+    need = max(hip.cactus_hip_attention_kv4_workspace(ref, B, S, H * G), hip.cactus_hip_kv4_pages_workspace(ref, 2))
+    work = cm.DeviceBuffer(need)
+    cm.call("cactus_hip_memset", work.ptr, 0, 4096, st)
+    cm.call("cactus_hip_stream_sync", st)
+    cm.call("cactus_hip_stream_sync", None)
+    graph = ctypes.c_void_p()
+    cm.call("cactus_hip_graph_capture_begin", st)
+    cm.call("cactus_hip_kv4_extend", ref, p["seqs"], p["counts"], B, 0, st)
+    for layer in range(2):
+        cm.call("cactus_hip_kv4_append_f16", ref, layer, p["seqs"], p["counts"], kv[0].ptr, kv[1].ptr, B, S, H * d, st)
+    cm.call("cactus_hip_attention_kv4_f16", ref, 1, p["seqs"], p["counts"], dq.ptr, H * G * d, do.ptr, B, S, H * G, 0.0, 0, 0, 1,
+            work.ptr, need, st)
+    cm.call("cactus_hip_kv4_fork", ref, p["src"], p["dst"], 2, work.ptr, need, st)
+    cm.call("cactus_hip_kv4_free", ref, p["gone"], 2, st)
+    cm.call("cactus_hip_kv4_compact", ref, work.ptr, need, st)
+    cm.call("cactus_hip_graph_capture_end", st, ctypes.byref(graph))
+    for i in range(4):
+        k, v = kv_rows(rng, B, S, H, d), kv_rows(rng, B, S, H, d)
+        q = rng.standard_normal((B, S, H * G, d)).astype(np.float16)
+        kv[0].upload(k, st), kv[1].upload(v, st), dq.upload(q, st)
+        cm.call("cactus_hip_graph_launch", graph, st)
+        o = do.to_numpy(np.float16, q.shape, st)
+        assert c.cpu.extend([1, 3], [40, 33]) == 0
+        for b, (slot, m) in enumerate(((1, 40), (3, 33))):
+            for layer in range(2):
+                for r in range(m):
+                    c.cpu.write(layer, slot, c.cpu.lens[slot] - m + r, k[b, r], v[b, r])
+            (kc, ks), (vc, vs) = c.cpu.read(1, slot)
+            want, tol = attention(q[b, :m], kc, ks, vc, vs, len(kc), 1 / math.sqrt(d))
+            assert (np.abs(o[b, :m] - want) <= tol).all(), (i, b)
+        assert c.cpu.fork([1, 3], [4, 1]) == 0
+        c.cpu.free([3, 4])
+        c.cpu.compact()
+        assert c.gpu.status(st) == 0
+        c.check()
+        c.attend(q, [0, 1], [30, 33], layer=0)          # eager, on the default stream
+        cm.call("cactus_hip_stream_sync", None)
+    cm.call("cactus_hip_graph_destroy", graph)
