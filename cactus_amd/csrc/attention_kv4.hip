@@ -756,6 +756,11 @@ __device__ __forceinline__ uint32_t high_values(uint32_t w, h16x2 s) {
                                               (h16x2){(_Float16)-72.0f, (_Float16)-72.0f});
     return __builtin_bit_cast(uint32_t, x * s);
 }
+// a pair of FP16 values, none of them NaN, cut to the largest finite ones
+__device__ __forceinline__ uint32_t finite(uint32_t w) {
+    const h16x2 top = {(_Float16)65504.0f, (_Float16)65504.0f};
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_elementwise_min(as_h2(w), top), -top));
+}
 
 // The line of stages: units (request, block of NV vectors, KV head) in that
 // order; 64 (request, block) pairs at a time, one per lane.
@@ -927,13 +932,19 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
             for (int o = 0; o + 1024 <= TB; o += 1024) lds_dma<16>(p + 16 * lane + o, raw_lds + o);
             if (16 * lane < TB % 1024) lds_dma<16>(p + 16 * lane + TB / 1024 * 1024, raw_lds + TB / 1024 * 1024);
         };
-        // A NaN or infinite scale of a value group: the key is marked and the group
-        // reads as 0 (0 times NaN would reach the rows that do not see the key)
-        auto mark = [&](int i, uint32_t (&vscl)[D / 16]) {
-            uint32_t bad = 0;        // an exponent of all ones carries into bits 15 and 31
+        // Every value operand has to be finite: a weight of 0 times NaN or infinity would
+        // reach the rows that do not see the key, and what a page holds behind the last
+        // token, in tokens that are not written yet, or in page 0 where it stands in for
+        // a missing one, is anything.  A NaN or infinite scale of a value group: the key
+        // is marked and the group reads as 0.  A scale from 8192 on, whose product with a
+        // code may be beyond FP16: the result says so, and the products are cut to
+        // 65504 (those of written tokens stay below, 7 x 9344).
+        auto mark = [&](int i, uint32_t (&vscl)[D / 16]) -> bool {
+            uint32_t bad = 0;        // an exponent field from 28 on carries into bits 15 and 31
 #pragma unroll
-            for (int k = 0; k < D / 16; k++) bad |= (vscl[k] & 0x7C007C00u) + 0x04000400u;
-            if (__builtin_expect(__ballot((bad & 0x80008000u) != 0) != 0, 0)) {
+            for (int k = 0; k < D / 16; k++) bad |= (vscl[k] & 0x7C007C00u) + 0x10001000u;
+            const bool large = __ballot((bad & 0x80008000u) != 0) != 0;
+            if (__builtin_expect(large, 0)) {
                 uint32_t groups[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < D / 16; k++)
@@ -952,6 +963,7 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                     }
                 }
             }
+            return large;
         };
         // stage i's tile, once it has arrived, to the operands of buffer `buf`
         auto put = [&](int i, int buf) {
@@ -975,7 +987,7 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
             uint32_t x[D / 32], vscl[D / 16];        // scales of keys 4 h + i
             load_words(x, raw + 9 * D + lane * (D / 8));
             load_words(vscl, raw + 17 * D + h * (D / 4));
-            mark(i, vscl);
+            const bool large = mark(i, vscl);
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 const uint32_t s01 = vscl[2 * g], s23 = vscl[2 * g + 1], w = x[g];
@@ -985,6 +997,14 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
                     make_uint2(low_values(w, se), low_values(w >> 8, so));
                 reinterpret_cast<uint2*>(&vf[buf][wid >> 1][2 * g + 1][lane])[wid & 1] =
                     make_uint2(high_values(w, se), high_values(w >> 8, so));
+            }
+            if (__builtin_expect(large, 0)) {
+#pragma unroll 1
+                for (int n = 0; n < NB; n++) {
+                    uint2* at = reinterpret_cast<uint2*>(&vf[buf][wid >> 1][n][lane]) + (wid & 1);
+                    const uint2 x = *at;
+                    *at = make_uint2(finite(x.x), finite(x.y));
+                }
             }
         };
 

@@ -432,6 +432,88 @@ def test_pages_that_do_not_exist_are_not_there(hip_ready):
         assert (got[16:32] == 3).all()
 
 
+def leftovers(c, bits, rng):
+    """Every page holds other data, as recycled memory does: slot 0's token takes page 0 and is never written."""
+    c.cpu.pages[:] = rng.integers(0, 256, c.cpu.pages.shape, np.uint8) if bits is None else bits
+    c.put_pages()
+    assert c.extend([0], [1]) == 0
+
+
+# 0x7B bytes: the scale 61280, with codes 3 and -1; 0x70: 8576 (with codes -8 a product of -68608), 0xF3: -15256; random bytes
+@pytest.mark.parametrize("bits", [0x7B, 0x70, 0xF3, 0xFB, None])
+@pytest.mark.parametrize("d,G,ps", [(64, 2, 16), (128, 4, 64), (256, 3, 256)])
+def test_what_unused_page_bytes_hold_reaches_no_row(hip_ready, d, G, ps, bits):
+    """Finite scales whose products with a code are beyond FP16, in the rest of a tile, behind the last one and in
+    page 0, which stands in for pages that are not there."""
+    rng = np.random.default_rng(d)
+    c = Cache(hip_ready, 1, 2, d, ps, 90, 6, 1 + 700 // ps)
+    leftovers(c, bits, rng)
+    lens = [40, 75, 128, 131, 600]
+    c.fill(rng, lens, seqs=range(1, 6))
+    for S in (1, 9, 40, 70):
+        q = rng.standard_normal((5, S, 2 * G, d)).astype(np.float16)
+        for window, causal in ((0, True), (30, True), (0, False)):
+            c.attend(q, range(1, 6), [min(S, n) for n in lens], window=window, sink=3, causal=causal)
+
+
+@pytest.mark.parametrize("bits", [0x7B, 0x70, None])
+@pytest.mark.parametrize("d,written,more", [(64, 30, 20), (64, 100, 50), (128, 70, 9), (256, 90, 70)])
+def test_tokens_that_are_not_written_yet_reach_only_the_rows_that_see_them(hip_ready, d, written, more, bits):
+    rng = np.random.default_rng(d + written)
+    c = Cache(hip_ready, 1, 1, d, 16, 20, 2, 16)
+    leftovers(c, bits, rng)
+    c.fill(rng, [written], seqs=[1])
+    (kc, ks), (vc, vs) = c.cpu.read(0, 1)
+    assert c.extend([1], [more]) == 0
+    m = written + more
+    q = rng.standard_normal((1, m, 1, d)).astype(np.float16)
+    dq, do = c.cm.DeviceBuffer.from_numpy(q), c.cm.DeviceBuffer(q.nbytes)
+    c.gpu.attention(0, dq.ptr, do.ptr, 1, m, 1, seqs=[1])
+    want, tol = attention(q[0, :written], kc, ks, vc, vs, written, 1 / math.sqrt(d))
+    assert (np.abs(do.to_numpy(np.float16, q.shape)[0, :written] - want) <= tol).all()
+
+
+@pytest.mark.parametrize("d,S", [(64, 1), (64, 12), (64, 80), (128, 33), (256, 70)])
+def test_the_largest_values_are_not_cut(hip_ready, d, S):
+    """Value groups of up to 65504 (scale 9344) beside ordinary ones; some rows see one such key alone."""
+    rng = np.random.default_rng(d + S)
+    c = Cache(hip_ready, 1, 1, d, 16, 20, 1, 16)
+    n = 150
+    assert c.extend([0], [n]) == 0
+    k, v = kv_rows(rng, 1, n, 1, d), kv_rows(rng, 1, n, 1, d)
+    v[0, ::5] = rng.choice([65504, -65504, 57000, 1], (30, 1, d)).astype(np.float16)
+    c.append(0, [0], [n], k, v)
+    q = rng.standard_normal((1, S, 2, d)).astype(np.float16)
+    c.attend(q, [0], [S])
+    c.attend(q, [0], [S], window=1)
+
+
+# pages of less than a stage's keys and of more, in every kernel of the attention
+@pytest.mark.parametrize("d,G,S", [(64, 2, 1), (64, 2, 10), (64, 2, 70), (128, 1, 40), (128, 1, 130), (256, 1, 10), (256, 2, 70)])
+@pytest.mark.parametrize("ps,gone", [(16, 1), (32, 3), (64, 0), (256, 1), (256, 2)])
+def test_missing_pages_in_every_kernel(hip_ready, d, G, S, ps, gone):
+    rng = np.random.default_rng(S + ps + gone)
+    n = 570
+    c = Cache(hip_ready, 1, 2, d, ps, 60, 2, 600 // ps + 1)
+    leftovers(c, 0x7B, rng)
+    c.fill(rng, [n], seqs=[1])
+    (kc, ks), (vc, vs) = c.cpu.read(0, 1)
+    table = c.cpu.table.copy()
+    table[1, gone] = (-1, 60, 1 << 30, -(1 << 31))[(S + gone) % 4]
+    c.gpu._buf["table"].upload(table)
+    q = rng.standard_normal((1, S, 2 * G, d)).astype(np.float16)
+    dq, do = c.cm.DeviceBuffer.from_numpy(q), c.cm.DeviceBuffer(q.nbytes)
+    for window in (0, 300):
+        c.gpu.attention(0, dq.ptr, do.ptr, 1, S, 2 * G, window=window, seqs=[1])
+        o = do.to_numpy(np.float16, q.shape)[0]
+        for r in range(S):
+            at = np.arange(max(0, n - S + r - window) if window else 0, n - S + r + 1)
+            at = at[at // ps != gone]
+            want, tol = attention(q[0, r:r + 1], kc[at], ks[at], vc[at], vs[at], len(at), 1 / math.sqrt(d), causal=False) \
+                if len(at) else (0, 0)
+            assert (np.abs(o[r] - want) <= tol).all(), (window, r)
+
+
 # ------------------------------------------------------------------ pages
 def test_extend_fork_free_compact_follow_the_model(hip_ready):
     rng = np.random.default_rng(10)
