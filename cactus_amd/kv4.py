@@ -24,16 +24,21 @@ class CacheDesc(ctypes.Structure):
         return ctypes.byref(self)
 
 
+class _List(DeviceBuffer):
+    """A list of slots, counts or pages that a call uploaded."""
+
+
 class KV4Cache:
     """Pages, tables and workspace of one cache, set up by cactus_hip_kv4_reset.
 
     The methods take device pointers (DeviceBuffer.ptr, or any integer) where
     the entry points do; slot and page lists may be sequences of ints, which
     are uploaded first (the call then waits for the stream).  `stream` is a
-    Stream's handle.  Scratch memory is kept per stream: calls on two streams may
-    overlap as the entry points say.  In a capture give pointers, and make the same
-    call once before it, so that the scratch memory is there; a graph that may
-    overlap eager calls needs the entry points and a workspace of its own."""
+    Stream's handle.  Scratch memory is kept per stream: calls on two streams, also
+    from two threads, may overlap as the entry points say.  In a capture give
+    pointers, and make the same call once before it, so that the scratch memory is
+    there; a graph that may overlap eager calls needs the entry points and a
+    workspace of its own."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, page_size: int, num_pages: int, max_seqs: int,
                  max_pages: int, stream=None):
@@ -45,11 +50,11 @@ class KV4Cache:
                      "lens": DeviceBuffer(4 * max_seqs), "refs": DeviceBuffer(4 * num_pages), "state": DeviceBuffer(16)}
         for name, b in self._buf.items():
             setattr(self.desc, name, b.ptr)
-        self._work, self._lists = {}, []
+        self._work = {}
         self.reset(stream)
 
     def _lst(self, v, n: int, stream=None):
-        """A device pointer as it is; a sequence of n ints or more uploaded (kept until the next such call ends)."""
+        """A device pointer as it is; a sequence of n ints or more uploaded, for the call that it is made for."""
         if v is None or isinstance(v, numbers.Integral):
             return None if v is None else int(v)
         a = np.asarray(v)
@@ -61,25 +66,27 @@ class KV4Cache:
             raise TypeError("a list of integers is needed")
         if a.min() < -(1 << 31) or a.max() >= 1 << 31:
             raise OverflowError("a list of 32-bit integers is needed")
-        b = DeviceBuffer.from_numpy(a.astype(np.int32), stream)
-        self._lists.append(b)
-        return b.ptr
+        return _List.from_numpy(a.astype(np.int32), stream)
 
     def _call(self, name, *args, stream=None):
-        call(name, self.desc.ref, *args, stream)
-        if self._lists:                       # uploaded lists go once the call has read them
-            call("cactus_hip_stream_sync", stream)
-            self._lists.clear()
+        # uploaded lists belong to this call, whatever other threads do, and go once it has read them
+        lists = [a for a in args if isinstance(a, _List)]
+        try:
+            call(name, self.desc.ref, *(a.ptr if isinstance(a, _List) else a for a in args), stream)
+        finally:
+            if lists:
+                call("cactus_hip_stream_sync", stream)
 
     def workspace(self, nbytes: int, stream=None):
         """At least nbytes of scratch memory for calls on `stream`, the first 4096 bytes zero."""
         work = self._work.setdefault(stream or 0, [])
-        if not work or work[-1].nbytes < nbytes:
+        last = work[-1] if work else None
+        if last is None or last.nbytes < nbytes:
             # a smaller one stays: a captured graph may hold its address
-            new = DeviceBuffer(max(nbytes, 4096))
-            call("cactus_hip_memset", new.ptr, 0, 4096, stream)
-            work.append(new)
-        return work[-1].ptr, work[-1].nbytes
+            last = DeviceBuffer(max(nbytes, 4096))
+            call("cactus_hip_memset", last.ptr, 0, 4096, stream)
+            work.append(last)
+        return last.ptr, last.nbytes
 
     def reset(self, stream=None):
         self._call("cactus_hip_kv4_reset", stream=stream)

@@ -1,6 +1,7 @@
 """The paged 4-bit KV cache without a GPU: refusals before any launch, sizes,
 and the restatement's own quantization."""
 import ctypes
+import gc
 
 import numpy as np
 import pytest
@@ -142,3 +143,76 @@ def test_the_quantized_values_are_exact_fp16_numbers_near_the_input():
     g = np.abs(x.astype(np.float64)).reshape(400, -1, 32).max(-1).repeat(32, -1)
     bound = np.repeat(s.astype(np.float64), 32, -1).reshape(x.shape) / 2 + g * 2.0 ** -9 + 7 * 2.0 ** -25
     assert (np.abs(y - x) <= bound).all()
+
+
+class Memory:
+    """Stands in for the library: which allocations live, and which lists the queued work of each stream reads."""
+
+    def __init__(self, monkeypatch):
+        import cactus_amd
+        self.live, self.queued, self.wrong, self.hooks = set(), {}, [], {}
+        self.next, self.uploads = 1 << 20, 0
+        monkeypatch.setattr(cactus_amd, "call", self.call)
+        monkeypatch.setattr("cactus_amd.kv4.call", self.call)
+        monkeypatch.setattr(cactus_amd, "hip", lambda: self)
+        monkeypatch.setattr("cactus_amd.kv4.hip", lambda: self)
+
+    def call(self, name, *args):
+        if name == "cactus_hip_malloc":
+            self.next += 4096
+            args[0]._obj.value = self.next
+            self.live.add(self.next)
+        elif name == "cactus_hip_kv4_bytes":
+            args[1]._obj.value = 4096
+        elif name == "cactus_hip_stream_sync":
+            self.queued[args[0]] = set()
+        elif name in ("cactus_hip_kv4_extend", "cactus_hip_kv4_fork"):
+            lists = set(args[1:3])
+            if not lists <= self.live:
+                self.wrong.append(f"{name} given freed lists on stream {args[-1]}")
+            self.queued.setdefault(args[-1], set()).update(lists)
+            if name in self.hooks:
+                self.hooks.pop(name)()
+            if name == "cactus_hip_kv4_fork":
+                raise RuntimeError("refused behind its first launch")
+        self.uploads += name == "cactus_hip_memcpy_h2d"
+        if self.uploads == 2 and "second upload" in self.hooks:
+            self.hooks.pop("second upload")()
+
+    def cactus_hip_free(self, p):
+        self.live.discard(p)
+        self.wrong += [f"list freed under stream {s}" for s, lists in self.queued.items() if p in lists]
+
+    def cactus_hip_kv4_pages_workspace(self, cache, n):
+        return 8192
+
+
+@pytest.mark.parametrize("when", ["second upload", "cactus_hip_kv4_extend"])
+def test_lists_of_a_call_outlive_another_threads_call(monkeypatch, when):
+    """A second thread's whole call falls between this one's upload, launch and wait."""
+    import threading
+    from cactus_amd.kv4 import KV4Cache
+    mem = Memory(monkeypatch)
+    c = KV4Cache(1, 1, 64, 16, 8, 4, 4)
+
+    def other():
+        t = threading.Thread(target=lambda: c.extend(2, seqs=[2, 3], counts=[1, 1], stream=7))
+        t.start()
+        t.join()
+
+    mem.hooks[when] = other
+    held = len(mem.live)
+    c.extend(2, seqs=[0, 1], counts=[1, 1], stream=5)
+    assert mem.wrong == [] and len(mem.live) == held
+
+
+def test_lists_of_a_call_that_fails_go_when_the_stream_is_done(monkeypatch):
+    from cactus_amd.kv4 import KV4Cache
+    mem = Memory(monkeypatch)
+    c = KV4Cache(1, 1, 64, 16, 8, 4, 4)
+    c.workspace(8192, 5)
+    held = len(mem.live)
+    with pytest.raises(RuntimeError):
+        c.fork([0, 1], [2, 3], stream=5)
+    gc.collect()                               # the exception's frames
+    assert mem.wrong == [] and len(mem.live) == held and not mem.queued[5]
