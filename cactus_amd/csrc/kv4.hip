@@ -322,6 +322,7 @@ __global__ void __launch_bounds__(BK_THREADS) kv4_extend_kernel(Kv4View c, const
     __shared__ int bad, total_s;
     const int tid = threadIdx.x, cap = c.max_pages << c.ps_log2;
     const int free_pages = c.state[KV4_FREE], hint = c.state[KV4_HINT];   // (before anything is waited for)
+    if (c.state[KV4_STATUS] != 0) return;     // the appends to come write nothing: no tokens for them
     for (int i = tid; i < (c.max_seqs + 31) / 32; i += BK_THREADS) bits[i] = 0;
     if (tid == 0) {
         bad = 0;
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(BK_THREADS) kv4_extend_kernel(Kv4View c, const
 
 // Lists of a fork in the workspace, behind the attention's counters.
 struct ForkPlan {
-    int32_t* ok;         // [2] whether the call is carried out, pages it takes
+    int32_t* ok;         // [3] whether the call is carried out, pages it takes, status bits
     int32_t* tail;       // [n] new page of the partly filled last one, -1
     int32_t* len;        // [n] the source's tokens before the call
     int32_t* rows;       // [n][max_pages] the source's pages before the call
@@ -428,16 +429,17 @@ __device__ bool fork_checked(const Kv4View& c, const int32_t* src, const int32_t
 // aside (row and length) and raises its full pages' counts.  Each checks the call
 // by itself, so that one launch does both: the counts of pages in use are raised
 // while workgroup 0 looks for pages whose count is 0, and the number of free
-// pages, which all of them read, changes in the second launch.
+// pages and the status, which all of them read, change in the second launch.
 __global__ void __launch_bounds__(BK_THREADS) kv4_fork_plan_kernel(Kv4View c, ForkPlan p, const int32_t* src,
                                                                    const int32_t* dst, int n) {
     __shared__ uint32_t bits[KV4_MAX_SEQS / 32];
     __shared__ int ids[BK_IDS], wave_sums[16], counts[2];
     const int tid = threadIdx.x, ps1 = (1 << c.ps_log2) - 1;
     const int free_pages = c.state[KV4_FREE], hint = c.state[KV4_HINT];   // (before anything is waited for)
+    const int status = c.state[KV4_STATUS];
     int total;
     const bool right = fork_checked(c, src, dst, n, bits, counts, &total);
-    const bool ok = right && total <= free_pages;
+    const bool ok = right && total <= free_pages && status == 0;
     if (blockIdx.x > 0) {
         const int i = blockIdx.x - 1;
         if (!ok) return;
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(BK_THREADS) kv4_fork_plan_kernel(Kv4View c, Fo
     if (tid == 0) {
         p.ok[0] = ok;
         p.ok[1] = total;
-        if (!ok) atomicOr((uint32_t*)c.state + KV4_STATUS, right ? CACTUS_HIP_KV4_NO_PAGES : CACTUS_HIP_KV4_BAD_REQUEST);
+        p.ok[2] = ok || status ? 0 : right ? CACTUS_HIP_KV4_NO_PAGES : CACTUS_HIP_KV4_BAD_REQUEST;
     }
     if (!ok) return;
     // at most max_seqs pages: dst slots differ
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(BK_THREADS) kv4_fork_plan_kernel(Kv4View c, Fo
         const int got = done < total ? collect_free(c, &at, total - done, ids, wave_sums) : 0;
         if (got == 0 && done < total) {
             // the free count was wrong: the pairs behind are left without a last page
-            if (tid == 0) atomicOr((uint32_t*)c.state + KV4_STATUS, CACTUS_HIP_KV4_NO_PAGES);
+            if (tid == 0) p.ok[2] = CACTUS_HIP_KV4_NO_PAGES;
             for (int i = tid; i < n; i += BK_THREADS) p.tail[i] = done ? p.tail[i] : -1;
             break;
         }
@@ -549,9 +551,12 @@ __device__ __forceinline__ void copy_piece(uint8_t* dst, const uint8_t* src, siz
 // block y 0: the destination's table row; from 1 on: a piece of the last page, a layer
 __global__ void __launch_bounds__(256) kv4_fork_apply_kernel(Kv4View c, ForkPlan p, const int32_t* src, const int32_t* dst,
                                                              int pieces) {
+    const int i = blockIdx.x;
+    const bool first = blockIdx.y == 0 && i == 0 && threadIdx.x == 0;
+    if (first && p.ok[2]) atomicOr((uint32_t*)c.state + KV4_STATUS, (uint32_t)p.ok[2]);
     if (!p.ok[0]) return;
-    const int i = blockIdx.x, d = kv4_slot(c, dst, i);
-    if (blockIdx.y == 0 && i == 0 && threadIdx.x == 0) atomicSub(&c.state[KV4_FREE], p.ok[1]);
+    const int d = kv4_slot(c, dst, i);
+    if (first) atomicSub(&c.state[KV4_FREE], p.ok[1]);
     if (kv4_slot(c, src, i) == d) return;
     const int32_t* row = p.rows + (size_t)i * c.max_pages;
     const int len = p.len[i], full = len >> c.ps_log2, tail = p.tail[i];

@@ -488,7 +488,8 @@ int cactus_hip_kv4_bytes(const cactus_hip_kv4_cache* cache, size_t* bytes);
 /* no tokens in any slot, every page free, status 0 (page contents stay) */
 int cactus_hip_kv4_reset(const cactus_hip_kv4_cache* cache, void* stream);
 /* Status bits since the last call or reset, which clears them; waits for the
- * stream.  While a bit is set, appends write nothing. */
+ * stream.  While a bit is set, extends, forks and appends change nothing, so that a
+ * slot never counts tokens whose append was held back; the other calls go on. */
 int cactus_hip_kv4_status(const cactus_hip_kv4_cache* cache, int* status, void* stream);
 /* Slot seqs[i] grows by counts[i] tokens (counts NULL: by `count` each): the
  * pages that it needs are the lowest free ones, in request order.  All or

@@ -604,6 +604,89 @@ def test_refused_requests_change_nothing(hip_ready):
     c.check()
 
 
+def test_nothing_grows_until_the_status_is_read(hip_ready):
+    """An append that the status holds back leaves no tokens behind: extend and fork are held back with it."""
+    rng = np.random.default_rng(16)
+    c = Cache(hip_ready, 2, 1, 64, 16, 12, 4, 8)
+    c.fill(rng, [40, 17])
+    k = c.cm.DeviceBuffer.from_numpy(kv_rows(rng, 2, 20, 1, 64))
+    for set_bit, bit in ((lambda: c.gpu.free([77]), 2), (lambda: c.gpu.copy_pages([0], [12]), 2),
+                         (lambda: c.gpu.extend(1, 128, seqs=[3]), 1), (lambda: c.gpu.fork([0, 0], [2, 2]), 2)):
+        set_bit()
+        c.gpu.extend(2, seqs=[0, 1], counts=[3, 20])
+        for layer in range(2):
+            c.gpu.append(layer, k.ptr, k.ptr, 2, 20, seqs=[0, 1], counts=[3, 20])
+        c.gpu.fork([0, 1], [2, 0])
+        c.check()
+        assert c.gpu.status() == bit and c.gpu.status() == 0
+    # pages are given up in any case, and what follows the reading goes on from there
+    c.gpu.free([1, 9])
+    c.cpu.free([1])
+    c.gpu.compact()
+    c.cpu.compact()
+    c.check()
+    assert c.gpu.status() == 2
+    c.fill(rng, [3, 20], seqs=[0, 1])
+    assert c.cpu.fork([0, 1], [2, 0]) == 0
+    c.gpu.fork([0, 1], [2, 0])
+    c.check()
+    assert c.gpu.status() == 0
+
+
+def test_a_captured_step_in_a_full_pool(hip_ready):
+    """Replays of extend and append past the last free page, then with pages free but the status not read yet."""
+    cm, rng = hip_ready, np.random.default_rng(17)
+    c = Cache(cm, 1, 1, 64, 16, 6, 3, 4)
+    c.fill(rng, [30, 14, 20])
+    stream = cm.Stream()
+    st = stream.handle
+    kv = [cm.DeviceBuffer(2 * 64 * 2) for _ in range(2)]
+    graph = ctypes.c_void_p()
+    cm.call("cactus_hip_graph_capture_begin", st)
+    cm.call("cactus_hip_kv4_extend", c.gpu.desc.ref, None, None, 2, 1, st)
+    cm.call("cactus_hip_kv4_append_f16", c.gpu.desc.ref, 0, None, None, kv[0].ptr, kv[1].ptr, 2, 1, 64, st)
+    cm.call("cactus_hip_graph_capture_end", st, ctypes.byref(graph))
+
+    def replay(grows):
+        k, v = kv_rows(rng, 2, 1, 1, 64), kv_rows(rng, 2, 1, 1, 64)
+        kv[0].upload(k, st), kv[1].upload(v, st)
+        cm.call("cactus_hip_graph_launch", graph, st)
+        stream.sync()
+        if grows:
+            assert c.cpu.extend([0, 1], [1, 1]) == 0
+            for b in range(2):
+                c.cpu.write(0, b, c.cpu.lens[b] - 1, k[b, 0], v[b, 0])
+        c.check()
+
+    replay(True)
+    replay(True)               # both pages are full now, and one page is free
+    replay(False)              # two are needed
+    replay(False)
+    c.gpu.free([2], stream=st)
+    c.cpu.free([2])
+    replay(False)              # there would be pages
+    assert c.gpu.status(st) == 1
+    for _ in range(3):
+        replay(True)
+    assert c.gpu.status(st) == 0
+    cm.call("cactus_hip_graph_destroy", graph)
+
+
+def test_a_fork_that_a_wrong_free_count_lets_through(hip_ready):
+    """state[0] promises a page that is not there: the status says so, and no page is used twice."""
+    rng = np.random.default_rng(18)
+    c = Cache(hip_ready, 1, 1, 64, 16, 4, 3, 4)
+    c.fill(rng, [40, 10])
+    before = c.gpu.tables()
+    c.gpu._buf["state"].upload(np.array([3, 0, 0, 0], np.int32))
+    c.gpu.fork([0], [2])
+    assert c.gpu.status() == 1
+    after = c.gpu.tables()
+    np.testing.assert_array_equal(after["refs"], before["refs"] + [1, 1, 0, 0])
+    np.testing.assert_array_equal(after["table"], np.vstack([before["table"][:2], [0, 1, -1, -1]]))
+    np.testing.assert_array_equal(c.pages(), c.cpu.pages)
+
+
 # ------------------------------------------------------------------ together
 def test_a_serving_run(hip_ready):
     """Prompts, beams, drafted tokens, conversations that end and a packed pool, every step's attention checked."""
