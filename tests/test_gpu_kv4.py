@@ -247,6 +247,37 @@ def test_offsets_past_32_bits(hip_ready):
         np.testing.assert_array_equal(*(b[i].to_numpy(np.uint16, k.shape) for b in back))
 
 
+@pytest.mark.parametrize("S,Hq", [(70, 8), (60, 32)])
+def test_many_rows_past_32_bits(hip_ready, S, Hq):
+    """The many-row kernel over pages that begin behind 4 GB of a pool."""
+    from cactus_amd.kv4 import CacheDesc
+    cm, rng = hip_ready, np.random.default_rng(24)
+    H, d, ps, N, n = 8, 256, 256, 8300, 600
+    page = H * ps * d * 9 // 8
+    ids = [N - 1, 8000, N - 7]
+    assert min(ids) * page > 1 << 32
+    one = Cache(cm, 1, H, d, ps, 4, 1, 4)                     # the same tokens in a small pool
+    assert one.extend([0], [n]) == 0
+    pool = cm.DeviceBuffer(N * page)
+    bufs = [cm.DeviceBuffer.from_numpy(np.array(x, np.int32)) for x in ([ids + [-1]], [n], [0] * N, [0] * 4)]
+    desc = CacheDesc(pages=pool.ptr, table=bufs[0].ptr, lens=bufs[1].ptr, refs=bufs[2].ptr, state=bufs[3].ptr, layers=1,
+                     kv_heads=H, head_dim=d, page_size=ps, num_pages=N, max_seqs=1, max_pages=4)
+    k, v = (cm.DeviceBuffer.from_numpy(kv_rows(rng, 1, n, H, d)) for _ in range(2))
+    q = rng.standard_normal((1, S, Hq, d)).astype(np.float16)
+    dq, outs = cm.DeviceBuffer.from_numpy(q), []
+    need = cm.hip().cactus_hip_attention_kv4_workspace(desc.ref, 1, S, Hq)
+    work = cm.DeviceBuffer(need)
+    cm.call("cactus_hip_memset", work.ptr, 0, 4096, None)
+    for c in (desc, one.gpu.desc):
+        cm.call("cactus_hip_kv4_append_f16", c.ref, 0, None, None, k.ptr, v.ptr, 1, n, H * d, None)
+        do = cm.DeviceBuffer.from_numpy(np.full(q.shape, np.float16(np.nan)))
+        cm.call("cactus_hip_attention_kv4_f16", c.ref, 0, None, None, dq.ptr, Hq * d, do.ptr, 1, S, Hq, 0.0, 0, 0, 1, work.ptr,
+                need, None)
+        outs.append(do.to_numpy(np.float16, q.shape))
+    assert np.isfinite(outs[0]).all()
+    np.testing.assert_array_equal(*outs)
+
+
 def test_two_streams_at_once(hip_ready):
     """Calls that overlap, with a workspace each, give what they give alone."""
     cm, rng = hip_ready, np.random.default_rng(22)
