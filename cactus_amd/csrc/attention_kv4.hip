@@ -223,6 +223,22 @@ __device__ __forceinline__ float sum_lanes(float v) {
     return v;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_fmaxf(__builtin_fmaxf(a, b), c); }
+// f over the four lanes of a column (16 apart), in each of them, by lane swaps: a step in
+// which the maximum rises waits for the result twice
+template <class F>
+__device__ __forceinline__ float column(float v, F f) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);     // rows 0, 0, 2, 2 and 1, 1, 3, 3
+    const uint32_t w = __builtin_bit_cast(uint32_t, f(bits_f(r[0]), bits_f(r[1])));
+    const auto t = __builtin_amdgcn_permlane32_swap(w, w, false, false);     // the lower half twice, and the upper one
+    return f(bits_f(t[0]), bits_f(t[1]));
+}
+__device__ __forceinline__ float column_max(float v) {
+    return column(v, [](float a, float b) { return __builtin_fmaxf(a, b); });
+}
+__device__ __forceinline__ float column_sum(float v) {
+    return column(v, [](float a, float b) { return a + b; });
+}
 
 // 16 bytes per active lane to LDS; ONCE: not to be kept in the caches
 template <bool ONCE>
@@ -411,15 +427,17 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
         const int last_pos = sq.len - sq.rows + a.by_g(v0 + nvec - 1);
         const int all = a.causal ? min(first_pos + 1, sq.len) : sq.len;
 
-        // The products p s are lifted by 2^(26 - top_exp), top_exp the exponent field of
-        // the largest value scale seen: s 2^lift is below 2^12 then, and below 2^15, which FP16 holds,
-        // until one eight times as large is met.  (Without it the weights of small
-        // values, or of many keys beside one that takes most of the weight, fell
-        // to FP16 subnormals or to zero; it costs 2% of a decode step of 32 requests,
-        // 8% of five drafted rows of heads of 64.)
-        int top_exp = 0;
-        uint32_t scale_end = 0;      // a scale from here on raises top_exp
+        // The products p s are lifted by 2^lift_exp before they become FP16: so that a
+        // step's largest is below 2^12 where it is chosen (as the maximum rises, or
+        // when a product reaches 2^15; FP16 holds 2^16).  It then keeps its 11 bits
+        // down to 2^-25 of that product.  (Without it the weights of small values, or of many
+        // keys beside one that takes most of the weight, fell to FP16 subnormals or
+        // to zero; chosen by the scales alone, one key of large values and no
+        // weight did that to the others.  It costs 2% of a decode step of 32 requests,
+        // 10% of five drafted rows of heads of 64.)
+        int lift_exp = 26;
         float lift = 0x1p26f;
+        uint32_t scale_end = 0;      // 2^15 / lift: below it no scale's products reach 2^15
         float m = -__builtin_inff(), mbase = 0.0f, l = 0.0f;
         f32x4 acc[NB], off[SG];       // O^T 2^-24 (odd blocks 2^-20) before the 8 comes off, -8 2^-24 sum p s_g
 #pragma unroll
@@ -485,38 +503,15 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
             // the running maximum, where one of the step's scores is above it (a
             // NaN score reaches the sum by itself)
             float top = max3(max3(x[0][0], x[0][1], x[0][2]), max3(x[0][3], x[1][0], x[1][1]), __builtin_fmaxf(x[1][2], x[1][3]));
-            u16x2 sc = __builtin_bit_cast(u16x2, vs[0][0]);
-#pragma unroll
-            for (int k = 1; k < 4 * SG; k++)
-                sc = __builtin_elementwise_max(sc, __builtin_bit_cast(u16x2, vs[k / (2 * SG)][k % (2 * SG)]));
-            const uint32_t top_scale = max((uint32_t)sc[0], (uint32_t)sc[1]);
-            if (__ballot((top > m) | (top_scale >= scale_end))) {
-                top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
-                top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
-                int se = (int)(top_scale >> 10);
-                if (__builtin_expect(__ballot(se > 30) != 0, 0)) {       // NaNs: not counted
-                    se = 0;
-#pragma unroll
-                    for (int k = 0; k < 4 * SG; k++) {
-                        const int lo = vs[k / (2 * SG)][k % (2 * SG)] >> 10 & 31, hi = vs[k / (2 * SG)][k % (2 * SG)] >> 26 & 31;
-                        se = max(se, max(lo > 30 ? 0 : lo, hi > 30 ? 0 : hi));
-                    }
-                }
-                se = max(se, __shfl_xor(se, 16, 64));
-                se = max(max(se, __shfl_xor(se, 32, 64)), top_exp);
+            const bool rises = __ballot(top > m) != 0;
+            float f = 1.0f;
+            if (rises) {
+                top = column_max(top);
                 const float mn = __builtin_fmaxf(m, top);
                 mbase = mn > -__builtin_inff() ? mn : 0.0f;
-                const float f = exp2_fast(m - mbase);      // 0 where nothing was there
+                f = exp2_fast(m - mbase);                  // 0 where nothing was there
                 m = mn;
                 l *= f;
-                const float fs = __builtin_ldexpf(f, top_exp - se);
-                top_exp = se;
-                scale_end = (uint32_t)(se + 4) << 10;
-                lift = __builtin_ldexpf(1.0f, 26 - se);
-#pragma unroll
-                for (int i = 0; i < NB; i++) acc[i] *= fs;
-#pragma unroll
-                for (int g = 0; g < SG; g++) off[g] *= fs;
             }
             float p[2][4];
 #pragma unroll
@@ -525,8 +520,39 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
                 for (int i = 0; i < 4; i++) {
                     p[t][i] = exp2_fast(x[t][i] - mbase);
                     l += p[t][i];
-                    p[t][i] *= lift;
                 }
+            u16x2 sc = __builtin_bit_cast(u16x2, vs[0][0]);
+#pragma unroll
+            for (int k = 1; k < 4 * SG; k++)
+                sc = __builtin_elementwise_max(sc, __builtin_bit_cast(u16x2, vs[k / (2 * SG)][k % (2 * SG)]));
+            // (no weight is above 1, and no product of the lane above that of its largest
+            // weight and largest scale)
+            const uint32_t top_scale = max((uint32_t)sc[0], (uint32_t)sc[1]);
+            if (rises || (__ballot(top_scale >= scale_end) &&
+                          __ballot(!(exp2_fast(top - mbase) * lift * h2f((uint16_t)top_scale) < 0x1p15f)))) {
+                float most = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4 * SG; k++) {
+                    const int t = k / (2 * SG), i = 2 * (k & 1);
+                    uint32_t s = vs[t][k % (2 * SG)];
+                    asm volatile("" : "+v"(s));      // (converted here: held until the products, the scales spilled)
+                    most = max3(most, __builtin_fabsf(mul_half<0>(p[t][i], s)), __builtin_fabsf(mul_half<1>(p[t][i + 1], s)));
+                }
+                most = column_max(most);             // (NaNs are not counted)
+                const int to = most > 0.0f ? min(12 - __builtin_amdgcn_frexp_expf(most), 26) : 26;
+                const float fs = __builtin_ldexpf(f, to - lift_exp);
+                lift_exp = to;
+                lift = __builtin_ldexpf(1.0f, to);
+                scale_end = (uint32_t)(30 - to) << 10;
+#pragma unroll
+                for (int i = 0; i < NB; i++) acc[i] *= fs;
+#pragma unroll
+                for (int g = 0; g < SG; g++) off[g] *= fs;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[t][i] *= lift;
             h16x8 pf[SG];
 #pragma unroll
             for (int g = 0; g < SG; g++) {
@@ -576,9 +602,8 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
         int et = tid;
         asm volatile("" : "+v"(et));
         const int eh = (et & 63) >> 4;
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
-        const float drop = __builtin_ldexpf(1.0f, top_exp - 26 + 24);      // the lift, and the codes' 2^-24
+        l = column_sum(l);
+        const float drop = __builtin_ldexpf(1.0f, 24 - lift_exp);      // the lift, and the codes' 2^-24
         if (live) {
 #pragma unroll
             for (int g = 0; g < NG; g++) {

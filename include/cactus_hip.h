@@ -523,10 +523,10 @@ int cactus_hip_kv4_read_f16(const cactus_hip_kv4_cache* cache, size_t layer, con
  * that sees no key gets zeros, rows behind m are left as they were.
  * window_size counts as cactus_hip_attention_f16's; sink_size without a
  * window has no effect.  Scores, softmax and sums in FP32; the weights are
- * rounded to FP16 for the matrix product with the values (for few rows: their
- * products with the value scales), to 2^-11 of each down to 2^-18 of the
- * largest.  A query vector with a NaN or an
- * infinity leaves its own output undefined, and no other.
+ * rounded to FP16 for the matrix product with the values (up to 64 query vectors per
+ * request and KV head: their products with the value scales), to 2^-11 of each down
+ * to 2^-21 of the row's largest.  A query vector with a NaN or an infinity leaves its
+ * own output undefined, and no other.
  * workspace: device memory of at least cactus_hip_attention_kv4_workspace
  * bytes, 256-byte aligned, its first 4096 bytes zero before the first call
  * that uses it (every call leaves them zero); calls that may overlap need

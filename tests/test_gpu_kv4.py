@@ -380,6 +380,28 @@ def test_many_small_weights_beside_a_large_one(hip_ready, d, S, G, size):
     c.attend(q, [0], [S], scale=1 / 8, small=False)
 
 
+@pytest.mark.parametrize("d,S,G", [(64, 1, 1), (128, 1, 2), (256, 1, 2), (64, 5, 3), (128, 9, 2), (256, 4, 4), (64, 80, 1)])
+@pytest.mark.parametrize("n,sink,outlier", [(3000, 3, 0), (3000, 3, 1999), (3000, 1500, 0), (3000, 1500, 1501), (200, 3, 0),
+                                            (200, 150, 60), (30, 3, 0), (30, 3, 20)])
+@pytest.mark.parametrize("size", [0.02, 2.0])
+def test_a_large_value_without_weight_leaves_the_others_their_bits(hip_ready, d, S, G, n, sink, outlier, size):
+    """As above, and one key with values of up to 60000 whose weight is 2^-100 of the largest: the products of weight and
+    value scale that count lie within 2^11 of each other, whatever the scales alone do (an output then is off by the
+    products' and its own rounding, 2^-11 each, and 2^-25; that key's share is below 2^-80)."""
+    rng = np.random.default_rng(d + S + outlier)
+    c = Cache(hip_ready, 1, 1, d, 64, 50, 1, 50)
+    assert c.extend([0], [n]) == 0
+    k = (0.1 * rng.standard_normal((1, n, 1, d))).astype(np.float16)
+    v = (size * (1 + 0.3 * rng.standard_normal((1, n, 1, d)))).astype(np.float16)
+    k[..., 0], k[0, sink, 0, 0], k[0, outlier, 0, 0] = 0, 12, -60
+    v[0, sink], v[0, outlier] = 0, (60000 * rng.uniform(-1, 1, (1, d))).astype(np.float16)
+    c.append(0, [0], [n], k, v)
+    S = min(S, n - 4)
+    q = rng.standard_normal((1, S, G, d)).astype(np.float16)
+    q[..., 0] = 8
+    c.attend(q, [0], [S], scale=1 / 8, small=False)
+
+
 def test_a_query_that_is_not_finite_leaves_the_others(hip_ready):
     rng = np.random.default_rng(23)
     c = Cache(hip_ready, 1, 2, 128, 16, 40, 2, 20)
