@@ -303,7 +303,8 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
     // longer stretches, for one or two such rounds, where that saves more (one row at
     // 9000 keys, 16 / 8 heads of 128, in stretches of 1, 2, 3 and 4 steps: 14.2, 12.8,
     // 11.3 and 12.7 us; at 4096, one round in any case: 9.1, 10.3, 11.1 and 12.0; at
-    // 32000: 24.8 -> 16.8).  With 16 vectors a step costs more than a round.
+    // 32000: 24.8 -> 16.8; heads of 64 and 256 were not timed).  With 16 vectors a
+    // step costs more than a round.
     if constexpr (PACK) {
         const uint32_t one = ((uint32_t)longest + (1u << a.join_log2) - 1) >> a.join_log2;   // steps of a part for one round
         const uint32_t rounds = (uint32_t)((float)(one + per - 1) * __builtin_amdgcn_rcpf((float)per));
@@ -744,7 +745,7 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
 
 // ------------------------------------------------------------ many rows
 // A workgroup takes 32 W query vectors of one KV head, 32 per wave in two
-// column blocks of 16, and walks the keys PF_KEYS at a time.  Each stage's codes
+// column blocks of 16, and walks the keys 16 W at a time.  Each stage's codes
 // become FP16 values once for all the waves: (u - 8) s is exact in FP16 (the
 // scale has 8 significant bits), so nothing is rounded that the few-row kernel
 // does not round, and the scores and outputs are plain products without a scale
@@ -755,8 +756,8 @@ __global__ void __launch_bounds__((64 * kv4_waves<D, PACK>()), (kv4_per_cu<D, PA
 // A column's maximum is raised only when a score exceeds it by 2^PF_SLACK, and
 // the outputs are rescaled a few times per row instead of at every new maximum.  The
 // weights are 2^PF_LIFT times those of the maximum, below 2^15 (FP16 holds 2^16):
-// where one key takes most of the weight, the many small ones keep their bits.  The sum of the weights is a
-// product with ones, of the rounded weights that the outputs use.
+// where one key takes most of the weight, the many small ones keep their bits.  The
+// sum of the weights is a product with ones, of the rounded weights that the outputs use.
 constexpr int PF_SLACK = 8, PF_LIFT = 7;
 //
 // More query vectors of a request per KV head than PF_FROM come here.  Its 256
@@ -764,7 +765,8 @@ constexpr int PF_SLACK = 8, PF_LIFT = 7;
 // launch: 40 vectors at 4096 keys, 8 heads of 128: 14.2 us there, 20.6 here; 8
 // requests of 40 at 9000: 62 and 73; 16 of 64 at 2000: 41 and 46.  With more the
 // codes are unpacked too often there: 4 requests of 68 at 4096: 33.5 there, 27.5
-// here; one of 128 at 32000: 71 and 46 (at 8000 25 and 26, at 2000 13 and 20).
+// here; one of 128 at 32000: 71 and 46 (at 8000 25 and 26, at 2000 13 and 20: the
+// rule goes by vectors alone, and a single request of few keys pays for that).
 constexpr size_t PF_FROM = 64;
 
 typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
@@ -1232,7 +1234,9 @@ __global__ void __launch_bounds__(64 * W, W == 8 ? 2 : 1) attn_kv4_prefill_kerne
         // Iteration i writes stage i + 1's operands and uses stage i's (from i0 - 1 on:
         // one copy of the code).  Two waves share a SIMD's units: the first four prepare
         // the next stage before their products, the others after theirs, so that one
-        // wave's vector instructions run beside the other's matrix ones.
+        // wave's vector instructions run beside the other's matrix ones.  (With four
+        // waves, heads of 256, there is no other: 2048 rows by 16384 keys, 32 / 8
+        // heads, at 592 TFLOP/s where heads of 128 reach 981.)
         uint32_t now = 0;
 #pragma unroll 1
         for (int i = i0 - 1; i < i1; i++) {

@@ -455,7 +455,9 @@ int cactus_hip_kv_window_shift(const cactus_hip_kv_layer* layers, size_t nlayers
  * hold the page (0: free); state[0] the number of free pages, state[1] a
  * page below which none is free, state[2] status bits (sticky, see
  * cactus_hip_kv4_status), state[3] 0.  Full pages may be shared by slots, a
- * partly filled one never is.  cactus_hip_kv4_reset sets up all four.
+ * partly filled one never is.  cactus_hip_kv4_reset sets up all four; after it
+ * only the calls below may change them (lens lowered by hand leaves pages that no call
+ * gives up, and may leave a shared page partly filled).
  *
  * `seqs` (device, NULL: request i is slot i) names the slot of each request;
  * `counts` (device, NULL: seq_len each) its rows, the first counts[i] of
@@ -501,7 +503,9 @@ int cactus_hip_kv4_extend(const cactus_hip_kv4_cache* cache, const int32_t* seqs
 /* Quantizes k, v [batch][seq_len] rows of [kv_heads][head_dim] fp16, kv_stride
  * values from row to row (a multiple of 8, at least kv_heads * head_dim; k and
  * v 16-byte aligned), into layer `layer`: request i's rows become the last
- * counts[i] tokens of its slot.  Slots have to differ from each other. */
+ * counts[i] tokens of its slot.  Slots have to differ from each other, and the
+ * tokens have to be on pages that no other slot holds, as those of an extend are
+ * until a fork: tokens written again on a shared page change for all its slots. */
 int cactus_hip_kv4_append_f16(const cactus_hip_kv4_cache* cache, size_t layer, const int32_t* seqs,
                               const int32_t* counts, const uint16_t* k, const uint16_t* v, size_t batch,
                               size_t seq_len, size_t kv_stride, void* stream);
