@@ -68,6 +68,12 @@ class KV4Cache:
             raise OverflowError("a list of 32-bit integers is needed")
         return _List.from_numpy(a.astype(np.int32), stream)
 
+    @staticmethod
+    def _pairs(src, dst) -> int:
+        if len(src) != len(dst):
+            raise ValueError(f"{len(src)} sources, {len(dst)} destinations")
+        return len(src)
+
     def _call(self, name, *args, stream=None):
         # uploaded lists belong to this call, whatever other threads do, and go once it has read them
         lists = [a for a in args if isinstance(a, _List)]
@@ -120,7 +126,7 @@ class KV4Cache:
                    stride, o, batch, seq_len, num_q_heads, scale, window, sink, int(causal), work, size, stream=stream)
 
     def fork(self, src, dst, n: int | None = None, stream=None):
-        n = len(src) if n is None else n
+        n = self._pairs(src, dst) if n is None else n
         work, size = self.workspace(hip().cactus_hip_kv4_pages_workspace(self.desc.ref, n), stream)
         self._call("cactus_hip_kv4_fork", self._lst(src, n, stream), self._lst(dst, n, stream), n, work, size, stream=stream)
 
@@ -133,7 +139,7 @@ class KV4Cache:
         self._call("cactus_hip_kv4_compact", work, size, stream=stream)
 
     def copy_pages(self, src, dst, n: int | None = None, stream=None):
-        n = len(src) if n is None else n
+        n = self._pairs(src, dst) if n is None else n
         self._call("cactus_hip_kv4_copy_pages", self._lst(src, n, stream), self._lst(dst, n, stream), n, stream=stream)
 
     def tables(self, stream=None) -> dict:

@@ -216,3 +216,16 @@ def test_lists_of_a_call_that_fails_go_when_the_stream_is_done(monkeypatch):
         c.fork([0, 1], [2, 3], stream=5)
     gc.collect()                               # the exception's frames
     assert mem.wrong == [] and len(mem.live) == held and not mem.queued[5]
+
+
+def test_pairs_of_different_lengths_are_refused(monkeypatch):
+    from cactus_amd.kv4 import KV4Cache
+    mem = Memory(monkeypatch)
+    c = KV4Cache(1, 1, 64, 16, 8, 4, 4)
+    held = set(mem.live)
+    for call in (c.fork, c.copy_pages):
+        for src, dst in (([0], [1, 2]), ([0, 1], [2])):
+            with pytest.raises(ValueError):
+                call(src, dst)
+    gc.collect()
+    assert mem.live == held and mem.queued == {}
