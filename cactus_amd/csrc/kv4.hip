@@ -14,72 +14,8 @@ namespace cactus_hip {
 // quad of lanes: the quads transpose 4 x 4 bytes in registers, so that pages are
 // read and written 4 bytes per group and lane, contiguous over the groups.
 //
-// Per value: x / s to the nearest integer, ties to even.  x has 11 significant
-// bits and (k + 1/2) s at most 12, so x / s is either exactly k + 1/2 or at least
-// 2^-13 away from it; x times the FP32 reciprocal of s is within 2^-20 of x / s, and
-// rounded to a multiple of 2^-14 it falls on the same side, ties included (an
-// exact division took twice the instructions).
-//
 // Bound by memory for prompts, by the chain of loads (slot, length, page, row) for
 // single tokens.
-
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
-
-// Scale of a group from the bits of its largest magnitude: a / 7 rounded to 8
-// significant bits (bf16) and then to fp16, which only rounds again where the
-// scale is an fp16 subnormal.  NaN for a NaN or an infinity.
-__device__ __forceinline__ uint16_t kv4_scale(uint32_t abits) {
-    const float q = h2f((uint16_t)abits) / 7.0f;
-    uint32_t b = __builtin_bit_cast(uint32_t, q);
-    b = (b + 0x7FFFu + ((b >> 16) & 1u)) & 0xFFFF0000u;   // finite: to nearest, ties to even
-    return abits >= 0x7C00u ? (uint16_t)0x7E00u : f2h(bits_f(b));
-}
-// code + 8 in the low byte of the result; inv: 1 / s, 0 where every code is 0
-__device__ __forceinline__ uint32_t kv4_code(uint16_t x, float inv) {
-    const float v = (h2f(x) * inv + 768.0f) - 768.0f;    // a multiple of 2^-14 (|v| < 16)
-    const float w = __builtin_amdgcn_fmed3f(v, -7.0f, 7.0f);
-    return __builtin_bit_cast(uint32_t, w + 12582920.0f);  // 3 2^22 + 8: the integer in the low bits
-}
-__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __builtin_amdgcn_perm(b, a, 0x0C0C0400u) | __builtin_amdgcn_perm(d, c, 0x04000C0Cu);
-}
-template <int CTRL>
-__device__ __forceinline__ uint32_t quad(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
-}
-// byte j of lane i's result: byte i of lane j's v, within each quad of lanes
-__device__ __forceinline__ uint32_t quad_transpose(uint32_t v, int i) {
-    // bytes (0, 1) and (2, 3) change places between lanes 1 apart, then pairs between lanes 2 apart
-    uint32_t o = quad<0xB1>(v);
-    v = i & 1 ? __builtin_amdgcn_perm(v, o, 0x07030501u) : __builtin_amdgcn_perm(o, v, 0x06020400u);
-    o = quad<0x4E>(v);
-    return i & 2 ? __builtin_amdgcn_perm(v, o, 0x07060302u) : __builtin_amdgcn_perm(o, v, 0x05040100u);
-}
-// N dwords at p, 4 N bytes aligned up to 16
-template <int N>
-__device__ __forceinline__ void load_dwords(uint32_t (&w)[N], const uint8_t* p) {
-    if constexpr (N == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[0] = u.x, w[1] = u.y;
-    } else {
-#pragma unroll
-        for (int k = 0; k < N / 4; k++) {
-            const uint4 u = reinterpret_cast<const uint4*>(p)[k];
-            w[4 * k] = u.x, w[4 * k + 1] = u.y, w[4 * k + 2] = u.z, w[4 * k + 3] = u.w;
-        }
-    }
-}
-template <int N>
-__device__ __forceinline__ void store_dwords(uint8_t* p, const uint32_t (&w)[N]) {
-    if constexpr (N == 2) {
-        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < N / 4; k++)
-            reinterpret_cast<uint4*>(p)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-    }
-}
 
 // grid (tile, KV head, request), two waves: keys and values
 template <int D>

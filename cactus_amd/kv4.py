@@ -112,6 +112,22 @@ class KV4Cache:
         self._call("cactus_hip_kv4_append_f16", layer, self._lst(seqs, batch, stream), self._lst(counts, batch, stream), k, v,
                    batch, seq_len, stride, stream=stream)
 
+    def append_rope(self, layer: int, q: int, q_out: int, num_q_heads: int, k: int, v: int, batch: int, seq_len: int,
+                    table: int, table_positions: int, q_stride: int | None = None, kv_stride: int | None = None,
+                    q_norm: int | None = None, k_norm: int | None = None, eps: float = 1e-6, seqs=None, counts=None,
+                    stream=None):
+        d = self.desc.head_dim
+        self._call("cactus_hip_kv4_append_rope_f16", layer, self._lst(seqs, batch, stream), self._lst(counts, batch, stream), q,
+                   q_stride or num_q_heads * d, q_out, num_q_heads, k, v, kv_stride or self.desc.kv_heads * d, q_norm, k_norm,
+                   eps, table, table_positions, batch, seq_len, stream=stream)
+
+    def rope_table(self, theta: float, stream=None) -> DeviceBuffer:
+        """The rotations of every position that a slot can have, max_pages * page_size of them, for append_rope."""
+        n, d = self.desc.max_pages * self.desc.page_size, self.desc.head_dim
+        table = DeviceBuffer(4 * n * d)
+        call("cactus_hip_rope_table_f32", table.ptr, n, d, theta, stream)
+        return table
+
     def read(self, layer: int, k: int, v: int, batch: int, seq_len: int, seqs=None, starts=None, counts=None, stream=None):
         self._call("cactus_hip_kv4_read_f16", layer, self._lst(seqs, batch, stream), self._lst(starts, batch, stream),
                    self._lst(counts, batch, stream), k, v, batch, seq_len, stream=stream)

@@ -166,6 +166,22 @@ int cactus_hip_matmul_int4_f16act_batched(const uint16_t* A, const uint8_t* B_pa
                                           size_t K, size_t N, size_t group_size, size_t batch,
                                           size_t stride_a, size_t stride_b, size_t stride_bs,
                                           size_t stride_c, void* stream);
+/* No counterpart in the reference.  Low-rank adapters of many requests beside a
+ * projection that they share: row j of request i, with adapter a = adapters[i],
+ *   y = fp16(base + scales[a] * B_a (A_a x))     (sums in FP32)
+ * x [batch][seq_len] rows of K, base (the projection's output) and y rows of N, each
+ * with its stride from row to row; A [num_adapters][rank][K], B [num_adapters][N][rank]
+ * fp16 (rows = outputs, like every weight here); scales [num_adapters] f32 (NULL: 1);
+ * adapters [batch] on the device, any number outside [0, num_adapters): none, y =
+ * base.  counts (device, NULL: seq_len each): the first counts[i] rows of request i are
+ * there, the others are not read and left as they were.  y may be base (with its stride);
+ * otherwise y overlaps no input.  rank: a multiple of 8 up to 256 (adapters of lower
+ * rank are padded with zeros); K and N multiples of 8; rows 16-byte aligned.  A NaN or
+ * an infinity in a row of x or base stays in that row of y. */
+int cactus_hip_lora_add_f16(const uint16_t* x, size_t x_stride, const uint16_t* A, const uint16_t* B,
+                            const float* scales, size_t num_adapters, size_t rank, const int32_t* adapters,
+                            const int32_t* counts, const uint16_t* base, size_t base_stride, uint16_t* y,
+                            size_t y_stride, size_t batch, size_t seq_len, size_t K, size_t N, void* stream);
 /* cactus_unpack_int4_to_int8 (kernel/kernel.h:162, kernel_quants.cpp:295-351) */
 int cactus_hip_unpack_int4_to_int8(const uint8_t* packed, int8_t* unpacked, size_t count,
                                    void* stream);
@@ -351,6 +367,51 @@ int cactus_hip_sample_f16(const uint16_t* logits, uint32_t* out, size_t vocab,
 int cactus_hip_sample_f32(const float* logits, uint32_t* out, size_t vocab, float temperature, float top_p,
                           size_t top_k, size_t random_seed, const float* bias_values,
                           const uint32_t* bias_indices, size_t bias_count, void* stream);
+/* No reference counterpart (the reference's samplers take one row, with a history that
+ * the process shares).  What each sequence's settings make of its logits:
+ * row i [vocab] (stride values from row to row), with s = seqs[i] (device, NULL: i)
+ * the slot whose settings apply, into out (FP32, out_stride):
+ *   n = how often the token is among history[s]'s first history_lens[s]
+ *   n > 0:  x = x > 0 ? x / repetition[s] : x * repetition[s];
+ *           x = x - frequency[s] * n;  x = x - presence[s]
+ *   x = x + bias, for every entry of the slot's list that names the token, in order
+ *   x = -infinity where the bit of the slot's mask is 0
+ * each operation in FP32, rounded by itself.  best[i] (NULL: not wanted): the first index of
+ * the largest value; NaN is never it; 0 where no value is above -infinity.  The
+ * rows of out are what cactus_hip_sample_f32 takes.  A slot outside [0, max_seqs)
+ * makes no access: its row of out and best are left as they were.  FP32 rows may be
+ * changed in place (out is logits, one stride).
+ * The settings are arrays on the device, so that a captured call follows them; each
+ * may be NULL, and is off then (history_lens, bias_counts: all of the stride;
+ * mask_ids: mask s for slot s).  Tokens outside the vocabulary are passed over.  masks
+ * [num_masks][mask_stride]: bit t % 32 of word t / 32, 1 = allowed; mask_ids[s] < 0:
+ * none, num_masks or more: no token is allowed.
+ * workspace: with best, device memory of cactus_hip_logits_rules_workspace(batch) bytes,
+ * 16-byte aligned, zero before the first call (every call leaves it zero); calls that may
+ * overlap need workspaces of their own, captured graphs among them. */
+#define CACTUS_HIP_LOGITS_MAX_BIAS 1024
+typedef struct {
+    const int32_t*  history;         /* [max_seqs][history_stride] tokens */
+    const int32_t*  history_lens;    /* [max_seqs] */
+    const float*    repetition;      /* [max_seqs] */
+    const float*    frequency;       /* [max_seqs] */
+    const float*    presence;        /* [max_seqs] */
+    const int32_t*  bias_tokens;     /* [max_seqs][bias_stride] */
+    const float*    bias_values;     /* [max_seqs][bias_stride] */
+    const int32_t*  bias_counts;     /* [max_seqs] */
+    const uint32_t* masks;           /* [num_masks][mask_stride] */
+    const int32_t*  mask_ids;        /* [max_seqs] */
+    size_t history_stride, bias_stride;      /* bias_stride at most CACTUS_HIP_LOGITS_MAX_BIAS */
+    size_t num_masks, mask_stride;           /* mask_stride in words */
+    size_t max_seqs;
+} cactus_hip_logits_rules;
+size_t cactus_hip_logits_rules_workspace(size_t batch);
+int cactus_hip_logits_rules_f16(const cactus_hip_logits_rules* rules, const int32_t* seqs, const uint16_t* logits,
+                                size_t stride, float* out, size_t out_stride, uint32_t* best, size_t batch,
+                                size_t vocab, void* workspace, size_t workspace_bytes, void* stream);
+int cactus_hip_logits_rules_f32(const cactus_hip_logits_rules* rules, const int32_t* seqs, const float* logits,
+                                size_t stride, float* out, size_t out_stride, uint32_t* best, size_t batch,
+                                size_t vocab, void* workspace, size_t workspace_bytes, void* stream);
 /* Model::decode's out_entropy (engine/engine_model.cpp:255-290): the
  * softmax entropy of fp16 logits [vocab] in double, divided by log(vocab),
  * written as one float to *out (device memory).  Floating point: within a
@@ -509,6 +570,33 @@ int cactus_hip_kv4_extend(const cactus_hip_kv4_cache* cache, const int32_t* seqs
 int cactus_hip_kv4_append_f16(const cactus_hip_kv4_cache* cache, size_t layer, const int32_t* seqs,
                               const int32_t* counts, const uint16_t* k, const uint16_t* v, size_t batch,
                               size_t seq_len, size_t kv_stride, void* stream);
+/* The rotations' table of cactus_hip_kv4_append_rope_f16: table [positions][2]
+ * [head_dim / 2], the cosines and the sines of p * theta^(-2 i / head_dim), computed in
+ * 64 bits and rounded to FP32.  A caller with scaled or other frequencies fills a
+ * table of its own. */
+int cactus_hip_rope_table_f32(float* table, size_t positions, size_t head_dim, float theta, void* stream);
+/* cactus_hip_kv4_append_f16 with the head norms and the position rotation of new
+ * queries and keys on the way, each row at its own position p in its sequence (lens
+ * - counts[i] + row, read on the device: a captured step may be replayed while the
+ * sequences grow).  Of a head's row x, with halves a and b of
+ *   y = x / sqrt(mean(x^2) + eps) * norm     (norm NULL: y = x)
+ *   (a cos - b sin, b cos + a sin),  cos and sin row p of `table`
+ * all in 64 bits, rounded once to FP16: for queries into q_out [batch][seq_len]
+ * [num_q_heads][head_dim], for keys the row that is quantized into the pages;
+ * values are quantized as they come.  q: num_q_heads heads per row, q_stride values from
+ * row to row; q_out may be q where the rows are dense (q_stride num_q_heads * head_dim);
+ * num_q_heads 0: keys and values only (q, q_out may be NULL).  q_norm, k_norm
+ * [head_dim] fp16, either may be NULL.  Strides are multiples of 8, every pointer but
+ * seqs and counts 16-byte aligned.  q, k and v may lie side by side in one buffer.
+ * `table` has at least max_pages * page_size positions (table_positions says how many).
+ * seqs, counts, slots that may not be named twice, pages that may not be shared and status
+ * bits as for cactus_hip_kv4_append_f16; where that writes nothing, rows of q_out are left
+ * as they were too (a row on a page that does not exist has its query all the same). */
+int cactus_hip_kv4_append_rope_f16(const cactus_hip_kv4_cache* cache, size_t layer, const int32_t* seqs,
+                                   const int32_t* counts, const uint16_t* q, size_t q_stride, uint16_t* q_out,
+                                   size_t num_q_heads, const uint16_t* k, const uint16_t* v, size_t kv_stride,
+                                   const uint16_t* q_norm, const uint16_t* k_norm, float eps, const float* table,
+                                   size_t table_positions, size_t batch, size_t seq_len, void* stream);
 /* The values of layer `layer`'s tokens: request i's tokens [starts[i],
  * starts[i] + counts[i]), or with starts NULL its last counts[i], into
  * k, v [batch][seq_len][kv_heads][head_dim] fp16 (16-byte aligned; either may

@@ -1,0 +1,169 @@
+"""Rotated appends, adapters per request and rules on logits without a GPU:
+refusals before any launch, sizes, the Python owners' checks, and the restatements."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import _serving as S
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import cactus_amd
+    return cactus_amd.hip()
+
+
+def refused(lib, rc, text):
+    assert rc == -1
+    assert text in lib.cactus_hip_last_error(), lib.cactus_hip_last_error()
+
+
+# ------------------------------------------------------------------ rotated append
+def cache(**kw):
+    from cactus_amd.kv4 import CacheDesc
+    shape = dict(layers=2, kv_heads=2, head_dim=128, page_size=64, num_pages=8, max_seqs=4, max_pages=4)
+    ptrs = dict(pages=1 << 20, table=1 << 21, lens=1 << 22, refs=1 << 23, state=1 << 24)   # never dereferenced
+    return CacheDesc(**{**shape, **ptrs, **kw})
+
+
+def append(lib, desc=None, layer=0, **kw):
+    a = dict(seqs=None, counts=None, q=4096, q_stride=512, q_out=8192, heads=4, k=4096, v=4096, kv_stride=256, q_norm=None,
+             k_norm=None, eps=1e-6, table=4096, positions=256, batch=2, seq_len=3)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.cactus_hip_kv4_append_rope_f16((desc or cache()).ref, layer, *a.values(), None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(k=None), b"null pointer"), (dict(v=None), b"null pointer"), (dict(q=None), b"null pointer"),
+    (dict(q_out=None), b"null pointer"), (dict(table=None), b"null pointer"), (dict(q=4104), b"aligned"),
+    (dict(q_out=4100), b"aligned"), (dict(k=4098), b"aligned"), (dict(v=4104), b"aligned"), (dict(kv_stride=260), b"aligned"),
+    (dict(q_stride=516), b"aligned"), (dict(q_norm=8), b"aligned"), (dict(k_norm=4100), b"aligned"), (dict(table=4104), b"aligned"),
+    (dict(kv_stride=248), b"kv_stride"), (dict(q_stride=504), b"q_stride"), (dict(eps=-1.0), b"eps"),
+    (dict(eps=float("nan")), b"eps"), (dict(eps=float("inf")), b"eps"), (dict(positions=255), b"table_positions"),
+    (dict(batch=5), b"slots"), (dict(seq_len=1 << 28), b"seq_len"), (dict(heads=1 << 17), b"num_q_heads"),
+    (dict(q=4096, q_out=4096, q_stride=520), b"in place")])
+def test_append_refusals(lib, kw, text):
+    refused(lib, append(lib, **kw), text)
+
+
+def test_append_checks_the_cache_and_the_layer(lib):
+    refused(lib, append(lib, cache(head_dim=96)), b"head_dim")
+    refused(lib, append(lib, cache(lens=None)), b"null buffer")
+    refused(lib, append(lib, layer=2), b"layer")
+    assert append(lib, batch=0) == 0 and append(lib, seq_len=0) == 0
+
+
+def test_rope_table_refusals(lib):
+    for kw, text in (((4096, 10, 63, 1e4), b"head_dim"), ((4096, 10, 0, 1e4), b"head_dim"), ((4096, 10, 64, 0.0), b"theta"),
+                     ((4096, 10, 64, float("nan")), b"theta"), ((4096, 1 << 31, 64, 1e4), b"positions"),
+                     ((None, 10, 64, 1e4), b"null")):
+        refused(lib, lib.cactus_hip_rope_table_f32(*kw, None), text)
+    assert lib.cactus_hip_rope_table_f32(None, 0, 64, 1e4, None) == 0
+
+
+def test_rotation_restated():
+    """A rotation keeps lengths, position 0 changes nothing, and scores depend on distances alone."""
+    rng = np.random.default_rng(1)
+    t = S.rope_table(50, 64, 1e4)
+    q, k = rng.standard_normal((2, 64))
+    y, _ = S.rotated(q, None, 0, t[0])
+    assert np.array_equal(y, q)
+    at = lambda x, p: S.rotated(x, None, 0, t[p])[0]  # noqa: E731
+    assert np.allclose(at(q, 17) @ at(k, 5), at(q, 40) @ at(k, 28), atol=64 * 2.0 ** -22 * np.abs(q).max() * np.abs(k).max())
+
+
+# ------------------------------------------------------------------ adapters
+def lora(lib, **kw):
+    a = dict(x=4096, x_stride=64, A=4096, B=4096, scales=None, n=3, rank=16, ids=4096, counts=None, base=4096, base_stride=128,
+             y=8192, y_stride=128, batch=2, seq_len=3, K=64, N=128)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.cactus_hip_lora_add_f16(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(rank=0), b"rank"), (dict(rank=12), b"rank"), (dict(rank=264), b"rank"), (dict(K=60, x_stride=60), b"multiples of 8"),
+    (dict(N=100), b"multiples of 8"), (dict(K=1 << 24, x_stride=1 << 24), b"2^24"), (dict(x=None), b"null pointer"),
+    (dict(A=None), b"null pointer"), (dict(B=None), b"null pointer"), (dict(ids=None), b"null pointer"),
+    (dict(base=None), b"null pointer"), (dict(y=None), b"null pointer"), (dict(x=4098), b"aligned"), (dict(A=4104), b"aligned"),
+    (dict(B=4104), b"aligned"), (dict(base=4104), b"aligned"), (dict(y=4104), b"aligned"), (dict(x_stride=68), b"aligned"),
+    (dict(x_stride=56), b"stride"), (dict(base_stride=120), b"stride"), (dict(y_stride=120), b"stride"),
+    (dict(y=4096, y_stride=136), b"in place"), (dict(batch=65536), b"batch"), (dict(seq_len=1 << 24), b"seq_len"),
+    (dict(n=1 << 24), b"num_adapters")])
+def test_lora_refusals(lib, kw, text):
+    refused(lib, lora(lib, **kw), text)
+
+
+def test_lora_without_rows_does_nothing(lib):
+    assert lora(lib, batch=0) == 0 and lora(lib, seq_len=0) == 0 and lora(lib, N=0) == 0
+
+
+# ------------------------------------------------------------------ rules on logits
+def call_rules(lib, half=True, change=(), **kw):
+    from cactus_amd.logits import RulesDesc
+    r = dict(history=4096, history_lens=4096, repetition=4096, frequency=4096, presence=4096, bias_tokens=4096, bias_values=4096,
+             bias_counts=4096, masks=4096, mask_ids=4096, history_stride=10, bias_stride=5, num_masks=2, mask_stride=4, max_seqs=6)
+    r.update(change)
+    a = dict(seqs=None, logits=4096, stride=100, out=8192, out_stride=100, best=4096, batch=3, vocab=100, work=4096, size=48)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return (lib.cactus_hip_logits_rules_f16 if half else lib.cactus_hip_logits_rules_f32)(RulesDesc(**r).ref, *a.values(), None)
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("change,kw,text", [
+    (dict(max_seqs=0), {}, b"max_seqs"), (dict(history_stride=1 << 31), {}, b"history_stride"),
+    (dict(bias_stride=1025), {}, b"bias_stride"), (dict(bias_values=None), {}, b"without values"),
+    (dict(mask_stride=3), {}, b"mask_stride"), (dict(mask_ids=None, num_masks=5), {}, b"mask"), ({}, dict(batch=65536, size=1 << 21), b"65535"),
+    ({}, dict(vocab=1 << 28, stride=1 << 28, out_stride=1 << 28), b"mask_stride"), ({}, dict(logits=None), b"null pointer"),
+    ({}, dict(out=None), b"null pointer"), ({}, dict(stride=99), b"stride"), ({}, dict(out_stride=99), b"stride"),
+    ({}, dict(out=8194), b"misaligned"), ({}, dict(logits=4097), b"misaligned"), ({}, dict(work=None), b"workspace"),
+    ({}, dict(work=4104), b"workspace"), ({}, dict(size=47), b"workspace"), ({}, dict(out=4096, stride=104), b"in place")])
+def test_rules_refusals(lib, half, change, kw, text):
+    refused(lib, call_rules(lib, half, change, **kw), text)
+
+
+def test_rules_more_refusals(lib):
+    refused(lib, call_rules(lib, True, dict(masks=None), vocab=1 << 28, stride=1 << 28, out_stride=1 << 28), b"vocab")
+    refused(lib, call_rules(lib, True, out=4096), b"in place")        # FP16 rows cannot become FP32 where they are
+    refused(lib, lib.cactus_hip_logits_rules_f16(None, None, 4096, 1, 4096, 1, None, 1, 1, None, 0, None), b"null rules")
+    assert call_rules(lib, batch=0) == 0 and call_rules(lib, vocab=0) == 0
+    assert lib.cactus_hip_logits_rules_workspace(3) == 48
+
+
+def test_rules_owner_checks(monkeypatch):
+    from cactus_amd import logits as L
+    sent = []
+
+    class Buffer:
+        def __init__(self, n):
+            self.nbytes, self.ptr = n, 1 << 20
+
+        @classmethod
+        def from_numpy(cls, a, stream=None):
+            return cls(a.nbytes)
+    monkeypatch.setattr(L, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(L, "call", lambda name, *a: sent.append((name, *a)))
+    r = L.LogitsRules(4, 50, max_history=8, max_bias=2, num_masks=1)
+    r.set_history(3, [1, 2, 3])
+    assert sent[0][1] == (1 << 20) + 4 * 3 * 8 and sent[0][3] == 12
+    for bad in (lambda: r.set_history(4, [1]), lambda: r.set_mask(1, [True] * 50), lambda: r.use_mask(-1, 0)):
+        with pytest.raises(IndexError):
+            bad()
+    for bad in (lambda: r.set_history(0, range(9)), lambda: r.set_bias(0, [1, 2, 3], [0, 0, 0]), lambda: r.set_bias(0, [1], []),
+                lambda: r.set_mask(0, [True] * 49), lambda: L.LogitsRules(1, 50, max_bias=1025),
+                lambda: L.LogitsRules(1, 50).set_history(0, [1])):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_rules_restated():
+    x = np.array([2.0, -2.0, 1.0, 0.0, 3.0], np.float32)
+    y, best = S.rules(x, hist=[0, 1, 1, -1, 7], rep=2.0, freq=0.5, pres=0.25, bias=[(3, 4.0), (3, -1.0), (9, 1.0)])
+    assert y.tolist() == [0.25, -5.25, 1.0, 3.0, 3.0] and best == 3
+    y, best = S.rules(x, mask=np.array([1, 1, 0, 0, 0], bool))
+    assert y.tolist() == [2.0, -2.0, -np.inf, -np.inf, -np.inf] and best == 0
+    assert S.rules(x, mask=np.zeros(5, bool))[1] == 0
+    assert S.rules([np.nan, -0.0, 0.0])[1] == 1
