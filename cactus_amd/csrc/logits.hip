@@ -22,34 +22,70 @@ __device__ __forceinline__ uint64_t best_key(float x, uint32_t i) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
     return (uint64_t)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (0xFFFFFFFFu - i);
 }
+__device__ __forceinline__ void load_words(uint32_t (&n)[8], const uint32_t* p) {
+    const uint4 u = reinterpret_cast<const uint4*>(p)[0], v = reinterpret_cast<const uint4*>(p)[1];
+    n[0] = u.x, n[1] = u.y, n[2] = u.z, n[3] = u.w, n[4] = v.x, n[5] = v.y, n[6] = v.z, n[7] = v.w;
+}
 __device__ __forceinline__ float penalized(float x, int n, float rep, float freq, float pres) {
     x = x > 0.0f ? x / rep : x * rep;
     const float f = freq * (float)n;
     return (x - f) - pres;
 }
 
-// A workgroup takes RULES_CHUNK tokens of a row.  It counts the history's tokens that
-// fall among them in LDS, then the biases' owners: the first entry that names a token
-// takes the whole chain of its entries, in order.
-constexpr int RULES_CHUNK = 4096, RULES_THREADS = 256, RULES_MAX_BIAS = CACTUS_HIP_LOGITS_MAX_BIAS;
-template <typename T>
-__global__ void __launch_bounds__(RULES_THREADS) logits_rules_kernel(RulesArgs a) {
-    // per token: occurrences; 2^31 + entry where a bias list's entry holds the value
-    __shared__ uint32_t counts[RULES_CHUNK];
-    __shared__ int b_tok[RULES_MAX_BIAS];
-    __shared__ float b_val[RULES_MAX_BIAS], b_out[RULES_MAX_BIAS];
-    __shared__ uint64_t w_key[RULES_THREADS / 64];
-    const int tid = threadIdx.x, row = blockIdx.y, c0 = (int)blockIdx.x * RULES_CHUNK, c1 = min(c0 + RULES_CHUNK, a.V);
+// A workgroup takes 16 THREADS tokens of a row, in groups of 8 per thread that start
+// where 16-byte loads of the row may (tokens before and behind the row are passed over).
+// The logits are on their way while it counts, in LDS, how often the history names each of
+// its tokens: every workgroup of a row reads the whole history, which the L2 holds, and
+// keeps what falls among its own.  Bias entries then count themselves into the same words:
+// a token that one entry names (most are) is that entry's thread's; of several the first
+// takes them all, in order.
+constexpr int RULES_MAX_BIAS = CACTUS_HIP_LOGITS_MAX_BIAS;
+constexpr uint32_t COUNT_BITS = 20;      // of the history; above it the entries, bit 31: value in b_out
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) logits_rules_kernel(RulesArgs a) {
+    constexpr int GROUPS = 2, CHUNK = 8 * GROUPS * THREADS, EPT = RULES_MAX_BIAS / THREADS;
+    __shared__ __attribute__((aligned(16))) uint32_t counts[CHUNK];
+    __shared__ float b_out[RULES_MAX_BIAS];
+    __shared__ uint64_t w_key[THREADS / 64];
+    const int tid = threadIdx.x, row = blockIdx.y;
     const int slot = a.seqs ? a.seqs[row] : row;
     if ((unsigned)slot >= (unsigned)a.r.max_seqs) return;
     const T* in = static_cast<const T*>(a.in) + (size_t)row * a.in_stride;
     float* out = a.out + (size_t)row * a.out_stride;
-    const auto load = [&](int t) -> float {
-        if constexpr (sizeof(T) == 2) return h2f(in[t]);
-        else return in[t];
-    };
-    const int hist = a.r.history ? (a.r.history_lens ? min(max(a.r.history_lens[slot], 0), (int)a.r.history_stride) : (int)a.r.history_stride) : 0;
-    const int nb = a.r.bias_tokens ? (a.r.bias_counts ? min(max(a.r.bias_counts[slot], 0), (int)a.r.bias_stride) : (int)a.r.bias_stride) : 0;
+    // tokens before the first one that starts 16 bytes of the row, and whether it does so in out too
+    const int shift = (int)(-(uintptr_t)in & 15) / (int)sizeof(T);
+    const bool vec = ((uintptr_t)(out + shift) & 15) == 0;
+    const int c0 = (shift ? shift - 8 : 0) + (int)blockIdx.x * CHUNK;      // (down to -7)
+    const int lo = max(c0, 0), hi = min(c0 + CHUNK, a.V);
+
+    float x[GROUPS][8];
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) {
+        const int t = c0 + 8 * (tid + THREADS * g);
+        if (vec && t >= 0 && t + 8 <= a.V) {
+            if constexpr (sizeof(T) == 2) {
+                const uint4 u = *reinterpret_cast<const uint4*>(in + t);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[g][j] = h2f((uint16_t)(w[j / 2] >> 16 * (j & 1)));
+            } else {
+                const f32x4 u = *reinterpret_cast<const f32x4*>(in + t), v = *reinterpret_cast<const f32x4*>(in + t + 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[g][j] = u[j], x[g][4 + j] = v[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[g][j] = 0.0f;
+                if (t + j >= 0 && t + j < a.V) {
+                    if constexpr (sizeof(T) == 2) x[g][j] = h2f(in[t + j]);
+                    else x[g][j] = in[t + j];
+                }
+            }
+        }
+    }
+    const int hist = !a.r.history ? 0 : a.r.history_lens ? min(max(a.r.history_lens[slot], 0), (int)a.r.history_stride) : (int)a.r.history_stride;
+    const int nb = !a.r.bias_tokens ? 0 : a.r.bias_counts ? min(max(a.r.bias_counts[slot], 0), (int)a.r.bias_stride) : (int)a.r.bias_stride;
     const float rep = a.r.repetition ? a.r.repetition[slot] : 1.0f, freq = a.r.frequency ? a.r.frequency[slot] : 0.0f,
                 pres = a.r.presence ? a.r.presence[slot] : 0.0f;
     const uint32_t* mask = nullptr;
@@ -61,47 +97,108 @@ __global__ void __launch_bounds__(RULES_THREADS) logits_rules_kernel(RulesArgs a
             mask = none ? nullptr : a.r.masks + (size_t)id * a.r.mask_stride;
         }
     }
-    for (int i = tid; i < RULES_CHUNK; i += RULES_THREADS) counts[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < hist; i += RULES_THREADS) {
-        const int t = a.r.history[(size_t)slot * a.r.history_stride + i];
-        if (t >= c0 && t < c1) atomicAdd(&counts[t - c0], 1u);
-    }
-    for (int i = tid; i < nb; i += RULES_THREADS) {
-        b_tok[i] = a.r.bias_tokens[(size_t)slot * a.r.bias_stride + i];
-        b_val[i] = a.r.bias_values[(size_t)slot * a.r.bias_stride + i];
-    }
-    __syncthreads();
-    for (int i = tid; i < nb; i += RULES_THREADS) {
-        const int t = b_tok[i];
-        if (t < c0 || t >= c1) continue;
-        bool first = true;
-        for (int j = 0; j < i; j++) first = first && b_tok[j] != t;
-        if (!first) continue;
-        float x = load(t);
-        const uint32_t n = counts[t - c0];
-        if (n) x = penalized(x, (int)n, rep, freq, pres);
-        for (int j = i; j < nb; j++)
-            if (b_tok[j] == t) x = x + b_val[j];
-        b_out[i] = x;
-        counts[t - c0] = 0x80000000u + i;
-    }
-    __syncthreads();
-    uint64_t key = 0;
-    for (int t = c0 + tid; t < c1; t += RULES_THREADS) {
-        const uint32_t n = counts[t - c0];
-        float x;
-        if (n >> 31) x = b_out[n & 0x7FFFFFFFu];
-        else {
-            x = load(t);
-            if (n) x = penalized(x, (int)n, rep, freq, pres);
+    const bool listed = hist > 0 || nb > 0;
+    if (listed) {
+#pragma unroll
+        for (int i = 0; i < CHUNK / 4 / THREADS; i++) reinterpret_cast<uint4*>(counts)[tid + THREADS * i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        const int32_t* h = a.r.history + (size_t)slot * a.r.history_stride;
+        for (int i0 = 0; i0 < hist; i0 += 8 * THREADS) {
+            int t[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int i = i0 + tid + THREADS * u;
+                t[u] = i < hist ? h[i] : -1;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if (t[u] >= lo && t[u] < hi) atomicAdd(&counts[t[u] - c0], 1u);
         }
-        if (none || (mask && !(mask[t >> 5] >> (t & 31) & 1u))) x = -__builtin_inff();
-        out[t] = x;
-        const uint64_t k = best_key(x, (uint32_t)t);
-        key = k > key ? k : key;
+        __syncthreads();
+    }
+    if (nb > 0) {
+        const int32_t* tokens = a.r.bias_tokens + (size_t)slot * a.r.bias_stride;
+        const float* values = a.r.bias_values + (size_t)slot * a.r.bias_stride;
+        int tok[EPT];
+        bool own[EPT];
+#pragma unroll
+        for (int e = 0; e < EPT; e++) {
+            const int i = tid + THREADS * e;
+            tok[e] = i < nb ? tokens[i] : -1;
+            own[e] = tok[e] >= lo && tok[e] < hi;
+            if (own[e]) atomicAdd(&counts[tok[e] - c0], 1u << COUNT_BITS);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < EPT; e++) {
+            if (!own[e]) continue;
+            const int i = tid + THREADS * e, t = tok[e];
+            const uint32_t w = counts[t - c0], n = w & ((1u << COUNT_BITS) - 1);
+            const bool single = w >> COUNT_BITS == 1;
+            if (!single)
+                for (int j = 0; j < i && own[e]; j++) own[e] = tokens[j] != t;
+            if (!own[e]) continue;
+            float v;
+            if constexpr (sizeof(T) == 2) v = h2f(in[t]);
+            else v = in[t];
+            if (n) v = penalized(v, (int)n, rep, freq, pres);
+            v = v + values[i];
+            if (!single)
+                for (int j = i + 1; j < nb; j++)
+                    if (tokens[j] == t) v = v + values[j];
+            b_out[i] = v;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < EPT; e++)
+            if (own[e]) counts[tok[e] - c0] = 0x80000000u + tid + THREADS * e;
+        __syncthreads();
+    }
+    float most = -__builtin_inff();
+    int at = 0;
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) {
+        const int l = 8 * (tid + THREADS * g), t = c0 + l;
+        if (t >= a.V || t + 8 <= 0) continue;
+        if (listed) {
+            uint32_t n[8];
+            load_words(n, counts + l);
+            if (n[0] | n[1] | n[2] | n[3] | n[4] | n[5] | n[6] | n[7]) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (n[j] >> 31) x[g][j] = b_out[n[j] & 0x7FFFFFFFu];
+                    else if (n[j]) x[g][j] = penalized(x[g][j], (int)n[j], rep, freq, pres);
+                }
+            }
+        }
+        if (none) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[g][j] = -__builtin_inff();
+        } else if (mask) {
+            const int t0 = max(t, 0), t1 = min(t + 7, a.V - 1);
+            const uint64_t w = (uint64_t)mask[t0 >> 5] | (uint64_t)mask[t1 >> 5] << 32;
+            // bit j: token t + j (words of tokens before the row hold nothing)
+            const uint32_t bits = t < 0 ? (uint32_t)w << -t : t0 >> 5 == t1 >> 5 ? (uint32_t)w >> (t0 & 31) : (uint32_t)(w >> (t0 & 31));
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[g][j] = bits >> j & 1 ? x[g][j] : -__builtin_inff();
+        }
+        if (vec && t >= 0 && t + 8 <= a.V) {
+            *reinterpret_cast<f32x4*>(out + t) = (f32x4){x[g][0], x[g][1], x[g][2], x[g][3]};
+            *reinterpret_cast<f32x4*>(out + t + 4) = (f32x4){x[g][4], x[g][5], x[g][6], x[g][7]};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (x[g][j] > most) most = x[g][j], at = t + j;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (t + j < 0 || t + j >= a.V) continue;
+                out[t + j] = x[g][j];
+                if (x[g][j] > most) most = x[g][j], at = t + j;
+            }
+        }
     }
     if (!a.best) return;
+    uint64_t key = best_key(most, (uint32_t)at);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         const uint64_t k = __shfl_xor((unsigned long long)key, o, 64);
@@ -110,7 +207,8 @@ __global__ void __launch_bounds__(RULES_THREADS) logits_rules_kernel(RulesArgs a
     if ((tid & 63) == 0) w_key[tid >> 6] = key;
     __syncthreads();
     if (tid != 0) return;
-    for (int w = 1; w < RULES_THREADS / 64; w++) key = w_key[w] > key ? w_key[w] : key;
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; w++) key = w_key[w] > key ? w_key[w] : key;
     // The row's largest key in the workspace; whoever comes last takes it and leaves zeros.  The
     // maximum is performed where the counter is, and has been when the counter is raised.
     uint64_t* best = reinterpret_cast<uint64_t*>(a.work + 4 * (size_t)row);
@@ -123,12 +221,21 @@ __global__ void __launch_bounds__(RULES_THREADS) logits_rules_kernel(RulesArgs a
     a.best[row] = key ? 0xFFFFFFFFu - (uint32_t)key : 0u;
 }
 
+template <typename T>
+static void rules_launch(const RulesArgs& a, size_t batch, hipStream_t st) {
+    const size_t tokens = (size_t)a.V + 7;      // (a row's groups may start up to 7 before it)
+    if (batch * ceil_div(tokens, 16384) >= 256)
+        hipLaunchKernelGGL((logits_rules_kernel<T, 1024>), dim3(ceil_div(tokens, 16384), (unsigned)batch), dim3(1024), 0, st, a);
+    else
+        hipLaunchKernelGGL((logits_rules_kernel<T, 256>), dim3(ceil_div(tokens, 4096), (unsigned)batch), dim3(256), 0, st, a);
+}
+
 static int rules(const cactus_hip_logits_rules* r, const int32_t* seqs, const void* logits, size_t stride, float* out,
                  size_t out_stride, uint32_t* best, size_t batch, size_t vocab, void* workspace, size_t workspace_bytes,
                  void* stream, bool half) {
     CH_REQUIRE(r, "logits_rules: null rules");
     CH_REQUIRE(r->max_seqs >= 1 && r->max_seqs < (1u << 30), "logits_rules: max_seqs out of range");
-    CH_REQUIRE(r->history_stride < (1u << 31) && r->bias_stride <= CACTUS_HIP_LOGITS_MAX_BIAS,
+    CH_REQUIRE(r->history_stride < (1u << COUNT_BITS) && r->bias_stride <= CACTUS_HIP_LOGITS_MAX_BIAS,
                "logits_rules: history_stride or bias_stride out of range");
     CH_REQUIRE(!r->bias_tokens || r->bias_values, "logits_rules: biases without values");
     CH_REQUIRE(!r->masks || r->mask_stride >= (vocab + 31) / 32, "logits_rules: mask_stride is shorter than a mask");
@@ -143,9 +250,8 @@ static int rules(const cactus_hip_logits_rules* r, const int32_t* seqs, const vo
     CH_REQUIRE(!best || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= 16 * batch),
                "logits_rules: workspace too small or not 16-byte aligned");
     RulesArgs a{*r, seqs, logits, out, best, static_cast<uint32_t*>(workspace), stride, out_stride, (int)vocab};
-    const dim3 grid(ceil_div(vocab, RULES_CHUNK), (unsigned)batch);
-    if (half) hipLaunchKernelGGL(logits_rules_kernel<uint16_t>, grid, dim3(RULES_THREADS), 0, as_stream(stream), a);
-    else hipLaunchKernelGGL(logits_rules_kernel<float>, grid, dim3(RULES_THREADS), 0, as_stream(stream), a);
+    if (half) rules_launch<uint16_t>(a, batch, as_stream(stream));
+    else rules_launch<float>(a, batch, as_stream(stream));
     return check_launch("logits_rules");
 }
 

@@ -401,7 +401,7 @@ typedef struct {
     const int32_t*  bias_counts;     /* [max_seqs] */
     const uint32_t* masks;           /* [num_masks][mask_stride] */
     const int32_t*  mask_ids;        /* [max_seqs] */
-    size_t history_stride, bias_stride;      /* bias_stride at most CACTUS_HIP_LOGITS_MAX_BIAS */
+    size_t history_stride, bias_stride;      /* below 2^20; at most CACTUS_HIP_LOGITS_MAX_BIAS */
     size_t num_masks, mask_stride;           /* mask_stride in words */
     size_t max_seqs;
 } cactus_hip_logits_rules;
