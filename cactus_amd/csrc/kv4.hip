@@ -22,7 +22,7 @@ template <int D>
 __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4View c, const int32_t* seqs, const int32_t* counts,
                                                          const uint16_t* k, const uint16_t* v, int seq_len, size_t stride) {
     constexpr int NG = D / 32;
-    const int lane = threadIdx.x & 63, key = lane & 15, h = lane >> 4, i = lane & 3;
+    const int lane = threadIdx.x & 63, key = lane & 15, h = lane >> 4;
     const bool vals = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) != 0;
     const int head = blockIdx.y, req = blockIdx.z;
     const int status = c.state[KV4_STATUS];
@@ -43,69 +43,7 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4View c, const int32_
     if (!kv4_page_ok(c, page)) return;
     uint8_t* out = kv4_tile(c, page, head, (pos0 & ((1 << c.ps_log2) - 1)) >> 4) + (vals ? 9 * D : 0);
 
-    // the groups' largest magnitudes, as fp16 bits (a NaN's or an infinity's are above every number's)
-    uint32_t amax[NG];
-#pragma unroll
-    for (int g = 0; g < NG; g++) {
-        const uint32_t m = 0x7FFF7FFFu;
-        u16x2 y = __builtin_bit_cast(u16x2, x[g].x & m);
-        y = __builtin_elementwise_max(y, __builtin_bit_cast(u16x2, x[g].y & m));
-        y = __builtin_elementwise_max(y, __builtin_bit_cast(u16x2, x[g].z & m));
-        y = __builtin_elementwise_max(y, __builtin_bit_cast(u16x2, x[g].w & m));
-        amax[g] = max((uint32_t)y[0], (uint32_t)y[1]);
-    }
-#pragma unroll
-    for (int g = 0; g < NG; g++) amax[g] = max(amax[g], (uint32_t)__shfl_xor((int)amax[g], 16, 64));
-#pragma unroll
-    for (int g = 0; g < NG; g++) amax[g] = max(amax[g], (uint32_t)__shfl_xor((int)amax[g], 32, 64));
-    uint32_t c0[NG], c1[NG];                                 // codes of dims 0-3 and 4-7, a byte each
-#pragma unroll
-    for (int g = 0; g < NG; g++) {
-        const uint16_t sb = kv4_scale(amax[g]);
-        const float s = h2f(sb), inv = s > 0.0f ? 1.0f / s : 0.0f;      // (NaN: codes 0)
-        // (a NaN or infinite value times 0 is NaN: its code is 0 too)
-        const bool zero = !(s > 0.0f);
-        const uint32_t w[4] = {x[g].x, x[g].y, x[g].z, x[g].w};
-        uint32_t u[8];
-#pragma unroll
-        for (int t = 0; t < 8; t++) u[t] = kv4_code((uint16_t)(t & 1 ? w[t / 2] >> 16 : w[t / 2]), inv);
-        c0[g] = zero ? 0x08080808u : low_bytes(u[0], u[1], u[2], u[3]);
-        c1[g] = zero ? 0x08080808u : low_bytes(u[4], u[5], u[6], u[7]);
-        if (mine && h == (g & 3))
-            reinterpret_cast<uint16_t*>(out + 8 * D)[((key >> 2) * NG + g) * 4 + (key & 3)] = sb;
-    }
-    if (!vals) {
-        uint32_t b[NG];
-#pragma unroll
-        for (int p = 0; p < NG / 2; p++) {
-            b[2 * p] = c0[2 * p] | c0[2 * p + 1] << 4;
-            b[2 * p + 1] = c1[2 * p] | c1[2 * p + 1] << 4;
-        }
-        if (mine) store_dwords(out + lane * (D / 8), b);
-        return;
-    }
-    // lanes h and h + 2 hold dims x and x + 16, which share a byte: lane h < 2 takes
-    // x = 8 h to 8 h + 3, lane h + 2 the four dims behind them
-    uint32_t b[NG];
-#pragma unroll
-    for (int g = 0; g < NG; g++) {
-        const uint32_t got = (uint32_t)__shfl_xor((int)(h < 2 ? c1[g] : c0[g]), 32, 64);
-        b[g] = h < 2 ? c0[g] | got << 4 : got | c1[g] << 4;
-    }
-    const int x0 = 8 * (h & 1) + (h < 2 ? 0 : 4);
-    const bool whole = pos0 >= lo && pos0 + 16 <= len;       // (the same for the wave)
-    if (whole) {
-#pragma unroll
-        for (int g = 0; g < NG; g++) b[g] = quad_transpose(b[g], i);
-        store_dwords(out + (key >> 2) * 2 * D + (x0 + i) * (D / 8), b);
-    } else if (mine) {
-        // other tokens of the tile stay: a byte at a time
-#pragma unroll
-        for (int g = 0; g < NG; g++)
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-                out[(key >> 2) * 2 * D + (x0 + t) * (D / 8) + 4 * g + i] = (uint8_t)(b[g] >> (8 * t));
-    }
+    kv4_write_tile<D>(x, out, vals, mine, pos0 >= lo && pos0 + 16 <= len);
 }
 
 // four codes (a byte each, low nibble: code + 8) times s, an exact fp16 value

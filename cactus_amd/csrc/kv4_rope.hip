@@ -122,6 +122,153 @@ __global__ void __launch_bounds__(64 * ROW_WAVES) kv4_rope_row_kernel(RopeArgs a
     }
 }
 
+// A wave takes one 16-token tile of several heads, lane 16 h + token with dims 8 h to 8 h + 7 of
+// each 32-dim group, the order in which the append writes pages: the halves of a rotation are in
+// one lane, and the table's values stay in registers from head to head (read anew for each they
+// were twice the bytes of the rows).
+// grid (tile, TILE_WAVES * heads_per_wave heads, request)
+constexpr int TILE_WAVES = 4;
+constexpr size_t ROPE_TILE_ROWS = 8;
+constexpr int ROPE_PER_WAVE = 4;
+template <int D>
+__global__ void __launch_bounds__(64 * TILE_WAVES) kv4_rope_tile_kernel(RopeArgs a, int per_wave) {
+    constexpr int NG = D / 32, NP = NG / 2;
+    const Kv4View& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), key = lane & 15, h = lane >> 4;
+    const int req = blockIdx.z, items = a.Hq + 2 * c.Hkv;
+    const int status = c.state[KV4_STATUS];
+    const int slot = kv4_slot(c, a.seqs, req);
+    if (slot < 0 || status != 0) return;
+    const int len = kv4_len(c, slot), first = len - kv4_count(a.counts, req, a.S);   // (negative: rows without a token)
+    const int lo = max(first, 0);
+    const int pos0 = (lo & ~15) + 16 * (int)blockIdx.x;
+    if (pos0 >= len) return;
+    const int pos = pos0 + key;
+    const bool mine = pos >= lo && pos < len, whole = pos0 >= lo && pos0 + 16 <= len;
+    const int at = mine ? pos : lo;
+    const size_t row = (size_t)req * a.S + (at - first);
+    float co[NP][8], si[NP][8];
+    {
+        const float* t = a.table + (size_t)at * D + 8 * h;
+#pragma unroll
+        for (int g = 0; g < NP; g++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const f32x4 u = *reinterpret_cast<const f32x4*>(t + 32 * g + 4 * j), v = *reinterpret_cast<const f32x4*>(t + D / 2 + 32 * g + 4 * j);
+#pragma unroll
+                for (int i = 0; i < 4; i++) co[g][4 * j + i] = u[i], si[g][4 * j + i] = v[i];
+            }
+    }
+    const int page = c.table[(size_t)slot * c.max_pages + (pos0 >> c.ps_log2)];
+    const int tile = (pos0 & ((1 << c.ps_log2) - 1)) >> 4;
+    const int item0 = (int)blockIdx.y * TILE_WAVES * per_wave + wave;
+    const auto source = [&](int item) {
+        const bool is_q = item < a.Hq, is_v = item >= a.Hq + c.Hkv;
+        return (is_q ? a.q + row * a.q_stride : (is_v ? a.v : a.k) + row * a.kv_stride) +
+               (size_t)(is_q ? item : is_v ? item - a.Hq - c.Hkv : item - a.Hq) * D + 8 * h;
+    };
+    uint4 next[NG];
+    if (item0 < items) {
+        const uint16_t* src = source(item0);
+#pragma unroll
+        for (int g = 0; g < NG; g++) next[g] = *reinterpret_cast<const uint4*>(src + 32 * g);
+    }
+    for (int n = 0; n < per_wave; n++) {
+        const int item = item0 + TILE_WAVES * n;
+        if (item >= items) return;
+        uint4 x[NG];
+#pragma unroll
+        for (int g = 0; g < NG; g++) x[g] = next[g];
+        if (n + 1 < per_wave && item + TILE_WAVES < items) {
+            const uint16_t* src = source(item + TILE_WAVES);
+#pragma unroll
+            for (int g = 0; g < NG; g++) next[g] = *reinterpret_cast<const uint4*>(src + 32 * g);
+        }
+        const bool is_q = item < a.Hq, is_v = item >= a.Hq + c.Hkv;
+        const auto half_of = [&](int g, int j) { return h2f((uint16_t)((&x[g].x)[j / 2] >> 16 * (j & 1))); };
+        if (is_q) {
+            // in 32 bits: an FP16 result has no border that 2^-22 beside it matters for
+            float f = 1.0f;
+            if (a.q_norm) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) ss = __builtin_fmaf(half_of(g, j), half_of(g, j), ss);
+                ss += __shfl_xor(ss, 16, 64);
+                ss += __shfl_xor(ss, 32, 64);
+                f = 1.0f / sqrtf(ss * (1.0f / D) + (float)a.eps);
+            }
+            uint16_t* dst = a.q_out + (row * a.Hq + item) * D + 8 * h;
+#pragma unroll
+            for (int g = 0; g < NP; g++) {
+                uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;
+                if (a.q_norm) {
+                    wa = *reinterpret_cast<const uint4*>(a.q_norm + 32 * g + 8 * h);
+                    wb = *reinterpret_cast<const uint4*>(a.q_norm + D / 2 + 32 * g + 8 * h);
+                }
+                uint32_t ra[4], rb[4];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    float u = half_of(g, j), v = half_of(g + NP, j);
+                    if (a.q_norm) {
+                        u = u * f * h2f((uint16_t)((&wa.x)[j / 2] >> 16 * (j & 1)));
+                        v = v * f * h2f((uint16_t)((&wb.x)[j / 2] >> 16 * (j & 1)));
+                    }
+                    const uint32_t p = f2h(__builtin_fmaf(u, co[g][j], -(v * si[g][j]))), r = f2h(__builtin_fmaf(v, co[g][j], u * si[g][j]));
+                    if (j & 1) ra[j / 2] |= p << 16, rb[j / 2] |= r << 16;
+                    else ra[j / 2] = p, rb[j / 2] = r;
+                }
+                if (mine) {
+                    *reinterpret_cast<uint4*>(dst + 32 * g) = make_uint4(ra[0], ra[1], ra[2], ra[3]);
+                    *reinterpret_cast<uint4*>(dst + D / 2 + 32 * g) = make_uint4(rb[0], rb[1], rb[2], rb[3]);
+                }
+            }
+            continue;
+        }
+        if (!kv4_page_ok(c, page)) return;        // (heads go up: keys and values are all that is left)
+        if (!is_v) {
+            double f = 1.0;
+            if (a.k_norm) {
+                double ss = 0.0;
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) ss += (double)(half_of(g, j) * half_of(g, j));     // (exact in FP32)
+                ss += __shfl_xor(ss, 16, 64);
+                ss += __shfl_xor(ss, 32, 64);
+                f = 1.0 / sqrt(ss * (1.0 / D) + a.eps);
+            }
+#pragma unroll
+            for (int g = 0; g < NP; g++) {
+                uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;
+                if (a.k_norm) {
+                    wa = *reinterpret_cast<const uint4*>(a.k_norm + 32 * g + 8 * h);
+                    wb = *reinterpret_cast<const uint4*>(a.k_norm + D / 2 + 32 * g + 8 * h);
+                }
+                uint32_t ra[4], rb[4];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    double u = half_of(g, j), v = half_of(g + NP, j);
+                    if (a.k_norm) {
+                        // (x w is exact in FP32)
+                        u = (double)(half_of(g, j) * h2f((uint16_t)((&wa.x)[j / 2] >> 16 * (j & 1)))) * f;
+                        v = (double)(half_of(g + NP, j) * h2f((uint16_t)((&wb.x)[j / 2] >> 16 * (j & 1)))) * f;
+                    }
+                    const double cs = co[g][j], sn = si[g][j];
+                    const uint32_t p = f64_to_h(__builtin_fma(u, cs, -(v * sn))), r = f64_to_h(__builtin_fma(v, cs, u * sn));
+                    if (j & 1) ra[j / 2] |= p << 16, rb[j / 2] |= r << 16;
+                    else ra[j / 2] = p, rb[j / 2] = r;
+                }
+                x[g] = make_uint4(ra[0], ra[1], ra[2], ra[3]);
+                x[g + NP] = make_uint4(rb[0], rb[1], rb[2], rb[3]);
+            }
+        }
+        const int head = is_v ? item - a.Hq - c.Hkv : item - a.Hq;
+        kv4_write_tile<D>(x, kv4_tile(c, page, head, tile) + (is_v ? 9 * D : 0), is_v, mine, whole);
+    }
+}
+
 // angles in 64 bits: p f up to 2^31 has 21 bits behind the point left
 __global__ void __launch_bounds__(256) rope_table_kernel(float* table, size_t positions, int half, double log2_theta) {
     const size_t n = positions * half;
@@ -193,7 +340,18 @@ int cactus_hip_kv4_append_rope_f16(const cactus_hip_kv4_cache* cache, size_t lay
     a.Hq = (int)num_q_heads;
     a.S = (int)seq_len;
     a.eps = eps;
-    const dim3 grid((unsigned)seq_len, ceil_div(num_q_heads + 2 * cache->kv_heads, ROW_WAVES), (unsigned)batch);
+    const size_t items = num_q_heads + 2 * cache->kv_heads;
+    if (seq_len >= ROPE_TILE_ROWS) {
+        const int per_wave = ROPE_PER_WAVE;
+        const dim3 grid(ceil_div(seq_len + 15, 16), ceil_div(items, TILE_WAVES * per_wave), (unsigned)batch);
+        switch (a.c.d) {
+            case 64: hipLaunchKernelGGL(kv4_rope_tile_kernel<64>, grid, dim3(64 * TILE_WAVES), 0, as_stream(stream), a, per_wave); break;
+            case 128: hipLaunchKernelGGL(kv4_rope_tile_kernel<128>, grid, dim3(64 * TILE_WAVES), 0, as_stream(stream), a, per_wave); break;
+            default: hipLaunchKernelGGL(kv4_rope_tile_kernel<256>, grid, dim3(64 * TILE_WAVES), 0, as_stream(stream), a, per_wave);
+        }
+        return check_launch("kv4_append_rope");
+    }
+    const dim3 grid((unsigned)seq_len, ceil_div(items, ROW_WAVES), (unsigned)batch);
     switch (a.c.d) {
         case 64: hipLaunchKernelGGL(kv4_rope_row_kernel<64>, grid, dim3(64 * ROW_WAVES), 0, as_stream(stream), a); break;
         case 128: hipLaunchKernelGGL(kv4_rope_row_kernel<128>, grid, dim3(64 * ROW_WAVES), 0, as_stream(stream), a); break;
