@@ -20,29 +20,52 @@ struct LoraArgs {
 
 // A workgroup takes 16 RT rows of a request and a share of the outputs.
 //   shrink  h^T = A x^T on v_mfma_f32_16x16x32_f16 (A's rows the operand's rows, x's the
-//           columns), the contraction over K dealt to the W waves in steps of 64 so that
-//           each element of A and x is loaded once per workgroup, straight in operand
-//           order (16 lanes' rows, 128 contiguous bytes of each); the partial sums meet in LDS
+//           columns), the contraction over K dealt to the W waves in steps of 32, so that
+//           each element of A and x is loaded once per workgroup; the partial sums meet in LDS
 //   expand  y^T = B h^T, h as two FP16 operands (h 2^e = hi + lo, 22 bits of it: the
-//           product's operands are FP16, and one of 11 bits would show in y); the rows of B
-//           are dealt to the operand's rows so that two tiles leave a lane eight
-//           neighbouring outputs of one row: 16-byte loads of base and stores of y
+//           product's operands are FP16, and one of 11 bits would show in y)
+// A wave loads 64 or 128 bytes of a row with neighbouring lanes, and its LDS turns them into
+// operands (the instruction wants 16 rows side by side: loads in that order take the L1 64
+// accesses each instead of 16, which was half of the time).  A and x go there by DMA, in a
+// ring of ST steps; B through registers; products of B come back the same way, so that base
+// and y move in whole lines too.  All of it is the wave's own: only the sums need barriers.
 // Where several workgroups share a tile's rows each computes h for itself: reading x and A
 // again from the L2 costs less than a second launch or a wait.
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
-constexpr int LORA_MAX_RANK = 256, LORA_WGS = 512;
-__device__ __forceinline__ h16x8 as_h8(uint4 u) { return __builtin_bit_cast(h16x8, u); }
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr int LORA_MAX_RANK = 256;
+__device__ __forceinline__ h16x8 as_h8(u32x4 u) { return __builtin_bit_cast(h16x8, u); }
+
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp_move_keep<0xB1>(v);      // within rows of 16 lanes
+    v += dpp_move_keep<0x4E>(v);
+    v += dpp_move_keep<0x141>(v);
+    v += dpp_move_keep<0x140>(v);
+    const auto of = [&](int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); };
+    return (of(0) + of(16)) + (of(32) + of(48));
+}
 
 // RB blocks of 16 ranks at a time, NP times; RB 1: ranks 8 and 16, hi and lo in one operand
 template <int RT, int RB, int NP, int W>
+struct LoraShape {
+    static constexpr int ROWS = 16 * RT, RP = 16 * RB * NP;
+    static constexpr int PS = 16 * RB + 4, HS = 2 * RP + 8;          // pitches of the sums and of h's halves
+    static constexpr int UN = RP <= 64 ? 64 : 32, DS = UN + 4;       // outputs at a time, pitch of their products
+    static constexpr int ST = RB + RT <= 3 ? 4 : 3;
+    static constexpr int STEP = 1024 * (RB + RT), PART = ROWS * PS * 4, BUF = UN * RP * 2, EXPAND = BUF + 16 * DS * 4;
+    static constexpr int SHRINK = ST * STEP > PART ? ST * STEP : PART, WAVE = SHRINK > EXPAND ? SHRINK : EXPAND;
+    static constexpr int LDS = W * WAVE + ROWS * HS * 2 + ROWS * 4;
+    static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+template <int RT, int RB, int NP, int W>
 __global__ void __launch_bounds__(64 * W) lora_tile_kernel(LoraArgs a) {
-    constexpr int ROWS = 16 * RT, RP = 16 * RB * NP, PS = 16 * RB + 4, HS = 2 * RP + 8, TPR = 64 * W / ROWS;
+    using Z = LoraShape<RT, RB, NP, W>;
+    constexpr int ROWS = Z::ROWS, RP = Z::RP, PS = Z::PS, HS = Z::HS, UN = Z::UN, DS = Z::DS, ST = Z::ST, TPR = 64 * W / ROWS;
     constexpr int VPT = 16 * RB / TPR > 0 ? 16 * RB / TPR : 1;       // ranks of a row that a thread sums, per pass
-    constexpr int LDS_A = W * ROWS * PS * 4, LDS_B = ROWS * HS * 2;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS_A > LDS_B ? LDS_A : LDS_B];
-    __shared__ float back[ROWS];                                     // 2^-e of a row
-    float* part = reinterpret_cast<float*>(lds);
-    uint16_t* hs = reinterpret_cast<uint16_t*>(lds);
+    __shared__ __attribute__((aligned(128))) uint8_t lds[Z::LDS];
+    uint16_t* hs = reinterpret_cast<uint16_t*>(lds + W * Z::WAVE);
+    float* back = reinterpret_cast<float*>(lds + W * Z::WAVE + ROWS * HS * 2);      // 2^-e of a row
 
     // workgroups of one tile on one XCD (workgroup i runs on XCD i % 8)
     const uint32_t xcd = blockIdx.x & 7u, local = blockIdx.x >> 3;
@@ -64,7 +87,7 @@ __global__ void __launch_bounds__(64 * W) lora_tile_kernel(LoraArgs a) {
             const int per = (n_hi - n_lo) / 8;
             for (int i = tid; i < rows * per; i += 64 * W) {
                 const int r = i / per, n = n_lo + i % per * 8;
-                *reinterpret_cast<uint4*>(y + r * a.y_stride + n) = *reinterpret_cast<const uint4*>(base + r * a.base_stride + n);
+                *reinterpret_cast<u32x4*>(y + r * a.y_stride + n) = *reinterpret_cast<const u32x4*>(base + r * a.base_stride + n);
             }
         }
         return;
@@ -73,72 +96,68 @@ __global__ void __launch_bounds__(64 * W) lora_tile_kernel(LoraArgs a) {
     const uint16_t* A = a.A + (size_t)id * a.r * a.K;
     const uint16_t* B = a.B + (size_t)id * a.N * a.r;
     const float scale = a.scales ? a.scales[id] : 1.0f;
+    uint8_t* own = lds + wave * Z::WAVE;
+    const uint32_t own_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)own;
 
     // rows and ranks behind the last one repeat it: their results are dropped
-    const uint16_t* xr[RT];
+    const int steps = (a.K + 31) / 32;
+    const int mine = steps > wave ? (steps - wave + W - 1) / W : 0;  // steps of this wave
+    const uint16_t* src[RB + RT];
 #pragma unroll
-    for (int t = 0; t < RT; t++) xr[t] = x + (size_t)min(16 * t + c16, rows - 1) * a.x_stride;
-    const int steps = (a.K + 63) / 64;
+    for (int i = 0; i < RT; i++) src[RB + i] = x + (size_t)min(16 * i + (lane >> 2), rows - 1) * a.x_stride;
     const int row = tid / TPR, sub = tid % TPR;
     float h[NP][VPT];
     float most = 0.0f;
 #pragma unroll
     for (int p = 0; p < NP; p++) {
-        const uint16_t* ar[RB];
 #pragma unroll
-        for (int b = 0; b < RB; b++) ar[b] = A + (size_t)min(16 * (p * RB + b) + c16, a.r - 1) * a.K;
-        f32x4 acc[RB][RT] = {};
-        struct Step {
-            uint4 A[RB][2], x[RT][2];
+        for (int i = 0; i < RB; i++) src[i] = A + (size_t)min(16 * (p * RB + i) + (lane >> 2), a.r - 1) * a.K;
+        // 16 bytes to slot s of row r: piece s ^ (r / 4), so that 8 rows' reads of a piece meet different banks
+        const auto issue = [&](int j) __attribute__((always_inline)) {
+            const int k = min(32 * (wave + W * j) + 8 * ((lane & 3) ^ (lane >> 4)), a.K - 8);
+            const uint32_t to = own_at + (uint32_t)(j % ST * Z::STEP);
+#pragma unroll
+            for (int i = 0; i < RB + RT; i++) lds_dma<16>(src[i] + k, to + 1024 * i);
         };
-        const auto load = [&](Step& s, int i) {
-            const int k = 64 * i + 16 * quad;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int ku = min(k + 8 * u, a.K - 8);
-#pragma unroll
-                for (int b = 0; b < RB; b++) s.A[b][u] = *reinterpret_cast<const uint4*>(ar[b] + ku);
-#pragma unroll
-                for (int t = 0; t < RT; t++) s.x[t][u] = *reinterpret_cast<const uint4*>(xr[t] + ku);
-            }
-        };
-        const auto mul = [&](Step& s, int i) {
-            if (64 * i + 64 > a.K) {          // (the same for the wave) the last step of a K that is no multiple of 64
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-                    if (64 * i + 16 * quad + 8 * u >= a.K) {
-#pragma unroll
-                        for (int b = 0; b < RB; b++) s.A[b][u] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                        for (int t = 0; t < RT; t++) s.x[t][u] = make_uint4(0, 0, 0, 0);
-                    }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int b = 0; b < RB; b++)
-#pragma unroll
-                    for (int t = 0; t < RT; t++)
-                        acc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(s.A[b][u]), as_h8(s.x[t][u]), acc[b][t], 0, 0, 0);
-        };
-        Step s0, s1;
-        int i = wave;
-        if (i < steps) load(s0, i);
-        while (i < steps) {
-            if (i + W < steps) load(s1, i + W);
-            mul(s0, i);
-            i += W;
-            if (i >= steps) break;
-            if (i + W < steps) load(s0, i + W);
-            mul(s1, i);
-            i += W;
-        }
         if (p > 0) __syncthreads();           // the sums of the pass before are read
+#pragma unroll
+        for (int j = 0; j < ST - 1; j++)
+            if (j < mine) issue(j);
+        f32x4 acc[RB][RT] = {};
+        for (int j = 0; j < mine; j++) {
+            if (j + ST - 1 < mine) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the step before has left its place
+                issue(j + ST - 1);
+            }
+            const int younger = min(ST - 1, mine - 1 - j);
+            if (ST > 3 && younger == 3) wait_dma<3 * (RB + RT)>();
+            else if (younger == 2) wait_dma<2 * (RB + RT)>();
+            else if (younger == 1) wait_dma<RB + RT>();
+            else wait_dma<0>();
+            const uint8_t* at_s = own + j % ST * Z::STEP + c16 * 64 + 16 * (quad ^ (c16 >> 2));
+            u32x4 fa[RB], fx[RT];
+#pragma unroll
+            for (int b = 0; b < RB; b++) fa[b] = *reinterpret_cast<const u32x4*>(at_s + 1024 * b);
+#pragma unroll
+            for (int t = 0; t < RT; t++) fx[t] = *reinterpret_cast<const u32x4*>(at_s + 1024 * (RB + t));
+            const int k0 = 32 * (wave + W * j);
+            if (k0 + 32 > a.K && k0 + 8 * quad >= a.K) {     // the last step of a K that is no multiple of 32
+#pragma unroll
+                for (int b = 0; b < RB; b++) fa[b] = (u32x4){0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < RT; t++) fx[t] = (u32x4){0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int b = 0; b < RB; b++)
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+                    acc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(fa[b]), as_h8(fx[t]), acc[b][t], 0, 0, 0);
+        }
 #pragma unroll
         for (int b = 0; b < RB; b++)
 #pragma unroll
             for (int t = 0; t < RT; t++)
-                *reinterpret_cast<f32x4*>(part + (wave * ROWS + 16 * t + c16) * PS + 16 * b + 4 * quad) = acc[b][t];
+                *reinterpret_cast<f32x4*>(own + ((16 * t + c16) * PS + 16 * b + 4 * quad) * 4) = acc[b][t];
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < VPT; v++) {
@@ -146,18 +165,40 @@ __global__ void __launch_bounds__(64 * W) lora_tile_kernel(LoraArgs a) {
             float s = 0.0f;
             if (TPR <= 16 * RB || j < 16 * RB) {
 #pragma unroll
-                for (int w = 0; w < W; w++) s += part[(w * ROWS + row) * PS + j];
+                for (int w = 0; w < W; w++) s += *reinterpret_cast<const float*>(lds + w * Z::WAVE + (row * PS + j) * 4);
             }
             h[p][v] = p * 16 * RB + j < a.r && j < 16 * RB ? s : 0.0f;
             const float u = __builtin_fabsf(h[p][v]);
             most = __builtin_fmaxf(most, u < __builtin_inff() ? u : 0.0f);      // (of the finite ones)
         }
     }
+    // what the outputs take, UN of them per step: B's rows of them, whole lines one after the other, and base
+    constexpr int KS = RB == 1 ? 1 : RP / 32, BI = UN * RP / 512, LPR = UN / 8, BJ = ROWS * LPR / 64;
+    const int lp = 31 - __builtin_clz(a.r / 8);
+    const bool pow2 = a.r == 8 << lp;         // pieces per row
+    const int swz = !pow2 || lp < 2 ? 0 : lp == 2 ? 3 : lp == 3 ? 7 : 15, swz_sh = lp == 2 ? 2 : 0;
+    const auto turn = [&](int n) { return (n >> swz_sh) & swz; };
+    const int all_b = a.N * (a.r / 8);        // pieces of B (below 2^24 * 32)
+    u32x4 bw[BI], bb[BJ];
+    const auto get = [&](int n0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < BI; i++) {
+            const int j = 64 * i + lane, n = j >> lp;
+            const int piece = swz ? (n << lp) + ((j & ((1 << lp) - 1)) ^ turn(n)) : j;
+            bw[i] = *reinterpret_cast<const u32x4*>(B + (size_t)min(n0 * (a.r / 8) + piece, all_b - 1) * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < BJ; i++) {
+            const int j = 64 * i + lane;
+            bb[i] = *reinterpret_cast<const u32x4*>(base + (size_t)min(j / LPR, rows - 1) * a.base_stride + min(n0 + j % LPR * 8, a.N - 8));
+        }
+    };
+    int n0 = n_lo + UN * wave;
+    if (n0 < n_hi) get(n0);                   // on its way before the sums have met
     // the row's largest to [2^14, 2^15)
 #pragma unroll
     for (int o = TPR / 2; o > 0; o >>= 1) most = __builtin_fmaxf(most, __shfl_xor(most, o, 64));
     const int e = most > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
-    __syncthreads();                          // (the halves lie where the sums did)
     if (sub == 0) back[row] = __builtin_ldexpf(1.0f, -e);
 #pragma unroll
     for (int p = 0; p < NP; p++)
@@ -175,67 +216,210 @@ __global__ void __launch_bounds__(64 * W) lora_tile_kernel(LoraArgs a) {
         }
     __syncthreads();
 
-    constexpr int KS = RB == 1 ? 1 : RP / 32;
-    float unlift[RT];
+    uint8_t* own_b = own;      // (the sums are read)
+    float* own_d = reinterpret_cast<float*>(own_b + Z::BUF);
+    for (; n0 < n_hi; n0 += UN * W) {
+        wave_lds_order();
 #pragma unroll
-    for (int t = 0; t < RT; t++) unlift[t] = back[16 * t + c16];
-    for (int n0 = n_lo + 32 * wave; n0 < n_hi; n0 += 32 * W) {
-        const int n = n0 + 8 * quad, nc = min(n, a.N - 8);
-        uint4 bs[RT];
+        for (int i = 0; i < BI; i++) *reinterpret_cast<u32x4*>(own_b + 1024 * i + 16 * lane) = bw[i];
+        u32x4 bc[BJ];
 #pragma unroll
-        for (int t = 0; t < RT; t++)
-            bs[t] = *reinterpret_cast<const uint4*>(base + (size_t)min(16 * t + c16, rows - 1) * a.base_stride + nc);
-        f32x4 acc[RT][2] = {};
-        const int nb = min(n0 + 8 * (c16 >> 2), a.N - 8) + (c16 & 3);
+        for (int i = 0; i < BJ; i++) bc[i] = bb[i];
+        if (n0 + UN * W < n_hi) get(n0 + UN * W);
+        wave_lds_order();
+        f32x4 acc[RT][UN / 16] = {};
 #pragma unroll
         for (int k = 0; k < KS; k++) {
             const int chunk = RB == 1 ? quad & 1 : 4 * k + quad;
             const bool there = 8 * chunk < a.r;
+            u32x4 z[RT][RB == 1 ? 1 : 2];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                uint4 w = *reinterpret_cast<const uint4*>(B + (size_t)(nb + 4 * u) * a.r + (there ? 8 * chunk : 0));
-                if (!there) w = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    const uint16_t* at_h = hs + (16 * t + c16) * HS + 8 * chunk;
-                    if constexpr (RB == 1) {
-                        const h16x8 z = *reinterpret_cast<const h16x8*>(at_h + (quad >> 1) * RP);
-                        acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w), z, acc[t][u], 0, 0, 0);
-                    } else {
-                        const h16x8 hi = *reinterpret_cast<const h16x8*>(at_h), lo = *reinterpret_cast<const h16x8*>(at_h + RP);
-                        acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w), hi, acc[t][u], 0, 0, 0);
-                        acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w), lo, acc[t][u], 0, 0, 0);
-                    }
+            for (int t = 0; t < RT; t++) {
+                const uint16_t* at_h = hs + (16 * t + c16) * HS + 8 * chunk;
+                if constexpr (RB == 1) {
+                    z[t][0] = *reinterpret_cast<const u32x4*>(at_h + (quad >> 1) * RP);
+                } else {
+                    z[t][0] = *reinterpret_cast<const u32x4*>(at_h);
+                    z[t][1] = *reinterpret_cast<const u32x4*>(at_h + RP);
                 }
             }
+#pragma unroll
+            for (int u = 0; u < UN / 16; u++) {
+                const int n = 16 * u + c16;
+                u32x4 w = *reinterpret_cast<const u32x4*>(own_b + 2 * n * a.r + (there ? 16 * (chunk ^ turn(n)) : 0));
+                if (!there) w = (u32x4){0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+#pragma unroll
+                    for (int q = 0; q < (RB == 1 ? 1 : 2); q++)
+                        acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w), as_h8(z[t][q]), acc[t][u], 0, 0, 0);
+            }
         }
-        if (n >= n_hi) continue;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
-            if (16 * t + c16 >= rows) continue;
-            const uint32_t w[4] = {bs[t].x, bs[t].y, bs[t].z, bs[t].w};
-            uint32_t o[4];
+            wave_lds_order();
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float d0 = acc[t][j >> 1][2 * (j & 1)] * unlift[t], d1 = acc[t][j >> 1][2 * (j & 1) + 1] * unlift[t];
-                o[j] = f2h(__builtin_fmaf(d0, scale, h2f((uint16_t)w[j]))) |
-                       (uint32_t)f2h(__builtin_fmaf(d1, scale, h2f((uint16_t)(w[j] >> 16)))) << 16;
+            for (int u = 0; u < UN / 16; u++) *reinterpret_cast<f32x4*>(own_d + c16 * DS + 16 * u + 4 * quad) = acc[t][u];
+            wave_lds_order();
+#pragma unroll
+            for (int i = 0; i < BJ / RT; i++) {
+                const int j = 64 * i + lane, r = j / LPR, n = n0 + j % LPR * 8;
+                const f32x4 d0 = *reinterpret_cast<const f32x4*>(own_d + r * DS + j % LPR * 8);
+                const f32x4 d1 = *reinterpret_cast<const f32x4*>(own_d + r * DS + j % LPR * 8 + 4);
+                const float unlift = back[16 * t + r];
+                const u32x4 u = bc[BJ / RT * t + i];
+                const u32x4 w = u;
+                uint32_t o[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const float e0 = (q < 2 ? d0 : d1)[2 * (q & 1)] * unlift, e1 = (q < 2 ? d0 : d1)[2 * (q & 1) + 1] * unlift;
+                    o[q] = f2h(__builtin_fmaf(e0, scale, h2f((uint16_t)w[q]))) |
+                           (uint32_t)f2h(__builtin_fmaf(e1, scale, h2f((uint16_t)(w[q] >> 16)))) << 16;
+                }
+                if (16 * t + r < rows && n < n_hi)
+                    *reinterpret_cast<u32x4*>(y + (size_t)(16 * t + r) * a.y_stride + n) = (u32x4){o[0], o[1], o[2], o[3]};
             }
-            *reinterpret_cast<uint4*>(y + (size_t)(16 * t + c16) * a.y_stride + n) = make_uint4(o[0], o[1], o[2], o[3]);
         }
     }
 }
 
+// Single rows (a decode step): nothing is shared by 16 rows, so the products are FP32 on the
+// vector units, with nothing to turn round in LDS.  Waves take ranks, RB of them side by side,
+// over the whole row; then lanes take 8 ranks of 8 neighbouring outputs.  Bound by the
+// chain of loads: id, A and x, (B and base on their way meanwhile,) store.
+template <int RB>
+__global__ void __launch_bounds__(512) lora_row_kernel(LoraArgs a) {
+    constexpr int W = 8;
+    __shared__ __attribute__((aligned(16))) float h[LORA_MAX_RANK];
+    const int req = blockIdx.y;
+    const int m = a.counts ? a.counts[req] : 1;
+    const int id = a.ids[req];
+    const uint16_t *x = a.x + (size_t)req * a.x_stride, *base = a.base + (size_t)req * a.base_stride;
+    uint16_t* y = a.y + (size_t)req * a.y_stride;
+    const int n_lo = (int)blockIdx.x * a.share, n_hi = min(n_lo + a.share, a.N);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (m < 1) return;
+    if ((unsigned)id >= (unsigned)a.adapters) {
+        if (y != base)
+            for (int n = n_lo + 8 * tid; n < n_hi; n += 512 * 8)
+                *reinterpret_cast<u32x4*>(y + n) = *reinterpret_cast<const u32x4*>(base + n);
+        return;
+    }
+    const uint16_t* A = a.A + (size_t)id * a.r * a.K;
+    const uint16_t* B = a.B + (size_t)id * a.N * a.r;
+    const float scale = a.scales ? a.scales[id] : 1.0f;
+    // outputs: 2^lp lanes (pieces of 8 ranks of a row of B) to 8 outputs, a wave 512 >> lp of them
+    const int pieces = a.r / 8, lp = pieces > 1 ? 32 - __builtin_clz(pieces - 1) : 0;
+    const int piece = lane & ((1 << lp) - 1), group = lane >> lp, per_wave = 512 >> lp;
+    const bool there = piece < pieces;
+    u32x4 bw[8], bb;
+    const auto get = [&](int n0) __attribute__((always_inline)) {
+        const int n = min(n0 + 8 * group, a.N - 8);
+#pragma unroll
+        for (int q = 0; q < 8; q++) bw[q] = *reinterpret_cast<const u32x4*>(B + (size_t)(n + q) * a.r + 8 * (there ? piece : 0));
+        bb = *reinterpret_cast<const u32x4*>(base + n);
+    };
+    int n0 = n_lo + per_wave * wave;
+
+    const int ranks = a.r / W;                // of each wave
+    for (int j0 = 0; j0 < ranks; j0 += RB) {
+        const uint16_t* ar[RB];
+#pragma unroll
+        for (int b = 0; b < RB; b++) ar[b] = A + (size_t)(wave * ranks + min(j0 + b, ranks - 1)) * a.K;
+        float acc[RB] = {};
+        constexpr int U = RB > 4 ? 1 : 2;
+        for (int k0 = 0; k0 < a.K; k0 += 512 * U) {
+            u32x4 xv[U], av[U][RB];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k = min(k0 + 512 * u + 8 * lane, a.K - 8);
+                xv[u] = *reinterpret_cast<const u32x4*>(x + k);
+#pragma unroll
+                for (int b = 0; b < RB; b++) av[u][b] = *reinterpret_cast<const u32x4*>(ar[b] + k);
+            }
+            if (k0 == 0 && j0 == 0 && n0 < n_hi) get(n0);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (k0 + 512 * u + 8 * lane >= a.K) continue;
+#pragma unroll
+                for (int b = 0; b < RB; b++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        acc[b] = __builtin_fmaf(h2f((uint16_t)(av[u][b][i / 2] >> 16 * (i & 1))), h2f((uint16_t)(xv[u][i / 2] >> 16 * (i & 1))), acc[b]);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < RB; b++) acc[b] = wave_sum(acc[b]);
+        if (lane == 0) {
+#pragma unroll
+            for (int b = 0; b < RB; b++)
+                if (j0 + b < ranks) h[wave * ranks + j0 + b] = acc[b];
+        }
+    }
+    if (a.K == 0 && n0 < n_hi) get(n0);
+    __syncthreads();
+    float hv[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) hv[i] = there ? h[8 * piece + i] : 0.0f;
+    for (; n0 < n_hi; n0 += per_wave * W) {
+        float s[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            s[q] = 0.0f;
+            if (there) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) s[q] = __builtin_fmaf(h2f((uint16_t)(bw[q][i / 2] >> 16 * (i & 1))), hv[i], s[q]);
+            }
+        }
+        const u32x4 w = bb;
+        const int n = n0 + 8 * group;
+        if (n0 + per_wave * W < n_hi) get(n0 + per_wave * W);
+        for (int o = 1; o < 1 << lp; o <<= 1)
+#pragma unroll
+            for (int q = 0; q < 8; q++) s[q] += __shfl_xor(s[q], o, 64);
+        if (piece == 0 && n < n_hi) {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                o[j] = f2h(__builtin_fmaf(s[2 * j], scale, h2f((uint16_t)w[j]))) |
+                       (uint32_t)f2h(__builtin_fmaf(s[2 * j + 1], scale, h2f((uint16_t)(w[j] >> 16)))) << 16;
+            *reinterpret_cast<u32x4*>(y + n) = (u32x4){o[0], o[1], o[2], o[3]};
+        }
+    }
+}
+
+// workgroups that a call is cut into, about: more share a tile's rows where there are fewer tiles
+constexpr size_t LORA_WGS = 256, LORA_TILE2 = 64;
+
+static void lora_rows(LoraArgs a, hipStream_t st) {
+    const int pieces = a.r / 8, lp = pieces > 1 ? 32 - __builtin_clz(pieces - 1) : 0, per_wave = 512 >> lp;
+    const size_t units = ceil_div(a.N, per_wave), want = ceil_div(LORA_WGS, a.batch);
+    const size_t share = ceil_div(units, want < units ? want : units);
+    a.share = (int)share * per_wave;
+    const dim3 grid(ceil_div(a.N, a.share), (unsigned)a.batch);
+    if (a.r <= 8) hipLaunchKernelGGL(lora_row_kernel<1>, grid, dim3(512), 0, st, a);
+    else if (a.r <= 16) hipLaunchKernelGGL(lora_row_kernel<2>, grid, dim3(512), 0, st, a);
+    else if (a.r <= 32) hipLaunchKernelGGL(lora_row_kernel<4>, grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL(lora_row_kernel<8>, grid, dim3(512), 0, st, a);
+}
+
 template <int RT, int RB, int NP, int W>
-static void lora_launch(LoraArgs a, int target, hipStream_t st) {
+static void lora_tiles(LoraArgs a, hipStream_t st) {
     a.tiles = (a.S + 16 * RT - 1) / (16 * RT);
     const size_t tiles = (size_t)a.tiles * a.batch;
-    const int units = (a.N + 31) / 32;
-    int splits = (int)((target + tiles - 1) / tiles);
-    splits = splits < 1 ? 1 : splits > (units + W - 1) / W ? (units + W - 1) / W : splits;
-    a.share = (units + splits - 1) / splits * 32;
+    // outputs are shared out in whole rounds of the W waves
+    const size_t rounds = ceil_div(a.N, LoraShape<RT, RB, NP, W>::UN * W), each = ceil_div(rounds * tiles, LORA_WGS);
+    a.share = (int)(each < rounds ? each : rounds) * LoraShape<RT, RB, NP, W>::UN * W;
     a.splits = (a.N + a.share - 1) / a.share;
     hipLaunchKernelGGL((lora_tile_kernel<RT, RB, NP, W>), dim3((unsigned)((tiles + 7) / 8 * 8 * a.splits)), dim3(64 * W), 0, st, a);
+}
+template <int RT>
+static void lora_ranks(const LoraArgs& a, hipStream_t st) {
+    if (a.r <= 16) lora_tiles<RT, 1, 1, 8>(a, st);
+    else if (a.r <= 32) lora_tiles<RT, 2, 1, 8>(a, st);
+    else if (a.r <= 64) lora_tiles<RT, 4, 1, 8>(a, st);
+    else if (a.r <= 128) lora_tiles<RT, 4, 2, 4>(a, st);
+    else lora_tiles<RT, 4, 4, 4>(a, st);
 }
 
 }  // namespace cactus_hip
@@ -261,24 +445,8 @@ extern "C" int cactus_hip_lora_add_f16(const uint16_t* x, size_t x_stride, const
                (int)rank, (int)batch, (int)seq_len, (int)K, (int)N, 0, 0, 0};
     CH_REQUIRE(batch * ceil_div(seq_len, 16) < (1u << 22), "lora_add: batch times seq_len out of range");
     const hipStream_t st = as_stream(stream);
-    const int rt = seq_len <= 16 ? 1 : batch * ceil_div(seq_len, 64) >= 128 && rank <= 64 ? 4 : batch * ceil_div(seq_len, 32) >= 64 ? 2 : 1;
-#define LORA_RANKS(RT, W)                                                     \
-    if (rank <= 16) lora_launch<RT, 1, 1, W>(a, LORA_WGS, st);                \
-    else if (rank <= 32) lora_launch<RT, 2, 1, W>(a, LORA_WGS, st);           \
-    else if (rank <= 64) lora_launch<RT, 4, 1, W>(a, LORA_WGS, st)
-#define LORA_MORE(RT, W)                                                      \
-    else if (rank <= 128) lora_launch<RT, 4, 2, W>(a, LORA_WGS, st);          \
-    else lora_launch<RT, 4, 4, W>(a, LORA_WGS, st)
-    if (rt == 4) {
-        LORA_RANKS(4, 4);
-    } else if (rt == 2) {
-        LORA_RANKS(2, 4);
-        LORA_MORE(2, 4);
-    } else {
-        LORA_RANKS(1, 8);
-        LORA_MORE(1, 8);
-    }
-#undef LORA_RANKS
-#undef LORA_MORE
+    if (seq_len == 1) lora_rows(a, st);
+    else if (seq_len > 16 && batch * ceil_div(seq_len, 32) >= LORA_TILE2) lora_ranks<2>(a, st);
+    else lora_ranks<1>(a, st);
     return check_launch("lora_add");
 }
