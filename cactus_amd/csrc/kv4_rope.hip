@@ -16,14 +16,39 @@ namespace cactus_hip {
 // set if any behind it is, which FP32 holds exactly and FP16 rounds as the whole.
 __device__ __forceinline__ uint16_t f64_to_h(double x) {
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
-    const uint32_t hi = (uint32_t)(b >> 32) | ((uint32_t)b != 0 ? 1u : 0u);
+    const uint32_t hi = (uint32_t)(b >> 32) | min((uint32_t)b, 1u);
     return f2h((float)__builtin_bit_cast(double, (uint64_t)hi << 32));
 }
-__device__ __forceinline__ double wave_sum_f64(double v) {
+// 1 / sqrt(v): the approximation's 2^-24 or so squared twice by Newton's steps; 0 for
+// infinity and infinity for 0, as the formula has them
+__device__ __forceinline__ double rsqrt_f64(double v) {
+    const double y0 = __builtin_amdgcn_rsq(v);
+    double y = y0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    for (int i = 0; i < 2; i++) y = __builtin_fma(0.5 * y, __builtin_fma(-(v * y), y, 1.0), y);
+    return v > 0.0 && v < __builtin_inf() ? y : y0;
 }
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    v += dpp_f64<0xB1>(v);        // within rows of 16 lanes
+    v += dpp_f64<0x4E>(v);
+    v += dpp_f64<0x141>(v);
+    v += dpp_f64<0x140>(v);
+    const auto of = [&](int l) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l);
+        return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    };
+    return (of(0) + of(16)) + (of(32) + of(48));
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct RopeArgs {
     Kv4View c;
@@ -52,21 +77,27 @@ __global__ void __launch_bounds__(64 * ROW_WAVES) kv4_rope_row_kernel(RopeArgs a
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int item = (int)blockIdx.y * ROW_WAVES + wave, row = blockIdx.x, req = blockIdx.z;
     if (item >= a.Hq + 2 * c.Hkv) return;
-    const int status = c.state[KV4_STATUS];
-    const int slot = kv4_slot(c, a.seqs, req);
-    if (slot < 0 || status != 0) return;
-    const int len = kv4_len(c, slot), m = kv4_count(a.counts, req, a.S);
-    const int pos = len - m + row;
-    if (row >= m || pos < 0) return;
     const bool is_q = item < a.Hq, is_v = item >= a.Hq + c.Hkv;
     const int head = is_q ? item : is_v ? item - a.Hq - c.Hkv : item - a.Hq;
     const size_t r = (size_t)req * a.S + row;
     const uint16_t* src = (is_q ? a.q + r * a.q_stride : (is_v ? a.v : a.k) + r * a.kv_stride) + (size_t)head * D + lane;
-    uint16_t x[E];
+    const uint16_t* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+    // what does not hang on the position is on its way while the slot's length is looked up
+    uint16_t x[E], wn[E] = {};
 #pragma unroll
     for (int e = 0; e < E; e++) x[e] = src[64 * e];
+    if (w) {
+#pragma unroll
+        for (int e = 0; e < E; e++) wn[e] = w[64 * e + lane];
+    }
+    const int status = c.state[KV4_STATUS];
+    const int slot = kv4_slot(c, a.seqs, req);
+    if (slot < 0) return;
+    const int len = kv4_len(c, slot), m = kv4_count(a.counts, req, a.S);
+    const int pos = len - m + row;
+    if (status != 0 || row >= m || pos < 0) return;
+    const int page = is_q ? 0 : c.table[(size_t)slot * c.max_pages + (pos >> c.ps_log2)];
     if (!is_v) {
-        const uint16_t* w = is_q ? a.q_norm : a.k_norm;
         double y[E];
 #pragma unroll
         for (int e = 0; e < E; e++) y[e] = (double)h2f(x[e]);
@@ -74,9 +105,9 @@ __global__ void __launch_bounds__(64 * ROW_WAVES) kv4_rope_row_kernel(RopeArgs a
             double ss = 0;
 #pragma unroll
             for (int e = 0; e < E; e++) ss = __builtin_fma(y[e], y[e], ss);
-            const double inv = 1.0 / sqrt(wave_sum_f64(ss) * (1.0 / D) + a.eps);
+            const double inv = rsqrt_f64(wave_sum_f64(ss) * (1.0 / D) + a.eps);
 #pragma unroll
-            for (int e = 0; e < E; e++) y[e] = y[e] * inv * (double)h2f(w[64 * e + lane]);
+            for (int e = 0; e < E; e++) y[e] = y[e] * (double)h2f(wn[e]) * inv;
         }
         const float* t = a.table + (size_t)pos * D;
         if constexpr (E == 1) {
@@ -97,17 +128,13 @@ __global__ void __launch_bounds__(64 * ROW_WAVES) kv4_rope_row_kernel(RopeArgs a
         for (int e = 0; e < E; e++) dst[64 * e] = x[e];
         return;
     }
-    const int page = c.table[(size_t)slot * c.max_pages + (pos >> c.ps_log2)];
     if (!kv4_page_ok(c, page)) return;
     uint8_t* out = kv4_tile(c, page, head, (pos & ((1 << c.ps_log2) - 1)) >> 4) + (is_v ? 9 * D : 0);
     const int key = pos & 15, l = lane & 31;
 #pragma unroll
     for (int e = 0; e < E; e++) {
         // group 2 e + lane / 32
-        uint32_t am = x[e] & 0x7FFFu;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) am = max(am, (uint32_t)__shfl_xor((int)am, o, 64));
-        const uint16_t sb = kv4_scale(am);
+        const uint16_t sb = kv4_scale((uint32_t)half_wave_max((float)(x[e] & 0x7FFFu)));     // (bits as numbers)
         const float s = h2f(sb), inv = s > 0.0f ? 1.0f / s : 0.0f;
         const uint32_t code = s > 0.0f ? kv4_code(x[e], inv) & 15u : 8u;
         const int g = 2 * e + (lane >> 5);
@@ -122,150 +149,200 @@ __global__ void __launch_bounds__(64 * ROW_WAVES) kv4_rope_row_kernel(RopeArgs a
     }
 }
 
-// A wave takes one 16-token tile of several heads, lane 16 h + token with dims 8 h to 8 h + 7 of
-// each 32-dim group, the order in which the append writes pages: the halves of a rotation are in
-// one lane, and the table's values stay in registers from head to head (read anew for each they
-// were twice the bytes of the rows).
-// grid (tile, TILE_WAVES * heads_per_wave heads, request)
+// Prompts.  Queries and keys: D / 16 lanes take a token, each two pieces of 8 dims that a rotation
+// pairs (so that neighbouring lanes load neighbouring bytes: with a lane per token, as the pages
+// have them, the L1 took a row's piece at a time), and a wave 1024 / D tokens of several heads one after
+// the other, the rotations staying in registers.  In each 8 lanes the pieces are 0 1 2 3 7 6 5 4:
+// the four of a scale's group are a quad, and the two whose codes share bytes mirror each other.
+// Values: a 16-token tile per wave in the pages' order, as the append without rotation.
+// grid (tile, 4 units each, request); units: TPT token groups times ceil(q and k heads / heads),
+// then ceil(v heads / heads)
 constexpr int TILE_WAVES = 4;
-constexpr size_t ROPE_TILE_ROWS = 8;
-constexpr int ROPE_PER_WAVE = 4;
+// Rows of a call from which tiles are faster than a wave per row and head (8 sequences of 8 rows 5.8
+// against 6.2 us, of 16 rows 6.7 against 6.4; 64 of 4 rows 8.5 against 10.0, of 8 rows 11.6
+// against 10.9: shorter sequences leave tiles too empty), and waves from which one takes two
+// heads (2000 waves 7.8 against 8.7 us, 14000 27.5 against 26.3; 16 query and 8 KV heads of 128).
+constexpr size_t ROPE_TILE_ROWS = 128, ROPE_TILE_SEQ = 8, ROPE_TWO_HEADS = 8192;
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
 template <int D>
-__global__ void __launch_bounds__(64 * TILE_WAVES) kv4_rope_tile_kernel(RopeArgs a, int per_wave) {
-    constexpr int NG = D / 32, NP = NG / 2;
+__global__ void __launch_bounds__(64 * TILE_WAVES, 3) kv4_rope_tile_kernel(RopeArgs a, int heads) {
+    constexpr int NG = D / 32, LPT = D / 16, TPW = 64 / LPT, TPT = 16 / TPW;
     const Kv4View& c = a.c;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), key = lane & 15, h = lane >> 4;
-    const int req = blockIdx.z, items = a.Hq + 2 * c.Hkv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int req = blockIdx.z, rot = a.Hq + c.Hkv, chunks = (rot + heads - 1) / heads;
+    const int unit = (int)blockIdx.y * TILE_WAVES + wave;
+    if (unit >= TPT * chunks) {
+        const int h0 = (unit - TPT * chunks) * heads;
+        if (h0 >= c.Hkv) return;
+        const int status = c.state[KV4_STATUS];
+        const int slot = kv4_slot(c, a.seqs, req);
+        if (slot < 0 || status != 0) return;
+        const int len = kv4_len(c, slot), first = len - kv4_count(a.counts, req, a.S);   // (negative: rows without a token)
+        const int lo = max(first, 0);
+        const int pos0 = (lo & ~15) + 16 * (int)blockIdx.x;
+        if (pos0 >= len) return;
+        const int key = lane & 15, h = lane >> 4, pos = pos0 + key;
+        const int page = c.table[(size_t)slot * c.max_pages + (pos0 >> c.ps_log2)];
+        if (!kv4_page_ok(c, page)) return;
+        const bool mine = pos >= lo && pos < len, whole = pos0 >= lo && pos0 + 16 <= len;
+        const uint16_t* src = a.v + ((size_t)req * a.S + ((mine ? pos : lo) - first)) * a.kv_stride + 8 * h;
+        for (int head = h0; head < min(h0 + heads, c.Hkv); head++) {
+            uint4 x[NG];
+#pragma unroll
+            for (int g = 0; g < NG; g++) x[g] = *reinterpret_cast<const uint4*>(src + (size_t)head * D + 32 * g);
+            kv4_write_tile<D>(x, kv4_tile(c, page, head, (pos0 & ((1 << c.ps_log2) - 1)) >> 4) + 9 * D, true, mine, whole);
+        }
+        return;
+    }
+    const int s = lane & (LPT - 1), j = LPT == 4 || !(s & 4) ? s : s ^ 3;       // piece (the other is j + LPT)
+    const int r0 = 16 * (int)blockIdx.x + unit / chunks * TPW, in_s = r0 + lane / LPT;
+    if (r0 >= a.S) return;
+    const size_t row = (size_t)req * a.S + min(in_s, a.S - 1);
+    const int item0 = unit % chunks * heads, item1 = min(item0 + heads, rot);
+    const auto source = [&](int item) {
+        return (item < a.Hq ? a.q + row * a.q_stride + (size_t)item * D : a.k + row * a.kv_stride + (size_t)(item - a.Hq) * D) + 8 * j;
+    };
+    const u32x4 ones = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};      // the weights of no norm
+    // the first rows do not hang on the position: on their way while the slot's length is looked up
+    u32x4 next[2];
+    {
+        const uint16_t* p = source(item0);
+        next[0] = *reinterpret_cast<const u32x4*>(p);
+        next[1] = *reinterpret_cast<const u32x4*>(p + D / 2);
+    }
     const int status = c.state[KV4_STATUS];
     const int slot = kv4_slot(c, a.seqs, req);
-    if (slot < 0 || status != 0) return;
-    const int len = kv4_len(c, slot), first = len - kv4_count(a.counts, req, a.S);   // (negative: rows without a token)
-    const int lo = max(first, 0);
-    const int pos0 = (lo & ~15) + 16 * (int)blockIdx.x;
-    if (pos0 >= len) return;
-    const int pos = pos0 + key;
-    const bool mine = pos >= lo && pos < len, whole = pos0 >= lo && pos0 + 16 <= len;
-    const int at = mine ? pos : lo;
-    const size_t row = (size_t)req * a.S + (at - first);
-    float co[NP][8], si[NP][8];
+    if (slot < 0) return;
+    const int len = kv4_len(c, slot), m = kv4_count(a.counts, req, a.S);
+    if (status != 0 || r0 >= m) return;
+    const int pos = len - m + in_s;
+    const bool mine = in_s < m && pos >= 0;
+    const int at = mine ? pos : 0;
+    float co[8], si[8];
     {
-        const float* t = a.table + (size_t)at * D + 8 * h;
+        const float* t = a.table + (size_t)at * D + 8 * j;
 #pragma unroll
-        for (int g = 0; g < NP; g++)
+        for (int i = 0; i < 2; i++) {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(t + 4 * i), v = *reinterpret_cast<const f32x4*>(t + D / 2 + 4 * i);
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const f32x4 u = *reinterpret_cast<const f32x4*>(t + 32 * g + 4 * j), v = *reinterpret_cast<const f32x4*>(t + D / 2 + 32 * g + 4 * j);
-#pragma unroll
-                for (int i = 0; i < 4; i++) co[g][4 * j + i] = u[i], si[g][4 * j + i] = v[i];
-            }
-    }
-    const int page = c.table[(size_t)slot * c.max_pages + (pos0 >> c.ps_log2)];
-    const int tile = (pos0 & ((1 << c.ps_log2) - 1)) >> 4;
-    const int item0 = (int)blockIdx.y * TILE_WAVES * per_wave + wave;
-    const auto source = [&](int item) {
-        const bool is_q = item < a.Hq, is_v = item >= a.Hq + c.Hkv;
-        return (is_q ? a.q + row * a.q_stride : (is_v ? a.v : a.k) + row * a.kv_stride) +
-               (size_t)(is_q ? item : is_v ? item - a.Hq - c.Hkv : item - a.Hq) * D + 8 * h;
-    };
-    uint4 next[NG];
-    if (item0 < items) {
-        const uint16_t* src = source(item0);
-#pragma unroll
-        for (int g = 0; g < NG; g++) next[g] = *reinterpret_cast<const uint4*>(src + 32 * g);
-    }
-    for (int n = 0; n < per_wave; n++) {
-        const int item = item0 + TILE_WAVES * n;
-        if (item >= items) return;
-        uint4 x[NG];
-#pragma unroll
-        for (int g = 0; g < NG; g++) x[g] = next[g];
-        if (n + 1 < per_wave && item + TILE_WAVES < items) {
-            const uint16_t* src = source(item + TILE_WAVES);
-#pragma unroll
-            for (int g = 0; g < NG; g++) next[g] = *reinterpret_cast<const uint4*>(src + 32 * g);
+            for (int k = 0; k < 4; k++) co[4 * i + k] = u[k], si[4 * i + k] = v[k];
         }
-        const bool is_q = item < a.Hq, is_v = item >= a.Hq + c.Hkv;
-        const auto half_of = [&](int g, int j) { return h2f((uint16_t)((&x[g].x)[j / 2] >> 16 * (j & 1))); };
-        if (is_q) {
+    }
+    // the tile of the lane's token
+    const int page = item1 > a.Hq ? c.table[(size_t)slot * c.max_pages + (at >> c.ps_log2)] : 0;
+    const bool keeps = mine && kv4_page_ok(c, page);
+    const int key = at & 15;
+    uint8_t* tile = kv4_tile(c, keeps ? page : 0, 0, (at & ((1 << c.ps_log2) - 1)) >> 4);
+    const size_t head_bytes = (size_t)(18 * D) << (c.ps_log2 - 4);
+    for (int item = item0; item < item1; item++) {
+        u32x4 x[2] = {next[0], next[1]}, w[2] = {ones, ones};
+        if (item + 1 < item1) {
+            const uint16_t* p = source(item + 1);
+            next[0] = *reinterpret_cast<const u32x4*>(p);
+            next[1] = *reinterpret_cast<const u32x4*>(p + D / 2);
+        }
+        const uint16_t* norm = item < a.Hq ? a.q_norm : a.k_norm;
+        if (norm) {
+            w[0] = *reinterpret_cast<const u32x4*>(norm + 8 * j);
+            w[1] = *reinterpret_cast<const u32x4*>(norm + D / 2 + 8 * j);
+        }
+        float xf[2][8], xw[2][8];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                xf[u][i] = h2f((uint16_t)(x[u][i / 2] >> 16 * (i & 1)));
+                xw[u][i] = xf[u][i] * h2f((uint16_t)(w[u][i / 2] >> 16 * (i & 1)));       // (exact)
+            }
+        if (item < a.Hq) {
             // in 32 bits: an FP16 result has no border that 2^-22 beside it matters for
             float f = 1.0f;
-            if (a.q_norm) {
+            if (norm) {
                 float ss = 0.0f;
 #pragma unroll
-                for (int g = 0; g < NG; g++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) ss = __builtin_fmaf(half_of(g, j), half_of(g, j), ss);
-                ss += __shfl_xor(ss, 16, 64);
-                ss += __shfl_xor(ss, 32, 64);
+                for (int i = 0; i < 8; i++) ss = __builtin_fmaf(xf[0][i], xf[0][i], __builtin_fmaf(xf[1][i], xf[1][i], ss));
+                ss += dpp_move_keep<0xB1>(ss);
+                ss += dpp_move_keep<0x4E>(ss);
+                if constexpr (LPT >= 8) ss += dpp_move_keep<0x141>(ss);
+                if constexpr (LPT >= 16) ss += dpp_move_keep<0x140>(ss);
                 f = 1.0f / sqrtf(ss * (1.0f / D) + (float)a.eps);
             }
-            uint16_t* dst = a.q_out + (row * a.Hq + item) * D + 8 * h;
+            uint16_t r[2][8];
 #pragma unroll
-            for (int g = 0; g < NP; g++) {
-                uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;
-                if (a.q_norm) {
-                    wa = *reinterpret_cast<const uint4*>(a.q_norm + 32 * g + 8 * h);
-                    wb = *reinterpret_cast<const uint4*>(a.q_norm + D / 2 + 32 * g + 8 * h);
-                }
-                uint32_t ra[4], rb[4];
+            for (int i = 0; i < 8; i++) {
+                const float u = xw[0][i] * f, v = xw[1][i] * f;
+                r[0][i] = f2h(__builtin_fmaf(u, co[i], -(v * si[i])));
+                r[1][i] = f2h(__builtin_fmaf(v, co[i], u * si[i]));
+            }
+            if (mine) {
+                uint16_t* dst = a.q_out + (row * a.Hq + item) * D + 8 * j;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    float u = half_of(g, j), v = half_of(g + NP, j);
-                    if (a.q_norm) {
-                        u = u * f * h2f((uint16_t)((&wa.x)[j / 2] >> 16 * (j & 1)));
-                        v = v * f * h2f((uint16_t)((&wb.x)[j / 2] >> 16 * (j & 1)));
-                    }
-                    const uint32_t p = f2h(__builtin_fmaf(u, co[g][j], -(v * si[g][j]))), r = f2h(__builtin_fmaf(v, co[g][j], u * si[g][j]));
-                    if (j & 1) ra[j / 2] |= p << 16, rb[j / 2] |= r << 16;
-                    else ra[j / 2] = p, rb[j / 2] = r;
-                }
-                if (mine) {
-                    *reinterpret_cast<uint4*>(dst + 32 * g) = make_uint4(ra[0], ra[1], ra[2], ra[3]);
-                    *reinterpret_cast<uint4*>(dst + D / 2 + 32 * g) = make_uint4(rb[0], rb[1], rb[2], rb[3]);
-                }
+                for (int u = 0; u < 2; u++)
+                    *reinterpret_cast<u32x4*>(dst + u * (D / 2)) =
+                        (u32x4){r[u][0] | (uint32_t)r[u][1] << 16, r[u][2] | (uint32_t)r[u][3] << 16,
+                                r[u][4] | (uint32_t)r[u][5] << 16, r[u][6] | (uint32_t)r[u][7] << 16};
             }
             continue;
         }
-        if (!kv4_page_ok(c, page)) return;        // (heads go up: keys and values are all that is left)
-        if (!is_v) {
-            double f = 1.0;
-            if (a.k_norm) {
-                double ss = 0.0;
+        double f = 1.0;
+        if (norm) {
+            double ss = 0.0;
 #pragma unroll
-                for (int g = 0; g < NG; g++)
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) ss += (double)(half_of(g, j) * half_of(g, j));     // (exact in FP32)
-                ss += __shfl_xor(ss, 16, 64);
-                ss += __shfl_xor(ss, 32, 64);
-                f = 1.0 / sqrt(ss * (1.0 / D) + a.eps);
-            }
+                for (int i = 0; i < 8; i++) ss += (double)(xf[u][i] * xf[u][i]);       // (exact in FP32)
+            ss += dpp_f64<0xB1>(ss);
+            ss += dpp_f64<0x4E>(ss);
+            if constexpr (LPT >= 8) ss += dpp_f64<0x141>(ss);
+            if constexpr (LPT >= 16) ss += dpp_f64<0x140>(ss);
+            f = rsqrt_f64(ss * (1.0 / D) + a.eps);
+        }
+        uint16_t r[2][8];
 #pragma unroll
-            for (int g = 0; g < NP; g++) {
-                uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;
-                if (a.k_norm) {
-                    wa = *reinterpret_cast<const uint4*>(a.k_norm + 32 * g + 8 * h);
-                    wb = *reinterpret_cast<const uint4*>(a.k_norm + D / 2 + 32 * g + 8 * h);
-                }
-                uint32_t ra[4], rb[4];
+        for (int i = 0; i < 8; i++) {
+            const double u = (double)xw[0][i] * f, v = (double)xw[1][i] * f, cs = co[i], sn = si[i];
+            r[0][i] = f64_to_h(__builtin_fma(u, cs, -(v * sn)));
+            r[1][i] = f64_to_h(__builtin_fma(v, cs, u * sn));
+        }
+        uint8_t* out = tile + (size_t)(item - a.Hq) * head_bytes;
+        uint32_t b[2][2];                         // codes of a piece, a byte each
+        uint16_t sb[2];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    double u = half_of(g, j), v = half_of(g + NP, j);
-                    if (a.k_norm) {
-                        // (x w is exact in FP32)
-                        u = (double)(half_of(g, j) * h2f((uint16_t)((&wa.x)[j / 2] >> 16 * (j & 1)))) * f;
-                        v = (double)(half_of(g + NP, j) * h2f((uint16_t)((&wb.x)[j / 2] >> 16 * (j & 1)))) * f;
-                    }
-                    const double cs = co[g][j], sn = si[g][j];
-                    const uint32_t p = f64_to_h(__builtin_fma(u, cs, -(v * sn))), r = f64_to_h(__builtin_fma(v, cs, u * sn));
-                    if (j & 1) ra[j / 2] |= p << 16, rb[j / 2] |= r << 16;
-                    else ra[j / 2] = p, rb[j / 2] = r;
-                }
-                x[g] = make_uint4(ra[0], ra[1], ra[2], ra[3]);
-                x[g + NP] = make_uint4(rb[0], rb[1], rb[2], rb[3]);
+        for (int u = 0; u < 2; u++) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = max(m, (uint32_t)(r[u][i] & 0x7FFFu));
+            m = max(m, dpp<0xB1>(m));
+            m = max(m, dpp<0x4E>(m));
+            sb[u] = kv4_scale(m);
+            const float sc = h2f(sb[u]), inv = sc > 0.0f ? 1.0f / sc : 0.0f;
+            uint32_t k[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) k[i] = kv4_code(r[u][i], inv);
+            b[u][0] = sc > 0.0f ? low_bytes(k[0], k[1], k[2], k[3]) : 0x08080808u;
+            b[u][1] = sc > 0.0f ? low_bytes(k[4], k[5], k[6], k[7]) : 0x08080808u;
+        }
+        uint2 bytes;
+        int p = 0;                                // 64-dim block of the bytes
+        if constexpr (LPT == 4) {
+            bytes = make_uint2(b[0][0] | b[1][0] << 4, b[0][1] | b[1][1] << 4);
+        } else {
+            // lanes with the low nibbles' pieces finish the first half's block, their mirrors the second's
+            const bool high = s & 4;
+            const uint32_t g0 = dpp<0x141>(high ? b[0][0] : b[1][0]), g1 = dpp<0x141>(high ? b[0][1] : b[1][1]);
+            bytes = high ? make_uint2(g0 | b[1][0] << 4, g1 | b[1][1] << 4) : make_uint2(b[0][0] | g0 << 4, b[0][1] | g1 << 4);
+            p = (j >> 3) + (high ? LPT / 8 : 0);
+        }
+        if (keeps) {
+            *reinterpret_cast<uint2*>(out + (j & 3) * 2 * D + key * (D / 8) + 8 * p) = bytes;
+            if ((s & 3) < 2) {
+                const int g = (j >> 2) + (s & 1 ? LPT / 4 : 0);
+                reinterpret_cast<uint16_t*>(out + 8 * D)[((key >> 2) * NG + g) * 4 + (key & 3)] = s & 1 ? sb[1] : sb[0];
             }
         }
-        const int head = is_v ? item - a.Hq - c.Hkv : item - a.Hq;
-        kv4_write_tile<D>(x, kv4_tile(c, page, head, tile) + (is_v ? 9 * D : 0), is_v, mine, whole);
     }
 }
 
@@ -341,13 +418,16 @@ int cactus_hip_kv4_append_rope_f16(const cactus_hip_kv4_cache* cache, size_t lay
     a.S = (int)seq_len;
     a.eps = eps;
     const size_t items = num_q_heads + 2 * cache->kv_heads;
-    if (seq_len >= ROPE_TILE_ROWS) {
-        const int per_wave = ROPE_PER_WAVE;
-        const dim3 grid(ceil_div(seq_len + 15, 16), ceil_div(items, TILE_WAVES * per_wave), (unsigned)batch);
+    if (seq_len >= ROPE_TILE_SEQ && batch * seq_len >= ROPE_TILE_ROWS) {
+        const auto units = [&](size_t heads) {
+            return cache->head_dim / 64 * ceil_div(num_q_heads + cache->kv_heads, heads) + ceil_div(cache->kv_heads, heads);
+        };
+        const int heads = batch * ceil_div(seq_len, 16) * units(1) < ROPE_TWO_HEADS ? 1 : 2;
+        const dim3 grid(ceil_div(seq_len + 15, 16), ceil_div(units(heads), TILE_WAVES), (unsigned)batch);
         switch (a.c.d) {
-            case 64: hipLaunchKernelGGL(kv4_rope_tile_kernel<64>, grid, dim3(64 * TILE_WAVES), 0, as_stream(stream), a, per_wave); break;
-            case 128: hipLaunchKernelGGL(kv4_rope_tile_kernel<128>, grid, dim3(64 * TILE_WAVES), 0, as_stream(stream), a, per_wave); break;
-            default: hipLaunchKernelGGL(kv4_rope_tile_kernel<256>, grid, dim3(64 * TILE_WAVES), 0, as_stream(stream), a, per_wave);
+            case 64: hipLaunchKernelGGL(kv4_rope_tile_kernel<64>, grid, dim3(64 * TILE_WAVES), 0, as_stream(stream), a, heads); break;
+            case 128: hipLaunchKernelGGL(kv4_rope_tile_kernel<128>, grid, dim3(64 * TILE_WAVES), 0, as_stream(stream), a, heads); break;
+            default: hipLaunchKernelGGL(kv4_rope_tile_kernel<256>, grid, dim3(64 * TILE_WAVES), 0, as_stream(stream), a, heads);
         }
         return check_launch("kv4_append_rope");
     }
