@@ -43,7 +43,7 @@ constexpr int RULES_MAX_BIAS = CACTUS_HIP_LOGITS_MAX_BIAS;
 constexpr uint32_t COUNT_BITS = 20;      // of the history; above it the entries, bit 31: value in b_out
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) logits_rules_kernel(RulesArgs a) {
-    constexpr int GROUPS = 2, CHUNK = 8 * GROUPS * THREADS, EPT = RULES_MAX_BIAS / THREADS;
+    constexpr int GROUPS = 2, CHUNK = 8 * GROUPS * THREADS, EPT = RULES_MAX_BIAS / THREADS, EARLY = 4;
     __shared__ __attribute__((aligned(16))) uint32_t counts[CHUNK];
     __shared__ float b_out[RULES_MAX_BIAS];
     __shared__ uint64_t w_key[THREADS / 64];
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(RulesArgs a) {
     const int shift = (int)(-(uintptr_t)in & 15) / (int)sizeof(T);
     const bool vec = ((uintptr_t)(out + shift) & 15) == 0;
     const int c0 = (shift ? shift - 8 : 0) + (int)blockIdx.x * CHUNK;      // (down to -7)
-    const int lo = max(c0, 0), hi = min(c0 + CHUNK, a.V);
+    const int lo = max(c0, 0), hi = max(lo, min(c0 + CHUNK, a.V));
 
     float x[GROUPS][8];
 #pragma unroll
@@ -84,17 +84,39 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(RulesArgs a) {
             }
         }
     }
-    const int hist = !a.r.history ? 0 : a.r.history_lens ? min(max(a.r.history_lens[slot], 0), (int)a.r.history_stride) : (int)a.r.history_stride;
-    const int nb = !a.r.bias_tokens ? 0 : a.r.bias_counts ? min(max(a.r.bias_counts[slot], 0), (int)a.r.bias_stride) : (int)a.r.bias_stride;
+    // The lists' first entries are on their way before it is known how many count: a list's length
+    // and then its entries, one after the other, cost more than the entries that go unused.
+    const int32_t* h = a.r.history + (size_t)slot * a.r.history_stride;
+    const int32_t* tokens = a.r.bias_tokens + (size_t)slot * a.r.bias_stride;
+    const float* values = a.r.bias_values + (size_t)slot * a.r.bias_stride;
+    int ht[EARLY], bt[EPT];
+    float bv[EPT], bx[EPT];
+    const int room = a.r.history ? (int)a.r.history_stride : 0, broom = a.r.bias_tokens ? (int)a.r.bias_stride : 0;
+#pragma unroll
+    for (int u = 0; u < EARLY; u++) ht[u] = tid + THREADS * u < room ? h[tid + THREADS * u] : -1;
+#pragma unroll
+    for (int e = 0; e < EPT; e++) {
+        bt[e] = tid + THREADS * e < broom ? tokens[tid + THREADS * e] : -1;
+        bv[e] = tid + THREADS * e < broom ? values[tid + THREADS * e] : 0.0f;
+    }
+    const int hist = a.r.history_lens && room ? min(max(a.r.history_lens[slot], 0), room) : room;
+    const int nb = a.r.bias_counts && broom ? min(max(a.r.bias_counts[slot], 0), broom) : broom;
     const float rep = a.r.repetition ? a.r.repetition[slot] : 1.0f, freq = a.r.frequency ? a.r.frequency[slot] : 0.0f,
                 pres = a.r.presence ? a.r.presence[slot] : 0.0f;
-    const uint32_t* mask = nullptr;
-    bool none = false;
+    uint32_t bits[GROUPS];                    // bit i of group g: its token i is allowed
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) bits[g] = 0xFFu;
     if (a.r.masks) {
         const int id = a.r.mask_ids ? a.r.mask_ids[slot] : slot;
         if (id >= 0) {
-            none = (size_t)id >= a.r.num_masks;
-            mask = none ? nullptr : a.r.masks + (size_t)id * a.r.mask_stride;
+            const bool none = (size_t)id >= a.r.num_masks;
+            const uint32_t* mask = a.r.masks + (none ? 0 : (size_t)id * a.r.mask_stride);
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                const int t = c0 + 8 * (tid + THREADS * g), t0 = min(max(t, 0), a.V - 1), t1 = min(max(t + 7, 0), a.V - 1);
+                const uint64_t w = none ? 0 : (uint64_t)mask[t0 >> 5] | (uint64_t)mask[t1 >> 5] << 32;
+                bits[g] = t < 0 ? (uint32_t)w << -t : t0 >> 5 == t1 >> 5 ? (uint32_t)w >> (t0 & 31) : (uint32_t)(w >> (t0 & 31));
+            }
         }
     }
     const bool listed = hist > 0 || nb > 0;
@@ -102,57 +124,52 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(RulesArgs a) {
 #pragma unroll
         for (int i = 0; i < CHUNK / 4 / THREADS; i++) reinterpret_cast<uint4*>(counts)[tid + THREADS * i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        const int32_t* h = a.r.history + (size_t)slot * a.r.history_stride;
-        for (int i0 = 0; i0 < hist; i0 += 8 * THREADS) {
+#pragma unroll
+        for (int u = 0; u < EARLY; u++)
+            if (tid + THREADS * u < hist && (uint32_t)(ht[u] - lo) < (uint32_t)(hi - lo)) atomicAdd(&counts[ht[u] - c0], 1u);
+        for (int i0 = EARLY * THREADS; i0 < hist; i0 += 8 * THREADS) {
             int t[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const int i = i0 + tid + THREADS * u;
-                t[u] = i < hist ? h[i] : -1;
-            }
+            for (int u = 0; u < 8; u++) t[u] = i0 + tid + THREADS * u < hist ? h[i0 + tid + THREADS * u] : -1;
 #pragma unroll
             for (int u = 0; u < 8; u++)
-                if (t[u] >= lo && t[u] < hi) atomicAdd(&counts[t[u] - c0], 1u);
+                if ((uint32_t)(t[u] - lo) < (uint32_t)(hi - lo)) atomicAdd(&counts[t[u] - c0], 1u);
+        }
+        if (nb > 0) {
+#pragma unroll
+            for (int e = 0; e < EPT; e++) {
+                if (tid + THREADS * e >= nb || bt[e] < lo || bt[e] >= hi) {
+                    bt[e] = -1;
+                    continue;
+                }
+                atomicAdd(&counts[bt[e] - c0], 1u << COUNT_BITS);
+                if constexpr (sizeof(T) == 2) bx[e] = h2f(in[bt[e]]);
+                else bx[e] = in[bt[e]];
+            }
         }
         __syncthreads();
-    }
-    if (nb > 0) {
-        const int32_t* tokens = a.r.bias_tokens + (size_t)slot * a.r.bias_stride;
-        const float* values = a.r.bias_values + (size_t)slot * a.r.bias_stride;
-        int tok[EPT];
-        bool own[EPT];
+        if (nb > 0) {
 #pragma unroll
-        for (int e = 0; e < EPT; e++) {
-            const int i = tid + THREADS * e;
-            tok[e] = i < nb ? tokens[i] : -1;
-            own[e] = tok[e] >= lo && tok[e] < hi;
-            if (own[e]) atomicAdd(&counts[tok[e] - c0], 1u << COUNT_BITS);
+            for (int e = 0; e < EPT; e++) {
+                const int i = tid + THREADS * e, t = bt[e];
+                if (t < 0) continue;
+                const uint32_t w = counts[t - c0], n = w & ((1u << COUNT_BITS) - 1);
+                bool own = !(w >> 31);            // (else the token's first entry has been here)
+                const bool single = w >> COUNT_BITS == 1;
+                if (!single)
+                    for (int j = 0; j < i && own; j++) own = tokens[j] != t;
+                if (!own) continue;
+                float v = bx[e];
+                if (n) v = penalized(v, (int)n, rep, freq, pres);
+                v = v + bv[e];
+                if (!single)
+                    for (int j = i + 1; j < nb; j++)
+                        if (tokens[j] == t) v = v + values[j];
+                b_out[i] = v;
+                counts[t - c0] = 0x80000000u + i;
+            }
+            __syncthreads();
         }
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < EPT; e++) {
-            if (!own[e]) continue;
-            const int i = tid + THREADS * e, t = tok[e];
-            const uint32_t w = counts[t - c0], n = w & ((1u << COUNT_BITS) - 1);
-            const bool single = w >> COUNT_BITS == 1;
-            if (!single)
-                for (int j = 0; j < i && own[e]; j++) own[e] = tokens[j] != t;
-            if (!own[e]) continue;
-            float v;
-            if constexpr (sizeof(T) == 2) v = h2f(in[t]);
-            else v = in[t];
-            if (n) v = penalized(v, (int)n, rep, freq, pres);
-            v = v + values[i];
-            if (!single)
-                for (int j = i + 1; j < nb; j++)
-                    if (tokens[j] == t) v = v + values[j];
-            b_out[i] = v;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < EPT; e++)
-            if (own[e]) counts[tok[e] - c0] = 0x80000000u + tid + THREADS * e;
-        __syncthreads();
     }
     float most = -__builtin_inff();
     int at = 0;
@@ -171,17 +188,8 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(RulesArgs a) {
                 }
             }
         }
-        if (none) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[g][j] = -__builtin_inff();
-        } else if (mask) {
-            const int t0 = max(t, 0), t1 = min(t + 7, a.V - 1);
-            const uint64_t w = (uint64_t)mask[t0 >> 5] | (uint64_t)mask[t1 >> 5] << 32;
-            // bit j: token t + j (words of tokens before the row hold nothing)
-            const uint32_t bits = t < 0 ? (uint32_t)w << -t : t0 >> 5 == t1 >> 5 ? (uint32_t)w >> (t0 & 31) : (uint32_t)(w >> (t0 & 31));
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[g][j] = bits >> j & 1 ? x[g][j] : -__builtin_inff();
-        }
+        for (int j = 0; j < 8; j++) x[g][j] = bits[g] >> j & 1 ? x[g][j] : -__builtin_inff();
         if (vec && t >= 0 && t + 8 <= a.V) {
             *reinterpret_cast<f32x4*>(out + t) = (f32x4){x[g][0], x[g][1], x[g][2], x[g][3]};
             *reinterpret_cast<f32x4*>(out + t + 4) = (f32x4){x[g][4], x[g][5], x[g][6], x[g][7]};
@@ -221,13 +229,11 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(RulesArgs a) {
     a.best[row] = key ? 0xFFFFFFFFu - (uint32_t)key : 0u;
 }
 
+constexpr int RULES_THREADS = 512;
 template <typename T>
 static void rules_launch(const RulesArgs& a, size_t batch, hipStream_t st) {
-    const size_t tokens = (size_t)a.V + 7;      // (a row's groups may start up to 7 before it)
-    if (batch * ceil_div(tokens, 16384) >= 256)
-        hipLaunchKernelGGL((logits_rules_kernel<T, 1024>), dim3(ceil_div(tokens, 16384), (unsigned)batch), dim3(1024), 0, st, a);
-    else
-        hipLaunchKernelGGL((logits_rules_kernel<T, 256>), dim3(ceil_div(tokens, 4096), (unsigned)batch), dim3(256), 0, st, a);
+    const dim3 grid(ceil_div((size_t)a.V + 7, 16 * RULES_THREADS), (unsigned)batch);      // (a row's groups may start up to 7 before it)
+    hipLaunchKernelGGL((logits_rules_kernel<T, RULES_THREADS>), grid, dim3(RULES_THREADS), 0, st, a);
 }
 
 static int rules(const cactus_hip_logits_rules* r, const int32_t* seqs, const void* logits, size_t stride, float* out,
