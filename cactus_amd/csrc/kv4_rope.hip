@@ -388,7 +388,7 @@ int cactus_hip_kv4_append_rope_f16(const cactus_hip_kv4_cache* cache, size_t lay
     if (rc) return rc;
     if (batch == 0 || seq_len == 0) return CACTUS_HIP_OK;
     CH_REQUIRE(k && v && table && (num_q_heads == 0 || (q && q_out)), "kv4_append_rope: null pointer");
-    CH_REQUIRE(num_q_heads <= 65536, "kv4_append_rope: num_q_heads out of range");
+    CH_REQUIRE(num_q_heads <= 16384, "kv4_append_rope: num_q_heads out of range");
     const auto aligned = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
     CH_REQUIRE(aligned(k) && aligned(v) && kv_stride % 8 == 0 &&
                    (num_q_heads == 0 || (aligned(q) && aligned(q_out) && q_stride % 8 == 0)),

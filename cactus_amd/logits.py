@@ -49,7 +49,10 @@ class LogitsRules:
             setattr(self.desc, name, self._buf[name].ptr)
 
     def _put(self, name: str, slot: int, values, dtype, stride: int, stream, rows: int | None = None):
-        a = np.ascontiguousarray(values, dtype)
+        a = np.asarray(values)
+        if np.issubdtype(dtype, np.integer) and a.size and (a.dtype.kind not in "iu" or a.min() < np.iinfo(dtype).min or a.max() > np.iinfo(dtype).max):
+            raise TypeError(f"{name}: 32-bit integers are needed")
+        a = np.ascontiguousarray(a, dtype)
         if not 0 <= slot < (self.desc.max_seqs if rows is None else rows):
             raise IndexError(f"no slot or mask {slot}")
         if name not in self._buf or a.size > stride:

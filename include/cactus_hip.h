@@ -380,7 +380,7 @@ int cactus_hip_sample_f32(const float* logits, uint32_t* out, size_t vocab, floa
  * the largest value; NaN is never it; 0 where no value is above -infinity.  The
  * rows of out are what cactus_hip_sample_f32 takes.  A slot outside [0, max_seqs)
  * makes no access: its row of out and best are left as they were.  FP32 rows may be
- * changed in place (out is logits, one stride).
+ * changed in place (out is logits, one stride); otherwise out overlaps no input.
  * The settings are arrays on the device, so that a captured call follows them; each
  * may be NULL, and is off then (history_lens, bias_counts: all of the stride;
  * mask_ids: mask s for slot s).  Tokens outside the vocabulary are passed over.  masks
@@ -581,13 +581,14 @@ int cactus_hip_rope_table_f32(float* table, size_t positions, size_t head_dim, f
  * sequences grow).  Of a head's row x, with halves a and b of
  *   y = x / sqrt(mean(x^2) + eps) * norm     (norm NULL: y = x)
  *   (a cos - b sin, b cos + a sin),  cos and sin row p of `table`
- * all in 64 bits, rounded once to FP16: for queries into q_out [batch][seq_len]
- * [num_q_heads][head_dim], for keys the row that is quantized into the pages;
- * values are quantized as they come.  q: num_q_heads heads per row, q_stride values from
- * row to row; q_out may be q where the rows are dense (q_stride num_q_heads * head_dim);
- * num_q_heads 0: keys and values only (q, q_out may be NULL).  q_norm, k_norm
- * [head_dim] fp16, either may be NULL.  Strides are multiples of 8, every pointer but
- * seqs and counts 16-byte aligned.  q, k and v may lie side by side in one buffer.
+ * keys in 64 bits and queries in 32 or more, rounded once to FP16: for queries into
+ * q_out [batch][seq_len][num_q_heads][head_dim], for keys the row that is quantized
+ * into the pages; values are quantized as they come.  q: num_q_heads (up to 16384) heads
+ * per row, q_stride values from row to row; q_out may be q where the rows are dense
+ * (q_stride num_q_heads * head_dim), otherwise it overlaps no input.  num_q_heads 0: keys
+ * and values only (q, q_out may be NULL).  q_norm, k_norm [head_dim] fp16, either may
+ * be NULL.  Strides are multiples of 8, every pointer but seqs and counts 16-byte
+ * aligned.  q, k and v may lie side by side in one buffer.
  * `table` has at least max_pages * page_size positions (table_positions says how many).
  * seqs, counts, slots that may not be named twice, pages that may not be shared and status
  * bits as for cactus_hip_kv4_append_f16; where that writes nothing, rows of q_out are left

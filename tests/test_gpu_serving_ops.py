@@ -509,3 +509,258 @@ def test_rules_owner(hip_ready):
     for i, want in enumerate((S.rules(x[0], [5, 5, 9], 1.5, 0.25, 0.5, [(9, 2.0), (100, -3.0)], allowed), S.rules(x[1]))):
         np.testing.assert_array_equal(got[i], want[0])
         assert top[i] == want[1]
+
+
+# ------------------------------------------------------------------ far offsets
+def test_lora_behind_4_gb(hip_ready):
+    """An adapter whose weights lie behind 2^32 bytes, and rows that do."""
+    rng = np.random.default_rng(11)
+    cm = hip_ready
+    r, K, N, n = 256, 16384, 16384, 520                       # 8 MB of each per adapter
+    A, B, _ = adapters(rng, 1, r, K, N)
+    dA, dB = cm.DeviceBuffer(n * A.nbytes), cm.DeviceBuffer(n * B.nbytes)
+    for buf, a in ((dA, A), (dB, B)):
+        cm.call("cactus_hip_memcpy_h2d", buf.ptr + (n - 1) * a.nbytes, a.ctypes.data, a.nbytes, None)
+    ids = dev(cm, np.int32([n - 1, n - 1]))
+    for S, stride in ((1, 1 << 31), (20, 1 << 27)):
+        x, base = f16(rng, 2, S, K), f16(rng, 2, S, N)
+        big = cm.DeviceBuffer((2 * S - 1) * stride * 2 + 2 * (K + N))          # rows of x and of y, far from each other
+        for b in range(2):
+            for i in range(S):
+                row = np.concatenate((x[b, i], base[b, i]))
+                cm.call("cactus_hip_memcpy_h2d", big.ptr + (b * S + i) * stride * 2, row.ctypes.data, row.nbytes, None)
+        y_at = big.ptr + 2 * K
+        cm.call("cactus_hip_lora_add_f16", big.ptr, stride, dA.ptr, dB.ptr, None, n, r, ids.ptr, None, y_at, stride, y_at, stride,
+                2, S, K, N, None)
+        got = np.zeros((2, S, N), np.float16)
+        for b in range(2):
+            for i in range(S):
+                cm.call("cactus_hip_memcpy_d2h", got[b, i].ctypes.data, y_at + (b * S + i) * stride * 2, 2 * N, None)
+        check_lora(got, x, A, B, None, [0, 0], None, base)
+        big.free()
+
+
+def test_rules_behind_4_gb(hip_ready):
+    rng = np.random.default_rng(12)
+    cm, V, stride, n = hip_ready, 5003, (1 << 29) + 4, 4
+    from cactus_amd.logits import RulesDesc
+    x = (4 * rng.standard_normal((n, V))).astype(np.float32)
+    big = cm.DeviceBuffer(((n - 1) * stride + V) * 4)
+    for i in range(n):
+        cm.call("cactus_hip_memcpy_h2d", big.ptr + 4 * i * stride, x[i].ctypes.data, x[i].nbytes, None)
+    best, work = cm.DeviceBuffer(4 * n), dev(cm, np.zeros(4 * n, np.uint32))
+    mask = rng.integers(0, 1 << 32, -(-V // 32), dtype=np.uint64).astype(np.uint32)
+    dm, di = dev(cm, mask), dev(cm, np.zeros(n, np.int32))
+    d = RulesDesc(max_seqs=n, masks=dm.ptr, mask_ids=di.ptr, num_masks=1, mask_stride=len(mask))
+    cm.call("cactus_hip_logits_rules_f32", d.ref, None, big.ptr, stride, big.ptr, stride, best.ptr, n, V, work.ptr, 16 * n, None)
+    got = np.zeros(V, np.float32)
+    for i in range(n):
+        cm.call("cactus_hip_memcpy_d2h", got.ctypes.data, big.ptr + 4 * i * stride, 4 * V, None)
+        want, b = S.rules(x[i], mask=np.unpackbits(mask.view(np.uint8), bitorder="little")[:V] > 0)
+        np.testing.assert_array_equal(got, want)
+        assert best.to_numpy(np.uint32, n)[i] == b
+
+
+@pytest.mark.parametrize("n", [1, 200])
+def test_append_on_pages_behind_4_gb(hip_ready, n):
+    rng = np.random.default_rng(13)
+    cm, d, H, ps, pages = hip_ready, 256, 8, 4096, 480        # 9.4 MB per page
+    from cactus_amd.kv4 import KV4Cache
+    c = KV4Cache(1, H, d, ps, pages, 2, 2)
+    c.extend(1, n)
+    t = c.tables()
+    t["table"][0, 0] = pages - 1
+    c._buf["table"].upload(t["table"])
+    table = S.rope_table(2 * ps, d, 1e6)
+    dt, q, k, v = dev(cm, table), f16(rng, 1, n, 4, d), f16(rng, 1, n, H, d), f16(rng, 1, n, H, d)
+    dq, dk, dv, do = dev(cm, q), dev(cm, k), dev(cm, v), cm.DeviceBuffer(q.nbytes)
+    c.append_rope(0, dq.ptr, do.ptr, 4, dk.ptr, dv.ptr, 1, n, dt.ptr, 2 * ps)
+    ok, ov = cm.DeviceBuffer(k.nbytes), cm.DeviceBuffer(v.nbytes)
+    c.read(0, ok.ptr, ov.ptr, 1, n)
+    key = np.stack([S.rotated(k[0, i], None, 0, table[i])[0] for i in range(n)]).astype(np.float16)
+    for buf, want in ((ok, key), (ov, v[0])):
+        np.testing.assert_array_equal(buf.to_numpy(np.float16, want.shape).astype(np.float64), values(*quantize(want)).reshape(want.shape))
+
+
+# ------------------------------------------------------------------ streams, graphs, a whole step
+def test_calls_on_two_streams(hip_ready):
+    """Calls that overlap, each with its own workspace and outputs, give what they give alone."""
+    from cactus_amd.logits import RulesDesc
+    rng = np.random.default_rng(14)
+    cm, V, rows = hip_ready, 30011, 24
+    x = (4 * rng.standard_normal((2, rows, V))).astype(np.float16)
+    s = settings(rng, rows, V)
+    keep = [dev(cm, a) for a in (s["hist"], s["lens"], *(np.float32(p) for p in s["pen"]), *s["bias"], s["bias_counts"])]
+    d = RulesDesc(max_seqs=rows, history_stride=s["hist"].shape[1], bias_stride=s["bias"][0].shape[1],
+                  **dict(zip(("history", "history_lens", "repetition", "frequency", "presence", "bias_tokens", "bias_values", "bias_counts"),
+                             (b.ptr for b in keep))))
+    streams = [cm.Stream(), cm.Stream()]
+    bufs = [(dev(cm, x[i]), cm.DeviceBuffer(4 * rows * V), cm.DeviceBuffer(4 * rows), dev(cm, np.zeros(4 * rows, np.uint32))) for i in range(2)]
+    A, B, sc = adapters(rng, 3, 16, 512, 1024)
+    xs, base = f16(rng, 2, 9, 40, 512), f16(rng, 2, 9, 40, 1024)
+    w = [dev(cm, a) for a in (A, B, sc)]
+    ids = dev(cm, np.int32([0, 1, 2, -1, 0, 1, 2, 0, 1]))
+    lb = [(dev(cm, xs[i]), dev(cm, base[i]), cm.DeviceBuffer(base[i].nbytes)) for i in range(2)]
+    for _ in range(20):
+        for i in (0, 1):
+            a, o, b, work = bufs[i]
+            cm.call("cactus_hip_logits_rules_f16", d.ref, None, a.ptr, V, o.ptr, V, b.ptr, rows, V, work.ptr, 16 * rows, streams[i].handle)
+            a, z, y = lb[i]
+            cm.call("cactus_hip_lora_add_f16", a.ptr, 512, w[0].ptr, w[1].ptr, w[2].ptr, 3, 16, ids.ptr, None, z.ptr, 1024, y.ptr,
+                    1024, 9, 40, 512, 1024, streams[i].handle)
+    for i in (0, 1):
+        streams[i].sync()
+        got, top = bufs[i][1].to_numpy(np.float32, (rows, V)), bufs[i][2].to_numpy(np.uint32, rows)
+        for r in range(rows):
+            want, b = S.rules(x[i, r], s["hist"][r, :s["lens"][r]], *(p[r] for p in s["pen"]),
+                              list(zip(s["bias"][0][r, :s["bias_counts"][r]], s["bias"][1][r])))
+            np.testing.assert_array_equal(got[r], want)
+            assert top[r] == b
+        check_lora(lb[i][2].to_numpy(np.float16, (9, 40, 1024)), xs[i], A, B, sc, [0, 1, 2, -1, 0, 1, 2, 0, 1], None, base[i])
+
+
+class Step:
+    """A layer and the head of a small model for many sequences: the projections that requests share with their
+    adapters, the rotated append, attention over the pages, the logits and their rules."""
+    HID, HQ, H, D, V, R = 256, 4, 2, 64, 3001, 8
+
+    def __init__(self, cm, B, rng):
+        from cactus_amd.kv4 import KV4Cache
+        from cactus_amd.logits import LogitsRules
+        from cactus_amd.lora import LoraAdapters
+        self.cm, self.B = cm, B
+        n = (self.HQ + 2 * self.H) * self.D
+        self.qkv_w = rng.integers(-127, 128, (n, self.HID)).astype(np.int8)
+        self.qkv_s = (0.001 + 0.001 * rng.random((n, self.HID // 32))).astype(np.float16)
+        self.head = f16(rng, self.V, self.HQ * self.D, scale=0.2)
+        self.norms = [(1 + 0.3 * rng.standard_normal(self.D)).astype(np.float16) for _ in range(2)]
+        self.A, self.Bw, self.sc = adapters(rng, 3, self.R, self.HID, n)
+        self.lora = LoraAdapters(3, self.R, self.HID, n)
+        for i in range(3):
+            self.lora.set(i, self.A[i], self.Bw[i], self.sc[i])
+        self.ids = [i % 4 - 1 for i in range(B)]
+        self.cache = KV4Cache(1, self.H, self.D, 16, 12 * B, B, 10)
+        cm.call("cactus_hip_memset", self.cache._buf["pages"].ptr, 0, self.cache._buf["pages"].nbytes, None)
+        self.table = S.rope_table(160, self.D, 1e4)
+        self.rules = LogitsRules(B, self.V, 20, 3, 2)
+        self.hist = [rng.integers(0, self.V, i % 20) for i in range(B)]
+        self.allowed = rng.random(self.V) < 0.3
+        for i in range(B):
+            self.rules.set_history(i, self.hist[i])
+            self.rules.set_penalties(i, 1.3, 0.2, 0.1)
+        self.rules.set_bias(0, [5, 5], [3.0, 1.0])
+        self.rules.set_mask(1, self.allowed)
+        self.rules.use_mask(B - 1, 1)
+        self.d = {k: dev(cm, v) for k, v in dict(w=self.qkv_w, s=self.qkv_s, head=self.head, qn=self.norms[0], kn=self.norms[1],
+                                                 table=self.table, ids=np.int32(self.ids)).items()}
+
+    def buffers(self, S_):
+        n, B = (self.HQ + 2 * self.H) * self.D, self.B
+        size = dict(x=2 * B * S_ * self.HID, proj=2 * B * S_ * n, qkv=2 * B * S_ * n, q=2 * B * S_ * self.HQ * self.D,
+                    o=2 * B * S_ * self.HQ * self.D, logits=2 * B * self.V, out=4 * B * self.V, best=4 * B, counts=4 * B)
+        return {k: self.cm.DeviceBuffer(v) for k, v in size.items()}
+
+    def run(self, b, S_, stream=None):
+        cm, B, HQ, H, D = self.cm, self.B, self.HQ, self.H, self.D
+        n = (HQ + 2 * H) * D
+        self.cache.extend(B, 0, None, b["counts"].ptr, stream)
+        cm.call("cactus_hip_matmul_int8_f16act_noalloc", b["x"].ptr, self.d["w"].ptr, self.d["s"].ptr, b["proj"].ptr, B * S_, self.HID, n, 32, stream)
+        self.lora.add(b["x"].ptr, b["proj"].ptr, b["qkv"].ptr, self.d["ids"].ptr, B, S_, b["counts"].ptr, stream=stream)
+        self.cache.append_rope(0, b["qkv"].ptr, b["q"].ptr, HQ, b["qkv"].ptr + 2 * HQ * D, b["qkv"].ptr + 2 * (HQ + H) * D, B, S_,
+                               self.d["table"].ptr, 160, n, n, self.d["qn"].ptr, self.d["kn"].ptr, 1e-6, None, b["counts"].ptr, stream)
+        self.cache.attention(0, b["q"].ptr, b["o"].ptr, B, S_, HQ, counts=b["counts"].ptr, stream=stream)
+        if S_ == 1:
+            cm.call("cactus_hip_matmul_f16", b["o"].ptr, self.d["head"].ptr, b["logits"].ptr, B, HQ * D, self.V, stream)
+            self.rules.apply(b["logits"].ptr, b["out"].ptr, B, b["best"].ptr, stream=stream)
+
+
+def test_a_step_of_many_sequences(hip_ready):
+    """Prompts of different lengths, then single tokens: every stage against its restatement."""
+    rng = np.random.default_rng(15)
+    B = 7
+    s = Step(hip_ready, B, rng)
+    HQ, H, D = s.HQ, s.H, s.D
+    cpu = Model(1, H, D, 16, 12 * B, B, 10)
+    s.cache._buf["pages"].upload(cpu.pages)
+    for S_, counts in ((40, [40, 3, 17, 0, 25, 1, 33]), (1, [1] * B), (3, [3, 1, 2, 0, 3, 3, 1]), (1, [1, 1, 0, 1, 1, 1, 1])):
+        b = s.buffers(S_)
+        x = f16(rng, B, S_, s.HID)
+        b["x"].upload(x)
+        b["counts"].upload(np.int32(counts))
+        b["q"].upload(np.zeros((B, S_, HQ, D), np.float16))
+        b["o"].upload(np.zeros((B, S_, HQ, D), np.float16))
+        b["qkv"].upload(np.zeros((B, S_, (HQ + 2 * H) * D), np.float16))
+        s.run(b, S_)
+        assert s.cache.status() == 0 and cpu.extend(list(range(B)), counts) == 0
+        proj, qkv = (b[k].to_numpy(np.float16, (B, S_, HQ + 2 * H, D)) for k in ("proj", "qkv"))
+        q, o = (b[k].to_numpy(np.float16, (B, S_, HQ, D)) for k in ("q", "o"))
+        for i, m in enumerate(counts):
+            n = (HQ + 2 * H) * D
+            flat, before = qkv[i, :m].reshape(m, n), proj[i, :m].reshape(m, n)
+            if s.ids[i] < 0:
+                np.testing.assert_array_equal(flat, before)
+            elif m:
+                y, err = S.lora(x[i, :m], s.A[s.ids[i]], s.Bw[s.ids[i]], float(np.float32(s.sc[s.ids[i]])), before)
+                assert (np.abs(flat - y) <= err).all()
+            for r in range(m):
+                pos = int(cpu.lens[i]) - m + r
+                y, err = S.rotated(qkv[i, r, :HQ], s.norms[0], 1e-6, s.table[pos])
+                assert (np.abs(q[i, r] - y) <= S.half_step(y) + err).all()
+                key = S.rotated(qkv[i, r, HQ:HQ + H], s.norms[1], 1e-6, s.table[pos])[0].astype(np.float16)
+                cpu.write(0, i, pos, key, qkv[i, r, HQ + H:])
+            if m:
+                (kc, ks), (vc, vs) = cpu.read(0, i)
+                want, tol = attention(q[i, :m], kc, ks, vc, vs, len(kc), D ** -0.5)
+                assert (np.abs(o[i, :m] - want) <= tol).all()
+        np.testing.assert_array_equal(s.cache._buf["pages"].to_numpy(np.uint8, cpu.pages.shape), cpu.pages)
+        if S_ == 1:
+            logits, out, best = b["logits"].to_numpy(np.float16, (B, s.V)), b["out"].to_numpy(np.float32, (B, s.V)), b["best"].to_numpy(np.uint32, B)
+            for i in range(B):
+                want, top = S.rules(logits[i], s.hist[i], 1.3, 0.2, 0.1, [(5, 3.0), (5, 1.0)] if i == 0 else [], s.allowed if i == B - 1 else None)
+                np.testing.assert_array_equal(out[i], want)
+                assert best[i] == top
+
+
+def test_a_captured_step(hip_ready):
+    """The step as a graph, replayed while the sequences grow, other work in between: what the eager step gives."""
+    cm, B = hip_ready, 5
+    a, e = (Step(cm, B, np.random.default_rng(16)) for _ in range(2))
+    rng = np.random.default_rng(17)
+    st = cm.Stream()
+    ba, be, prompt = a.buffers(1), e.buffers(1), f16(rng, B, 20, a.HID)
+    for s in (a, e):
+        b = s.buffers(20)
+        b["x"].upload(prompt)
+        b["counts"].upload(np.int32([20, 1, 7, 16, 13]))
+        s.run(b, 20, st.handle)
+        st.sync()
+    # one eager step before the capture, so that scratch memory is there
+    xs = f16(rng, 9, B, 1, a.HID)
+    for s, b in ((a, ba), (e, be)):
+        b["counts"].upload(np.int32([1] * B))
+        b["x"].upload(xs[0])
+        s.run(b, 1, st.handle)
+        st.sync()
+    graph = ctypes.c_void_p()
+    cm.call("cactus_hip_graph_capture_begin", st.handle)
+    a.run(ba, 1, st.handle)
+    cm.call("cactus_hip_graph_capture_end", st.handle, ctypes.byref(graph))
+    for i, counts in enumerate([[1] * 5, [1, 0, 1, 1, 1], [1] * 5, [0, 0, 0, 1, 0], [1] * 5, [1] * 5, [1] * 5, [1] * 5]):
+        for b in (ba, be):
+            b["x"].upload(xs[i + 1])
+            b["counts"].upload(np.int32(counts))
+        cm.call("cactus_hip_graph_launch", graph, st.handle)
+        e.run(be, 1, None)                 # on another stream, at the same time
+        st.sync()
+        cm.call("cactus_hip_stream_sync", None)
+        assert a.cache.status(st.handle) == 0 and e.cache.status() == 0
+        for k, kind in (("q", np.uint16), ("o", np.uint16), ("out", np.uint32), ("best", np.uint32)):
+            n = ba[k].nbytes // np.dtype(kind).itemsize
+            got, want = ba[k].to_numpy(kind, n), be[k].to_numpy(kind, n)
+            rows = np.repeat(np.array(counts) > 0, n // B)      # (without a token: an old output's logits)
+            np.testing.assert_array_equal(got[rows], want[rows], err_msg=f"replay {i}: {k}")
+        for name, v in a.cache.tables().items():
+            np.testing.assert_array_equal(v, e.cache.tables()[name])
+        size = a.cache._buf["pages"].nbytes
+        np.testing.assert_array_equal(a.cache._buf["pages"].to_numpy(np.uint8, size), e.cache._buf["pages"].to_numpy(np.uint8, size))
+    cm.call("cactus_hip_graph_destroy", graph)

@@ -42,7 +42,7 @@ def append(lib, desc=None, layer=0, **kw):
     (dict(q_stride=516), b"aligned"), (dict(q_norm=8), b"aligned"), (dict(k_norm=4100), b"aligned"), (dict(table=4104), b"aligned"),
     (dict(kv_stride=248), b"kv_stride"), (dict(q_stride=504), b"q_stride"), (dict(eps=-1.0), b"eps"),
     (dict(eps=float("nan")), b"eps"), (dict(eps=float("inf")), b"eps"), (dict(positions=255), b"table_positions"),
-    (dict(batch=5), b"slots"), (dict(seq_len=1 << 28), b"seq_len"), (dict(heads=1 << 17), b"num_q_heads"),
+    (dict(batch=5), b"slots"), (dict(seq_len=1 << 28), b"seq_len"), (dict(heads=16385), b"num_q_heads"),
     (dict(q=4096, q_out=4096, q_stride=520), b"in place")])
 def test_append_refusals(lib, kw, text):
     refused(lib, append(lib, **kw), text)
@@ -91,7 +91,7 @@ def lora(lib, **kw):
     (dict(B=4104), b"aligned"), (dict(base=4104), b"aligned"), (dict(y=4104), b"aligned"), (dict(x_stride=68), b"aligned"),
     (dict(x_stride=56), b"stride"), (dict(base_stride=120), b"stride"), (dict(y_stride=120), b"stride"),
     (dict(y=4096, y_stride=136), b"in place"), (dict(batch=65536), b"batch"), (dict(seq_len=1 << 24), b"seq_len"),
-    (dict(n=1 << 24), b"num_adapters")])
+    (dict(n=1 << 24), b"num_adapters"), (dict(batch=65535, seq_len=1 << 20), b"batch times seq_len")])
 def test_lora_refusals(lib, kw, text):
     refused(lib, lora(lib, **kw), text)
 
@@ -114,7 +114,7 @@ def call_rules(lib, half=True, change=(), **kw):
 
 @pytest.mark.parametrize("half", [True, False])
 @pytest.mark.parametrize("change,kw,text", [
-    (dict(max_seqs=0), {}, b"max_seqs"), (dict(history_stride=1 << 31), {}, b"history_stride"),
+    (dict(max_seqs=0), {}, b"max_seqs"), (dict(history_stride=1 << 20), {}, b"history_stride"),
     (dict(bias_stride=1025), {}, b"bias_stride"), (dict(bias_values=None), {}, b"without values"),
     (dict(mask_stride=3), {}, b"mask_stride"), (dict(mask_ids=None, num_masks=5), {}, b"mask"), ({}, dict(batch=65536, size=1 << 21), b"65535"),
     ({}, dict(vocab=1 << 28, stride=1 << 28, out_stride=1 << 28), b"mask_stride"), ({}, dict(logits=None), b"null pointer"),
@@ -157,6 +157,51 @@ def test_rules_owner_checks(monkeypatch):
                 lambda: L.LogitsRules(1, 50).set_history(0, [1])):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_rules_owner_takes_integers(monkeypatch):
+    from cactus_amd import logits as L
+
+    class Buffer:
+        def __init__(self, n):
+            self.nbytes, self.ptr = n, 1 << 20
+
+        @classmethod
+        def from_numpy(cls, a, stream=None):
+            return cls(a.nbytes)
+    monkeypatch.setattr(L, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(L, "call", lambda name, *a: None)
+    r = L.LogitsRules(4, 50, max_history=8, max_bias=2)
+    for bad in ([1.5], np.array([1 << 32]), [1 << 31], [True]):
+        with pytest.raises(TypeError):
+            r.set_history(0, bad)
+        with pytest.raises(TypeError):
+            r.set_bias(0, bad, [1.0])
+    r.set_history(0, [])
+    r.set_history(0, np.arange(8, dtype=np.uint8))
+
+
+def test_lora_owner_checks(monkeypatch):
+    from cactus_amd import lora as L
+    sent = []
+
+    class Buffer:
+        def __init__(self, n):
+            self.nbytes, self.ptr = n, 1 << 20
+    monkeypatch.setattr(L, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(L, "call", lambda name, *a: sent.append((name, *a)))
+    a = L.LoraAdapters(3, 16, 32, 24)
+    sent.clear()
+    a.set(2, np.ones((4, 32)), np.ones((24, 4)), 0.5)
+    assert [(s[1] - (1 << 20), s[3]) for s in sent] == [(2 * 16 * 32 * 2, 16 * 32 * 2), (2 * 16 * 24 * 2, 16 * 24 * 2), (8, 4)]
+    with pytest.raises(IndexError):
+        a.set(3, np.ones((4, 32)), np.ones((24, 4)))
+    for A, B in (((17, 32), (24, 17)), ((4, 31), (24, 4)), ((4, 32), (24, 5)), ((4, 32), (23, 4)), ((32,), (24, 1))):
+        with pytest.raises(ValueError):
+            a.set(0, np.ones(A), np.ones(B))
+    for bad in ((3, 12, 32, 24), (3, 0, 32, 24), (3, 264, 32, 24), (3, 8, 30, 24), (3, 8, 32, 20)):
+        with pytest.raises(ValueError):
+            L.LoraAdapters(*bad)
 
 
 def test_rules_restated():
