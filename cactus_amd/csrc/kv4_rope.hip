@@ -281,9 +281,9 @@ __global__ void __launch_bounds__(64 * TILE_WAVES, 3) kv4_rope_tile_kernel(RopeA
                 uint16_t* dst = a.q_out + (row * a.Hq + item) * D + 8 * j;
 #pragma unroll
                 for (int u = 0; u < 2; u++)
-                    *reinterpret_cast<u32x4*>(dst + u * (D / 2)) =
-                        (u32x4){r[u][0] | (uint32_t)r[u][1] << 16, r[u][2] | (uint32_t)r[u][3] << 16,
-                                r[u][4] | (uint32_t)r[u][5] << 16, r[u][6] | (uint32_t)r[u][7] << 16};
+                    __builtin_nontemporal_store((u32x4){r[u][0] | (uint32_t)r[u][1] << 16, r[u][2] | (uint32_t)r[u][3] << 16,
+                                r[u][4] | (uint32_t)r[u][5] << 16, r[u][6] | (uint32_t)r[u][7] << 16},
+                                                reinterpret_cast<u32x4*>(dst + u * (D / 2)));
             }
             continue;
         }

@@ -64,12 +64,11 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(RulesArgs a) {
         const int t = c0 + 8 * (tid + THREADS * g);
         if (vec && t >= 0 && t + 8 <= a.V) {
             if constexpr (sizeof(T) == 2) {
-                const uint4 u = *reinterpret_cast<const uint4*>(in + t);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                const i32x4 w = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(in + t));
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[g][j] = h2f((uint16_t)(w[j / 2] >> 16 * (j & 1)));
+                for (int j = 0; j < 8; j++) x[g][j] = h2f((uint16_t)((uint32_t)w[j / 2] >> 16 * (j & 1)));
             } else {
-                const f32x4 u = *reinterpret_cast<const f32x4*>(in + t), v = *reinterpret_cast<const f32x4*>(in + t + 4);
+                const f32x4 u = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(in + t)), v = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(in + t + 4));
 #pragma unroll
                 for (int j = 0; j < 4; j++) x[g][j] = u[j], x[g][4 + j] = v[j];
             }
@@ -191,8 +190,8 @@ __global__ void __launch_bounds__(THREADS) logits_rules_kernel(RulesArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; j++) x[g][j] = bits[g] >> j & 1 ? x[g][j] : -__builtin_inff();
         if (vec && t >= 0 && t + 8 <= a.V) {
-            *reinterpret_cast<f32x4*>(out + t) = (f32x4){x[g][0], x[g][1], x[g][2], x[g][3]};
-            *reinterpret_cast<f32x4*>(out + t + 4) = (f32x4){x[g][4], x[g][5], x[g][6], x[g][7]};
+            __builtin_nontemporal_store((f32x4){x[g][0], x[g][1], x[g][2], x[g][3]}, reinterpret_cast<f32x4*>(out + t));
+            __builtin_nontemporal_store((f32x4){x[g][4], x[g][5], x[g][6], x[g][7]}, reinterpret_cast<f32x4*>(out + t + 4));
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (x[g][j] > most) most = x[g][j], at = t + j;

@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(64 * W) lora_tile_kernel(LoraArgs a) {
                            (uint32_t)f2h(__builtin_fmaf(e1, scale, h2f((uint16_t)(w[q] >> 16)))) << 16;
                 }
                 if (16 * t + r < rows && n < n_hi)
-                    *reinterpret_cast<u32x4*>(y + (size_t)(16 * t + r) * a.y_stride + n) = (u32x4){o[0], o[1], o[2], o[3]};
+                    __builtin_nontemporal_store((u32x4){o[0], o[1], o[2], o[3]}, reinterpret_cast<u32x4*>(y + (size_t)(16 * t + r) * a.y_stride + n));
             }
         }
     }
