@@ -90,7 +90,7 @@ __device__ __forceinline__ uint16_t kv4_scale(uint32_t abits) {
 }
 // code + 8 in the low byte of the result; inv: 1 / s, 0 where every code is 0
 __device__ __forceinline__ uint32_t kv4_code(uint16_t x, float inv) {
-    const float v = (h2f(x) * inv + 768.0f) - 768.0f;    // a multiple of 2^-14 (|v| < 16)
+    const float v = __builtin_fmaf(h2f(x), inv, 768.0f) - 768.0f;    // a multiple of 2^-14 (|v| < 16)
     const float w = __builtin_amdgcn_fmed3f(v, -7.0f, 7.0f);
     return __builtin_bit_cast(uint32_t, w + 12582920.0f);  // 3 2^22 + 8: the integer in the low bits
 }

@@ -3,10 +3,18 @@
 //
 //   y = x / sqrt(mean(x^2) + eps) w,   halves a, b of y at position p:
 //   a cos(p f_i) - b sin(p f_i),  b cos(p f_i) + a sin(p f_i)
-// Queries and keys are computed in 64 bits and rounded once, to FP16.  For the
-// keys that keeps the 4-bit codes what the formula says: an FP32 sum that falls
-// on the other side of an FP16 value's border moves a key by 2^-11, and where
-// that crosses the border of two codes, by a seventh of its group's largest.
+// Keys are computed in 64 bits and rounded once, to FP16, which keeps their 4-bit
+// codes what the formula says: an FP32 sum that falls on the other side of an
+// FP16 value's border moves a key by 2^-11, and where that crosses the border of
+// two codes, by a seventh of its group's largest.  Queries have no codes: 64 bits
+// where a wave has one row, 32 where it has many, rounded once too.
+//
+// Single rows are bound by the chain of loads (length, position, rotation and page), prompts by
+// memory with the vector units 60% busy.  Four prompts of up to 2048 rows, 16 query and 8 KV
+// heads of 128 dims with norms: 25.9 us, 84 MB, 3.2 TB/s (16 more query heads add 48.8 MB in
+// 10 us, 4.9 TB/s; the keys' 64-bit sums are what the rest waits for).  64 single rows 3.4 us,
+// one row of 4 and 1 heads of 256 dims 3.4.  Queries go past the caches: 39.9 -> 38.4 us with the
+// read of the keys and values.
 #include "kv4_device.h"
 
 namespace cactus_hip {
@@ -249,40 +257,38 @@ __global__ void __launch_bounds__(64 * TILE_WAVES, 3) kv4_rope_tile_kernel(RopeA
             w[0] = *reinterpret_cast<const u32x4*>(norm + 8 * j);
             w[1] = *reinterpret_cast<const u32x4*>(norm + D / 2 + 8 * j);
         }
-        float xf[2][8], xw[2][8];
+        const auto xh = [&](int u, int i) { return h2f((uint16_t)(x[u][i / 2] >> 16 * (i & 1))); };
+        float xw[2][8];                           // times the weights, exact (fma_mix takes FP16 operands as they are)
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                xf[u][i] = h2f((uint16_t)(x[u][i / 2] >> 16 * (i & 1)));
-                xw[u][i] = xf[u][i] * h2f((uint16_t)(w[u][i / 2] >> 16 * (i & 1)));       // (exact)
-            }
+            for (int i = 0; i < 8; i++) xw[u][i] = __builtin_fmaf(xh(u, i), h2f((uint16_t)(w[u][i / 2] >> 16 * (i & 1))), -0.0f);
         if (item < a.Hq) {
             // in 32 bits: an FP16 result has no border that 2^-22 beside it matters for
             float f = 1.0f;
             if (norm) {
                 float ss = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) ss = __builtin_fmaf(xf[0][i], xf[0][i], __builtin_fmaf(xf[1][i], xf[1][i], ss));
+                for (int i = 0; i < 8; i++) ss = __builtin_fmaf(xh(0, i), xh(0, i), __builtin_fmaf(xh(1, i), xh(1, i), ss));
                 ss += dpp_move_keep<0xB1>(ss);
                 ss += dpp_move_keep<0x4E>(ss);
                 if constexpr (LPT >= 8) ss += dpp_move_keep<0x141>(ss);
                 if constexpr (LPT >= 16) ss += dpp_move_keep<0x140>(ss);
-                f = 1.0f / sqrtf(ss * (1.0f / D) + (float)a.eps);
+                f = __builtin_amdgcn_rsqf(ss * (1.0f / D) + (float)a.eps);
             }
-            uint16_t r[2][8];
+            h16x2 r[2][4];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float u = xw[0][i] * f, v = xw[1][i] * f;
-                r[0][i] = f2h(__builtin_fmaf(u, co[i], -(v * si[i])));
-                r[1][i] = f2h(__builtin_fmaf(v, co[i], u * si[i]));
+                const float cf = co[i] * f, sf = si[i] * f;
+                r[0][i / 2][i & 1] = (_Float16)__builtin_fmaf(xw[0][i], cf, -(xw[1][i] * sf));
+                r[1][i / 2][i & 1] = (_Float16)__builtin_fmaf(xw[1][i], cf, xw[0][i] * sf);
             }
             if (mine) {
                 uint16_t* dst = a.q_out + (row * a.Hq + item) * D + 8 * j;
 #pragma unroll
                 for (int u = 0; u < 2; u++)
-                    __builtin_nontemporal_store((u32x4){r[u][0] | (uint32_t)r[u][1] << 16, r[u][2] | (uint32_t)r[u][3] << 16,
-                                r[u][4] | (uint32_t)r[u][5] << 16, r[u][6] | (uint32_t)r[u][7] << 16},
+                    __builtin_nontemporal_store((u32x4){__builtin_bit_cast(uint32_t, r[u][0]), __builtin_bit_cast(uint32_t, r[u][1]),
+                                                        __builtin_bit_cast(uint32_t, r[u][2]), __builtin_bit_cast(uint32_t, r[u][3])},
                                                 reinterpret_cast<u32x4*>(dst + u * (D / 2)));
             }
             continue;
@@ -293,7 +299,7 @@ __global__ void __launch_bounds__(64 * TILE_WAVES, 3) kv4_rope_tile_kernel(RopeA
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) ss += (double)(xf[u][i] * xf[u][i]);       // (exact in FP32)
+                for (int i = 0; i < 8; i++) ss += (double)__builtin_fmaf(xh(u, i), xh(u, i), 0.0f);      // (exact in FP32)
             ss += dpp_f64<0xB1>(ss);
             ss += dpp_f64<0x4E>(ss);
             if constexpr (LPT >= 8) ss += dpp_f64<0x141>(ss);
