@@ -275,8 +275,7 @@ __global__ void __launch_bounds__(64 * W) lora_tile_kernel(LoraArgs a) {
                 const f32x4 d0 = *reinterpret_cast<const f32x4*>(own_d + r * DS + j % LPR * 8);
                 const f32x4 d1 = *reinterpret_cast<const f32x4*>(own_d + r * DS + j % LPR * 8 + 4);
                 const float unlift = back[16 * t + r];
-                const u32x4 u = bc[BJ / RT * t + i];
-                const u32x4 w = u;
+                const u32x4 w = bc[BJ / RT * t + i];
                 uint32_t o[4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
