@@ -446,7 +446,7 @@ extern "C" int cactus_hip_lora_add_f16(const uint16_t* x, size_t x_stride, const
     CH_REQUIRE(num_adapters < (1u << 24), "lora_add: num_adapters out of range");
     CH_REQUIRE(batch <= 65535 && seq_len < (1u << 24), "lora_add: batch or seq_len out of range");
     if (batch == 0 || seq_len == 0 || N == 0) return CACTUS_HIP_OK;
-    CH_REQUIRE(adapters && base && y && (num_adapters == 0 || (A && B && x) || K == 0), "lora_add: null pointer");
+    CH_REQUIRE(adapters && base && y && (num_adapters == 0 || (B && ((A && x) || K == 0))), "lora_add: null pointer");
     const auto aligned = [](const void* p, size_t stride) { return ((uintptr_t)p & 15) == 0 && stride % 8 == 0; };
     CH_REQUIRE(aligned(x, x_stride) && aligned(A, 0) && aligned(B, 0) && aligned(base, base_stride) && aligned(y, y_stride),
                "lora_add: rows are not 16-byte aligned");

@@ -96,6 +96,12 @@ def test_lora_refusals(lib, kw, text):
     refused(lib, lora(lib, **kw), text)
 
 
+@pytest.mark.parametrize("S", [1, 3, 100])
+def test_lora_without_inputs_needs_its_second_weights(lib, S):
+    """K 0: A and x may be missing, but the outputs' product still reads B."""
+    refused(lib, lora(lib, K=0, x_stride=0, x=None, A=None, B=None, seq_len=S), b"null pointer")
+
+
 def test_lora_without_rows_does_nothing(lib):
     assert lora(lib, batch=0) == 0 and lora(lib, seq_len=0) == 0 and lora(lib, N=0) == 0
 
