@@ -451,6 +451,7 @@ extern "C" int cactus_hip_lora_add_f16(const uint16_t* x, size_t x_stride, const
     CH_REQUIRE(aligned(x, x_stride) && aligned(A, 0) && aligned(B, 0) && aligned(base, base_stride) && aligned(y, y_stride),
                "lora_add: rows are not 16-byte aligned");
     CH_REQUIRE(x_stride >= K && base_stride >= N && y_stride >= N, "lora_add: a stride is shorter than its row");
+    CH_REQUIRE(y != x || num_adapters == 0 || K == 0, "lora_add: y in place of x, which other workgroups still read");
     CH_REQUIRE(y != base || y_stride == base_stride, "lora_add: y in place of base needs its stride");
     LoraArgs a{x,        A,           B,        scales, adapters, counts, base, y, x_stride, base_stride, y_stride, (int)num_adapters,
                (int)rank, (int)batch, (int)seq_len, (int)K, (int)N, 0, 0, 0};

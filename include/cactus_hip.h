@@ -174,8 +174,8 @@ int cactus_hip_matmul_int4_f16act_batched(const uint16_t* A, const uint8_t* B_pa
  * fp16 (rows = outputs, like every weight here); scales [num_adapters] f32 (NULL: 1);
  * adapters [batch] on the device, any number outside [0, num_adapters): none, y =
  * base.  counts (device, NULL: seq_len each): the first counts[i] rows of request i are
- * there, the others are not read and left as they were.  y may be base (with its stride);
- * otherwise y overlaps no input.  rank: a multiple of 8 up to 256 (adapters of lower
+ * there, the others are not read and left as they were.  y may be base (with its stride),
+ * but not x; otherwise y overlaps no input.  rank: a multiple of 8 up to 256 (adapters of lower
  * rank are padded with zeros); K and N multiples of 8; rows 16-byte aligned.  A NaN or
  * an infinity in a row of x or base stays in that row of y. */
 int cactus_hip_lora_add_f16(const uint16_t* x, size_t x_stride, const uint16_t* A, const uint16_t* B,

@@ -102,6 +102,13 @@ def test_lora_without_inputs_needs_its_second_weights(lib, S):
     refused(lib, lora(lib, K=0, x_stride=0, x=None, A=None, B=None, seq_len=S), b"null pointer")
 
 
+@pytest.mark.parametrize("S", [1, 3, 100])
+@pytest.mark.parametrize("base", [4096, 16384])
+def test_lora_refuses_outputs_in_place_of_x(lib, S, base):
+    """Workgroups that share a row read all of x: one would overwrite what another still reads."""
+    refused(lib, lora(lib, K=64, N=64, x=4096, y=4096, base=base, x_stride=64, base_stride=64, y_stride=64, seq_len=S), b"place of x")
+
+
 def test_lora_without_rows_does_nothing(lib):
     assert lora(lib, batch=0) == 0 and lora(lib, seq_len=0) == 0 and lora(lib, N=0) == 0
 
