@@ -11,7 +11,8 @@ MAX_RANK = 256
 
 class LoraAdapters:
     """Adapters of one projection [N][K]: up to `count` of them, of any rank up to `rank` (a multiple of 8; lower
-    ranks are padded with zeros).  An adapter that was never set adds nothing.  `stream` is a Stream's handle."""
+    ranks are padded with zeros).  An adapter that was never set adds nothing.  `stream` is a Stream's handle; the
+    constructor waits for it, so that calls may follow on any stream."""
 
     def __init__(self, count: int, rank: int, K: int, N: int, stream=None):
         if rank % 8 or not 8 <= rank <= MAX_RANK:
@@ -22,6 +23,7 @@ class LoraAdapters:
         self._A, self._B, self._scales = DeviceBuffer(2 * count * rank * K), DeviceBuffer(2 * count * N * rank), DeviceBuffer(4 * count)
         for b in (self._A, self._B, self._scales):
             call("cactus_hip_memset", b.ptr, 0, b.nbytes, stream)
+        call("cactus_hip_stream_sync", stream)      # calls on other streams are not ordered behind the fills
 
     def set(self, i: int, A, B, scale: float = 1.0, stream=None):
         """A [r][K] and B [N][r], r at most the rank: y += scale * B (A x).  Waits for the stream."""

@@ -217,6 +217,25 @@ def test_lora_owner_checks(monkeypatch):
             L.LoraAdapters(*bad)
 
 
+def test_lora_owner_waits_for_its_first_weights(monkeypatch):
+    """The zeros that the adapters start with are there when the owner is: a call on another stream, the
+    upload of an adapter among them, is not ordered behind a fill that is still on its way."""
+    from cactus_amd import lora as L
+    sent = []
+
+    class Buffer:
+        def __init__(self, n):
+            self.nbytes, self.ptr = n, 1 << 20
+    monkeypatch.setattr(L, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(L, "call", lambda name, *a: sent.append((name, a)))
+    for stream in (None, 77):
+        sent.clear()
+        L.LoraAdapters(3, 16, 32, 24, stream)
+        fills = [i for i, (name, a) in enumerate(sent) if name == "cactus_hip_memset" and a[-1] == stream]
+        assert len(fills) == 3
+        assert sent[-1] == ("cactus_hip_stream_sync", (stream,)) and fills[-1] < len(sent) - 1
+
+
 def test_rules_restated():
     x = np.array([2.0, -2.0, 1.0, 0.0, 3.0], np.float32)
     y, best = S.rules(x, hist=[0, 1, 1, -1, 7], rep=2.0, freq=0.5, pres=0.25, bias=[(3, 4.0), (3, -1.0), (9, 1.0)])
