@@ -52,6 +52,7 @@ class KV4Cache:
             setattr(self.desc, name, b.ptr)
         self._work = {}
         self.reset(stream)
+        self.status(stream)      # waits: calls on other streams are not ordered behind the reset
 
     def _lst(self, v, n: int, stream=None):
         """A device pointer as it is; a sequence of n ints or more uploaded, for the call that it is made for."""
@@ -122,10 +123,12 @@ class KV4Cache:
                    eps, table, table_positions, batch, seq_len, stream=stream)
 
     def rope_table(self, theta: float, stream=None) -> DeviceBuffer:
-        """The rotations of every position that a slot can have, max_pages * page_size of them, for append_rope."""
+        """The rotations of every position that a slot can have, max_pages * page_size of them, for append_rope.
+        Waits for the stream, so that any stream may read the table."""
         n, d = self.desc.max_pages * self.desc.page_size, self.desc.head_dim
         table = DeviceBuffer(4 * n * d)
         call("cactus_hip_rope_table_f32", table.ptr, n, d, theta, stream)
+        call("cactus_hip_stream_sync", stream)
         return table
 
     def read(self, layer: int, k: int, v: int, batch: int, seq_len: int, seqs=None, starts=None, counts=None, stream=None):

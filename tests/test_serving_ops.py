@@ -74,6 +74,29 @@ def test_rotation_restated():
     assert np.allclose(at(q, 17) @ at(k, 5), at(q, 40) @ at(k, 28), atol=64 * 2.0 ** -22 * np.abs(q).max() * np.abs(k).max())
 
 
+def test_cache_owner_waits_for_what_it_sets_up(monkeypatch):
+    """Tables and rotations that the owner makes are there when it returns them: other streams' calls are not ordered
+    behind the kernels that fill them."""
+    from cactus_amd import kv4
+    sent = []
+
+    class Buffer:
+        def __init__(self, n):
+            self.nbytes, self.ptr = n, 1 << 20
+    monkeypatch.setattr(kv4, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(kv4, "call", lambda name, *a: sent.append((name, a)))
+    waits = ("cactus_hip_stream_sync", "cactus_hip_kv4_status")      # (the status waits for the stream)
+    for stream in (None, 77):
+        sent.clear()
+        c = kv4.KV4Cache(1, 1, 64, 16, 8, 4, 4, stream)
+        names = [n for n, a in sent if a[-1] == stream]
+        assert "cactus_hip_kv4_reset" in names and names[-1] in waits
+        sent.clear()
+        c.rope_table(1e4, stream)
+        names = [n for n, a in sent if a[-1] == stream]
+        assert "cactus_hip_rope_table_f32" in names and names[-1] in waits
+
+
 # ------------------------------------------------------------------ adapters
 def lora(lib, **kw):
     a = dict(x=4096, x_stride=64, A=4096, B=4096, scales=None, n=3, rank=16, ids=4096, counts=None, base=4096, base_stride=128,
