@@ -97,10 +97,12 @@ class LogitsRules:
         if best is not None:
             size = hip().cactus_hip_logits_rules_workspace(batch)
             kept = self._work.setdefault(stream or 0, [])
-            if not kept or kept[-1].nbytes < size:
+            last = kept[-1] if kept else None
+            if last is None or last.nbytes < size:
                 # a smaller one stays: a captured graph may hold its address
-                kept.append(DeviceBuffer(size))
-                call("cactus_hip_memset", kept[-1].ptr, 0, size, stream)
-            work, size = kept[-1].ptr, kept[-1].nbytes
+                last = DeviceBuffer(size)
+                call("cactus_hip_memset", last.ptr, 0, size, stream)
+                kept.append(last)
+            work, size = last.ptr, last.nbytes
         call("cactus_hip_logits_rules_f32" if fp32 else "cactus_hip_logits_rules_f16", self.desc.ref, seqs, logits,
              stride or self.vocab, out, out_stride or self.vocab, best, batch, self.vocab, work, size, stream)

@@ -195,6 +195,44 @@ def test_rules_owner_checks(monkeypatch):
             bad()
 
 
+def test_rules_owner_keeps_scratch_memory_once_it_is_zero(monkeypatch):
+    """A workspace is kept for later calls only behind its fill: not where that fails, and not for another
+    thread's call in between."""
+    from cactus_amd import logits as L
+
+    class Buffer:
+        made = 0
+
+        def __init__(self, n):
+            Buffer.made += 1
+            self.nbytes, self.ptr = n, Buffer.made << 20
+    monkeypatch.setattr(L, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(L, "hip", lambda: type("Lib", (), {"cactus_hip_logits_rules_workspace": staticmethod(lambda n: 16 * n)}))
+    filled, used, during = set(), [], []
+
+    def call(name, *a):
+        if name == "cactus_hip_memset":
+            if during:
+                during.pop()()
+            filled.add(a[0])
+        else:
+            used.append(a[-3])
+            assert used[-1] in filled, "scratch memory that is not zero"
+    monkeypatch.setattr(L, "call", call)
+
+    def fail():
+        raise RuntimeError("refused")
+    r = L.LogitsRules(4, 50)
+    during.append(fail)
+    with pytest.raises(RuntimeError):
+        r.apply(4096, 8192, 4, 4096)
+    r.apply(4096, 8192, 4, 4096)
+    during.append(lambda: r.apply(4096, 8192, 8, 4096, stream=5))
+    r.apply(4096, 8192, 8, 4096, stream=5)
+    r.apply(4096, 8192, 2, 4096, stream=5)
+    assert len(used) == 4
+
+
 def test_rules_owner_takes_integers(monkeypatch):
     from cactus_amd import logits as L
 
