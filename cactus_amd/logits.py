@@ -33,7 +33,7 @@ class LogitsRules:
         self.vocab, words = vocab, -(-vocab // 32)
         self.desc = RulesDesc(history_stride=max_history, bias_stride=max_bias, num_masks=num_masks, mask_stride=words,
                               max_seqs=max_seqs)
-        self._buf, self._work = {}, {}
+        self._buf, self._part, self._work = {}, {}, {}
         start = {}
         if max_history:
             start.update(history=np.full((max_seqs, max_history), -1, np.int32), history_lens=np.zeros(max_seqs, np.int32),
@@ -46,35 +46,38 @@ class LogitsRules:
             start.update(masks=np.full((num_masks, words), 0xFFFFFFFF, np.uint32), mask_ids=np.full(max_seqs, -1, np.int32))
         for name, a in start.items():
             self._buf[name] = DeviceBuffer.from_numpy(a, stream)
+            self._part[name] = a.dtype.type, a.shape[1] if a.ndim > 1 else 1
             setattr(self.desc, name, self._buf[name].ptr)
 
-    def _put(self, name: str, slot: int, values, dtype, stride: int, stream, rows: int | None = None):
-        a = np.asarray(values)
-        if np.issubdtype(dtype, np.integer) and a.size and (a.dtype.kind not in "iu" or a.min() < np.iinfo(dtype).min or a.max() > np.iinfo(dtype).max):
-            raise TypeError(f"{name}: 32-bit integers are needed")
-        a = np.ascontiguousarray(a, dtype)
+    def _put(self, slot: int, stream, rows: int | None = None, **parts):
+        """Uploads a slot's (or a mask's) part of each named array; checks all of them first."""
         if not 0 <= slot < (self.desc.max_seqs if rows is None else rows):
             raise IndexError(f"no slot or mask {slot}")
-        if name not in self._buf or a.size > stride:
-            raise ValueError(f"{name}: room for {stride if name in self._buf else 0} values, {a.size} given")
-        if a.size:
-            call("cactus_hip_memcpy_h2d", self._buf[name].ptr + 4 * slot * stride, a.ctypes.data, a.nbytes, stream)
-        return a.size
+        ready = []
+        for name, values in parts.items():
+            kind, stride = self._part.get(name, (None, 0))
+            a = np.asarray(values)
+            if kind is None or a.size > stride:
+                raise ValueError(f"{name}: room for {stride} values, {a.size} given")
+            if a.size and kind != np.float32 and (a.dtype.kind not in "iu" or a.min() < np.iinfo(kind).min or a.max() > np.iinfo(kind).max):
+                raise TypeError(f"{name}: 32-bit integers are needed")
+            if a.size and kind == np.float32 and a.dtype.kind not in "fiub":
+                raise TypeError(f"{name}: numbers are needed")
+            ready.append((self._buf[name].ptr + 4 * slot * stride, np.ascontiguousarray(a, kind)))
+        for ptr, a in ready:
+            if a.size:
+                call("cactus_hip_memcpy_h2d", ptr, a.ctypes.data, a.nbytes, stream)
 
     def set_history(self, slot: int, tokens, stream=None):
-        n = self._put("history", slot, tokens, np.int32, self.desc.history_stride, stream)
-        self._put("history_lens", slot, [n], np.int32, 1, stream)
+        self._put(slot, stream, history=tokens, history_lens=[np.size(tokens)])
 
     def set_penalties(self, slot: int, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0, stream=None):
-        for name, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-            self._put(name, slot, [v], np.float32, 1, stream)
+        self._put(slot, stream, repetition=[repetition], frequency=[frequency], presence=[presence])
 
     def set_bias(self, slot: int, tokens, values, stream=None):
-        if len(tokens) != len(values):
-            raise ValueError(f"{len(tokens)} tokens, {len(values)} values")
-        n = self._put("bias_tokens", slot, tokens, np.int32, self.desc.bias_stride, stream)
-        self._put("bias_values", slot, values, np.float32, self.desc.bias_stride, stream)
-        self._put("bias_counts", slot, [n], np.int32, 1, stream)
+        if np.size(tokens) != np.size(values):
+            raise ValueError(f"{np.size(tokens)} tokens, {np.size(values)} values")
+        self._put(slot, stream, bias_tokens=tokens, bias_values=values, bias_counts=[np.size(tokens)])
 
     def set_mask(self, mask: int, allowed, stream=None):
         """allowed: a truth value per token."""
@@ -82,11 +85,11 @@ class LogitsRules:
         if a.shape != (self.vocab,):
             raise ValueError(f"{self.vocab} truth values are needed")
         bits = np.packbits(np.pad(a, (0, -len(a) % 32)), bitorder="little").view(np.uint32)
-        self._put("masks", mask, bits, np.uint32, self.desc.mask_stride, stream, self.desc.num_masks)
+        self._put(mask, stream, self.desc.num_masks, masks=bits)
 
     def use_mask(self, slot: int, mask: int, stream=None):
-        """Mask number `mask` for the slot; -1: none."""
-        self._put("mask_ids", slot, [mask], np.int32, 1, stream)
+        """Mask number `mask` for the slot; -1: none; num_masks or more: no token is allowed."""
+        self._put(slot, stream, mask_ids=[mask])
 
     def apply(self, logits: int, out: int, batch: int, best: int | None = None, fp32: bool = False, stride: int | None = None,
               out_stride: int | None = None, seqs: int | None = None, stream=None):

@@ -255,6 +255,38 @@ def test_rules_owner_takes_integers(monkeypatch):
     r.set_history(0, np.arange(8, dtype=np.uint8))
 
 
+def test_rules_owner_changes_a_setting_whole_or_not_at_all(monkeypatch):
+    """Every part of a setting is checked before the first is uploaded."""
+    from cactus_amd import logits as L
+    sent = []
+
+    class Buffer:
+        def __init__(self, n):
+            self.nbytes, self.ptr = n, 1 << 20
+
+        @classmethod
+        def from_numpy(cls, a, stream=None):
+            return cls(a.nbytes)
+    monkeypatch.setattr(L, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(L, "call", lambda name, *a: sent.append((name, *a)))
+    r = L.LogitsRules(4, 50, max_history=8, max_bias=6, num_masks=1)
+    for bad in (lambda: r.set_bias(0, [1, 2], ["a", "b"]), lambda: r.set_bias(0, [1], [None]), lambda: r.set_bias(0, [[1, 2, 3]], [1.0]),
+                lambda: r.set_bias(0, [1, 2], [[1.0, 2.0], [3.0, 4.0]]), lambda: r.set_bias(0, [1, 2, 3], np.float32(1)),
+                lambda: r.set_history(0, ["a"]), lambda: r.set_penalties(0, 1.1, 0.5, "none"),
+                lambda: r.set_penalties(0, 1.1, None), lambda: r.set_penalties(0, [1.0, 2.0]), lambda: r.use_mask(0, [0, 0])):
+        with pytest.raises((TypeError, ValueError)):
+            bad()
+        assert sent == []
+    r.set_bias(1, np.array([3, 4]), (0.5, -1))
+    assert [c[3] for c in sent] == [8, 8, 4]
+    sent.clear()
+    r.set_penalties(1, 2, np.float64(0.5))
+    r.set_bias(1, [], [])
+    r.set_history(1, [[1, 2, 3]])
+    assert [c[3] for c in sent] == [4] * 4 + [12, 4]
+    L.LogitsRules(0, 50, max_history=8, max_bias=6, num_masks=0)
+
+
 def test_lora_owner_checks(monkeypatch):
     from cactus_amd import lora as L
     sent = []
