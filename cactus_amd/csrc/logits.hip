@@ -134,14 +134,14 @@ __global__ void __launch_bounds__(RULES_THREADS) logits_rules_kernel(RulesArgs a
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < EARLY; u++)
-            if (tid + THREADS * u < hist && (uint32_t)(ht[u] - lo) < (uint32_t)(hi - lo)) atomicAdd(&counts[ht[u] - c0], 1u);
+            if (tid + THREADS * u < hist && (uint32_t)ht[u] - (uint32_t)lo < (uint32_t)(hi - lo)) atomicAdd(&counts[ht[u] - c0], 1u);
         for (int i0 = EARLY * THREADS; i0 < hist; i0 += 8 * THREADS) {
             int t[8];
 #pragma unroll
             for (int u = 0; u < 8; u++) t[u] = i0 + tid + THREADS * u < hist ? h[i0 + tid + THREADS * u] : -1;
 #pragma unroll
             for (int u = 0; u < 8; u++)
-                if ((uint32_t)(t[u] - lo) < (uint32_t)(hi - lo)) atomicAdd(&counts[t[u] - c0], 1u);
+                if ((uint32_t)t[u] - (uint32_t)lo < (uint32_t)(hi - lo)) atomicAdd(&counts[t[u] - c0], 1u);
         }
         if (nb > 0) {
 #pragma unroll

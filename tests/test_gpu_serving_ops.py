@@ -483,6 +483,20 @@ def test_rules_long_histories_and_lists(hip_ready):
     run_rules(hip_ready, (4 * rng.standard_normal((3, V))).astype(np.float16), V, **s)
 
 
+def test_rules_tokens_at_the_ends_of_32_bits(hip_ready):
+    """Outside the vocabulary by as much as there is, in histories on either side of the entries that are read early."""
+    rng = np.random.default_rng(18)
+    ends = np.int32([-(1 << 31), -(1 << 31) + 1, -(1 << 31) + 8192, (1 << 31) - 1, (1 << 31) - 8192, -8192, -1])
+    for V, H in ((5, 7), (20011, 40), (9001, 5000)):
+        s = settings(rng, 2, V, H=H)
+        s["hist"][:, rng.permutation(H)[:max(7, H // 3)]] = np.resize(ends, max(7, H // 3))
+        s["lens"][:] = H
+        s["bias"][0][:, 3:7] = ends[:4]
+        s["bias_counts"][:] = 9
+        for kind in (np.float16, np.float32):
+            run_rules(hip_ready, (4 * rng.standard_normal((2, V))).astype(kind), V, **s)
+
+
 def test_rules_many_rows(hip_ready):
     rng = np.random.default_rng(9)
     for n, V in ((300, 1111), (40, 30000)):
