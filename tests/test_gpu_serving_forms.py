@@ -1,0 +1,124 @@
+"""The forms that the rotated append takes for prompts: sizes that the rules of its dispatch
+send to each, against the plain restatements."""
+import re
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+from test_gpu_serving_ops import Rope
+
+pytestmark = pytest.mark.gpu
+
+EPS = float(np.float32(1e-6))       # what the kernels are given of it
+CSRC = Path(__file__).resolve().parent.parent / "cactus_amd" / "csrc"
+
+
+def rule(source, name):
+    """A constant of a kernel's dispatch: the sizes below are held against it, so that they keep reaching
+    what they are meant for."""
+    return int(re.search(rf"\b{name} = (\d+)", (CSRC / source).read_text()).group(1))
+
+
+# ------------------------------------------------------------------ rotated append
+def tiled(B, n):
+    return n >= rule("kv4_rope.hip", "ROPE_TILE_SEQ") and B * n >= rule("kv4_rope.hip", "ROPE_TILE_ROWS")
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [65, 80])
+def test_tiles_with_queries_in_place(hip_ready, d, n):
+    rng = np.random.default_rng(d)
+    c = Rope(hip_ready, 1, 2, d, 16, 40, 3, 8)
+    assert tiled(2, n)
+    c.extend([0, 2], [n, n - 1])
+    c.append([0, 2], [n, n - 1], *c.rows(rng, 2, n, 4), *c.norms(rng), EPS, in_place=True)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("Hq,H", [(0, 1), (0, 3), (1, 1), (5, 1), (12, 3), (8, 8)])
+def test_tiles_of_few_and_odd_heads(hip_ready, Hq, H, d):
+    rng = np.random.default_rng(Hq + H + d)
+    n = 45
+    c = Rope(hip_ready, 1, H, d, 16, 40, 3, 8)
+    assert tiled(3, n)
+    c.extend([0, 1, 2], [5, 0, 20])
+    c.extend([0, 1, 2], [n, n, n])
+    c.append([0, 1, 2], [n] * 3, *c.rows(rng, 3, n, Hq), *c.norms(rng), EPS)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("q_normed", [True, False])
+def test_tiles_with_one_norm_of_two(hip_ready, q_normed, d):
+    rng = np.random.default_rng(3)
+    n = 130
+    c = Rope(hip_ready, 1, 2, d, 16, 40, 3, 12)
+    assert tiled(1, n)
+    c.extend([0], [n])
+    w = next(c.norms(rng))
+    c.append([0], [n], *c.rows(rng, 1, n, 4), w if q_normed else None, None if q_normed else w, eps=2.0 ** -7)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_tiles_of_requests_that_write_nothing(hip_ready, d):
+    rng = np.random.default_rng(d)
+    n = 66
+    c = Rope(hip_ready, 1, 2, d, 16, 60, 6, 12)
+    assert tiled(2, n)
+    c.extend([0, 1, 3], [n - 2, 70, 33])              # slots 0 and 3 have fewer tokens than rows
+    c.append([0, -1, 6, 1, 1 << 30], [n] * 5, *c.rows(rng, 5, n, 2))
+    c.append([3, 1], [n, 0], *c.rows(rng, 2, n, 2))
+    # a page that the table does not name: the query is rotated all the same
+    c.cpu.table[3, 1] = -1
+    c.gpu._buf["table"].upload(c.cpu.table)
+    c.append([3, 1], [33, n], *c.rows(rng, 2, n, 2), *c.norms(rng), EPS)
+    c.gpu.extend(1, seqs=[99], counts=[1])
+    c.append([1, 0], [n, 1], *c.rows(rng, 2, n, 2), write=False)
+    assert c.gpu.status() == 2
+
+
+def extremes(rng, d, q, k, v):
+    for x in (q, k, v):
+        x[0, 0, 0], x[0, 1, 0] = 0, 65504
+        x[0, 0, 1] = np.float16(2.0 ** -24) * rng.integers(-9, 10, d)
+        x[0, 0, 2, 7], x[0, 1, 3, d - 1], x[1, 2, 4, 3] = np.nan, np.inf, -np.inf
+        x[1, 0, 5] *= np.float16(2.0 ** -12)
+        x[1, 1, 6] = np.where(np.arange(d) % 32 == 5, 60000, 1)
+        x[1, 1, 7] = (np.arange(d) % 14 - 6.5)
+        x[1, 1, 7, ::32] = 7
+        x[1, 40:44, 2] *= np.float16(2.0 ** -18)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("normed", [False, True])
+def test_tiles_of_extreme_values(hip_ready, d, normed):
+    rng = np.random.default_rng(d)
+    n = 70
+    c = Rope(hip_ready, 1, 8, d, 16, 40, 3, 8)
+    assert tiled(2, n)
+    c.extend([0, 1], [n + 5, n])
+    q, k, v = c.rows(rng, 2, n, 8)
+    extremes(rng, d, q, k, v)
+    c.append([0, 1], [n, n], q, k, v, *(c.norms(rng) if normed else (None, None)), EPS)
+
+
+def test_tiles_at_far_positions(hip_ready):
+    rng = np.random.default_rng(2)
+    c = Rope(hip_ready, 1, 1, 64, 4096, 70, 2, 40, theta=1e6)
+    assert tiled(2, 70)
+    c.extend([0, 1], [163840, 100000])
+    c.append([0, 1], [70, 70], *c.rows(rng, 2, 70, 2), *c.norms(rng), EPS)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_and_tiles_meet(hip_ready, d):
+    """On either side of both borders of the rule between a wave per row and tiles."""
+    rng = np.random.default_rng(d)
+    rows, seq = rule("kv4_rope.hip", "ROPE_TILE_ROWS"), rule("kv4_rope.hip", "ROPE_TILE_SEQ")
+    sizes = [(-(-rows // seq), seq), (-(-rows // seq) - 1, seq), (-(-rows // (seq - 1)), seq - 1), (1, rows - 1), (1, rows)]
+    assert [tiled(*s) for s in sizes] == [True, False, False, False, True]
+    for B, n in sizes:
+        c = Rope(hip_ready, 1, 1, d, 16, 60, 24, 12)
+        c.extend(list(range(B)), rng.integers(0, 20, B).tolist())
+        c.extend(list(range(B)), [n] * B)
+        c.append(list(range(B)), [n] * B, *c.rows(rng, B, n, 2), *c.norms(rng), EPS)
