@@ -25,6 +25,10 @@ def tiled(B, n):
     return n >= rule("kv4_rope.hip", "ROPE_TILE_SEQ") and B * n >= rule("kv4_rope.hip", "ROPE_TILE_ROWS")
 
 
+def waves(B, n, Hq, H, d):
+    return B * -(-n // 16) * (d // 64 * (Hq + H) + H)
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("n", [65, 80])
 def test_tiles_with_queries_in_place(hip_ready, d, n):
@@ -122,3 +126,31 @@ def test_rows_and_tiles_meet(hip_ready, d):
         c.extend(list(range(B)), rng.integers(0, 20, B).tolist())
         c.extend(list(range(B)), [n] * B)
         c.append(list(range(B)), [n] * B, *c.rows(rng, B, n, 2), *c.norms(rng), EPS)
+
+
+@pytest.mark.parametrize("d,B,n", [(64, 8, 257), (128, 5, 257), (256, 4, 176)])
+@pytest.mark.parametrize("Hq,normed,in_place", [(33, True, False), (32, False, False), (33, False, True), (32, True, True)])
+def test_waves_of_two_heads(hip_ready, d, B, n, Hq, normed, in_place):
+    """Ragged prompts of so many waves that each takes two heads: with 33 query heads one takes the last of them and
+    the first key head, with 32 the last wave has one key head; of 15 KV heads the last wave has one's values."""
+    rng = np.random.default_rng(d + Hq)
+    H = 15
+    assert tiled(B, n) and waves(B, n, Hq, H, d) >= rule("kv4_rope.hip", "ROPE_TWO_HEADS")
+    c = Rope(hip_ready, 1, H, d, 16, 200, B, 20)
+    counts = [n, n - 1, n // 2 + 3, n - 16, 1, n, 0, n // 3][:B]
+    c.extend(list(range(B)), [3, 0, 16, 31, 15, 7, 1, 40][:B])
+    c.extend(list(range(B)), counts)
+    q, k, v = c.rows(rng, B, n, Hq)
+    extremes(rng, d, q, k, v)
+    c.append(list(range(B)), counts, q, k, v, *(c.norms(rng) if normed else (None, None)), EPS, pad=0 if in_place else 16, in_place=in_place)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_two_heads_of_keys_alone(hip_ready, d):
+    rng = np.random.default_rng(d)
+    B, H = 8, 15
+    n = {64: 560, 128: 370, 256: 225}[d]
+    assert tiled(B, n) and waves(B, n, 0, H, d) >= rule("kv4_rope.hip", "ROPE_TWO_HEADS")
+    c = Rope(hip_ready, 1, H, d, 64, 90, B, 10)
+    c.extend(list(range(B)), [n] * B)
+    c.append(list(range(B)), [n] * B, *c.rows(rng, B, n, 0), None, next(c.norms(rng)), EPS)
