@@ -581,9 +581,11 @@ int cactus_hip_rope_table_f32(float* table, size_t positions, size_t head_dim, f
  * sequences grow).  Of a head's row x, with halves a and b of
  *   y = x / sqrt(mean(x^2) + eps) * norm     (norm NULL: y = x)
  *   (a cos - b sin, b cos + a sin),  cos and sin row p of `table`
- * keys in 64 bits and queries in 32 or more, rounded once to FP16: for queries into
- * q_out [batch][seq_len][num_q_heads][head_dim], for keys the row that is quantized
- * into the pages; values are quantized as they come.  q: num_q_heads (up to 16384) heads
+ * rounded once to FP16: for queries into q_out [batch][seq_len][num_q_heads][head_dim],
+ * for keys the row that is quantized into the pages; values are quantized as they come.
+ * Keys are computed in 64 bits; queries too where seq_len is below 8 or batch * seq_len
+ * below 128, and in 32 above: a query may differ by an FP16 step with the size of the
+ * call that it is in, pages do not.  q: num_q_heads (up to 16384) heads
  * per row, q_stride values from row to row; q_out may be q where the rows are dense
  * (q_stride num_q_heads * head_dim), otherwise it overlaps no input.  num_q_heads 0: keys
  * and values only (q, q_out may be NULL).  q_norm, k_norm [head_dim] fp16, either may

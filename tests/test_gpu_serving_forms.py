@@ -1,12 +1,13 @@
-"""The forms that the rotated append takes for prompts: sizes that the rules of its dispatch
-send to each, against the plain restatements."""
+"""The forms that the rotated append takes: sizes that the rules of its dispatch send to
+each, against the plain restatements."""
 import re
 from pathlib import Path
 
 import numpy as np
 import pytest
 
-from test_gpu_serving_ops import Rope
+import _serving as S
+from test_gpu_serving_ops import Rope, dev
 
 pytestmark = pytest.mark.gpu
 
@@ -154,3 +155,31 @@ def test_two_heads_of_keys_alone(hip_ready, d):
     c = Rope(hip_ready, 1, H, d, 64, 90, B, 10)
     c.extend(list(range(B)), [n] * B)
     c.append(list(range(B)), [n] * B, *c.rows(rng, B, n, 0), None, next(c.norms(rng)), EPS)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("normed", [False, True])
+def test_single_rows_queries_are_rounded_once(hip_ready, d, normed):
+    """Where a wave has one row, queries are computed in 64 bits: the FP16 value next to the formula's, but where that
+    lies so close to the middle of two that 64 bits cannot tell.
+
+    Of |a cos| + |b sin|, the sum of d squares (d / 64 + 6 roundings, half of them in the root), its
+    root, and four products and a sum err by less than 32 of 2^-53: 2^-48."""
+    rng = np.random.default_rng(d)
+    B, n, Hq = 20, 6, 16
+    assert not tiled(B, n)
+    c = Rope(hip_ready, 1, 1, d, 16, 200, B, 8)
+    lens = rng.integers(n, 100, B).tolist()
+    c.extend(list(range(B)), lens)
+    q, k, v = c.rows(rng, B, n, Hq)
+    q_norm, k_norm = c.norms(rng) if normed else (None, None)
+    b = [dev(hip_ready, a) for a in (q, k, v)] + [hip_ready.DeviceBuffer(q.nbytes)]
+    w = [None if a is None else dev(hip_ready, a) for a in (q_norm, k_norm)]
+    c.gpu.append_rope(0, b[0].ptr, b[3].ptr, Hq, b[1].ptr, b[2].ptr, B, n, c.dtable.ptr, len(c.table), None, None,
+                      *(a and a.ptr for a in w), EPS)
+    got = b[3].to_numpy(np.float16, q.shape)
+    for i in range(B):
+        for r in range(n):
+            y, err = S.rotated(q[i, r], q_norm, EPS, c.table[lens[i] - n + r])
+            e = err / ((d / 2 + 12) * S.E32) * 2.0 ** -48
+            assert ((y - e).astype(np.float16) <= got[i, r]).all() and (got[i, r] <= (y + e).astype(np.float16)).all()
