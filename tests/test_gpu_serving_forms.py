@@ -1,5 +1,5 @@
-"""The forms that the rotated append takes: sizes that the rules of its dispatch send to
-each, against the plain restatements."""
+"""The forms that the rotated append and the adapters take: sizes that the rules of their
+dispatch send to each, against the plain restatements."""
 import re
 from pathlib import Path
 
@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import _serving as S
-from test_gpu_serving_ops import Rope, dev
+from test_gpu_serving_ops import Rope, adapters, check_lora, dev, f16, run_lora
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +183,106 @@ def test_single_rows_queries_are_rounded_once(hip_ready, d, normed):
             y, err = S.rotated(q[i, r], q_norm, EPS, c.table[lens[i] - n + r])
             e = err / ((d / 2 + 12) * S.E32) * 2.0 ** -48
             assert ((y - e).astype(np.float16) <= got[i, r]).all() and (got[i, r] <= (y + e).astype(np.float16)).all()
+
+
+# ------------------------------------------------------------------ adapters
+def tiles32(b, n):
+    return n > 16 and b * -(-n // 32) >= rule("lora.hip", "LORA_TILE2")
+
+
+def requests(rng, b, n):
+    """Ragged rows, some requests without any or with more than there are; adapters 0 to 3, a third of them none."""
+    counts = rng.integers(1, n + 1, b)
+    counts[[1, 4, 7]] = 0, n + 9, -2
+    ids = rng.integers(-2, 4, b)
+    ids[:3] = 3, 0, -1
+    return counts.tolist(), ids.tolist()
+
+
+@pytest.mark.parametrize("r", [8, 16, 24, 32, 40, 64, 72, 128, 136, 256])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_lora_prompts_in_tiles_of_32_rows(hip_ready, r, in_place):
+    """Several steps of K per wave and more than one round of outputs per workgroup, both with a remainder."""
+    rng = np.random.default_rng(r)
+    b, n, K, N = 33, 50, 1160, 1544
+    assert tiles32(b, n)
+    A, B, s = adapters(rng, 4, r, K, N)
+    x, base = f16(rng, b, n, K), f16(rng, b, n, N)
+    counts, ids = requests(rng, b, n)
+    for i, m in enumerate(counts):
+        x[i, max(m, 0):] = np.nan            # not read: no row that is there is touched by them
+    got = run_lora(hip_ready, x, A, B, s, ids, counts, base, (8, 16, 24), in_place)
+    check_lora(got, x, A, B, s, ids, counts, base, in_place)
+
+
+@pytest.mark.parametrize("r", [8, 16, 48, 64, 128, 200])
+def test_lora_more_tiles_than_workgroups_at_a_time(hip_ready, r):
+    """Every workgroup takes all outputs of its rows."""
+    rng = np.random.default_rng(r)
+    b, n, K, N = 90, 70, 72, 1032
+    assert tiles32(b, n) and b * -(-n // 32) > rule("lora.hip", "LORA_WGS")
+    A, B, s = adapters(rng, 4, r, K, N)
+    x, base = f16(rng, b, n, K), f16(rng, b, n, N)
+    counts, ids = requests(rng, b, n)
+    check_lora(run_lora(hip_ready, x, A, B, s, ids, counts, base), x, A, B, s, ids, counts, base)
+
+
+@pytest.mark.parametrize("r", [16, 32, 64, 128, 256])
+def test_lora_32_row_tiles_keep_nan_and_infinity_in_their_rows(hip_ready, r):
+    rng = np.random.default_rng(r)
+    b, n, K, N = 32, 50, 136, 200
+    assert tiles32(b, n)
+    A, B, s = adapters(rng, 2, r, K, N)
+    x, base = f16(rng, b, n, K), f16(rng, b, n, N)
+    ids = [i % 2 for i in range(b)]
+    clean = run_lora(hip_ready, x, A, B, s, ids, None, base)
+    check_lora(clean, x, A, B, s, ids, None, base)
+    for bad in (np.nan, np.inf, -np.inf):
+        y = x.copy()
+        y[0, 17, 5], y[5, 31, 135], y[31, 49, 0] = bad, bad, bad
+        got = run_lora(hip_ready, y, A, B, s, ids, None, base)
+        for i, j in ((0, 17), (5, 31), (31, 49)):
+            assert not np.isfinite(got[i, j]).any()
+            got[i, j] = clean[i, j]
+        np.testing.assert_array_equal(got, clean)
+
+
+@pytest.mark.parametrize("r", [8, 64])
+def test_lora_32_row_tiles_ranges(hip_ready, r):
+    """The ranks' values pass FP16's range on both sides."""
+    rng = np.random.default_rng(r)
+    b, n, K, N = 32, 40, 264, 72
+    assert tiles32(b, n)
+    for ax, aa, ab, s in ((2.0 ** -14, 2.0 ** -14, 1.0, 1.0), (200.0, 200.0, 2.0 ** -12, 2.0 ** -8), (3000.0, 3000.0, 2.0 ** -24, 2.0 ** -10),
+                          (0.0, 1.0, 1.0, 1.0)):
+        A, B = f16(rng, 2, r, K, scale=aa), f16(rng, 2, N, r, scale=ab)
+        x, base = f16(rng, b, n, K, scale=ax), f16(rng, b, n, N, scale=1e-3)
+        sc, ids = np.array([s, -s], np.float32), [i % 2 for i in range(b)]
+        check_lora(run_lora(hip_ready, x, A, B, sc, ids, None, base), x, A, B, sc, ids, None, base)
+
+
+def test_lora_tiles_of_16_and_32_rows_meet(hip_ready):
+    rng = np.random.default_rng(1)
+    K, N, most = 104, 136, rule("lora.hip", "LORA_TILE2")
+    A, B, s = adapters(rng, 4, 32, K, N)
+    sizes = [(most - 1, 17), (most, 17), (most, 16), (most // 2, 33), (most // 2 - 1, 64), (1, 32 * most), (1, 32 * (most - 1))]
+    assert [tiles32(*z) for z in sizes] == [False, True, False, True, False, True, False]
+    for b, n in sizes:
+        x, base, ids = f16(rng, b, n, K), f16(rng, b, n, N), rng.integers(-1, 4, b).tolist()
+        check_lora(run_lora(hip_ready, x, A, B, s, ids, None, base), x, A, B, s, ids, None, base)
+
+
+@pytest.mark.parametrize("r,N", [(8, 16392), (16, 8200), (24, 8200), (64, 4104), (128, 4104), (256, 4104)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_lora_single_rows_in_several_rounds(hip_ready, r, N, in_place):
+    """So many requests that a workgroup's waves take outputs more than once, with a remainder."""
+    rng = np.random.default_rng(r)
+    b, K = 130, 1544
+    pieces = 1 << (r // 8 - 1).bit_length()
+    assert -(-N // (512 // pieces)) > 8 * -(-rule("lora.hip", "LORA_WGS") // b), "one round"
+    A, B, s = adapters(rng, 5, r, K, N)
+    x, base = f16(rng, b, 1, K), f16(rng, b, 1, N)
+    ids = rng.integers(-1, 6, b).tolist()
+    counts = rng.integers(-1, 3, b).tolist()
+    got = run_lora(hip_ready, x, A, B, s, ids, counts, base, (8, 16, 24), in_place)
+    check_lora(got, x, A, B, s, ids, counts, base, in_place)
