@@ -10,11 +10,12 @@
 // where a wave has one row, 32 where it has many, rounded once too.
 //
 // Single rows are bound by the chain of loads (length, position, rotation and page), prompts by
-// memory with the vector units 60% busy.  Four prompts of up to 2048 rows, 16 query and 8 KV
-// heads of 128 dims with norms: 25.9 us, 84 MB, 3.2 TB/s (16 more query heads add 48.8 MB in
-// 10 us, 4.9 TB/s; the keys' 64-bit sums are what the rest waits for).  64 single rows 3.4 us,
-// one row of 4 and 1 heads of 256 dims 3.4.  Queries go past the caches: 39.9 -> 38.4 us with the
-// read of the keys and values.
+// memory with the vector units 60% busy.  Four prompts of up to 2048 rows (6427 in all), 16 query
+// and 8 KV heads of 128 dims with norms: 24.7 us in a graph, 26.4 traced; 89.7 MB, 3.6 TB/s (16 more
+// query heads add 52.6 MB in 11.6 us, 4.5 TB/s; the keys' 64-bit sums are what the rest waits
+// for).  The same with 64 dims 13.6 us (3.3 TB/s), with 256 dims 47.1 (3.8), with 4 and 1 heads of 256
+// dims 11.8 (3.5).  64 single rows 4.3 us traced, one row of 4 and 1 heads of 256 dims 3.9.  Queries
+// go past the caches: 39.9 -> 38.4 us with the read of the keys and values.
 #include "kv4_device.h"
 
 namespace cactus_hip {
@@ -169,7 +170,12 @@ constexpr int TILE_WAVES = 4;
 // Rows of a call from which tiles are faster than a wave per row and head (8 sequences of 8 rows 5.8
 // against 6.2 us, of 16 rows 6.7 against 6.4; 64 of 4 rows 8.5 against 10.0, of 8 rows 11.6
 // against 10.9: shorter sequences leave tiles too empty), and waves from which one takes two
-// heads (2000 waves 7.8 against 8.7 us, 14000 27.5 against 26.3; 16 query and 8 KV heads of 128).
+// heads, by them one and two heads per wave (us):
+//   waves        16 / 8 of 64     16 / 8 of 128    16 / 8 of 256    32 / 8 of 128    4 / 1 of 256
+//   2000          4.6   5.5        4.9   6.7        6.4   9.7        4.7   5.8        6.3   5.7
+//   8200         10.5  10.7       11.1  11.5       13.1  13.2       10.7  11.1       13.0  11.3
+//   12300        14.2  13.4       14.4  14.1       17.1  17.1       14.0  13.3       16.7  14.6
+//   28000        26.9  24.8       32.3  29.2       34.7  32.0       30.7  27.6       36.1  30.5
 constexpr size_t ROPE_TILE_ROWS = 128, ROPE_TILE_SEQ = 8, ROPE_TWO_HEADS = 8192;
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {

@@ -4,8 +4,13 @@
 // Bound by memory: x, base and y are 2 (K + 2 N) bytes a row for 2 r (K + N) operations.  8 x
 // 1024 rows of 4096 by 4096: rank 16 46 us and rank 32 48 (4.4 and 4.3 TB/s; a copy of 2 GiB runs
 // at 4.9), rank 64 56 us, where the weights that 256 workgroups read from the L2, 1 MB each, tell.
-// Five prompts of up to 701 rows, 1024 by 2048, rank 32: 9.6 us; 64 single rows with 24 adapters,
-// 2048 by 1024, rank 16: 4.6 us; one row 3.3 (an empty launch 2.4).
+// That is 256 tiles of 32 rows on 256 CUs.  A workgroup's 91 to 156 KB of LDS leave room for one per CU, so
+// that more rows come in rounds: 8224 rows 57 and 84 us (ranks 16 and 64), 16384 83 and 101.  Ranks above 64
+// have four waves per workgroup and read x again in every pass: 95 us (rank 128) and 157 (256)
+// for 8192 rows, 151 and 247 for 8224.
+// Five prompts of up to 701 rows, 1024 by 2048, rank 32: 9.4 us (rank 64 12.3, 128 27.7,
+// 256 47.9); 64 single rows with 24 adapters, 2048 by 1024, rank 16: 4.6 us; one row 3.3 (an empty
+// launch 2.4).
 #include "hip_common.h"
 
 namespace cactus_hip {

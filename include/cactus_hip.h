@@ -168,7 +168,8 @@ int cactus_hip_matmul_int4_f16act_batched(const uint16_t* A, const uint8_t* B_pa
                                           size_t stride_c, void* stream);
 /* No counterpart in the reference.  Low-rank adapters of many requests beside a
  * projection that they share: row j of request i, with adapter a = adapters[i],
- *   y = fp16(base + scales[a] * B_a (A_a x))     (sums in FP32)
+ *   y = fp16(base + scales[a] * B_a (A_a x))     (sums in FP32; with seq_len above 1, A_a x
+ * enters the second product with 22 bits, or to 2^-39 of its row's largest)
  * x [batch][seq_len] rows of K, base (the projection's output) and y rows of N, each
  * with its stride from row to row; A [num_adapters][rank][K], B [num_adapters][N][rank]
  * fp16 (rows = outputs, like every weight here); scales [num_adapters] f32 (NULL: 1);
@@ -376,7 +377,7 @@ int cactus_hip_sample_f32(const float* logits, uint32_t* out, size_t vocab, floa
  *           x = x - frequency[s] * n;  x = x - presence[s]
  *   x = x + bias, for every entry of the slot's list that names the token, in order
  *   x = -infinity where the bit of the slot's mask is 0
- * each operation in FP32, rounded by itself.  best[i] (NULL: not wanted): the first index of
+ * each operation in FP32, rounded by itself; one list of tokens for all three penalties.  best[i] (NULL: not wanted): the first index of
  * the largest value; NaN is never it; 0 where no value is above -infinity.  The
  * rows of out are what cactus_hip_sample_f32 takes.  A slot outside [0, max_seqs)
  * makes no access: its row of out and best are left as they were.  FP32 rows may be
