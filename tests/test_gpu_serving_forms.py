@@ -1,5 +1,6 @@
 """The forms that the rotated append and the adapters take: sizes that the rules of their
 dispatch send to each, against the plain restatements."""
+import ctypes
 import re
 from pathlib import Path
 
@@ -7,7 +8,7 @@ import numpy as np
 import pytest
 
 import _serving as S
-from test_gpu_serving_ops import Rope, adapters, check_lora, dev, f16, run_lora
+from test_gpu_serving_ops import Rope, Step, adapters, check_lora, dev, f16, run_lora
 
 pytestmark = pytest.mark.gpu
 
@@ -286,3 +287,46 @@ def test_lora_single_rows_in_several_rounds(hip_ready, r, N, in_place):
     counts = rng.integers(-1, 3, b).tolist()
     got = run_lora(hip_ready, x, A, B, s, ids, counts, base, (8, 16, 24), in_place)
     check_lora(got, x, A, B, s, ids, counts, base, in_place)
+
+
+# ------------------------------------------------------------------ a step of prompts
+def test_captured_prompts(hip_ready):
+    """Prompts as a graph, replayed while the sequences grow, an eager step on another stream at the same time:
+    both have what they have alone."""
+    cm, B, n = hip_ready, 33, 40
+    a, e = (Step(cm, B, np.random.default_rng(16)) for _ in range(2))
+    assert tiled(B, n) and tiles32(B, n)
+    rng = np.random.default_rng(17)
+    st = cm.Stream()
+    ba, be = a.buffers(n), e.buffers(n)
+
+    def rows(counts):
+        x = f16(rng, B, n, a.HID)
+        for b in (ba, be):
+            b["x"].upload(x)
+            b["counts"].upload(np.int32(counts))
+            for k in ("qkv", "q", "o"):
+                b[k].upload(np.zeros(b[k].nbytes // 2, np.float16))
+    rows([n] * B)
+    for s, b in ((a, ba), (e, be)):            # once before the capture, so that scratch memory is there
+        s.run(b, n, st.handle)
+        st.sync()
+    graph = ctypes.c_void_p()
+    cm.call("cactus_hip_graph_capture_begin", st.handle)
+    a.run(ba, n, st.handle)
+    cm.call("cactus_hip_graph_capture_end", st.handle, ctypes.byref(graph))
+    for i in range(3):
+        rows(rng.integers(0, n + 1, B))
+        cm.call("cactus_hip_graph_launch", graph, st.handle)
+        e.run(be, n, None)
+        st.sync()
+        cm.call("cactus_hip_stream_sync", None)
+        assert a.cache.status(st.handle) == 0 and e.cache.status() == 0
+        for k in ("qkv", "q", "o"):
+            size = ba[k].nbytes // 2
+            np.testing.assert_array_equal(ba[k].to_numpy(np.uint16, size), be[k].to_numpy(np.uint16, size), err_msg=f"replay {i}: {k}")
+        for name, v in a.cache.tables().items():
+            np.testing.assert_array_equal(v, e.cache.tables()[name])
+        size = a.cache._buf["pages"].nbytes
+        np.testing.assert_array_equal(a.cache._buf["pages"].to_numpy(np.uint8, size), e.cache._buf["pages"].to_numpy(np.uint8, size))
+    cm.call("cactus_hip_graph_destroy", graph)
