@@ -173,6 +173,7 @@ constexpr int TILE_WAVES = 4;
 // heads, by them one and two heads per wave (us):
 //   waves        16 / 8 of 64     16 / 8 of 128    16 / 8 of 256    32 / 8 of 128    4 / 1 of 256
 //   2000          4.6   5.5        4.9   6.7        6.4   9.7        4.7   5.8        6.3   5.7
+//   6100          9.2   7.3        9.4   9.0       10.8  10.8        9.0   8.9       10.8   9.3
 //   8200         10.5  10.7       11.1  11.5       13.1  13.2       10.7  11.1       13.0  11.3
 //   12300        14.2  13.4       14.4  14.1       17.1  17.1       14.0  13.3       16.7  14.6
 //   28000        26.9  24.8       32.3  29.2       34.7  32.0       30.7  27.6       36.1  30.5
